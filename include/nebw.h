@@ -227,6 +227,157 @@ int nebw_layernorm_quant(nebw_dev *dev, float *x, const float *y, const float *g
                          const float *beta, float eps, int64_t rows, int64_t H, const float *ias,
                          int8_t *q, float *scale, void *stream);
 
+/* ---- rotary positions and norms of the query and key heads ----------------
+ * For a maintainer whose encoder rotates other than the model passes do
+ * (adjacent pairs, a part of each head, positions past the trained length,
+ * few key heads), or norms each query and key head first.  They go between
+ * nebw_gemm (Q|K|V) and nebw_attention.  Device buffers, asynchronous on
+ * `stream`, no allocation, no workspace: they can be captured in a graph.  No
+ * counterpart in the reference, whose one form (rotate-half over the whole
+ * head) the QKV epilogue of a rotary model applies. */
+
+/* Which elements of a head turn together, n = rot_dim / 2: HALF i and n + i,
+ * PAIRS 2i and 2i + 1.  Elements from rot_dim on do not turn. */
+enum { NEBW_ROPE_HALF = 0, NEBW_ROPE_PAIRS = 1 };
+/* Frequencies for positions past the trained length, f_i = theta^(-i/n):
+ *   LINEAR  f_i / factor
+ *   NTK     f_i of the base theta * factor^(n / (n - 1))
+ *   YARN    f_i where it turns more than `fast` (0: 32) times within orig_len
+ *           positions, f_i / factor where fewer than `slow` (0: 1) times,
+ *           blended linearly over the index in between; the rotated values
+ *           times attn_scale (0: 0.1 ln(factor) + 1)
+ *   BANDS   the same two ends (fast 0: 4, slow 0: 1), blended linearly over
+ *           the number of turns, and no scale */
+enum {
+  NEBW_ROPE_PLAIN = 0, NEBW_ROPE_LINEAR = 1, NEBW_ROPE_NTK = 2, NEBW_ROPE_YARN = 3,
+  NEBW_ROPE_BANDS = 4
+};
+typedef struct nebw_rope_scaling {
+  int32_t kind;       /* NEBW_ROPE_PLAIN ..                  */
+  int32_t reserved0;
+  int64_t orig_len;   /* YARN, BANDS: the trained length     */
+  double factor;      /* >= 1                                */
+  double fast, slow;  /* YARN, BANDS: 0 for the defaults     */
+  double attn_scale;  /* YARN: 0 for the default             */
+} nebw_rope_scaling;
+/* inv_freq[rot_dim / 2] and the tables' scale (NULL scaling: PLAIN).  Host
+ * only.  The set also suits nebw_model_set_rope_freq where *scale is 1.
+ * theta > 1; rot_dim even, up to 256. */
+int nebw_rope_freqs(double theta, int32_t rot_dim, const nebw_rope_scaling *scaling,
+                    double *inv_freq, double *scale);
+/* The table cos, sin (position * inv_freq[i]) * scale of positions
+ * [0, max_pos) for n host frequencies: taken in double, rounded once, kept on
+ * the device (8 bytes an entry, 2^28 entries at most).  rot_dim = 2n.
+ * Released with nebw_release_weight.  Synchronous. */
+int nebw_stage_rope(nebw_dev *dev, const double *inv_freq, int32_t n, int64_t max_pos,
+                    double scale, uint64_t *handle);
+/* pos[seq_off[b] + s] = s for s < seq_len[b] (at most max_len): the packed
+ * rows' positions in their sequences, from nebw_pack_offsets' outputs. */
+int nebw_row_positions(nebw_dev *dev, const int32_t *seq_off, const int32_t *seq_len, int32_t B,
+                       int32_t max_len, int32_t *pos, void *stream);
+
+/* The query or the key heads of packed rows: row r's head h is the head_dim
+ * elements at x + r * stride + h * head_dim (stride in elements: 3H for the Q
+ * or K block of a Q|K|V row).  The results go to out in the same manner: out
+ * == x with out_stride == stride works in place, otherwise the two must not
+ * overlap.  Query and key head counts are independent. */
+typedef struct nebw_heads {
+  const void *x;
+  void *out;
+  int64_t stride, out_stride;
+  int32_t heads;
+  int32_t reserved0;
+  const float *gamma; /* [head_dim] fp32, the norm's weight               */
+  const float *beta;  /* [head_dim] fp32, NEBW_HEADNORM_LAYER only         */
+} nebw_heads;
+/* NEBW_HEADNORM_RMS: x / sqrt(mean(x^2) + eps) * gamma.
+ * NEBW_HEADNORM_LAYER: (x - mean) / sqrt(var + eps) * gamma + beta. */
+enum { NEBW_HEADNORM_NONE = 0, NEBW_HEADNORM_RMS = 1, NEBW_HEADNORM_LAYER = 2 };
+
+/* Rotary positions: the pair (a, b) of a head of row r becomes
+ * (a cos - b sin, b cos + a sin) of pos[r]'s table entry; fp32 arithmetic,
+ * one rounding.  q or k may be NULL (or have no heads).  dtype NEBW_BF16 or
+ * NEBW_F32; head_dim even, up to 256, at least the handle's rot_dim.  pos
+ * [rows] int32 device; a position outside the table is an NEBW_EDEVICE error
+ * at the next sync, and the nearest entry is used.  rows_dev (may be NULL):
+ * device count of live rows; rows from min(*rows_dev, rows) on are left as
+ * they are. */
+int nebw_rope(nebw_dev *dev, const nebw_heads *q, const nebw_heads *k, int dtype, int64_t rows,
+              const int32_t *rows_dev, int32_t head_dim, uint64_t rope, int layout,
+              const int32_t *pos, void *stream);
+/* A norm of every query and key head over its head_dim, then the rotation of
+ * nebw_rope (rope 0: none, pos may then be NULL), in one pass. */
+int nebw_qk_norm_rope(nebw_dev *dev, const nebw_heads *q, const nebw_heads *k, int dtype,
+                      int64_t rows, const int32_t *rows_dev, int32_t head_dim, int norm,
+                      float eps, uint64_t rope, int layout, const int32_t *pos, void *stream);
+
+/* ---- experts ----------------------------------------------------------------
+ * The feed-forward of an expert layer, in place of the two FFN nebw_gemm
+ * calls: nebw_gemm (router logits) -> nebw_moe_route -> nebw_gemm_grouped (up)
+ * -> nebw_gemm_grouped (down) -> nebw_moe_combine -> nebw_layernorm.  The
+ * group sizes stay on the device, so the chain is asynchronous and one
+ * captured graph serves every routing of its shape.  No counterpart in the
+ * reference, which has no expert models. */
+
+/* The weights of `experts` (up to 512) experts, [experts, K, N] row-major,
+ * each the container's [K, N] operand, fp32 or bf16, in host memory or on
+ * this device (then read on `stream`); staged once as bf16 RNE [experts, N,
+ * K].  gated != 0: N = 2F = [up | gate] along N, F % 32 == 0, and the
+ * grouped product forms up * act(gate).  K % 8 == 0, K >= 64, N % 8 == 0.
+ * Released with nebw_release_weight.  Synchronous. */
+int nebw_stage_experts(nebw_dev *dev, const void *kn, int dtype, int32_t experts, int64_t K,
+                       int64_t N, int gated, void *stream, uint64_t *handle);
+
+enum { NEBW_ROUTE_SOFTMAX = 0, NEBW_ROUTE_SIGMOID = 1 };
+/* Bytes of device workspace nebw_moe_route needs (-1: refused sizes).  A
+ * workspace belongs to one call at a time. */
+int64_t nebw_moe_route_workspace(int64_t rows, int32_t experts, int32_t top_k);
+/* The top_k (up to 16) of `experts` (up to 512) experts of each row, and the
+ * rows grouped by expert.  logits [rows, stride] device, fp32 or bf16 (stride
+ * >= experts in elements: a padded GEMM output's N).  The largest logits are
+ * chosen, ties to the lower expert; -inf and NaN are never chosen.  Their
+ * scores are the softmax over all experts or the sigmoid; renorm != 0 divides
+ * by the sum of the chosen; then times scale.  Outputs, all device:
+ *   ids [rows, top_k], weights [rows, top_k] fp32, by falling logit
+ *   group_off [experts + 1]: expert e has the places group_off[e] ..
+ *     group_off[e + 1], its rows ascending
+ *   row_src [rows * top_k]: the row at each place
+ *   row_dst [rows, top_k]: the place of each chosen expert
+ * Where fewer than top_k can be chosen the rest have id -1, weight 0, row_dst
+ * -1 and no place.  rows_dev (may be NULL): device count of live rows; the
+ * outputs of rows behind it, and row_src from group_off[experts] on, are left
+ * as they are.  The result does not depend on scheduling. */
+int nebw_moe_route(nebw_dev *dev, const void *logits, int dtype, int64_t stride, int64_t rows,
+                   const int32_t *rows_dev, int32_t experts, int32_t top_k, int score, int renorm,
+                   float scale, int32_t *ids, float *weights, int32_t *group_off,
+                   int32_t *row_src, int32_t *row_dst, void *workspace, int64_t workspace_bytes,
+                   void *stream);
+
+/* One product per expert over its group of rows:
+ *   C[p] = act(A[row_src[p]] . W[e] + bias[e]), group_off[e] <= p < group_off[e + 1]
+ * (row_src NULL: A[p]).  A bf16 [a_rows, K]; C [rows, N] (gated: [rows, N / 2]
+ * = up * act(gate)), bf16, or fp32 with act NONE; bias [experts, N] fp32 in
+ * the container's column order, or NULL; act NEBW_ACT_*, for gated weights
+ * NEBW_GATE_*.  rows bounds group_off[experts]; rows of C in no group are
+ * left as they are.  Products accumulate in fp32, one rounding.  group_off
+ * that falls or leaves [0, rows], or a row_src outside A, is an NEBW_EDEVICE
+ * error at the next sync (clamped, so nothing is read out of bounds).  A, C
+ * and bias 16-byte aligned; C must not overlap A. */
+int nebw_gemm_grouped(nebw_dev *dev, uint64_t weight, const void *A, int64_t a_rows,
+                      const int32_t *row_src, const int32_t *group_off, int64_t rows, int64_t K,
+                      int64_t N, const float *bias, int act, void *C, int c_dtype, void *stream);
+
+/* out[t] = residual[t] + sum_j weights[t, j] * y[row_dst[t, j]], j ascending
+ * in fp32, one rounding: the experts' rows y [y_rows, H] (bf16 or fp32) back
+ * in row order, bf16 or fp32.  row_dst < 0 adds nothing and reads nothing;
+ * row_dst >= y_rows is an NEBW_EDEVICE error at the next sync (and adds
+ * nothing).  residual [rows, H] fp32 (NULL: none) may be out itself where out
+ * is fp32.  rows_dev as in nebw_moe_route. */
+int nebw_moe_combine(nebw_dev *dev, const void *y, int y_dtype, int64_t y_rows,
+                     const int32_t *row_dst, const float *weights, int64_t rows,
+                     const int32_t *rows_dev, int32_t top_k, int64_t H, const float *residual,
+                     void *out, int out_dtype, void *stream);
+
 /* ---- the whole encoder -------------------------------------------------- */
 
 /* Geometry a container's config carries (set_model_shape,

@@ -1,0 +1,589 @@
+// The operators of rotary and expert encoder layers, C ABI part of
+// include/nebw.h: rotary positions, per-head norms, expert routing, grouped
+// products and the combine.  This file is part of the nebw.cu translation
+// unit (included at its end): it uses that file's device handle, tensor maps
+// and error reporting.  None of these has a counterpart in the reference.
+
+namespace {
+
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// Host or this device's memory; *on_device says which.
+int where_is(nebw_dev *d, const void *p, bool *on_device) {
+  cudaPointerAttributes a;
+  NEBW_CUDA(cudaPointerGetAttributes(&a, p));
+  *on_device = a.type == cudaMemoryTypeDevice || a.type == cudaMemoryTypeManaged;
+  NEBW_REQUIRE(a.type != cudaMemoryTypeDevice || a.device == d->device,
+               "the data is on device %d, the handle on device %d", a.device, d->device);
+  return NEBW_OK;
+}
+
+template <int BN, int EPI>
+int set_grouped_attr() {
+  const int smem = nebw::GroupedShape<BN>::kSmemBytes;
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<BN, EPI, false>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<BN, EPI, true>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  return NEBW_OK;
+}
+
+template <int BN>
+int set_grouped_attrs_bn() {
+  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16>()) return rc;
+  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16Gelu8>()) return rc;
+  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16Erf>()) return rc;
+  if (int rc = set_grouped_attr<BN, nebw::kGrpF32>()) return rc;
+  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16SwiGLU>()) return rc;
+  return set_grouped_attr<BN, nebw::kGrpBf16GeGLU>();
+}
+
+int set_layer_op_attrs() {
+  if (int rc = set_grouped_attrs_bn<128>()) return rc;
+  if (int rc = set_grouped_attrs_bn<256>()) return rc;
+  NEBW_CUDA(cudaFuncSetAttribute(
+      nebw::route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      (nebw::kRouteWarps + 1) * nebw::kRouteMaxExperts * static_cast<int>(sizeof(int))));
+  return NEBW_OK;
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------
+// rotary positions and per-head norms
+// ---------------------------------------------------------------------------
+
+extern "C" int nebw_rope_freqs(double theta, int32_t rot_dim, const nebw_rope_scaling *s,
+                               double *inv_freq, double *scale) {
+  NEBW_REQUIRE(inv_freq && scale, "null frequency output");
+  NEBW_REQUIRE(rot_dim >= 2 && rot_dim % 2 == 0 && rot_dim <= nebw::kHeadMaxDim,
+               "rotary width %d refused: even, 2 .. %d", rot_dim, nebw::kHeadMaxDim);
+  NEBW_REQUIRE(theta > 1.0 && std::isfinite(theta), "rotary base %g refused", theta);
+  const int n = rot_dim / 2;
+  const int kind = s ? s->kind : NEBW_ROPE_PLAIN;
+  *scale = 1.0;
+  if (kind != NEBW_ROPE_PLAIN) {
+    NEBW_REQUIRE(kind == NEBW_ROPE_LINEAR || kind == NEBW_ROPE_NTK || kind == NEBW_ROPE_YARN ||
+                     kind == NEBW_ROPE_BANDS,
+                 "rotary scaling %d refused", kind);
+    NEBW_REQUIRE(s->factor >= 1.0 && std::isfinite(s->factor), "rotary factor %g refused: >= 1",
+                 s->factor);
+  }
+  const bool trained = kind == NEBW_ROPE_YARN || kind == NEBW_ROPE_BANDS;
+  double fast = 0.0, slow = 0.0;
+  if (trained) {
+    NEBW_REQUIRE(s->orig_len > 0, "this rotary scaling needs the trained length");
+    fast = s->fast > 0.0 ? s->fast : kind == NEBW_ROPE_YARN ? 32.0 : 4.0;
+    slow = s->slow > 0.0 ? s->slow : 1.0;
+    NEBW_REQUIRE(fast > slow, "rotary bounds refused: fast %g must be above slow %g", fast, slow);
+  }
+  constexpr double kTwoPi = 6.283185307179586476925;
+  double base = theta;
+  if (kind == NEBW_ROPE_NTK) base = n > 1 ? theta * std::pow(s->factor, n / (n - 1.0)) : theta;
+  double lo = 0.0, hi = 0.0;
+  if (kind == NEBW_ROPE_YARN) {
+    // the index whose frequency turns beta times within the trained length
+    const double len = static_cast<double>(s->orig_len);
+    lo = std::max(0.0, std::floor(n * std::log(len / (fast * kTwoPi)) / std::log(theta)));
+    hi = std::min(n - 1.0, std::ceil(n * std::log(len / (slow * kTwoPi)) / std::log(theta)));
+    *scale = s->attn_scale > 0.0 ? s->attn_scale : 0.1 * std::log(s->factor) + 1.0;
+  }
+  for (int i = 0; i < n; ++i) {
+    const double f = std::pow(base, -static_cast<double>(i) / n);
+    double keep = 1.0;  // the share that stays unscaled
+    if (kind == NEBW_ROPE_LINEAR) keep = 0.0;
+    if (kind == NEBW_ROPE_YARN)
+      keep = 1.0 - std::min(1.0, std::max(0.0, (i - lo) / std::max(hi - lo, 1e-3)));
+    if (kind == NEBW_ROPE_BANDS)
+      keep = std::min(1.0, std::max(0.0, (s->orig_len * f / kTwoPi - slow) / (fast - slow)));
+    inv_freq[i] = keep == 1.0 ? f : f * keep + f / s->factor * (1.0 - keep);
+  }
+  return NEBW_OK;
+}
+
+extern "C" int nebw_stage_rope(nebw_dev *d, const double *inv_freq, int32_t n, int64_t max_pos,
+                               double scale, uint64_t *handle) {
+  if (int rc = use_dev(d)) return rc;
+  NEBW_REQUIRE(inv_freq && handle, "null rotary operand");
+  NEBW_REQUIRE(n >= 1 && n <= nebw::kHeadMaxDim / 2, "%d rotary frequencies refused: 1 .. %d", n,
+               nebw::kHeadMaxDim / 2);
+  NEBW_REQUIRE(max_pos >= 1 && max_pos <= (1ll << 28) / n,
+               "rotary table of %lld positions refused", static_cast<long long>(max_pos));
+  NEBW_REQUIRE(std::isfinite(scale) && scale != 0.0, "rotary scale %g refused", scale);
+  for (int i = 0; i < n; ++i)
+    NEBW_REQUIRE(std::isfinite(inv_freq[i]), "rotary frequency %d is not finite", i);
+  RopeTable t;
+  t.n = n;
+  t.max_pos = max_pos;
+  double *freq = nullptr;
+  const size_t entries = static_cast<size_t>(max_pos) * n;
+  if (cudaMalloc(&t.table, entries * sizeof(float2)) != cudaSuccess ||
+      cudaMalloc(&freq, n * sizeof(double)) != cudaSuccess) {
+    cudaGetLastError();
+    cudaFree(t.table);
+    return set_error(NEBW_ENOMEM, "cudaMalloc for a rotary table [%lld, %d] failed",
+                     static_cast<long long>(max_pos), n);
+  }
+  cudaError_t e =
+      cudaMemcpyAsync(freq, inv_freq, n * sizeof(double), cudaMemcpyHostToDevice, d->stream);
+  if (e == cudaSuccess) {
+    nebw::rope_table_kernel<<<static_cast<unsigned>((entries + 255) / 256), 256, 0, d->stream>>>(
+        freq, n, max_pos, scale, t.table);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) e = cudaStreamSynchronize(d->stream);
+  cudaFree(freq);
+  if (e != cudaSuccess) {
+    cudaFree(t.table);
+    return set_error(NEBW_ECUDA, "rotary table staging failed: %s", cudaGetErrorString(e));
+  }
+  try {
+    d->ropes[d->next_handle] = t;
+  } catch (const std::exception &) {
+    cudaFree(t.table);
+    return set_error(NEBW_ENOMEM, "no host memory for a rotary handle");
+  }
+  *handle = d->next_handle++;
+  return NEBW_OK;
+}
+
+extern "C" int nebw_row_positions(nebw_dev *d, const int32_t *off, const int32_t *len, int32_t B,
+                                  int32_t max_len, int32_t *pos, void *stream) {
+  if (int rc = use_dev(d)) return rc;
+  NEBW_REQUIRE(off && len && pos, "null position operand");
+  NEBW_REQUIRE(B >= 0 && B <= 65535 && max_len >= 0, "positions of %d sequences up to %d refused",
+               B, max_len);
+  if (B == 0 || max_len == 0) return NEBW_OK;
+  nebw::row_pos_kernel<<<dim3((max_len + 255) / 256, B), 256, 0, pick_stream(d, stream)>>>(off, len,
+                                                                                          pos);
+  NEBW_CUDA(cudaGetLastError());
+  return NEBW_OK;
+}
+
+namespace {
+
+int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t rows, size_t esz,
+                int norm, nebw::HeadSide *side) {
+  *side = nebw::HeadSide{};
+  if (!h || h->heads == 0) return NEBW_OK;
+  NEBW_REQUIRE(h->heads > 0 && h->heads <= 4096, "%d %s heads refused", h->heads, what);
+  const int64_t width = static_cast<int64_t>(h->heads) * head_dim;
+  NEBW_REQUIRE(h->x && h->out, "null %s operand", what);
+  NEBW_REQUIRE(aligned(h->x, esz) && aligned(h->out, esz), "%s heads are not element-aligned", what);
+  NEBW_REQUIRE(rows <= 1 || (h->stride >= width && h->out_stride >= width),
+               "%s row stride refused: %lld and %lld for %lld elements a row", what,
+               static_cast<long long>(h->stride), static_cast<long long>(h->out_stride),
+               static_cast<long long>(width));
+  NEBW_REQUIRE(h->stride < (1ll << 31) && h->out_stride < (1ll << 31), "%s row stride refused",
+               what);
+  NEBW_REQUIRE(h->out != h->x || rows <= 1 || h->out_stride == h->stride,
+               "%s heads in place need one row stride", what);
+  if (norm != NEBW_HEADNORM_NONE) {
+    NEBW_REQUIRE(h->gamma, "%s norm without its weight", what);
+    NEBW_REQUIRE(norm != NEBW_HEADNORM_LAYER || h->beta, "%s LayerNorm without its bias", what);
+    NEBW_REQUIRE(aligned(h->gamma, 4) && aligned(h->beta, 4), "%s norm weights are not aligned",
+                 what);
+  }
+  side->x = h->x;
+  side->out = h->out;
+  side->stride = h->stride;
+  side->out_stride = h->out_stride;
+  side->heads = h->heads;
+  side->gamma = h->gamma;
+  side->beta = h->beta;
+  return NEBW_OK;
+}
+
+template <typename T, int NORM, bool PAIRS>
+int launch_heads(const nebw::HeadArgs &a, cudaStream_t st) {
+  const int heads = a.q.heads + a.k.heads;
+  const int64_t blocks = (a.rows * heads + 7) / 8;
+  NEBW_REQUIRE(blocks < (1ll << 31), "too many heads: %lld rows of %d",
+               static_cast<long long>(a.rows), heads);
+  nebw::heads_any_kernel<T, NORM, PAIRS><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
+  NEBW_CUDA(cudaGetLastError());
+  return NEBW_OK;
+}
+
+template <typename T, int NORM>
+int launch_heads_layout(const nebw::HeadArgs &a, int layout, cudaStream_t st) {
+  return layout == NEBW_ROPE_PAIRS ? launch_heads<T, NORM, true>(a, st)
+                                   : launch_heads<T, NORM, false>(a, st);
+}
+
+template <typename T>
+int launch_heads_norm(const nebw::HeadArgs &a, int norm, int layout, cudaStream_t st) {
+  switch (norm) {
+    case NEBW_HEADNORM_RMS: return launch_heads_layout<T, nebw::kHeadNormRms>(a, layout, st);
+    case NEBW_HEADNORM_LAYER: return launch_heads_layout<T, nebw::kHeadNormLayer>(a, layout, st);
+    default: return launch_heads_layout<T, nebw::kHeadNormNone>(a, layout, st);
+  }
+}
+
+int run_heads(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype, int64_t rows,
+              const int32_t *rows_dev, int32_t head_dim, int norm, float eps, uint64_t rope,
+              int layout, const int32_t *pos, void *stream) {
+  if (int rc = use_dev(d)) return rc;
+  NEBW_REQUIRE(dtype == NEBW_F32 || dtype == NEBW_BF16, "head dtype %d refused", dtype);
+  NEBW_REQUIRE(rows >= 0 && rows < (1ll << 31), "rows %lld refused", static_cast<long long>(rows));
+  NEBW_REQUIRE(head_dim >= 2 && head_dim % 2 == 0 && head_dim <= nebw::kHeadMaxDim,
+               "head_dim %d refused: even, 2 .. %d", head_dim, nebw::kHeadMaxDim);
+  NEBW_REQUIRE(norm == NEBW_HEADNORM_NONE || norm == NEBW_HEADNORM_RMS ||
+                   norm == NEBW_HEADNORM_LAYER,
+               "head norm %d refused", norm);
+  NEBW_REQUIRE(norm == NEBW_HEADNORM_NONE || (eps >= 0.0f && std::isfinite(eps)),
+               "head norm eps %g refused", static_cast<double>(eps));
+  NEBW_REQUIRE(layout == NEBW_ROPE_HALF || layout == NEBW_ROPE_PAIRS, "rotary layout %d refused",
+               layout);
+  nebw::HeadArgs a{};
+  if (rope) {
+    auto it = d->ropes.find(rope);
+    NEBW_REQUIRE(it != d->ropes.end(), "unknown rotary handle %llu",
+                 static_cast<unsigned long long>(rope));
+    NEBW_REQUIRE(2 * it->second.n <= head_dim, "a rotary width of %d is more than head_dim %d",
+                 2 * it->second.n, head_dim);
+    NEBW_REQUIRE(pos || rows == 0, "rotation without positions");
+    a.n = it->second.n;
+    a.table = it->second.table;
+    a.max_pos = it->second.max_pos;
+    a.pos = pos;
+  }
+  const size_t esz = dtype == NEBW_F32 ? 4 : 2;
+  if (int rc = check_heads(q, "query", head_dim, rows, esz, norm, &a.q)) return rc;
+  if (int rc = check_heads(k, "key", head_dim, rows, esz, norm, &a.k)) return rc;
+  NEBW_REQUIRE(a.q.heads + a.k.heads > 0, "no heads given");
+  if (rows == 0) return NEBW_OK;
+  a.rows = rows;
+  a.rows_dev = rows_dev;
+  a.head_dim = head_dim;
+  a.eps = eps;
+  a.err = d->d_err;
+  const cudaStream_t st = pick_stream(d, stream);
+  return dtype == NEBW_F32 ? launch_heads_norm<float>(a, norm, layout, st)
+                           : launch_heads_norm<__nv_bfloat16>(a, norm, layout, st);
+}
+
+}  // namespace
+
+extern "C" int nebw_rope(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype,
+                         int64_t rows, const int32_t *rows_dev, int32_t head_dim, uint64_t rope,
+                         int layout, const int32_t *pos, void *stream) {
+  NEBW_REQUIRE(rope != 0, "nebw_rope without a rotary handle");
+  return run_heads(d, q, k, dtype, rows, rows_dev, head_dim, NEBW_HEADNORM_NONE, 0.0f, rope, layout,
+                   pos, stream);
+}
+
+extern "C" int nebw_qk_norm_rope(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype,
+                                 int64_t rows, const int32_t *rows_dev, int32_t head_dim, int norm,
+                                 float eps, uint64_t rope, int layout, const int32_t *pos,
+                                 void *stream) {
+  NEBW_REQUIRE(norm == NEBW_HEADNORM_RMS || norm == NEBW_HEADNORM_LAYER, "head norm %d refused",
+               norm);
+  return run_heads(d, q, k, dtype, rows, rows_dev, head_dim, norm, eps, rope, layout, pos, stream);
+}
+
+// ---------------------------------------------------------------------------
+// experts
+// ---------------------------------------------------------------------------
+
+namespace {
+
+int64_t route_blocks(int64_t rows) {
+  return (rows + nebw::kRouteBlockRows - 1) / nebw::kRouteBlockRows;
+}
+
+int check_route(int64_t rows, int32_t experts, int32_t top_k) {
+  NEBW_REQUIRE(experts >= 1 && experts <= nebw::kRouteMaxExperts, "%d experts refused: 1 .. %d",
+               experts, nebw::kRouteMaxExperts);
+  NEBW_REQUIRE(top_k >= 1 && top_k <= nebw::kRouteMaxK && top_k <= experts,
+               "top_k %d of %d experts refused: 1 .. %d", top_k, experts, nebw::kRouteMaxK);
+  NEBW_REQUIRE(rows >= 0 && rows < (1ll << 30) && rows * top_k < (1ll << 30),
+               "%lld rows of %d experts refused", static_cast<long long>(rows), top_k);
+  return NEBW_OK;
+}
+
+template <typename T>
+void launch_topk(const nebw::RouteArgs &a, cudaStream_t st) {
+  const unsigned g = static_cast<unsigned>(a.blocks);
+  const int b = nebw::kRouteThreads;
+  if (a.experts <= 32) nebw::route_topk_kernel<T, 1><<<g, b, 0, st>>>(a);
+  else if (a.experts <= 64) nebw::route_topk_kernel<T, 2><<<g, b, 0, st>>>(a);
+  else if (a.experts <= 128) nebw::route_topk_kernel<T, 4><<<g, b, 0, st>>>(a);
+  else if (a.experts <= 256) nebw::route_topk_kernel<T, 8><<<g, b, 0, st>>>(a);
+  else nebw::route_topk_kernel<T, 16><<<g, b, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" int64_t nebw_moe_route_workspace(int64_t rows, int32_t experts, int32_t top_k) {
+  if (check_route(rows, experts, top_k)) return -1;
+  return route_blocks(rows) * experts * static_cast<int64_t>(sizeof(int));
+}
+
+extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_t stride,
+                              int64_t rows, const int32_t *rows_dev, int32_t experts,
+                              int32_t top_k, int score, int renorm, float scale, int32_t *ids,
+                              float *weights, int32_t *group_off, int32_t *row_src,
+                              int32_t *row_dst, void *ws, int64_t ws_bytes, void *stream) {
+  if (int rc = use_dev(d)) return rc;
+  if (int rc = check_route(rows, experts, top_k)) return rc;
+  NEBW_REQUIRE(dtype == NEBW_F32 || dtype == NEBW_BF16, "logit dtype %d refused", dtype);
+  NEBW_REQUIRE(score == NEBW_ROUTE_SOFTMAX || score == NEBW_ROUTE_SIGMOID, "score %d refused",
+               score);
+  NEBW_REQUIRE(std::isfinite(scale), "routing scale %g refused", static_cast<double>(scale));
+  NEBW_REQUIRE(group_off, "null routing output");
+  const cudaStream_t st = pick_stream(d, stream);
+  if (rows == 0) {
+    NEBW_CUDA(cudaMemsetAsync(group_off, 0, (experts + 1) * sizeof(int), st));
+    return NEBW_OK;
+  }
+  NEBW_REQUIRE(logits && ids && weights && row_src && row_dst && ws, "null routing operand");
+  NEBW_REQUIRE(stride >= experts && stride < (1ll << 31),
+               "logit row stride %lld refused for %d experts", static_cast<long long>(stride),
+               experts);
+  NEBW_REQUIRE(aligned(logits, dtype == NEBW_F32 ? 4 : 2) && aligned(ws, 4),
+               "routing operands are not aligned");
+  const int64_t need = route_blocks(rows) * experts * static_cast<int64_t>(sizeof(int));
+  NEBW_REQUIRE(ws_bytes >= need, "routing workspace of %lld bytes refused: %lld are needed",
+               static_cast<long long>(ws_bytes), static_cast<long long>(need));
+  nebw::RouteArgs a{};
+  a.logits = logits;
+  a.stride = stride;
+  a.rows = rows;
+  a.rows_dev = rows_dev;
+  a.experts = experts;
+  a.k = top_k;
+  a.sigmoid = score == NEBW_ROUTE_SIGMOID;
+  a.renorm = renorm != 0;
+  a.scale = scale;
+  a.ids = ids;
+  a.weights = weights;
+  a.group_off = group_off;
+  a.row_src = row_src;
+  a.row_dst = row_dst;
+  a.hist = static_cast<int *>(ws);
+  a.blocks = static_cast<int>(route_blocks(rows));
+  if (dtype == NEBW_F32) launch_topk<float>(a, st);
+  else launch_topk<__nv_bfloat16>(a, st);
+  NEBW_CUDA(cudaGetLastError());
+  const size_t smem = (nebw::kRouteWarps + 1) * static_cast<size_t>(experts) * sizeof(int);
+  nebw::route_place_kernel<<<static_cast<unsigned>(a.blocks), nebw::kRouteThreads, smem, st>>>(a);
+  NEBW_CUDA(cudaGetLastError());
+  return NEBW_OK;
+}
+
+extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_t experts,
+                                  int64_t K, int64_t N, int gated, void *stream,
+                                  uint64_t *handle) {
+  if (int rc = use_dev(d)) return rc;
+  NEBW_REQUIRE(kn && handle, "null expert weight operand");
+  NEBW_REQUIRE(dtype == NEBW_F32 || dtype == NEBW_BF16, "weight dtype %d refused", dtype);
+  NEBW_REQUIRE(experts >= 1 && experts <= nebw::kGroupMaxExperts, "%d experts refused: 1 .. %d",
+               experts, nebw::kGroupMaxExperts);
+  NEBW_REQUIRE(K >= 64 && N >= 8 && K % 8 == 0 && N % 8 == 0 && K <= (1 << 20) &&
+                   N < (1ll << 30) && N * experts < (1ll << 30),
+               "expert weights [%d, K=%lld, N=%lld] refused: K >= 64, K %% 8 == 0, N %% 8 == 0",
+               experts, static_cast<long long>(K), static_cast<long long>(N));
+  NEBW_REQUIRE(!gated || N % 64 == 0,
+               "gated expert weights of N=%lld refused: [up | gate] of a multiple of 32 each",
+               static_cast<long long>(N));
+  bool on_device = false;
+  if (int rc = where_is(d, kn, &on_device)) return rc;
+  const cudaStream_t st = pick_stream(d, stream);
+  const size_t esz = dtype == NEBW_F32 ? 4 : 2;
+  const size_t one = static_cast<size_t>(K) * N * esz;
+  Experts w;
+  w.experts = experts;
+  w.K = K;
+  w.N = N;
+  w.gated = gated != 0;
+  void *tmp = nullptr;
+  if (cudaMalloc(&w.ptr, static_cast<size_t>(experts) * K * N * 2) != cudaSuccess ||
+      (!on_device && cudaMalloc(&tmp, one) != cudaSuccess)) {
+    cudaGetLastError();
+    cudaFree(w.ptr);
+    return set_error(NEBW_ENOMEM, "cudaMalloc for [%d, %lld, %lld] expert weights failed", experts,
+                     static_cast<long long>(N), static_cast<long long>(K));
+  }
+  const unsigned gx = static_cast<unsigned>((N + 31) / 32), gy = static_cast<unsigned>((K + 31) / 32);
+  cudaError_t e = cudaSuccess;
+  if (on_device) {
+    nebw::stage_experts_kernel<<<dim3(gx, gy, experts), dim3(32, 8), 0, st>>>(
+        kn, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, 0, w.ptr);
+    e = cudaGetLastError();
+  } else {
+    for (int i = 0; i < experts && e == cudaSuccess; ++i) {  // one expert's copy at a time
+      e = cudaMemcpyAsync(tmp, static_cast<const char *>(kn) + i * one, one,
+                          cudaMemcpyHostToDevice, st);
+      if (e != cudaSuccess) break;
+      nebw::stage_experts_kernel<<<dim3(gx, gy, 1), dim3(32, 8), 0, st>>>(
+          tmp, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, i, w.ptr);
+      e = cudaGetLastError();
+    }
+  }
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  cudaFree(tmp);
+  int rc = NEBW_OK;
+  if (e != cudaSuccess)
+    rc = set_error(NEBW_ECUDA, "expert weight staging failed: %s", cudaGetErrorString(e));
+  if (!rc) rc = make_tmap_kmajor(&w.map128, w.ptr, experts * N, K, 128);
+  if (!rc) rc = make_tmap_kmajor(&w.map256, w.ptr, experts * N, K, 256);
+  if (!rc) {
+    try {
+      d->experts[d->next_handle] = w;
+    } catch (const std::exception &) {
+      rc = set_error(NEBW_ENOMEM, "no host memory for an expert weight handle");
+    }
+  }
+  if (rc) {
+    cudaFree(w.ptr);
+    return rc;
+  }
+  *handle = d->next_handle++;
+  return NEBW_OK;
+}
+
+namespace {
+
+template <int BN, int EPI>
+void launch_grouped_epi(const CUtensorMap &mA, const CUtensorMap &mW, const nebw::GroupedArgs &a,
+                        unsigned grid, cudaStream_t st) {
+  const size_t smem = nebw::GroupedShape<BN>::kSmemBytes;
+  if (a.row_src)
+    nebw::gemm_grouped_kernel<BN, EPI, true><<<grid, nebw::kGemmThreads, smem, st>>>(mA, mW, a);
+  else
+    nebw::gemm_grouped_kernel<BN, EPI, false><<<grid, nebw::kGemmThreads, smem, st>>>(mA, mW, a);
+}
+
+template <int BN>
+int launch_grouped(nebw_dev *d, const CUtensorMap &mA, const CUtensorMap &mW, int epi,
+                   const nebw::GroupedArgs &a, cudaStream_t st) {
+  // every group may end in a part tile
+  const int64_t tiles = (a.rows / nebw::kGemmBM + std::min(a.experts, a.rows)) *
+                        int64_t{(a.N + BN - 1) / BN};
+  NEBW_REQUIRE(tiles < (1ll << 31), "grouped product too large");
+  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, d->sm_count));
+  switch (epi) {
+    case nebw::kGrpBf16: launch_grouped_epi<BN, nebw::kGrpBf16>(mA, mW, a, grid, st); break;
+    case nebw::kGrpBf16Gelu8: launch_grouped_epi<BN, nebw::kGrpBf16Gelu8>(mA, mW, a, grid, st); break;
+    case nebw::kGrpBf16Erf: launch_grouped_epi<BN, nebw::kGrpBf16Erf>(mA, mW, a, grid, st); break;
+    case nebw::kGrpF32: launch_grouped_epi<BN, nebw::kGrpF32>(mA, mW, a, grid, st); break;
+    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<BN, nebw::kGrpBf16SwiGLU>(mA, mW, a, grid, st); break;
+    case nebw::kGrpBf16GeGLU: launch_grouped_epi<BN, nebw::kGrpBf16GeGLU>(mA, mW, a, grid, st); break;
+  }
+  NEBW_CUDA(cudaGetLastError());
+  return NEBW_OK;
+}
+
+}  // namespace
+
+extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, int64_t a_rows,
+                                 const int32_t *row_src, const int32_t *group_off, int64_t rows,
+                                 int64_t K, int64_t N, const float *bias, int act, void *C,
+                                 int c_dtype, void *stream) {
+  if (int rc = use_dev(d)) return rc;
+  auto it = d->experts.find(weight);
+  NEBW_REQUIRE(it != d->experts.end(), "unknown expert weight handle %llu",
+               static_cast<unsigned long long>(weight));
+  const Experts &w = it->second;
+  NEBW_REQUIRE(K == w.K && N == w.N,
+               "grouped product [rows, %lld] x [%lld, %lld] does not match the staged experts "
+               "[%d, K=%lld, N=%lld]",
+               static_cast<long long>(K), static_cast<long long>(K), static_cast<long long>(N),
+               w.experts, static_cast<long long>(w.K), static_cast<long long>(w.N));
+  NEBW_REQUIRE(rows >= 0 && rows < (1 << 30) && a_rows >= 0 && a_rows < (1 << 30),
+               "grouped rows %lld of %lld refused", static_cast<long long>(rows),
+               static_cast<long long>(a_rows));
+  NEBW_REQUIRE(c_dtype == NEBW_F32 || c_dtype == NEBW_BF16, "output dtype %d refused", c_dtype);
+  if (w.gated) {
+    NEBW_REQUIRE(act == NEBW_GATE_SILU || act == NEBW_GATE_GELU_ERF, "gate activation %d refused",
+                 act);
+    NEBW_REQUIRE(c_dtype == NEBW_BF16, "a gated product writes bf16 output");
+  } else {
+    NEBW_REQUIRE(act == NEBW_ACT_NONE || act == NEBW_ACT_GELU8 || act == NEBW_ACT_GELU_ERF,
+                 "activation %d refused", act);
+    NEBW_REQUIRE(act == NEBW_ACT_NONE || c_dtype == NEBW_BF16,
+                 "an activation epilogue writes bf16 output");
+  }
+  if (rows == 0) return NEBW_OK;
+  NEBW_REQUIRE(A && C && group_off, "null grouped operand");
+  NEBW_REQUIRE(a_rows > 0, "grouped rows of an empty A");
+  NEBW_REQUIRE(row_src || a_rows >= rows, "A has %lld rows, the groups up to %lld",
+               static_cast<long long>(a_rows), static_cast<long long>(rows));
+  NEBW_REQUIRE(aligned(A, 16) && aligned(C, 16) && aligned(bias, 16),
+               "grouped operands must be 16-byte aligned");
+  nebw::GroupedArgs a{};
+  a.off = group_off;
+  a.experts = w.experts;
+  a.rows = static_cast<int>(rows);
+  a.row_src = row_src;
+  a.a_rows = static_cast<int>(a_rows);
+  a.N = static_cast<int>(N);
+  a.K = static_cast<int>(K);
+  a.bias = bias;
+  a.out = C;
+  a.err = d->d_err;
+  int epi = nebw::kGrpBf16;
+  if (w.gated) epi = act == NEBW_GATE_SILU ? nebw::kGrpBf16SwiGLU : nebw::kGrpBf16GeGLU;
+  else if (c_dtype == NEBW_F32) epi = nebw::kGrpF32;
+  else if (act == NEBW_ACT_GELU8) epi = nebw::kGrpBf16Gelu8;
+  else if (act == NEBW_ACT_GELU_ERF) epi = nebw::kGrpBf16Erf;
+  CUtensorMap mA;
+  if (int rc = make_tmap_kmajor(&mA, A, a_rows, K, row_src ? 1 : nebw::kGemmBM)) return rc;
+  const cudaStream_t st = pick_stream(d, stream);
+  if (N % 256 == 0) return launch_grouped<256>(d, mA, w.map256, epi, a, st);
+  return launch_grouped<128>(d, mA, w.map128, epi, a, st);
+}
+
+namespace {
+
+template <typename TY, typename TO>
+void launch_combine(const nebw::CombineArgs &a, bool vec, cudaStream_t st) {
+  const int64_t items = a.rows * (vec ? a.H / 8 : a.H);
+  const unsigned g = static_cast<unsigned>((items + 255) / 256);
+  if (vec) nebw::moe_combine_kernel<TY, TO, 8><<<g, 256, 0, st>>>(a);
+  else nebw::moe_combine_kernel<TY, TO, 1><<<g, 256, 0, st>>>(a);
+}
+
+}  // namespace
+
+extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t y_rows,
+                                const int32_t *row_dst, const float *weights, int64_t rows,
+                                const int32_t *rows_dev, int32_t top_k, int64_t H,
+                                const float *residual, void *out, int out_dtype, void *stream) {
+  if (int rc = use_dev(d)) return rc;
+  NEBW_REQUIRE(y_dtype == NEBW_F32 || y_dtype == NEBW_BF16, "expert row dtype %d refused", y_dtype);
+  NEBW_REQUIRE(out_dtype == NEBW_F32 || out_dtype == NEBW_BF16, "output dtype %d refused",
+               out_dtype);
+  NEBW_REQUIRE(top_k >= 1 && top_k <= nebw::kRouteMaxK, "top_k %d refused: 1 .. %d", top_k,
+               nebw::kRouteMaxK);
+  NEBW_REQUIRE(H >= 1 && H <= (1 << 20), "width %lld refused", static_cast<long long>(H));
+  NEBW_REQUIRE(rows >= 0 && rows < (1ll << 30) && rows * top_k < (1ll << 30) && y_rows >= 0 &&
+                   y_rows < (1ll << 30) && rows * H < (1ll << 38),
+               "%lld rows of %d experts refused", static_cast<long long>(rows), top_k);
+  if (rows == 0) return NEBW_OK;
+  NEBW_REQUIRE(y && row_dst && weights && out, "null combine operand");
+  nebw::CombineArgs a{};
+  a.y = y;
+  a.row_dst = row_dst;
+  a.weights = weights;
+  a.residual = residual;
+  a.out = out;
+  a.rows = rows;
+  a.y_rows = y_rows;
+  a.rows_dev = rows_dev;
+  a.k = top_k;
+  a.H = H;
+  a.err = d->d_err;
+  const bool vec = H % 8 == 0 && aligned(y, 16) && aligned(out, 16) && aligned(residual, 16);
+  const cudaStream_t st = pick_stream(d, stream);
+  if (y_dtype == NEBW_F32) {
+    if (out_dtype == NEBW_F32) launch_combine<float, float>(a, vec, st);
+    else launch_combine<float, __nv_bfloat16>(a, vec, st);
+  } else {
+    if (out_dtype == NEBW_F32) launch_combine<__nv_bfloat16, float>(a, vec, st);
+    else launch_combine<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
+  }
+  NEBW_CUDA(cudaGetLastError());
+  return NEBW_OK;
+}

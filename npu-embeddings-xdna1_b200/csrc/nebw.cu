@@ -45,8 +45,11 @@
 #include "attention.cuh"
 #include "attention_tc.cuh"
 #include "gated.cuh"
+#include "gemm_grouped.cuh"
 #include "gemm_i8.cuh"
 #include "gemm_tc.cuh"
+#include "heads.cuh"
+#include "moe.cuh"
 #include "npue_file.h"
 #include "npue_pack.h"
 #include "ptx.cuh"
@@ -91,6 +94,8 @@ const char *dev_err_name(int code) {
     case nebw::kDevBadTokenId: return "a token id is outside [0, vocab_size)";
     case nebw::kDevBadLength: return "a sequence length is outside [1, seq]";
     case nebw::kDevBadShape: return "a kernel was handed a shape its launch cannot cover";
+    case nebw::kDevBadPosition: return "a position is outside the staged rotary table";
+    case nebw::kDevBadGroup: return "a group offset or grouped row index is out of range";
     default: return "unknown device error";
   }
 }
@@ -219,6 +224,23 @@ struct WeightI8 {
   CUtensorMap map64, map128, map256;  // box rows 64 / 128 / 256, 128-byte K boxes
 };
 
+// The weights of a set of experts (nebw_stage_experts): bf16 [experts, N, K],
+// a gated set's N interleaved in groups of 64 = [32 up | 32 gate].
+struct Experts {
+  __nv_bfloat16 *ptr = nullptr;
+  int experts = 0;
+  int64_t K = 0, N = 0;
+  bool gated = false;
+  CUtensorMap map128, map256;  // [experts * N, K], box rows 128 / 256
+};
+
+// cos and sin of every position and frequency (nebw_stage_rope).
+struct RopeTable {
+  float2 *table = nullptr;  // [max_pos, n]
+  int n = 0;
+  int64_t max_pos = 0;
+};
+
 struct nebw_dev {
   int device = 0;
   int sm_count = 0;
@@ -231,6 +253,8 @@ struct nebw_dev {
   int *d_err = nullptr;
   std::map<uint64_t, Weight> weights;
   std::map<uint64_t, WeightI8> weights_i8;  // int8 GEMM operands (nebw_stage_weight_i8)
+  std::map<uint64_t, Experts> experts;
+  std::map<uint64_t, RopeTable> ropes;
   uint64_t next_handle = 1;
   // CTA pairs the GPU can hold at once for the 2-CTA GEMM (0: use the
   // single-CTA kernel); NEBW_GEMM_CTAS=1 in the environment forces 0.
@@ -703,6 +727,10 @@ int set_gemm_i8_attrs() {
   return NEBW_OK;
 }
 
+namespace {
+int set_layer_op_attrs();  // layer_ops.cuh
+}
+
 extern "C" int nebw_open(int device, nebw_dev **out) {
   NEBW_REQUIRE(out != nullptr, "null output handle");
   *out = nullptr;
@@ -727,6 +755,7 @@ extern "C" int nebw_open(int device, nebw_dev **out) {
   if (int rc = set_all_gemm_attrs()) return rc;
   if (int rc = set_gemm_i8_attrs<128>()) return rc;
   if (int rc = set_gemm_i8_attrs<256>()) return rc;
+  if (int rc = set_layer_op_attrs()) return rc;
   NEBW_CUDA(cudaFuncSetAttribute(nebw::attention_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  nebw::AttnTcShape<64>::kSmemBytes));
   NEBW_CUDA(cudaFuncSetAttribute(nebw::attention_tc_kernel<64>, cudaFuncAttributePreferredSharedMemoryCarveout,
@@ -748,6 +777,8 @@ extern "C" int nebw_close(nebw_dev *d) {
   cudaStreamSynchronize(d->stream);
   for (auto &kv : d->weights) cudaFree(kv.second.ptr);
   for (auto &kv : d->weights_i8) cudaFree(kv.second.ptr);
+  for (auto &kv : d->experts) cudaFree(kv.second.ptr);
+  for (auto &kv : d->ropes) cudaFree(kv.second.table);
   cudaFree(d->d_err);
   cudaStreamDestroy(d->stream);
   if (d->cap_stream) cudaStreamDestroy(d->cap_stream);
@@ -937,12 +968,21 @@ extern "C" int nebw_release_weight(nebw_dev *d, uint64_t handle) {
   if (int rc = use_dev(d)) return rc;
   auto it = d->weights.find(handle);
   auto it8 = d->weights_i8.find(handle);
-  NEBW_REQUIRE(it != d->weights.end() || it8 != d->weights_i8.end(),
+  auto itx = d->experts.find(handle);
+  auto itr = d->ropes.find(handle);
+  NEBW_REQUIRE(it != d->weights.end() || it8 != d->weights_i8.end() || itx != d->experts.end() ||
+                   itr != d->ropes.end(),
                "unknown weight handle %llu", static_cast<unsigned long long>(handle));
   NEBW_CUDA(cudaStreamSynchronize(d->stream));
   if (it != d->weights.end()) {
     cudaFree(it->second.ptr);
     d->weights.erase(it);
+  } else if (itx != d->experts.end()) {
+    cudaFree(itx->second.ptr);
+    d->experts.erase(itx);
+  } else if (itr != d->ropes.end()) {
+    cudaFree(itr->second.table);
+    d->ropes.erase(itr);
   } else {
     cudaFree(it8->second.ptr);
     d->weights_i8.erase(it8);
@@ -2689,6 +2729,12 @@ extern "C" int nebw_encode_device_static(nebw_model *m, const int32_t *ids, cons
 // ---------------------------------------------------------------------------
 
 #include "vit.cuh"
+
+// ---------------------------------------------------------------------------
+// Operators of rotary and expert layers.
+// ---------------------------------------------------------------------------
+
+#include "layer_ops.cuh"
 
 // ---------------------------------------------------------------------------
 // Several GPUs: the sharded pass and the NCCL gather.

@@ -21,6 +21,8 @@ enum DevErr : int {
   kDevBadTokenId = 2,    // a token id outside [0, vocab)
   kDevBadLength = 3,     // a sequence length outside [1, seq]
   kDevBadShape = 4,      // a kernel was handed a shape its launch cannot cover
+  kDevBadPosition = 5,   // a position outside the rotary table
+  kDevBadGroup = 6,      // a group offset or a grouped row index out of range
 };
 
 constexpr uint64_t kWaitTimeoutNs = 2000ull * 1000ull * 1000ull;  // 2 s

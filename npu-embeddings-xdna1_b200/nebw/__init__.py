@@ -27,6 +27,9 @@ F32, BF16 = 0, 1
 ACT_NONE, ACT_GELU8, ACT_GELU_ERF = 0, 1, 2
 GATE_SILU, GATE_GELU_ERF = 0, 1
 POOL_MEAN, POOL_CLS = 0, 1
+ROPE_HALF, ROPE_PAIRS = 0, 1
+HEADNORM_NONE, HEADNORM_RMS, HEADNORM_LAYER = 0, 1, 2
+ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
 
 
 class NebwError(RuntimeError):
@@ -47,6 +50,41 @@ class VitConfig(C.Structure):
     _fields_ = [(n, C.c_int32) for n in (
         "num_layers", "hidden", "num_heads", "head_dim", "intermediate", "image_size",
         "patch_size", "num_channels")] + [("layer_norm_eps", C.c_float)]
+
+
+class RopeScaling(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("reserved0", C.c_int32), ("orig_len", C.c_int64),
+                ("factor", C.c_double), ("fast", C.c_double), ("slow", C.c_double),
+                ("attn_scale", C.c_double)]
+
+
+class Heads(C.Structure):
+    """The query or key heads of packed rows (nebw_heads)."""
+
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("stride", C.c_int64),
+                ("out_stride", C.c_int64), ("heads", C.c_int32), ("reserved0", C.c_int32),
+                ("gamma", C.c_void_p), ("beta", C.c_void_p)]
+
+    @classmethod
+    def of(cls, x, heads: int, out=None, gamma=None, beta=None):
+        """Heads of a 2-D torch CUDA tensor [rows, heads * head_dim] (a column
+        slice of Q|K|V rows, say), in place or into `out` of the same shape.
+        The object keeps the tensors alive."""
+        out = x if out is None else out
+        for t in (x, out):
+            if t.dim() != 2 or t.stride(1) != 1 or t.shape[1] % heads:
+                raise ValueError("heads are rows of a 2-D tensor with adjacent elements")
+        if out.shape != x.shape or out.dtype != x.dtype:
+            raise ValueError("the heads' output must have their shape and dtype")
+        for t in (gamma, beta):
+            if t is not None and (str(t.dtype) != "torch.float32" or not t.is_contiguous()
+                                  or t.numel() != x.shape[1] // heads):
+                raise ValueError("a head norm's weights are head_dim contiguous fp32 values")
+        h = cls(x.data_ptr(), out.data_ptr(), x.stride(0), out.stride(0), heads, 0, _addr(gamma),
+                _addr(beta))
+        h.dtype = _dtype(x)
+        h.tensors = (x, out, gamma, beta)
+        return h
 
 
 _lib = None
@@ -128,6 +166,24 @@ def lib() -> C.CDLL:
         "nebw_model_set_int8_operand": ([vp, C.c_char_p, vp, vp, vp, i64, i64], C.c_int),
         "nebw_model_set_datapath": ([vp, i32], C.c_int),
         "nebw_model_set_graphs": ([vp, i32], C.c_int),
+        "nebw_rope_freqs": ([C.c_double, i32, C.POINTER(RopeScaling), C.POINTER(C.c_double),
+                             C.POINTER(C.c_double)], C.c_int),
+        "nebw_stage_rope": ([vp, C.POINTER(C.c_double), i32, i64, C.c_double,
+                             C.POINTER(C.c_uint64)], C.c_int),
+        "nebw_row_positions": ([vp, vp, vp, i32, i32, vp, vp], C.c_int),
+        "nebw_rope": ([vp, C.POINTER(Heads), C.POINTER(Heads), C.c_int, i64, vp, i32, C.c_uint64,
+                       C.c_int, vp, vp], C.c_int),
+        "nebw_qk_norm_rope": ([vp, C.POINTER(Heads), C.POINTER(Heads), C.c_int, i64, vp, i32,
+                               C.c_int, C.c_float, C.c_uint64, C.c_int, vp, vp], C.c_int),
+        "nebw_stage_experts": ([vp, vp, C.c_int, i32, i64, i64, C.c_int, vp,
+                                C.POINTER(C.c_uint64)], C.c_int),
+        "nebw_moe_route_workspace": ([i64, i32, i32], i64),
+        "nebw_moe_route": ([vp, vp, C.c_int, i64, i64, vp, i32, i32, C.c_int, C.c_int, C.c_float,
+                            vp, vp, vp, vp, vp, vp, i64, vp], C.c_int),
+        "nebw_gemm_grouped": ([vp, C.c_uint64, vp, i64, vp, vp, i64, i64, i64, vp, C.c_int, vp,
+                               C.c_int, vp], C.c_int),
+        "nebw_moe_combine": ([vp, vp, C.c_int, i64, vp, vp, i64, vp, i32, i64, vp, vp, C.c_int,
+                              vp], C.c_int),
         "nebw_pack_checkpoint": ([C.c_char_p, C.c_char_p, C.c_char_p, i32, i32,
                                   C.POINTER(C.c_uint64)], C.c_int),
         "nebw_comm_unique_id": ([vp], C.c_int),
@@ -167,6 +223,16 @@ def _addr(x):
     if isinstance(x, np.ndarray):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)}")
+
+
+def _dtype(t) -> int:
+    """F32 or BF16 of a torch tensor."""
+    name = str(t.dtype)
+    if name == "torch.bfloat16":
+        return BF16
+    if name == "torch.float32":
+        return F32
+    raise TypeError(f"fp32 or bf16 is required, not {name}")
 
 
 CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy: the legacy default stream's handle
@@ -311,6 +377,116 @@ class Device:
 
     def narrow_bf16(self, x, n, y, stream=None):
         _check(lib().nebw_narrow_bf16(self.h, _addr(x), n, _addr(y), self._s(stream)))
+
+    # ---- rotary positions, head norms --------------------------------------
+    def stage_rope(self, inv_freq, max_pos: int, scale: float = 1.0) -> int:
+        """The rotary table of positions [0, max_pos) (nebw_stage_rope)."""
+        f = np.ascontiguousarray(inv_freq, np.float64)
+        hnd = C.c_uint64()
+        _check(lib().nebw_stage_rope(self.h, f.ctypes.data_as(C.POINTER(C.c_double)), f.size,
+                                     max_pos, scale, C.byref(hnd)))
+        return hnd.value
+
+    def row_positions(self, seq_off, seq_len, B, max_len, pos, stream=None):
+        _check(lib().nebw_row_positions(self.h, _addr(seq_off), _addr(seq_len), B, max_len,
+                                        _addr(pos), self._s(stream)))
+
+    @staticmethod
+    def _heads_dtype(q, k, dtype):
+        """The dtype of heads made by Heads.of, or the one given."""
+        for h in (q, k):
+            d = getattr(h, "dtype", None)
+            if d is not None:
+                if dtype is not None and dtype != d:
+                    raise TypeError("query and key heads of different dtypes")
+                dtype = d
+        return BF16 if dtype is None else dtype
+
+    def rope(self, q, k, rows, head_dim, rope, pos, layout=ROPE_HALF, dtype=None, rows_dev=None,
+             stream=None):
+        """Rotary positions on the heads q and k (Heads, either may be None) (nebw_rope)."""
+        _check(lib().nebw_rope(self.h, q, k, self._heads_dtype(q, k, dtype), rows,
+                               _addr(rows_dev), head_dim, rope, layout, _addr(pos),
+                               self._s(stream)))
+
+    def qk_norm_rope(self, q, k, rows, head_dim, norm=HEADNORM_RMS, eps=1e-6, rope=0, pos=None,
+                     layout=ROPE_HALF, dtype=None, rows_dev=None, stream=None):
+        """A norm of every head, then the rotation (rope 0: none) (nebw_qk_norm_rope)."""
+        _check(lib().nebw_qk_norm_rope(self.h, q, k, self._heads_dtype(q, k, dtype), rows,
+                                       _addr(rows_dev), head_dim, norm, eps, rope, layout,
+                                       _addr(pos), self._s(stream)))
+
+    # ---- experts -----------------------------------------------------------
+    def stage_experts(self, w_ekn, gated: bool = False, stream=None) -> int:
+        """Expert weights [experts, K, N] (nebw_stage_experts): numpy fp32, or
+        bf16 bits as uint16, or a contiguous fp32 / bf16 torch tensor."""
+        if isinstance(w_ekn, np.ndarray):
+            w = np.ascontiguousarray(w_ekn)
+            if w.dtype not in (np.float32, np.uint16):
+                raise TypeError("weights are fp32, or bf16 bit patterns as uint16")
+            dt = F32 if w.dtype == np.float32 else BF16
+        else:
+            w, dt = w_ekn.contiguous(), _dtype(w_ekn)
+        E, K, N = w.shape
+        hnd = C.c_uint64()
+        _check(lib().nebw_stage_experts(self.h, _addr(w), dt, E, K, N, int(gated),
+                                        self._s(stream), C.byref(hnd)))
+        return hnd.value
+
+    def moe_route(self, logits, rows, experts, top_k, ids, weights, group_off, row_src, row_dst,
+                  workspace, score=ROUTE_SOFTMAX, renorm=False, scale=1.0, rows_dev=None,
+                  stream=None):
+        """The top_k experts of each row of logits (a 2-D fp32 / bf16 torch
+        tensor, its row stride kept) and the rows grouped by expert
+        (nebw_moe_route)."""
+        if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < experts:
+            raise ValueError("logits are rows of at least `experts` adjacent values")
+        _check(lib().nebw_moe_route(self.h, logits.data_ptr(), _dtype(logits),
+                                    max(logits.stride(0), experts), rows, _addr(rows_dev),
+                                    experts, top_k, score, int(renorm), scale, _addr(ids),
+                                    _addr(weights), _addr(group_off), _addr(row_src),
+                                    _addr(row_dst), _addr(workspace),
+                                    workspace.numel() * workspace.element_size(),
+                                    self._s(stream)))
+
+    def gemm_grouped(self, weight, A, a_rows, group_off, rows, K, N, C_out, row_src=None,
+                     bias=None, act=ACT_NONE, c_dtype=BF16, stream=None):
+        """One product per expert over its group of rows (nebw_gemm_grouped)."""
+        _check(lib().nebw_gemm_grouped(self.h, weight, _addr(A), a_rows, _addr(row_src),
+                                       _addr(group_off), rows, K, N, _addr(bias), act,
+                                       _addr(C_out), c_dtype, self._s(stream)))
+
+    def moe_combine(self, y, row_dst, weights, rows, top_k, H, out, residual=None, rows_dev=None,
+                    stream=None):
+        """The experts' rows y (torch, [places, H]) weighted and summed per
+        row (nebw_moe_combine)."""
+        _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y.shape[0], _addr(row_dst),
+                                      _addr(weights), rows, _addr(rows_dev), top_k, H,
+                                      _addr(residual), out.data_ptr(), _dtype(out),
+                                      self._s(stream)))
+
+
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}
+
+
+def rope_freqs(theta: float, rot_dim: int, scaling: str = "none", factor: float = 1.0,
+               orig_len: int = 0, fast: float = 0.0, slow: float = 0.0, attn_scale: float = 0.0):
+    """(inv_freq [rot_dim / 2], scale) of rotary positions, scaled for
+    positions past the trained length (nebw_rope_freqs)."""
+    inv = np.empty(max(1, rot_dim // 2), np.float64)
+    scale = C.c_double()
+    s = RopeScaling(ROPE_SCALINGS[scaling], 0, orig_len, factor, fast, slow, attn_scale)
+    _check(lib().nebw_rope_freqs(theta, rot_dim, C.byref(s),
+                                 inv.ctypes.data_as(C.POINTER(C.c_double)), C.byref(scale)))
+    return inv, scale.value
+
+
+def moe_route_workspace(rows: int, experts: int, top_k: int) -> int:
+    """Bytes of device workspace of Device.moe_route."""
+    n = lib().nebw_moe_route_workspace(rows, experts, top_k)
+    if n < 0:
+        raise NebwError(1, lib().nebw_last_error().decode())
+    return n
 
 
 class Model:

@@ -1,0 +1,134 @@
+"""Host side of the rotary and expert operators (CPU, no device): the rotary
+frequency sets against their formulas, the workspace sizes and the refusals
+that need no GPU."""
+
+import math
+
+import numpy as np
+import pytest
+
+
+@pytest.mark.parametrize("n", [1, 2, 16, 32, 128])
+@pytest.mark.parametrize("theta", [1000.0, 160000.0])
+def test_rope_freqs_plain_linear_ntk(n, theta):
+    import nebw
+    i = np.arange(n)
+    # a few roundings of pow in double
+    tol = dict(rtol=1e-13, atol=0)
+    inv, scale = nebw.rope_freqs(theta, 2 * n)
+    assert scale == 1.0
+    np.testing.assert_allclose(inv, theta ** (-i / n), **tol)
+    inv, scale = nebw.rope_freqs(theta, 2 * n, "linear", factor=8.0)
+    assert scale == 1.0
+    np.testing.assert_allclose(inv, theta ** (-i / n) / 8.0, **tol)
+    inv, scale = nebw.rope_freqs(theta, 2 * n, "ntk", factor=8.0)
+    assert scale == 1.0
+    np.testing.assert_allclose(inv[0], 1.0, **tol)
+    if n > 1:  # the slowest frequency is the linear one, the fastest is kept
+        np.testing.assert_allclose(inv[-1], theta ** (-(n - 1) / n) / 8.0, rtol=1e-12)
+
+
+def test_rope_freqs_yarn_and_bands():
+    import nebw
+    n, theta, length, factor = 64, 10000.0, 4096, 16.0
+    plain = theta ** (-np.arange(n) / n)
+    turns = length * plain / (2 * math.pi)
+    inv, scale = nebw.rope_freqs(theta, 2 * n, "yarn", factor=factor, orig_len=length)
+    assert scale == pytest.approx(0.1 * math.log(factor) + 1.0, rel=1e-15)
+    ratio = plain / inv
+    # a few roundings of pow in double
+    np.testing.assert_allclose(ratio[turns > 40], 1.0, rtol=1e-13)      # fast ones are kept
+    np.testing.assert_allclose(ratio[turns < 0.9], factor, rtol=1e-12)  # slow ones are divided
+    assert np.all(np.diff(ratio) >= -1e-12)            # and between them it only grows
+    assert nebw.rope_freqs(theta, 2 * n, "yarn", factor, length, attn_scale=1.5)[1] == 1.5
+    inv, scale = nebw.rope_freqs(theta, 2 * n, "bands", factor=factor, orig_len=length)
+    assert scale == 1.0
+    ratio = plain / inv
+    np.testing.assert_allclose(ratio[turns >= 4.0], 1.0, rtol=1e-13)
+    np.testing.assert_allclose(ratio[turns <= 1.0], factor, rtol=1e-12)
+    mid = (turns > 1.0) & (turns < 4.0)
+    keep = (turns[mid] - 1.0) / 3.0
+    np.testing.assert_allclose(inv[mid], plain[mid] * (keep + (1 - keep) / factor), rtol=1e-12)
+    inv, _ = nebw.rope_freqs(theta, 2 * n, "bands", factor, length, fast=2.0, slow=0.5)
+    np.testing.assert_allclose((plain / inv)[turns >= 2.0], 1.0, rtol=1e-13)
+
+
+@pytest.mark.parametrize("args,word", [
+    ((10000.0, 7), "rotary width"),
+    ((10000.0, 0), "rotary width"),
+    ((10000.0, 258), "rotary width"),
+    ((1.0, 64), "rotary base"),
+    ((float("inf"), 64), "rotary base"),
+    ((float("nan"), 64), "rotary base"),
+    ((10000.0, 64, "linear", 0.5), "factor"),
+    ((10000.0, 64, "ntk", float("nan")), "factor"),
+    ((10000.0, 64, "yarn", 4.0), "trained length"),
+    ((10000.0, 64, "bands", 4.0, 4096, 1.0, 2.0), "bounds"),
+])
+def test_rope_freqs_refusals(args, word):
+    import nebw
+    with pytest.raises(nebw.NebwError, match=word) as e:
+        nebw.rope_freqs(*args)
+    assert e.value.code == 1
+
+
+def test_rope_freqs_null_outputs_and_unknown_kind():
+    import ctypes as C
+
+    import nebw
+    L = nebw.lib()
+    assert L.nebw_rope_freqs(10000.0, 64, None, None, None) == 1
+    inv, scale = (C.c_double * 32)(), C.c_double()
+    s = nebw.RopeScaling(9, 0, 4096, 2.0, 0, 0, 0)
+    assert L.nebw_rope_freqs(10000.0, 64, C.byref(s), inv, C.byref(scale)) == 1
+    assert "scaling 9" in L.nebw_last_error().decode()
+    assert L.nebw_rope_freqs(10000.0, 64, None, inv, C.byref(scale)) == 0  # NULL: plain
+    assert inv[0] == 1.0 and scale.value == 1.0
+
+
+def test_route_workspace():
+    import nebw
+    assert nebw.moe_route_workspace(0, 8, 2) == 0
+    small, big = nebw.moe_route_workspace(1, 8, 2), nebw.moe_route_workspace(131072, 256, 8)
+    assert 0 <= small <= big <= 16 << 20
+    for rows, experts, k in [(1, 0, 1), (1, 513, 1), (1, 8, 0), (1, 8, 17), (1, 4, 5), (-1, 8, 2),
+                             (1 << 30, 8, 2), (1 << 62, 8, 4)]:
+        with pytest.raises(nebw.NebwError):
+            nebw.moe_route_workspace(rows, experts, k)
+
+
+def test_null_device_is_refused_by_name():
+    import nebw
+    L = nebw.lib()
+    calls = {
+        "nebw_stage_rope": (None, None, 1, 1, 1.0, None),
+        "nebw_row_positions": (None,) * 3 + (1, 1, None, None),
+        "nebw_rope": (None, None, None, 1, 1, None, 64, 1, 0, None, None),
+        "nebw_qk_norm_rope": (None, None, None, 1, 1, None, 64, 1, 1e-6, 0, 0, None, None),
+        "nebw_stage_experts": (None, None, 0, 1, 64, 64, 0, None, None),
+        "nebw_moe_route": (None, None, 0, 8, 1, None, 8, 2, 0, 0, 1.0) + (None,) * 6 + (0, None),
+        "nebw_gemm_grouped": (None, 1, None, 1, None, None, 1, 64, 64, None, 0, None, 1, None),
+        "nebw_moe_combine": (None, None, 1, 1, None, None, 1, None, 2, 64, None, None, 1, None),
+    }
+    for name, args in calls.items():
+        assert getattr(L, name)(*args) == 1, name
+        assert "null device handle" in L.nebw_last_error().decode(), name
+
+
+def test_heads_of_refuses_what_it_cannot_describe():
+    torch = pytest.importorskip("torch")
+    import nebw
+    x = torch.zeros(4, 96)
+    h = nebw.Heads.of(x[:, 32:], 2)
+    assert (h.x, h.out, h.stride, h.heads) == (x.data_ptr() + 128, x.data_ptr() + 128, 96, 2)
+    for bad in (x.t(), x[:, ::2], x.reshape(2, 2, 96)):
+        with pytest.raises(ValueError):
+            nebw.Heads.of(bad, 2)
+    with pytest.raises(ValueError):
+        nebw.Heads.of(x, 5)
+    with pytest.raises(ValueError):
+        nebw.Heads.of(x, 2, out=torch.zeros(4, 96, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        nebw.Heads.of(x, 2, gamma=torch.zeros(96))
+    with pytest.raises(TypeError):
+        nebw.Heads.of(x.double(), 2)
