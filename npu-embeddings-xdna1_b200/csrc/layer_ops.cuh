@@ -41,9 +41,6 @@ int set_grouped_attrs_bn() {
 int set_layer_op_attrs() {
   if (int rc = set_grouped_attrs_bn<128>()) return rc;
   if (int rc = set_grouped_attrs_bn<256>()) return rc;
-  NEBW_CUDA(cudaFuncSetAttribute(
-      nebw::route_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      (nebw::kRouteWarps + 1) * nebw::kRouteMaxExperts * static_cast<int>(sizeof(int))));
   return NEBW_OK;
 }
 
@@ -194,8 +191,39 @@ int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t
   return NEBW_OK;
 }
 
+template <typename T, int NORM, bool PAIRS, int IT>
+void launch_heads_vec(const nebw::HeadArgs &a, int lg, unsigned blocks, int q_chunks, int chunks,
+                      cudaStream_t st) {
+  nebw::heads_vec_kernel<T, NORM, PAIRS, IT><<<blocks, 256, 0, st>>>(a, lg, q_chunks, chunks);
+}
+
+bool heads_vec_side(const nebw::HeadSide &s, size_t esz) {
+  return aligned(s.x, 16) && aligned(s.out, 16) && s.stride * esz % 16 == 0 &&
+         s.out_stride * esz % 16 == 0 && aligned(s.gamma, 16) && aligned(s.beta, 16);
+}
+
 template <typename T, int NORM, bool PAIRS>
 int launch_heads(const nebw::HeadArgs &a, cudaStream_t st) {
+  constexpr int V = nebw::HeadVec<T>::V;
+  if (a.head_dim % (2 * V) == 0 && a.n % V == 0 && heads_vec_side(a.q, sizeof(T)) &&
+      heads_vec_side(a.k, sizeof(T))) {
+    int lg = 0;  // lanes a head
+    while ((2 * V << lg) < a.head_dim) ++lg;
+    const int per = 32 >> lg;  // heads a warp takes at once
+    const int most = std::max(a.q.heads, a.k.heads);
+    const int it = most > 2 * per ? 4 : most > per ? 2 : 1;
+    const int q_chunks = (a.q.heads + per * it - 1) / (per * it);
+    const int chunks = q_chunks + (a.k.heads + per * it - 1) / (per * it);
+    const int64_t blocks = (a.rows * chunks + 7) / 8;
+    NEBW_REQUIRE(blocks < (1ll << 31), "too many heads: %lld rows of %d",
+                 static_cast<long long>(a.rows), a.q.heads + a.k.heads);
+    const unsigned g = static_cast<unsigned>(blocks);
+    if (it == 4) launch_heads_vec<T, NORM, PAIRS, 4>(a, lg, g, q_chunks, chunks, st);
+    else if (it == 2) launch_heads_vec<T, NORM, PAIRS, 2>(a, lg, g, q_chunks, chunks, st);
+    else launch_heads_vec<T, NORM, PAIRS, 1>(a, lg, g, q_chunks, chunks, st);
+    NEBW_CUDA(cudaGetLastError());
+    return NEBW_OK;
+  }
   const int heads = a.q.heads + a.k.heads;
   const int64_t blocks = (a.rows * heads + 7) / 8;
   NEBW_REQUIRE(blocks < (1ll << 31), "too many heads: %lld rows of %d",
@@ -288,8 +316,13 @@ extern "C" int nebw_qk_norm_rope(nebw_dev *d, const nebw_heads *q, const nebw_he
 
 namespace {
 
-int64_t route_blocks(int64_t rows) {
-  return (rows + nebw::kRouteBlockRows - 1) / nebw::kRouteBlockRows;
+constexpr int kRouteMostBlocks = 256;  // no sm_100 GPU has more SMs
+
+// Blocks of the two-kernel form (1: the fused one): one an SM at most, which
+// keeps the counts that every block sums small, of 32 rows at least.
+int64_t route_blocks(int64_t rows, int sms) {
+  if (rows <= nebw::kRouteFusedRows) return 1;
+  return std::min<int64_t>((rows + 31) / 32, std::min(sms, kRouteMostBlocks));
 }
 
 int check_route(int64_t rows, int32_t experts, int32_t top_k) {
@@ -302,22 +335,36 @@ int check_route(int64_t rows, int32_t experts, int32_t top_k) {
   return NEBW_OK;
 }
 
+template <typename T, int K>
+int launch_route(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
+  const size_t smem = (nebw::kRouteWarps + 2) * static_cast<size_t>(a.experts) * sizeof(int);
+  if (blocks == 1) {
+    nebw::route_fused_kernel<T, K><<<1, nebw::kRouteThreads, smem, st>>>(a);
+  } else {
+    nebw::route_choose_kernel<T, K><<<blocks, nebw::kRouteThreads, 0, st>>>(a);
+    NEBW_CUDA(cudaGetLastError());
+    nebw::route_place_kernel<<<blocks, nebw::kRouteThreads, smem, st>>>(a);
+  }
+  NEBW_CUDA(cudaGetLastError());
+  return NEBW_OK;
+}
+
+// The list a lane keeps: the next power of two of top_k.
 template <typename T>
-void launch_topk(const nebw::RouteArgs &a, cudaStream_t st) {
-  const unsigned g = static_cast<unsigned>(a.blocks);
-  const int b = nebw::kRouteThreads;
-  if (a.experts <= 32) nebw::route_topk_kernel<T, 1><<<g, b, 0, st>>>(a);
-  else if (a.experts <= 64) nebw::route_topk_kernel<T, 2><<<g, b, 0, st>>>(a);
-  else if (a.experts <= 128) nebw::route_topk_kernel<T, 4><<<g, b, 0, st>>>(a);
-  else if (a.experts <= 256) nebw::route_topk_kernel<T, 8><<<g, b, 0, st>>>(a);
-  else nebw::route_topk_kernel<T, 16><<<g, b, 0, st>>>(a);
+int launch_route_k(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
+  if (a.k == 1) return launch_route<T, 1>(a, blocks, st);
+  if (a.k == 2) return launch_route<T, 2>(a, blocks, st);
+  if (a.k <= 4) return launch_route<T, 4>(a, blocks, st);
+  if (a.k <= 8) return launch_route<T, 8>(a, blocks, st);
+  return launch_route<T, 16>(a, blocks, st);
 }
 
 }  // namespace
 
 extern "C" int64_t nebw_moe_route_workspace(int64_t rows, int32_t experts, int32_t top_k) {
   if (check_route(rows, experts, top_k)) return -1;
-  return route_blocks(rows) * experts * static_cast<int64_t>(sizeof(int));
+  if (rows <= nebw::kRouteFusedRows) return 0;
+  return int64_t{kRouteMostBlocks} * experts * static_cast<int64_t>(sizeof(int));
 }
 
 extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_t stride,
@@ -337,19 +384,20 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
     NEBW_CUDA(cudaMemsetAsync(group_off, 0, (experts + 1) * sizeof(int), st));
     return NEBW_OK;
   }
-  NEBW_REQUIRE(logits && ids && weights && row_src && row_dst && ws, "null routing operand");
+  NEBW_REQUIRE(logits && ids && weights && row_src && row_dst, "null routing operand");
   NEBW_REQUIRE(stride >= experts && stride < (1ll << 31),
                "logit row stride %lld refused for %d experts", static_cast<long long>(stride),
                experts);
-  NEBW_REQUIRE(aligned(logits, dtype == NEBW_F32 ? 4 : 2) && aligned(ws, 4),
-               "routing operands are not aligned");
-  const int64_t need = route_blocks(rows) * experts * static_cast<int64_t>(sizeof(int));
-  NEBW_REQUIRE(ws_bytes >= need, "routing workspace of %lld bytes refused: %lld are needed",
+  const size_t esz = dtype == NEBW_F32 ? 4 : 2;
+  NEBW_REQUIRE(aligned(logits, esz) && aligned(ws, 4), "routing operands are not aligned");
+  const int64_t need = nebw_moe_route_workspace(rows, experts, top_k);
+  NEBW_REQUIRE(ws_bytes >= need && (ws || need == 0),
+               "routing workspace of %lld bytes refused: %lld are needed",
                static_cast<long long>(ws_bytes), static_cast<long long>(need));
   nebw::RouteArgs a{};
   a.logits = logits;
   a.stride = stride;
-  a.rows = rows;
+  a.rows = static_cast<int>(rows);
   a.rows_dev = rows_dev;
   a.experts = experts;
   a.k = top_k;
@@ -362,14 +410,15 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
   a.row_src = row_src;
   a.row_dst = row_dst;
   a.hist = static_cast<int *>(ws);
-  a.blocks = static_cast<int>(route_blocks(rows));
-  if (dtype == NEBW_F32) launch_topk<float>(a, st);
-  else launch_topk<__nv_bfloat16>(a, st);
-  NEBW_CUDA(cudaGetLastError());
-  const size_t smem = (nebw::kRouteWarps + 1) * static_cast<size_t>(experts) * sizeof(int);
-  nebw::route_place_kernel<<<static_cast<unsigned>(a.blocks), nebw::kRouteThreads, smem, st>>>(a);
-  NEBW_CUDA(cudaGetLastError());
-  return NEBW_OK;
+  const int eights = (experts + 7) / 8;
+  // four lanes a row up to 128 experts, then as many as leave each 32
+  while (a.lg < 4 && (1 << a.lg) < eights && (a.lg < 2 || (eights >> a.lg) > 4)) ++a.lg;
+  a.per = (eights + (1 << a.lg) - 1) / (1 << a.lg) * 8;
+  a.vec = experts % 8 == 0 && aligned(logits, 16) && stride * esz % 16 == 0;
+  const int blocks = static_cast<int>(route_blocks(rows, d->sm_count));
+  a.block_rows = static_cast<int>((rows + blocks - 1) / blocks);
+  return dtype == NEBW_F32 ? launch_route_k<float>(a, blocks, st)
+                           : launch_route_k<__nv_bfloat16>(a, blocks, st);
 }
 
 extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_t experts,
@@ -539,10 +588,13 @@ namespace {
 
 template <typename TY, typename TO>
 void launch_combine(const nebw::CombineArgs &a, bool vec, cudaStream_t st) {
-  const int64_t items = a.rows * (vec ? a.H / 8 : a.H);
-  const unsigned g = static_cast<unsigned>((items + 255) / 256);
-  if (vec) nebw::moe_combine_kernel<TY, TO, 8><<<g, 256, 0, st>>>(a);
-  else nebw::moe_combine_kernel<TY, TO, 1><<<g, 256, 0, st>>>(a);
+  const int cols = vec ? a.H / 8 : a.H;  // threads a row would take
+  int tx = 32;
+  while (tx < cols && tx < 256) tx <<= 1;
+  const dim3 b(tx, 256 / tx);
+  const unsigned g = static_cast<unsigned>((a.rows + b.y - 1) / b.y);
+  if (vec) nebw::moe_combine_kernel<TY, TO, 8><<<g, b, 0, st>>>(a);
+  else nebw::moe_combine_kernel<TY, TO, 1><<<g, b, 0, st>>>(a);
 }
 
 }  // namespace
@@ -559,7 +611,7 @@ extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t
                nebw::kRouteMaxK);
   NEBW_REQUIRE(H >= 1 && H <= (1 << 20), "width %lld refused", static_cast<long long>(H));
   NEBW_REQUIRE(rows >= 0 && rows < (1ll << 30) && rows * top_k < (1ll << 30) && y_rows >= 0 &&
-                   y_rows < (1ll << 30) && rows * H < (1ll << 38),
+                   y_rows < (1ll << 30),
                "%lld rows of %d experts refused", static_cast<long long>(rows), top_k);
   if (rows == 0) return NEBW_OK;
   NEBW_REQUIRE(y && row_dst && weights && out, "null combine operand");
@@ -569,11 +621,11 @@ extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t
   a.weights = weights;
   a.residual = residual;
   a.out = out;
-  a.rows = rows;
-  a.y_rows = y_rows;
+  a.rows = static_cast<int>(rows);
+  a.y_rows = static_cast<int>(y_rows);
   a.rows_dev = rows_dev;
   a.k = top_k;
-  a.H = H;
+  a.H = static_cast<int>(H);
   a.err = d->d_err;
   const bool vec = H % 8 == 0 && aligned(y, 16) && aligned(out, 16) && aligned(residual, 16);
   const cudaStream_t st = pick_stream(d, stream);

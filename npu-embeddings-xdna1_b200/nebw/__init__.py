@@ -266,7 +266,7 @@ class Device:
             return _stream(stream)
         if self.torch_stream:
             import torch
-            return _stream(torch.cuda.current_stream())
+            return _stream(torch.cuda.current_stream(self.index))
         return None
 
     def close(self):
