@@ -9,13 +9,25 @@
 // a gated weight's N columns are interleaved in groups of 64 = [32 up |
 // 32 gate] and the product is up * act(gate), N / 2 wide.
 //
-// Tiles are 128 x BN of one expert; a list of tile counts per expert, built
-// by every block from off, gives a tile its expert.  The roles, the shared
-// memory ring, the double-buffered accumulator and the bounded waits are
-// gemm_tc_kernel's.  A's rows come by a tiled TMA load where they are grouped
-// already (rows past the group are the next group's and are not stored), or
-// by 32 four-row gathers, one from each lane of the producer warp, the lane
-// keeping its four row indices in registers for the whole tile.
+// A tile is 128 * CTAS rows of one expert by bn columns: a CTA pair on 256 x
+// 256 (tcgen05 cta_group::2, each CTA loading its 128 rows of A and of W) or
+// one CTA on 128 x bn, bn <= 128.  A list of tile counts per expert, built by
+// every block from off, gives a tile its expert, so the persistent blocks walk
+// one list whatever the groups are.  Roles of a block:
+//   warp 0        W by TMA (and A, where its rows are grouped already), and
+//                 the stage's transaction bytes
+//   warp 1        tcgen05.mma (the pair's leader)
+//   warps 2-9     epilogue: TMEM -> bias, activation -> shared memory -> TMA
+//                 store of 32 x 32 chunks; the chunk in which a group ends is
+//                 stored row by row
+//   warps 10-13   GATHER: A's rows, four at a time (tile::gather4), each warp
+//                 a quarter of the tile's rows with their indices in registers
+// A gather is issued by one lane for uniform operands; from 32 lanes of one
+// warp the same 32 gathers take turns on the issue path (80 clocks each,
+// measured: 2457 us for 65,542 rows, K 1024, N 8192).  Rows past the group
+// are not loaded: what lies in their place in shared memory reaches only
+// accumulator rows that are not stored.  All waits are bounded as in
+// gemm_tc_pair_kernel, whose barriers these are.
 #pragma once
 
 #include <cuda.h>
@@ -46,21 +58,70 @@ struct GroupedArgs {
   const int *row_src;  // [rows] or null
   int a_rows;          // A's rows
   int N, K;            // N as staged (2F for a gated weight)
+  int bn;              // tile columns: 256 (pairs); 128, 64 or 32
   const float *bias;   // [experts, N] in the container's column order, or null
   void *out;           // [rows, N or N / 2]
   int *err;
 };
 
+// Shared memory, the same for both: 128 rows of A and up to 128 of W a stage.
+struct GroupedShape {
+  static constexpr int kABytes = kGemmBM * kGemmBK * 2;
+  static constexpr int kStageBytes = 2 * kABytes;
+  static constexpr int kStages = 5;
+  static constexpr int kWarpStaging = 6 * 1024;  // one fp32 or three bf16 chunks
+  static constexpr int kStagingBytes = 8 * kWarpStaging;
+  static constexpr int kBarBytes = 256;
+  static constexpr int kTableBytes = 2 * (kGroupMaxExperts + 1) * 4;
+  static constexpr int kSmemBytes =
+      1024 + kStages * kStageBytes + kStagingBytes + kBarBytes + kTableBytes;
+};
+constexpr int kGroupedBox = 32;           // rows a TMA box of A or W
+constexpr int kGroupedThreads = 320;
+constexpr int kGroupedGatherThreads = 448;  // four more warps
+
+// A box of a K-major map into this CTA's shared memory, completing on the
+// barrier at `bar` (a shared::cluster address: the pair leader's).
+template <int CTAS>
+__device__ __forceinline__ void grp_load(void *smem_dst, const void *tmap, uint32_t bar, int32_t c0,
+                                         int32_t c1) {
+  if constexpr (CTAS == 2)
+    tma_load_2d_pair(smem_dst, tmap, bar, c0, c1);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+
+// Arrive on a barrier of this cluster without ordering any memory access of
+// this thread before it.
+__device__ __forceinline__ void grp_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+
 // Four rows of a K-major map (box 64 x 1) into 512 consecutive bytes of a
 // 128-byte-swizzled tile.
-__device__ __forceinline__ void tma_gather4(void *smem_dst, const void *tmap, uint64_t *bar,
-                                            int32_t c0, const int (&r)[4]) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_u32(smem_dst)),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
-      "r"(smem_u32(bar))
-      : "memory");
+template <int CTAS>
+__device__ __forceinline__ void grp_gather4(uint32_t dst, const void *tmap, uint32_t bar,
+                                            int32_t c0, int32_t r0, int32_t r1, int32_t r2,
+                                            int32_t r3) {
+  if constexpr (CTAS == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+        ".cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
+        "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
+        "r"(bar)
+        : "memory");
 }
 
 // The groups in shared memory: off clamped to [0, rows] and ascending (a
@@ -69,6 +130,7 @@ struct GroupTable {
   int off[kGroupMaxExperts + 1];
   int tile[kGroupMaxExperts + 1];
 };
+static_assert(sizeof(GroupTable) == GroupedShape::kTableBytes, "table size");
 
 __device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedArgs &p, int bm,
                                                   int n_blocks) {
@@ -126,41 +188,90 @@ __device__ __forceinline__ GroupTile group_tile(const GroupTable &g, int t, int 
   return {e, g.off[e] + mb * bm, g.off[e + 1], i - mb * n_blocks};
 }
 
-// 32 accumulator columns [col0, col0 + 32) of one row, biased, activated and
-// stored; a gated epilogue's come with the 32 columns of their gate.
+// 32 accumulator columns of one row from GEMM column col0 on (a gated
+// epilogue: up columns, with their gates in rg), biased and activated: output
+// columns [c0, c0 + ncols).
 template <int EPI>
-__device__ __forceinline__ void grp_store32(const GroupedArgs &p, int e, int64_t row, int col0,
-                                            const uint32_t (&r)[32], const uint32_t (&rg)[32]) {
-  constexpr bool kGated = grp_gated(EPI);
-  const int width = kGated ? p.N / 2 : p.N;
-  const int c0 = kGated ? col0 / 2 : col0;  // col0 % 64 == 0 there
-  const int ncols = min(32, width - c0);    // width % 8 == 0
-  float v[32];
+__device__ __forceinline__ void grp_finish(const float *bias, int width, int c0, int ncols,
+                                           const uint32_t (&r)[32], const uint32_t (&rg)[32],
+                                           float (&v)[32]) {
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-  const float *bias = p.bias ? p.bias + static_cast<int64_t>(e) * p.N + c0 : nullptr;
+  if (bias) {
+    const float4 *b4 = reinterpret_cast<const float4 *>(bias + c0);
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    if (i < ncols) {
-      if (bias) v[i] += __ldg(bias + i);
-      if constexpr (kGated) {
-        float g = __uint_as_float(rg[i]);
-        if (bias) g += __ldg(bias + width + i);
-        v[i] *= EPI == kGrpBf16SwiGLU ? silu_fast(g) : gelu_erf(g);
-      } else if constexpr (EPI == kGrpBf16Gelu8) {
-        v[i] = gelu8(v[i]);
-      } else if constexpr (EPI == kGrpBf16Erf) {
-        v[i] = gelu_erf(v[i]);
+    for (int i = 0; i < 8; ++i) {
+      if (i * 4 < ncols) {
+        const float4 b = __ldg(b4 + i);
+        v[4 * i] += b.x;
+        v[4 * i + 1] += b.y;
+        v[4 * i + 2] += b.z;
+        v[4 * i + 3] += b.w;
       }
     }
   }
+  if constexpr (grp_gated(EPI)) {
+    const float4 *b4 = bias ? reinterpret_cast<const float4 *>(bias + width + c0) : nullptr;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float g[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = __uint_as_float(rg[4 * i + j]);
+      if (b4) {  // a gated width is a multiple of 32
+        const float4 b = __ldg(b4 + i);
+        g[0] += b.x;
+        g[1] += b.y;
+        g[2] += b.z;
+        g[3] += b.w;
+      }
+      if constexpr (EPI == kGrpBf16SwiGLU) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * i + j] *= silu_fast(g[j]);
+      } else {
+        gelu_erf_x2(g[0], g[1]);
+        gelu_erf_x2(g[2], g[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[4 * i + j] *= g[j];
+      }
+    }
+  } else if constexpr (EPI == kGrpBf16Gelu8) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) gelu8_x2(v[i], v[i + 1]);
+  } else if constexpr (EPI == kGrpBf16Erf) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) gelu_erf_x2(v[i], v[i + 1]);
+  }
+}
+
+// This lane's row of a 32 x 32 chunk in shared memory, in the output map's
+// swizzle (make_tmap_out): fp32 rows of 128 bytes, bf16 rows of 64.
+template <int EPI>
+__device__ __forceinline__ void grp_stage(const float (&v)[32], uint8_t *chunk, int lane) {
   if constexpr (EPI == kGrpF32) {
-    float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + row * width + c0);
+#pragma unroll
+    for (int q = 0; q < 8; ++q)
+      *reinterpret_cast<float4 *>(chunk + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<uint4 *>(chunk + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
+          make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
+                     pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
+                     pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
+  }
+}
+
+// The same row straight to C.
+template <int EPI>
+__device__ __forceinline__ void grp_store(void *out, int64_t at, int ncols, const float (&v)[32]) {
+  if constexpr (EPI == kGrpF32) {
+    float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       if (i * 4 < ncols) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   } else {
-    uint4 *o = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.out) + row * width + c0);
+    uint4 *o = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(out) + at);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (i * 8 < ncols)
@@ -171,192 +282,308 @@ __device__ __forceinline__ void grp_store32(const GroupedArgs &p, int e, int64_t
   }
 }
 
-template <int BN>
-struct GroupedShape {
-  using S = GemmShape<BN>;
-  static constexpr int kSmemBytes = S::kSmemBytes + static_cast<int>(sizeof(GroupTable));
-};
-
-template <int BN, int EPI, bool GATHER>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+template <int CTAS, int EPI, bool GATHER>
+__global__ void __cluster_dims__(CTAS, 1, 1)
+    __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA,
-                        const __grid_constant__ CUtensorMap tmW, const GroupedArgs p) {
-  using S = GemmShape<BN>;
+                        const __grid_constant__ CUtensorMap tmW,
+                        const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
+  using S = GroupedShape;
   constexpr int kStages = S::kStages;
+  constexpr int kTileM = CTAS * kGemmBM;
+  constexpr int kAccCols = CTAS == 2 ? 256 : 128;  // TMEM columns of an accumulator
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t *sA = smem;
   uint8_t *sW = smem + kStages * S::kABytes;
-  uint64_t *full = reinterpret_cast<uint64_t *>(smem + kStages * S::kStageBytes);
+  uint8_t *staging = smem + kStages * S::kStageBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(staging + S::kStagingBytes);
   uint64_t *empty = full + kStages;
   uint64_t *tfull = empty + kStages;
   uint64_t *tempty = tfull + 2;
   uint64_t *drain = tempty + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-  GroupTable &table = *reinterpret_cast<GroupTable *>(smem + kStages * S::kStageBytes + S::kBarBytes);
+  GroupTable &table =
+      *reinterpret_cast<GroupTable *>(staging + S::kStagingBytes + S::kBarBytes);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int n_blocks = (p.N + BN - 1) / BN;
+  const int rank = CTAS == 2 ? static_cast<int>(cluster_ctarank()) : 0;
+  const bool leader = rank == 0;
+  const int bn = CTAS == 2 ? 256 : p.bn;
+  const int n_blocks = (p.N + bn - 1) / bn;
   const int num_kb = (p.K + kGemmBK - 1) / kGemmBK;
+  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmA);
     tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmC);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
+      // every gather warp arrives on every stage, also with no row to load:
+      // one that did not could fall a phase behind the ring, whose parity
+      // then reads the wrong way round
+      mbar_init(&full[s], 1 + (GATHER ? 4 * CTAS : 0));
       mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 8);
+      mbar_init(&tempty[a], 8 * CTAS);
     }
     mbar_init(drain, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, S::kTmemCols);
-    tmem_relinquish();
+    if constexpr (CTAS == 2) {
+      tmem_alloc_pair(tmem_slot, 2 * kAccCols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 2 * kAccCols);
+      tmem_relinquish();
+    }
   }
-  group_table_build(table, p, kGemmBM, n_blocks);
+  group_table_build(table, p, kTileM, n_blocks);
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();
+  else __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int num_tiles = table.tile[p.experts];
   auto wait_all = [&](uint64_t *bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
   };
+  auto leader_bar = [&](uint64_t *bar) -> uint32_t {
+    return CTAS == 2 ? map_to_cta(smem_u32(bar), 0) : smem_u32(bar);
+  };
+  // of a tile's rows, how many lie in CTA c's 128
+  auto cta_rows = [&](const GroupTile &t, int c) -> int {
+    return min(max(t.end - t.row - c * kGemmBM, 0), kGemmBM);
+  };
 
   if (warp == 0) {
-    // ---------------- TMA producer (the whole warp walks the schedule) -----
-    int stage = 0, e = 0;
-    uint32_t phase = 0;
-    uint32_t issued_mask = 0, last_phase = 0;
-    bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
-      int src[4];
-      if constexpr (GATHER) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          // past the group: its last row again, not stored
-          int r = __ldg(p.row_src + min(t.row + 4 * lane + i, t.end - 1));
-          if (r < 0 || r >= p.a_rows) {
-            record_err(p.err, kDevBadGroup);
-            r = 0;
+    // ---------------- W (and grouped A) producer ----------------
+    if (lane == 0) {
+      int stage = 0, e = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
+        const GroupTile t = group_tile(table, tile, kTileM, n_blocks, e);
+        const int a_boxes = GATHER ? 0 : (cta_rows(t, rank) + kGroupedBox - 1) / kGroupedBox;
+        uint32_t bytes = static_cast<uint32_t>(bn) * kGemmBK * 2;
+        for (int c = 0; c < CTAS; ++c) {
+          const int m = cta_rows(t, c);
+          bytes += GATHER ? (m + 3) / 4 * 512
+                          : (m + kGroupedBox - 1) / kGroupedBox * (kGroupedBox * 128);
+        }
+        const int w_row = t.e * p.N + t.nb * bn + rank * (bn / CTAS);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) {
+            ok = false;
+            break;
           }
-          src[i] = r;
+          if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
+          const uint32_t bar = leader_bar(&full[stage]);
+          if constexpr (CTAS == 2) {
+            grp_load<CTAS>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
+          } else {
+            for (int i = 0; i < bn / kGroupedBox; ++i)
+              grp_load<CTAS>(sW + stage * S::kABytes + i * kGroupedBox * 128, &tmW, bar,
+                             kb * kGemmBK, w_row + i * kGroupedBox);
+          }
+          for (int i = 0; i < a_boxes; ++i)
+            grp_load<CTAS>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
+                           kb * kGemmBK, t.row + rank * kGemmBM + i * kGroupedBox);
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
         }
       }
+      // Tail: the MMAs have released every stage, so all loads of this CTA
+      // (the gathers too) have landed and all commits aimed at its barriers
+      // have arrived before it may exit.
+      for (int i = 0; i < kStages && ok; ++i) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) break;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (the pair's leader) ----------------
+    if (leader) {
+      const uint32_t idesc = idesc_bf16_f32(kTileM, bn);
+      const bool elect = elect_one_sync();
+      int stage = 0;
+      uint32_t phase = 0;
+      bool issued_any = false, ok = true;
+      int local = 0;
+      for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
+        const int acc = local & 1;
+        if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kAccCols);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!wait_all(&full[stage], phase)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t da = sdesc_kmajor_sw128(smem_u32(sA + stage * S::kABytes));
+          const uint64_t dw = sdesc_kmajor_sw128(smem_u32(sW + stage * S::kABytes));
+          if (elect) {
+#pragma unroll
+            for (int k = 0; k < kGemmBK / 16; ++k) {
+              if constexpr (CTAS == 2)
+                umma_bf16_pair(d_tmem, da + k * 2, dw + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
+              else
+                umma_bf16(d_tmem, da + k * 2, dw + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
+            }
+            if constexpr (CTAS == 2) umma_commit_pair(&empty[stage], 0x3);
+            else umma_commit(&empty[stage]);
+          }
+          __syncwarp();
+          issued_any = true;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok && elect) {
+          if constexpr (CTAS == 2) umma_commit_pair(&tfull[acc], 0x3);
+          else umma_commit(&tfull[acc]);
+        }
+        __syncwarp();
+      }
+      if (issued_any) {
+        if (elect) {
+          if constexpr (CTAS == 2) umma_commit_pair(drain, 0x1);
+          else umma_commit(drain);
+        }
+        __syncwarp();
+        wait_all(drain, 0);
+      }
+    }
+  } else if (warp < 10) {
+    // ---------------- epilogue ----------------
+    // Two warps per TMEM lane quarter, half of the columns each.
+    constexpr bool kGated = grp_gated(EPI);
+    constexpr int kStep = kGated ? 64 : 32;  // accumulator columns a chunk takes
+    constexpr int kChunkBytes = EPI == kGrpF32 ? 4096 : 2048;
+    constexpr int kSlots = S::kWarpStaging / kChunkBytes;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    // whole chunks to each half, the first taking the larger share
+    const int split = (bn / kStep + 1) / 2 * kStep;
+    const int begin = half ? split : 0, end = half ? bn : split;
+    const int width = kGated ? p.N / 2 : p.N;
+    uint8_t *mine = staging + (warp - 2) * S::kWarpStaging;
+    int slot = 0;
+    int local = 0, e = 0;
+    for (int tile = first; tile < num_tiles; tile += step, ++local) {
+      const int acc = local & 1;
+      if (!wait_all(&tfull[acc], (local >> 1) & 1)) break;
+      tc_fence_after();
+      const GroupTile t = group_tile(table, tile, kTileM, n_blocks, e);
+      const int row0 = t.row + rank * kGemmBM + quarter * 32;
+      const float *bias = p.bias ? p.bias + static_cast<int64_t>(t.e) * p.N : nullptr;
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(acc * kAccCols);
+      if (row0 < t.end) {  // warp-uniform
+#pragma unroll 1
+        for (int c = begin; c < end; c += kStep) {
+          const int col0 = t.nb * bn + c;
+          if (col0 >= p.N) break;
+          uint32_t r[32], rg[32];
+          tmem_ld_32x32b_x32(t_row + c, r);
+          if constexpr (kGated) tmem_ld_32x32b_x32(t_row + c + 32, rg);
+          tmem_wait_ld_regs(r);
+          if constexpr (kGated) tmem_wait_ld_regs(rg);
+          const int c0 = kGated ? col0 / 2 : col0;
+          const int ncols = min(32, width - c0);
+          float v[32];
+          grp_finish<EPI>(bias, width, c0, ncols, r, rg, v);
+          if (row0 + 32 <= t.end) {
+            uint8_t *chunk = mine + slot * kChunkBytes;
+            if (++slot == kSlots) slot = 0;
+            if (lane == 0) bulk_wait_group_read<kSlots - 1>();
+            __syncwarp();
+            grp_stage<EPI>(v, chunk, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmC, chunk, c0, row0);
+              bulk_commit_group();
+            }
+          } else if (row0 + lane < t.end) {
+            grp_store<EPI>(p.out, static_cast<int64_t>(row0 + lane) * width + c0, ncols, v);
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        if constexpr (CTAS == 2) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty[acc]), 0));
+        else mbar_arrive(&tempty[acc]);
+      }
+    }
+    if (lane == 0) bulk_wait_group_all();
+  } else if constexpr (GATHER) {
+    // ---------------- A by gathers (warps 10..13) ----------------
+    const int part = warp - 10;  // rows [32 * part, +32) of this CTA's 128
+    const bool elect = elect_one_sync();
+    int stage = 0, e = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first; tile < num_tiles && ok; tile += step) {
+      const GroupTile t = group_tile(table, tile, kTileM, n_blocks, e);
+      const int count = min(max(cta_rows(t, rank) - 32 * part, 0), 32);
+      int mine = 0;
+      if (count > 0) {
+        // past the group: its last row again, to fill a gather of four
+        const int at = t.row + rank * kGemmBM + 32 * part + min(lane, count - 1);
+        mine = __ldg(p.row_src + at);
+        if (mine < 0 || mine >= p.a_rows) {
+          record_err(p.err, kDevBadGroup);
+          mine = 0;
+        }
+      }
+      int src[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) src[i] = __shfl_sync(0xffffffffu, mine, i);
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!wait_all(&empty[stage], phase ^ 1u)) {
           ok = false;
           break;
         }
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&full[stage], S::kStageBytes);
-          tma_load_2d(sW + stage * S::kBBytes, &tmW, &full[stage], kb * kGemmBK,
-                      t.e * p.N + t.nb * BN);
-          if constexpr (!GATHER)
-            tma_load_2d(sA + stage * S::kABytes, &tmA, &full[stage], kb * kGemmBK, t.row);
-        }
-        __syncwarp();
-        if constexpr (GATHER)
-          tma_gather4(sA + stage * S::kABytes + lane * 512, &tmA, &full[stage], kb * kGemmBK, src);
-        issued_mask |= 1u << stage;
-        last_phase = (last_phase & ~(1u << stage)) | (phase << stage);
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-    // Drain: every stage this warp loaded has landed before the CTA exits.
-    for (int s = 0; s < kStages; ++s)
-      if (issued_mask & (1u << s)) wait_all(&full[s], (last_phase >> s) & 1u);
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    constexpr uint32_t idesc = idesc_bf16_f32(kGemmBM, BN);
-    const bool elect = elect_one_sync();
-    int stage = 0;
-    uint32_t phase = 0;
-    bool issued_any = false, ok = true;
-    int local = 0;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
-      const int acc = local & 1;
-      if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
-      tc_fence_after();
-      const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * BN);
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!wait_all(&full[stage], phase)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint64_t da = sdesc_kmajor_sw128(smem_u32(sA + stage * S::kABytes));
-        const uint64_t dw = sdesc_kmajor_sw128(smem_u32(sW + stage * S::kBBytes));
         if (elect) {
+          const uint32_t dst = smem_u32(sA + stage * S::kABytes) + part * 4096;
+          const uint32_t bar = leader_bar(&full[stage]);
 #pragma unroll
-          for (int k = 0; k < kGemmBK / 16; ++k)
-            umma_bf16(d_tmem, da + k * 2, dw + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
-          umma_commit(&empty[stage]);
+          for (int i = 0; i < 8; ++i)
+            if (4 * i < count)
+              grp_gather4<CTAS>(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
+                                src[4 * i + 2], src[4 * i + 3]);
+          grp_arrive(bar);
         }
         __syncwarp();
-        issued_any = true;
         if (++stage == kStages) {
           stage = 0;
           phase ^= 1u;
         }
-      }
-      if (ok && elect) umma_commit(&tfull[acc]);
-      __syncwarp();
-    }
-    if (issued_any) {
-      if (elect) umma_commit(drain);
-      __syncwarp();
-      wait_all(drain, 0);
-    }
-  } else {
-    // ---------------- epilogue (warps 2..9) ----------------
-    constexpr int kHalf = BN / 2;
-    constexpr int kChunks = kHalf / 32;
-    const int quarter = warp & 3;
-    const int col_half = ((warp - 2) >> 2) * kHalf;
-    int local = 0, e = 0;
-    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
-      const int acc = local & 1;
-      if (!wait_all(&tfull[acc], (local >> 1) & 1)) break;
-      tc_fence_after();
-      const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
-      const int row = t.row + quarter * 32 + lane;
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                             static_cast<uint32_t>(acc * BN + col_half);
-      constexpr int kStep = grp_gated(EPI) ? 2 : 1;
-#pragma unroll
-      for (int c = 0; c < kChunks; c += kStep) {
-        uint32_t r[32], rg[32];
-        tmem_ld_32x32b_x32(t_row + c * 32, r);
-        if constexpr (kStep == 2) tmem_ld_32x32b_x32(t_row + (c + 1) * 32, rg);
-        tmem_wait_ld_regs(r);
-        if constexpr (kStep == 2) tmem_wait_ld_regs(rg);
-        if (c + kStep == kChunks) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&tempty[acc]);
-        }
-        const int col0 = t.nb * BN + col_half + c * 32;
-        if (row < t.end && col0 < p.N) grp_store32<EPI>(p, t.e, row, col0, r, rg);
       }
     }
   }
 
   tc_fence_before();
-  __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();  // no CTA leaves while its pair may still signal it
+  else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, S::kTmemCols);
+    if constexpr (CTAS == 2) tmem_dealloc_pair(tmem_base, 2 * kAccCols);
+    else tmem_dealloc(tmem_base, 2 * kAccCols);
   }
 }
 

@@ -18,30 +18,29 @@ int where_is(nebw_dev *d, const void *p, bool *on_device) {
   return NEBW_OK;
 }
 
-template <int BN, int EPI>
+template <int CTAS, int EPI>
 int set_grouped_attr() {
-  const int smem = nebw::GroupedShape<BN>::kSmemBytes;
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<BN, EPI, false>,
+  const int smem = nebw::GroupedShape::kSmemBytes;
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<CTAS, EPI, false>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<BN, EPI, true>,
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<CTAS, EPI, true>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   return NEBW_OK;
 }
 
-template <int BN>
-int set_grouped_attrs_bn() {
-  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16>()) return rc;
-  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16Gelu8>()) return rc;
-  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16Erf>()) return rc;
-  if (int rc = set_grouped_attr<BN, nebw::kGrpF32>()) return rc;
-  if (int rc = set_grouped_attr<BN, nebw::kGrpBf16SwiGLU>()) return rc;
-  return set_grouped_attr<BN, nebw::kGrpBf16GeGLU>();
+template <int CTAS>
+int set_grouped_attrs_ctas() {
+  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16>()) return rc;
+  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16Gelu8>()) return rc;
+  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16Erf>()) return rc;
+  if (int rc = set_grouped_attr<CTAS, nebw::kGrpF32>()) return rc;
+  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16SwiGLU>()) return rc;
+  return set_grouped_attr<CTAS, nebw::kGrpBf16GeGLU>();
 }
 
 int set_layer_op_attrs() {
-  if (int rc = set_grouped_attrs_bn<128>()) return rc;
-  if (int rc = set_grouped_attrs_bn<256>()) return rc;
-  return NEBW_OK;
+  if (int rc = set_grouped_attrs_ctas<1>()) return rc;
+  return set_grouped_attrs_ctas<2>();
 }
 
 }  // namespace
@@ -476,7 +475,7 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   if (e != cudaSuccess)
     rc = set_error(NEBW_ECUDA, "expert weight staging failed: %s", cudaGetErrorString(e));
   if (!rc) rc = make_tmap_kmajor(&w.map128, w.ptr, experts * N, K, 128);
-  if (!rc) rc = make_tmap_kmajor(&w.map256, w.ptr, experts * N, K, 256);
+  if (!rc) rc = make_tmap_kmajor(&w.map32, w.ptr, experts * N, K, nebw::kGroupedBox);
   if (!rc) {
     try {
       d->experts[d->next_handle] = w;
@@ -494,31 +493,39 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
 
 namespace {
 
-template <int BN, int EPI>
-void launch_grouped_epi(const CUtensorMap &mA, const CUtensorMap &mW, const nebw::GroupedArgs &a,
-                        unsigned grid, cudaStream_t st) {
-  const size_t smem = nebw::GroupedShape<BN>::kSmemBytes;
+template <int CTAS, int EPI>
+void launch_grouped_epi(const CUtensorMap &mA, const CUtensorMap &mW, const CUtensorMap &mC,
+                        const nebw::GroupedArgs &a, unsigned grid, cudaStream_t st) {
+  const size_t smem = nebw::GroupedShape::kSmemBytes;
   if (a.row_src)
-    nebw::gemm_grouped_kernel<BN, EPI, true><<<grid, nebw::kGemmThreads, smem, st>>>(mA, mW, a);
+    nebw::gemm_grouped_kernel<CTAS, EPI, true>
+        <<<grid, nebw::kGroupedGatherThreads, smem, st>>>(mA, mW, mC, a);
   else
-    nebw::gemm_grouped_kernel<BN, EPI, false><<<grid, nebw::kGemmThreads, smem, st>>>(mA, mW, a);
+    nebw::gemm_grouped_kernel<CTAS, EPI, false>
+        <<<grid, nebw::kGroupedThreads, smem, st>>>(mA, mW, mC, a);
 }
 
-template <int BN>
-int launch_grouped(nebw_dev *d, const CUtensorMap &mA, const CUtensorMap &mW, int epi,
-                   const nebw::GroupedArgs &a, cudaStream_t st) {
-  // every group may end in a part tile
-  const int64_t tiles = (a.rows / nebw::kGemmBM + std::min(a.experts, a.rows)) *
-                        int64_t{(a.N + BN - 1) / BN};
+// The most tiles that groups of `rows` rows in all can make: every group may
+// end in a part tile.
+int64_t grouped_tiles(int64_t rows, int64_t experts, int64_t tile_rows, int64_t n_blocks) {
+  return (rows / tile_rows + std::min(experts, rows)) * n_blocks;
+}
+
+template <int CTAS>
+int launch_grouped(nebw_dev *d, const CUtensorMap &mA, const CUtensorMap &mW,
+                   const CUtensorMap &mC, int epi, const nebw::GroupedArgs &a, cudaStream_t st) {
+  const int64_t tiles = grouped_tiles(a.rows, a.experts, CTAS * nebw::kGemmBM,
+                                      (a.N + a.bn - 1) / a.bn);
   NEBW_REQUIRE(tiles < (1ll << 31), "grouped product too large");
-  const unsigned grid = static_cast<unsigned>(std::min<int64_t>(tiles, d->sm_count));
+  const unsigned g = static_cast<unsigned>(
+      CTAS * std::min<int64_t>(tiles, CTAS == 2 ? d->gemm_pairs : d->sm_count));
   switch (epi) {
-    case nebw::kGrpBf16: launch_grouped_epi<BN, nebw::kGrpBf16>(mA, mW, a, grid, st); break;
-    case nebw::kGrpBf16Gelu8: launch_grouped_epi<BN, nebw::kGrpBf16Gelu8>(mA, mW, a, grid, st); break;
-    case nebw::kGrpBf16Erf: launch_grouped_epi<BN, nebw::kGrpBf16Erf>(mA, mW, a, grid, st); break;
-    case nebw::kGrpF32: launch_grouped_epi<BN, nebw::kGrpF32>(mA, mW, a, grid, st); break;
-    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<BN, nebw::kGrpBf16SwiGLU>(mA, mW, a, grid, st); break;
-    case nebw::kGrpBf16GeGLU: launch_grouped_epi<BN, nebw::kGrpBf16GeGLU>(mA, mW, a, grid, st); break;
+    case nebw::kGrpBf16: launch_grouped_epi<CTAS, nebw::kGrpBf16>(mA, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16Gelu8: launch_grouped_epi<CTAS, nebw::kGrpBf16Gelu8>(mA, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16Erf: launch_grouped_epi<CTAS, nebw::kGrpBf16Erf>(mA, mW, mC, a, g, st); break;
+    case nebw::kGrpF32: launch_grouped_epi<CTAS, nebw::kGrpF32>(mA, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16SwiGLU>(mA, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16GeGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16GeGLU>(mA, mW, mC, a, g, st); break;
   }
   NEBW_CUDA(cudaGetLastError());
   return NEBW_OK;
@@ -577,11 +584,20 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   else if (c_dtype == NEBW_F32) epi = nebw::kGrpF32;
   else if (act == NEBW_ACT_GELU8) epi = nebw::kGrpBf16Gelu8;
   else if (act == NEBW_ACT_GELU_ERF) epi = nebw::kGrpBf16Erf;
-  CUtensorMap mA;
-  if (int rc = make_tmap_kmajor(&mA, A, a_rows, K, row_src ? 1 : nebw::kGemmBM)) return rc;
+  CUtensorMap mA, mC;
+  if (int rc = make_tmap_kmajor(&mA, A, a_rows, K, row_src ? 1 : nebw::kGroupedBox)) return rc;
+  if (int rc = make_tmap_out(&mC, C, rows, w.gated ? N / 2 : N, c_dtype == NEBW_BF16)) return rc;
   const cudaStream_t st = pick_stream(d, stream);
-  if (N % 256 == 0) return launch_grouped<256>(d, mA, w.map256, epi, a, st);
-  return launch_grouped<128>(d, mA, w.map128, epi, a, st);
+  const int64_t groups = std::min<int64_t>(w.experts, rows);
+  if (d->gemm_pairs > 0 && rows >= 384 * groups && N >= 256) {
+    a.bn = 256;
+    return launch_grouped<2>(d, mA, w.map128, mC, epi, a, st);
+  }
+  // one CTA a tile; narrower tiles while the groups' columns leave SMs idle
+  a.bn = 128;
+  const int least = w.gated ? 64 : 32;
+  while (a.bn > least && groups * ((N + a.bn - 1) / a.bn) < d->sm_count) a.bn /= 2;
+  return launch_grouped<1>(d, mA, w.map32, mC, epi, a, st);
 }
 
 namespace {

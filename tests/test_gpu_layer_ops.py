@@ -618,6 +618,9 @@ GROUP_CASES = [
     ([64, 17, 1, 0, 290, 3], 512, 1536),
     ([20, 31, 32, 33, 63, 64, 65, 96], 768, 768),
     ([3000, 1, 0, 1200], 256, 1024),
+    # several tiles a block, with part tiles among them: one CTA, and a pair
+    ([130, 3, 257, 1, 90, 128, 0, 200] * 10, 192, 1024),
+    ([2100, 1, 900, 513, 40, 2500] * 2, 192, 1536),
 ]
 EPILOGUES = [  # gated, act, output
     (False, 0, "bf16"), (False, 0, "f32"), (False, 1, "bf16"), (False, 2, "bf16"),
