@@ -20,8 +20,8 @@
 //   warps 2-9     epilogue: TMEM -> bias, activation -> shared memory -> TMA
 //                 store of 32 x 32 chunks; the chunk in which a group ends is
 //                 stored row by row
-//   warps 10-13   GATHER: A's rows, four at a time (tile::gather4), each warp
-//                 a quarter of the tile's rows with their indices in registers
+//   warps 10-17   GATHER: A's rows, four at a time (tile::gather4), each warp
+//                 a share of the tile's rows with their indices in registers
 // A gather is issued by one lane for uniform operands; from 32 lanes of one
 // warp the same 32 gathers take turns on the issue path (80 clocks each,
 // measured: 2457 us for 65,542 rows, K 1024, N 8192).  Rows past the group
@@ -76,9 +76,11 @@ struct GroupedShape {
   static constexpr int kSmemBytes =
       1024 + kStages * kStageBytes + kStagingBytes + kBarBytes + kTableBytes;
 };
-constexpr int kGroupedBox = 32;           // rows a TMA box of A or W
+constexpr int kGroupedBox = 32;  // rows of the TMA boxes that end a group of A
 constexpr int kGroupedThreads = 320;
-constexpr int kGroupedGatherThreads = 448;  // four more warps
+constexpr int kGatherWarps = 8;
+constexpr int kGatherRows = kGemmBM / kGatherWarps;
+constexpr int kGroupedGatherThreads = 320 + 32 * kGatherWarps;
 
 // A box of a K-major map into this CTA's shared memory, completing on the
 // barrier at `bar` (a shared::cluster address: the pair leader's).
@@ -286,6 +288,7 @@ template <int CTAS, int EPI, bool GATHER>
 __global__ void __cluster_dims__(CTAS, 1, 1)
     __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA,
+                        const __grid_constant__ CUtensorMap tmA128,
                         const __grid_constant__ CUtensorMap tmW,
                         const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
   using S = GroupedShape;
@@ -324,7 +327,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       // every gather warp arrives on every stage, also with no row to load:
       // one that did not could fall a phase behind the ring, whose parity
       // then reads the wrong way round
-      mbar_init(&full[s], 1 + (GATHER ? 4 * CTAS : 0));
+      mbar_init(&full[s], 1 + (GATHER ? kGatherWarps * CTAS : 0));
       mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
@@ -384,16 +387,15 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
           }
           if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
           const uint32_t bar = leader_bar(&full[stage]);
-          if constexpr (CTAS == 2) {
-            grp_load<CTAS>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
+          grp_load<CTAS>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
+          if (a_boxes == kGemmBM / kGroupedBox) {
+            grp_load<CTAS>(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK,
+                           t.row + rank * kGemmBM);
           } else {
-            for (int i = 0; i < bn / kGroupedBox; ++i)
-              grp_load<CTAS>(sW + stage * S::kABytes + i * kGroupedBox * 128, &tmW, bar,
-                             kb * kGemmBK, w_row + i * kGroupedBox);
+            for (int i = 0; i < a_boxes; ++i)
+              grp_load<CTAS>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
+                             kb * kGemmBK, t.row + rank * kGemmBM + i * kGroupedBox);
           }
-          for (int i = 0; i < a_boxes; ++i)
-            grp_load<CTAS>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
-                           kb * kGemmBK, t.row + rank * kGemmBM + i * kGroupedBox);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
@@ -525,44 +527,46 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        if constexpr (CTAS == 2) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty[acc]), 0));
+        // (the fence orders the TMEM reads; a releasing arrive would also wait
+        // for this thread's outstanding global accesses)
+        if constexpr (CTAS == 2) grp_arrive(map_to_cta(smem_u32(&tempty[acc]), 0));
         else mbar_arrive(&tempty[acc]);
       }
     }
     if (lane == 0) bulk_wait_group_all();
   } else if constexpr (GATHER) {
-    // ---------------- A by gathers (warps 10..13) ----------------
-    const int part = warp - 10;  // rows [32 * part, +32) of this CTA's 128
+    // ---------------- A by gathers (warps 10..17) ----------------
+    const int part = warp - 10;  // a share of this CTA's 128 rows
     const bool elect = elect_one_sync();
     int stage = 0, e = 0;
     uint32_t phase = 0;
     bool ok = true;
     for (int tile = first; tile < num_tiles && ok; tile += step) {
       const GroupTile t = group_tile(table, tile, kTileM, n_blocks, e);
-      const int count = min(max(cta_rows(t, rank) - 32 * part, 0), 32);
+      const int count = min(max(cta_rows(t, rank) - kGatherRows * part, 0), kGatherRows);
       int mine = 0;
       if (count > 0) {
         // past the group: its last row again, to fill a gather of four
-        const int at = t.row + rank * kGemmBM + 32 * part + min(lane, count - 1);
+        const int at = t.row + rank * kGemmBM + kGatherRows * part + min(lane, count - 1);
         mine = __ldg(p.row_src + at);
         if (mine < 0 || mine >= p.a_rows) {
           record_err(p.err, kDevBadGroup);
           mine = 0;
         }
       }
-      int src[32];
+      int src[kGatherRows];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) src[i] = __shfl_sync(0xffffffffu, mine, i);
+      for (int i = 0; i < kGatherRows; ++i) src[i] = __shfl_sync(0xffffffffu, mine, i);
       for (int kb = 0; kb < num_kb; ++kb) {
         if (!wait_all(&empty[stage], phase ^ 1u)) {
           ok = false;
           break;
         }
         if (elect) {
-          const uint32_t dst = smem_u32(sA + stage * S::kABytes) + part * 4096;
+          const uint32_t dst = smem_u32(sA + stage * S::kABytes) + part * (kGatherRows * 128);
           const uint32_t bar = leader_bar(&full[stage]);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < kGatherRows / 4; ++i)
             if (4 * i < count)
               grp_gather4<CTAS>(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
                                 src[4 * i + 2], src[4 * i + 3]);

@@ -165,72 +165,69 @@ __global__ void __launch_bounds__(256) heads_any_kernel(const HeadArgs p) {
 // shuffles of the 2^lg lanes that share a head.  A warp takes 32 / 2^lg heads
 // of one side of one row at a time, IT times: the table entries and the
 // norm's weights are read once for all of them, and all loads are issued
-// before the first is used.
+// before the first is used.  The arithmetic is packed, two values an
+// instruction, which keeps the issue slots below half of what the bytes take.
 template <typename T>
 struct HeadVec;
 template <>
 struct HeadVec<__nv_bfloat16> {
   static constexpr int V = 8;
-  static __device__ __forceinline__ void unpack(const uint4 &u, float (&f)[8]) {
+  static __device__ __forceinline__ void unpack(const uint4 &u, uint64_t (&f)[4]) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+    for (int i = 0; i < 4; ++i)
+      f[i] = pk2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
-  static __device__ __forceinline__ uint4 pack(const float (&f)[8]) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                      pack_bf16x2(f[6], f[7]));
+  static __device__ __forceinline__ uint32_t pack1(uint64_t f) {
+    float a, b;
+    unpk2(f, a, b);
+    return pack_bf16x2(a, b);
+  }
+  static __device__ __forceinline__ uint4 pack(const uint64_t (&f)[4]) {
+    return make_uint4(pack1(f[0]), pack1(f[1]), pack1(f[2]), pack1(f[3]));
   }
 };
 template <>
 struct HeadVec<float> {
   static constexpr int V = 4;
-  static __device__ __forceinline__ void unpack(const uint4 &u, float (&f)[4]) {
-    f[0] = __uint_as_float(u.x);
-    f[1] = __uint_as_float(u.y);
-    f[2] = __uint_as_float(u.z);
-    f[3] = __uint_as_float(u.w);
+  static __device__ __forceinline__ void unpack(const uint4 &u, uint64_t (&f)[2]) {
+    f[0] = pk2(__uint_as_float(u.x), __uint_as_float(u.y));
+    f[1] = pk2(__uint_as_float(u.z), __uint_as_float(u.w));
   }
-  static __device__ __forceinline__ uint4 pack(const float (&f)[4]) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                      __float_as_uint(f[3]));
+  static __device__ __forceinline__ uint4 pack(const uint64_t (&f)[2]) {
+    float a, b, c, d;
+    unpk2(f[0], a, b);
+    unpk2(f[1], c, d);
+    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c),
+                      __float_as_uint(d));
   }
 };
 
-template <int V>
-__device__ __forceinline__ void head_weights(const float *w, float (&f)[V]) {
+template <int P>
+__device__ __forceinline__ void head_weights(const float *w, uint64_t (&f)[P]) {
 #pragma unroll
-  for (int i = 0; i < V; i += 4) {
-    const float4 x = __ldg(reinterpret_cast<const float4 *>(w + i));
-    f[i] = x.x;
-    f[i + 1] = x.y;
-    f[i + 2] = x.z;
-    f[i + 3] = x.w;
+  for (int i = 0; i < P; i += 2) {
+    const float4 x = __ldg(reinterpret_cast<const float4 *>(w + 2 * i));
+    f[i] = pk2(x.x, x.y);
+    f[i + 1] = pk2(x.z, x.w);
   }
 }
 
 template <typename T, int NORM, bool PAIRS, int IT>
 __global__ void __launch_bounds__(256)
-    heads_vec_kernel(const HeadArgs p, int lg, int q_chunks, int chunks) {
-  constexpr int V = HeadVec<T>::V;
+    heads_vec_kernel(const HeadArgs p, int lg, int q_chunks, float inv_dim) {
+  constexpr int V = HeadVec<T>::V, P = V / 2;
   const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t row = item / chunks;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   int64_t rows = p.rows;
   if (p.rows_dev) rows = min(rows, static_cast<int64_t>(max(0, __ldg(p.rows_dev))));
   if (row >= rows) return;
-  int chunk = static_cast<int>(item - row * chunks);
-  const bool key = chunk >= q_chunks;
-  if (key) chunk -= q_chunks;
+  const bool key = static_cast<int>(blockIdx.y) >= q_chunks;
+  const int chunk = key ? blockIdx.y - q_chunks : blockIdx.y;
   const T *x = static_cast<const T *>(key ? p.k.x : p.q.x);
   T *out = static_cast<T *>(key ? p.k.out : p.q.out);
   const int heads = key ? p.k.heads : p.q.heads;
   const bool in_place = x == out;
-  x += row * (key ? p.k.stride : p.q.stride);
-  out += row * (key ? p.k.out_stride : p.q.out_stride);
-
   const int per = 32 >> lg, slot = lane & ((1 << lg) - 1);
   const int head0 = chunk * IT * per + (lane >> lg);
   const bool turn = slot * V < p.n;
@@ -239,102 +236,124 @@ __global__ void __launch_bounds__(256)
   if (NORM == kHeadNormNone && in_place) live = live && turn;
   const int e0 = turn && !PAIRS ? slot * V : slot * 2 * V;
   const int e1 = turn && !PAIRS ? p.n + slot * V : e0 + V;
+  x += row * (key ? p.k.stride : p.q.stride) + head0 * p.head_dim;
+  out += row * (key ? p.k.out_stride : p.q.out_stride) + head0 * p.head_dim;
+  const int hop = per * p.head_dim;  // elements between a lane's heads
 
   uint4 ua[IT], ub[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    const int h = head0 + i * per;
     ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
-    if (live && h < heads) {
-      ua[i] = *reinterpret_cast<const uint4 *>(x + h * p.head_dim + e0);
-      ub[i] = *reinterpret_cast<const uint4 *>(x + h * p.head_dim + e1);
+    if (live && head0 + i * per < heads) {
+      ua[i] = *reinterpret_cast<const uint4 *>(x + i * hop + e0);
+      ub[i] = *reinterpret_cast<const uint4 *>(x + i * hop + e1);
     }
   }
-  float c[V], s[V];  // of the thread's pairs
+  // cos and sin of the thread's pairs: two pairs a packed value (half), or
+  // one at a time (pairs)
+  uint64_t c2[P], s2[P];
   if (turn) {
     const float4 *t =
         reinterpret_cast<const float4 *>(p.table + head_position(p, row) * p.n + slot * V);
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
+    for (int i = 0; i < P; ++i) {
       const float4 v = __ldg(t + i);
-      c[2 * i] = v.x;
-      s[2 * i] = v.y;
-      c[2 * i + 1] = v.z;
-      s[2 * i + 1] = v.w;
+      c2[i] = pk2(v.x, v.z);
+      s2[i] = pk2(v.y, v.w);
     }
   }
-  float ga[V], gb[V], ba[V], bb[V];
+  uint64_t ga[P], gb[P], ba[P], bb[P];
   if constexpr (NORM != kHeadNormNone) {
     if (live) {
       const float *g = key ? p.k.gamma : p.q.gamma;
-      head_weights<V>(g + e0, ga);
-      head_weights<V>(g + e1, gb);
+      head_weights<P>(g + e0, ga);
+      head_weights<P>(g + e1, gb);
       if constexpr (NORM == kHeadNormLayer) {
         const float *b = key ? p.k.beta : p.q.beta;
-        head_weights<V>(b + e0, ba);
-        head_weights<V>(b + e1, bb);
+        head_weights<P>(b + e0, ba);
+        head_weights<P>(b + e1, bb);
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    float a[V], b[V];
+    uint64_t a[P], b[P];
     HeadVec<T>::unpack(ua[i], a);
     HeadVec<T>::unpack(ub[i], b);
     if constexpr (NORM != kHeadNormNone) {
-      float mean = 0.f;
       if constexpr (NORM == kHeadNormLayer) {
+        uint64_t m2 = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) mean += a[v] + b[v];
+        for (int v = 0; v < P; ++v) m2 = add_x2(m2, add_x2(a[v], b[v]));
+        float mean, m1;
+        unpk2(m2, mean, m1);
+        mean += m1;
         for (int o = 1; o < 1 << lg; o <<= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
-        mean /= static_cast<float>(p.head_dim);
-      }
-      float q = 0.f;
-      if (live) {
+        mean *= -inv_dim;
+        const uint64_t n2 = live ? pk2(mean, mean) : 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          a[v] -= mean;
-          b[v] -= mean;
-          q = fmaf(a[v], a[v], q);
-          q = fmaf(b[v], b[v], q);
+        for (int v = 0; v < P; ++v) {
+          a[v] = add_x2(a[v], n2);
+          b[v] = add_x2(b[v], n2);
         }
       }
-      for (int o = 1; o < 1 << lg; o <<= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
-      const float is = 1.0f / sqrtf(q / static_cast<float>(p.head_dim) + p.eps);
+      uint64_t q2 = 0;
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
+      for (int v = 0; v < P; ++v) {
+        q2 = fma_x2(a[v], a[v], q2);
+        q2 = fma_x2(b[v], b[v], q2);
+      }
+      float q, q1;
+      unpk2(q2, q, q1);
+      q += q1;
+      for (int o = 1; o < 1 << lg; o <<= 1) q += __shfl_xor_sync(0xffffffffu, q, o);
+      const float is = rsqrtf(fmaf(q, inv_dim, p.eps));
+      const uint64_t is2 = pk2(is, is);
+#pragma unroll
+      for (int v = 0; v < P; ++v) {
+        a[v] = mul_x2(a[v], is2);
+        b[v] = mul_x2(b[v], is2);
         if constexpr (NORM == kHeadNormLayer) {
-          a[v] = fmaf(a[v] * is, ga[v], ba[v]);
-          b[v] = fmaf(b[v] * is, gb[v], bb[v]);
+          a[v] = fma_x2(a[v], ga[v], ba[v]);
+          b[v] = fma_x2(b[v], gb[v], bb[v]);
         } else {
-          a[v] = a[v] * is * ga[v];
-          b[v] = b[v] * is * gb[v];
+          a[v] = mul_x2(a[v], ga[v]);
+          b[v] = mul_x2(b[v], gb[v]);
         }
       }
     }
     if (turn) {
       if constexpr (PAIRS) {
+        // a[v] and b[v] are a pair each; the table entries of pair v of a are
+        // half v % 2 of entry v / 2, those of b follow
 #pragma unroll
-        for (int v = 0; v < V; v += 2) {
-          const float a0 = a[v], b0 = b[v];
-          a[v] = fmaf(-a[v + 1], s[v / 2], a0 * c[v / 2]);
-          a[v + 1] = fmaf(a0, s[v / 2], a[v + 1] * c[v / 2]);
-          b[v] = fmaf(-b[v + 1], s[(V + v) / 2], b0 * c[(V + v) / 2]);
-          b[v + 1] = fmaf(b0, s[(V + v) / 2], b[v + 1] * c[(V + v) / 2]);
+        for (int v = 0; v < P; ++v) {
+          float ca, cb, sa, sb, lo, hi, x0, x1;
+          unpk2(c2[v / 2], lo, hi);
+          ca = v & 1 ? hi : lo;
+          unpk2(s2[v / 2], lo, hi);
+          sa = v & 1 ? hi : lo;
+          unpk2(c2[(P + v) / 2], lo, hi);
+          cb = v & 1 ? hi : lo;
+          unpk2(s2[(P + v) / 2], lo, hi);
+          sb = v & 1 ? hi : lo;
+          unpk2(a[v], x0, x1);
+          a[v] = pk2(fmaf(-x1, sa, x0 * ca), fmaf(x0, sa, x1 * ca));
+          unpk2(b[v], x0, x1);
+          b[v] = pk2(fmaf(-x1, sb, x0 * cb), fmaf(x0, sb, x1 * cb));
         }
       } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-          const float a0 = a[v];
-          a[v] = fmaf(-b[v], s[v], a0 * c[v]);
-          b[v] = fmaf(a0, s[v], b[v] * c[v]);
+        for (int v = 0; v < P; ++v) {
+          const uint64_t a0 = a[v], ns = s2[v] ^ 0x8000000080000000ull;
+          a[v] = fma_x2(b[v], ns, mul_x2(a0, c2[v]));
+          b[v] = fma_x2(a0, s2[v], mul_x2(b[v], c2[v]));
         }
       }
     }
-    const int h = head0 + i * per;
-    if (live && h < heads) {
-      *reinterpret_cast<uint4 *>(out + h * p.head_dim + e0) = HeadVec<T>::pack(a);
-      *reinterpret_cast<uint4 *>(out + h * p.head_dim + e1) = HeadVec<T>::pack(b);
+    if (live && head0 + i * per < heads) {
+      *reinterpret_cast<uint4 *>(out + i * hop + e0) = HeadVec<T>::pack(a);
+      *reinterpret_cast<uint4 *>(out + i * hop + e1) = HeadVec<T>::pack(b);
     }
   }
 }

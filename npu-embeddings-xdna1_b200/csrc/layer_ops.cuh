@@ -38,7 +38,25 @@ int set_grouped_attrs_ctas() {
   return set_grouped_attr<CTAS, nebw::kGrpBf16GeGLU>();
 }
 
+constexpr int kRouteSmem =
+    (nebw::kRouteWarps + 2) * nebw::kRouteMaxExperts * static_cast<int>(sizeof(int));
+
+template <typename T>
+int set_route_attrs() {
+  const auto a = cudaFuncAttributeMaxDynamicSharedMemorySize;
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 1>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 2>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 4>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 8>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 16>, a, kRouteSmem));
+  return NEBW_OK;
+}
+
 int set_layer_op_attrs() {
+  if (int rc = set_route_attrs<float>()) return rc;
+  if (int rc = set_route_attrs<__nv_bfloat16>()) return rc;
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_place_kernel,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteSmem));
   if (int rc = set_grouped_attrs_ctas<1>()) return rc;
   return set_grouped_attrs_ctas<2>();
 }
@@ -191,9 +209,12 @@ int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t
 }
 
 template <typename T, int NORM, bool PAIRS, int IT>
-void launch_heads_vec(const nebw::HeadArgs &a, int lg, unsigned blocks, int q_chunks, int chunks,
-                      cudaStream_t st) {
-  nebw::heads_vec_kernel<T, NORM, PAIRS, IT><<<blocks, 256, 0, st>>>(a, lg, q_chunks, chunks);
+void launch_heads_vec(const nebw::HeadArgs &a, int lg, int per, cudaStream_t st) {
+  const int q_chunks = (a.q.heads + per * IT - 1) / (per * IT);
+  const int chunks = q_chunks + (a.k.heads + per * IT - 1) / (per * IT);
+  const dim3 grid(static_cast<unsigned>((a.rows + 7) / 8), chunks);
+  nebw::heads_vec_kernel<T, NORM, PAIRS, IT>
+      <<<grid, 256, 0, st>>>(a, lg, q_chunks, 1.0f / static_cast<float>(a.head_dim));
 }
 
 bool heads_vec_side(const nebw::HeadSide &s, size_t esz) {
@@ -210,16 +231,11 @@ int launch_heads(const nebw::HeadArgs &a, cudaStream_t st) {
     while ((2 * V << lg) < a.head_dim) ++lg;
     const int per = 32 >> lg;  // heads a warp takes at once
     const int most = std::max(a.q.heads, a.k.heads);
-    const int it = most > 2 * per ? 4 : most > per ? 2 : 1;
-    const int q_chunks = (a.q.heads + per * it - 1) / (per * it);
-    const int chunks = q_chunks + (a.k.heads + per * it - 1) / (per * it);
-    const int64_t blocks = (a.rows * chunks + 7) / 8;
-    NEBW_REQUIRE(blocks < (1ll << 31), "too many heads: %lld rows of %d",
-                 static_cast<long long>(a.rows), a.q.heads + a.k.heads);
-    const unsigned g = static_cast<unsigned>(blocks);
-    if (it == 4) launch_heads_vec<T, NORM, PAIRS, 4>(a, lg, g, q_chunks, chunks, st);
-    else if (it == 2) launch_heads_vec<T, NORM, PAIRS, 2>(a, lg, g, q_chunks, chunks, st);
-    else launch_heads_vec<T, NORM, PAIRS, 1>(a, lg, g, q_chunks, chunks, st);
+    static const int kIt = std::getenv("HD_IT") ? std::atoi(std::getenv("HD_IT")) : 4;
+    const int it = std::min(kIt, most > 2 * per ? 4 : most > per ? 2 : 1);
+    if (it == 4) launch_heads_vec<T, NORM, PAIRS, 4>(a, lg, per, st);
+    else if (it == 2) launch_heads_vec<T, NORM, PAIRS, 2>(a, lg, per, st);
+    else launch_heads_vec<T, NORM, PAIRS, 1>(a, lg, per, st);
     NEBW_CUDA(cudaGetLastError());
     return NEBW_OK;
   }
@@ -334,9 +350,13 @@ int check_route(int64_t rows, int32_t experts, int32_t top_k) {
   return NEBW_OK;
 }
 
+size_t route_smem(int experts) {
+  return (nebw::kRouteWarps + 2) * static_cast<size_t>(experts) * sizeof(int);
+}
+
 template <typename T, int K>
 int launch_route(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
-  const size_t smem = (nebw::kRouteWarps + 2) * static_cast<size_t>(a.experts) * sizeof(int);
+  const size_t smem = route_smem(a.experts);
   if (blocks == 1) {
     nebw::route_fused_kernel<T, K><<<1, nebw::kRouteThreads, smem, st>>>(a);
   } else {
@@ -475,7 +495,8 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   if (e != cudaSuccess)
     rc = set_error(NEBW_ECUDA, "expert weight staging failed: %s", cudaGetErrorString(e));
   if (!rc) rc = make_tmap_kmajor(&w.map128, w.ptr, experts * N, K, 128);
-  if (!rc) rc = make_tmap_kmajor(&w.map32, w.ptr, experts * N, K, nebw::kGroupedBox);
+  if (!rc) rc = make_tmap_kmajor(&w.map64, w.ptr, experts * N, K, 64);
+  if (!rc) rc = make_tmap_kmajor(&w.map32, w.ptr, experts * N, K, 32);
   if (!rc) {
     try {
       d->experts[d->next_handle] = w;
@@ -494,15 +515,16 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
 namespace {
 
 template <int CTAS, int EPI>
-void launch_grouped_epi(const CUtensorMap &mA, const CUtensorMap &mW, const CUtensorMap &mC,
-                        const nebw::GroupedArgs &a, unsigned grid, cudaStream_t st) {
+void launch_grouped_epi(const CUtensorMap &mA, const CUtensorMap &mA128, const CUtensorMap &mW,
+                        const CUtensorMap &mC, const nebw::GroupedArgs &a, unsigned grid,
+                        cudaStream_t st) {
   const size_t smem = nebw::GroupedShape::kSmemBytes;
   if (a.row_src)
     nebw::gemm_grouped_kernel<CTAS, EPI, true>
-        <<<grid, nebw::kGroupedGatherThreads, smem, st>>>(mA, mW, mC, a);
+        <<<grid, nebw::kGroupedGatherThreads, smem, st>>>(mA, mA128, mW, mC, a);
   else
     nebw::gemm_grouped_kernel<CTAS, EPI, false>
-        <<<grid, nebw::kGroupedThreads, smem, st>>>(mA, mW, mC, a);
+        <<<grid, nebw::kGroupedThreads, smem, st>>>(mA, mA128, mW, mC, a);
 }
 
 // The most tiles that groups of `rows` rows in all can make: every group may
@@ -512,20 +534,20 @@ int64_t grouped_tiles(int64_t rows, int64_t experts, int64_t tile_rows, int64_t 
 }
 
 template <int CTAS>
-int launch_grouped(nebw_dev *d, const CUtensorMap &mA, const CUtensorMap &mW,
-                   const CUtensorMap &mC, int epi, const nebw::GroupedArgs &a, cudaStream_t st) {
+int launch_grouped(nebw_dev *d, const CUtensorMap &mA, const CUtensorMap &mA128,
+                   const CUtensorMap &mW, const CUtensorMap &mC, int epi, const nebw::GroupedArgs &a, cudaStream_t st) {
   const int64_t tiles = grouped_tiles(a.rows, a.experts, CTAS * nebw::kGemmBM,
                                       (a.N + a.bn - 1) / a.bn);
   NEBW_REQUIRE(tiles < (1ll << 31), "grouped product too large");
   const unsigned g = static_cast<unsigned>(
       CTAS * std::min<int64_t>(tiles, CTAS == 2 ? d->gemm_pairs : d->sm_count));
   switch (epi) {
-    case nebw::kGrpBf16: launch_grouped_epi<CTAS, nebw::kGrpBf16>(mA, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16Gelu8: launch_grouped_epi<CTAS, nebw::kGrpBf16Gelu8>(mA, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16Erf: launch_grouped_epi<CTAS, nebw::kGrpBf16Erf>(mA, mW, mC, a, g, st); break;
-    case nebw::kGrpF32: launch_grouped_epi<CTAS, nebw::kGrpF32>(mA, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16SwiGLU>(mA, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16GeGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16GeGLU>(mA, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16: launch_grouped_epi<CTAS, nebw::kGrpBf16>(mA, mA128, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16Gelu8: launch_grouped_epi<CTAS, nebw::kGrpBf16Gelu8>(mA, mA128, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16Erf: launch_grouped_epi<CTAS, nebw::kGrpBf16Erf>(mA, mA128, mW, mC, a, g, st); break;
+    case nebw::kGrpF32: launch_grouped_epi<CTAS, nebw::kGrpF32>(mA, mA128, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16SwiGLU>(mA, mA128, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16GeGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16GeGLU>(mA, mA128, mW, mC, a, g, st); break;
   }
   NEBW_CUDA(cudaGetLastError());
   return NEBW_OK;
@@ -584,33 +606,41 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   else if (c_dtype == NEBW_F32) epi = nebw::kGrpF32;
   else if (act == NEBW_ACT_GELU8) epi = nebw::kGrpBf16Gelu8;
   else if (act == NEBW_ACT_GELU_ERF) epi = nebw::kGrpBf16Erf;
-  CUtensorMap mA, mC;
+  CUtensorMap mA, mA128, mC;
   if (int rc = make_tmap_kmajor(&mA, A, a_rows, K, row_src ? 1 : nebw::kGroupedBox)) return rc;
+  if (row_src) mA128 = mA;  // not used
+  else if (int rc = make_tmap_kmajor(&mA128, A, a_rows, K, nebw::kGemmBM)) return rc;
   if (int rc = make_tmap_out(&mC, C, rows, w.gated ? N / 2 : N, c_dtype == NEBW_BF16)) return rc;
   const cudaStream_t st = pick_stream(d, stream);
   const int64_t groups = std::min<int64_t>(w.experts, rows);
-  if (d->gemm_pairs > 0 && rows >= 384 * groups && N >= 256) {
+  static const int kThr = std::getenv("GRP_THR") ? std::atoi(std::getenv("GRP_THR")) : 384;
+  if (d->gemm_pairs > 0 && rows >= kThr * groups && N >= 256) {
     a.bn = 256;
-    return launch_grouped<2>(d, mA, w.map128, mC, epi, a, st);
+    return launch_grouped<2>(d, mA, mA128, w.map128, mC, epi, a, st);
   }
   // one CTA a tile; narrower tiles while the groups' columns leave SMs idle
   a.bn = 128;
   const int least = w.gated ? 64 : 32;
   while (a.bn > least && groups * ((N + a.bn - 1) / a.bn) < d->sm_count) a.bn /= 2;
-  return launch_grouped<1>(d, mA, w.map32, mC, epi, a, st);
+  const CUtensorMap &mW = a.bn == 128 ? w.map128 : a.bn == 64 ? w.map64 : w.map32;
+  return launch_grouped<1>(d, mA, mA128, mW, mC, epi, a, st);
 }
 
 namespace {
 
 template <typename TY, typename TO>
 void launch_combine(const nebw::CombineArgs &a, bool vec, cudaStream_t st) {
-  const int cols = vec ? a.H / 8 : a.H;  // threads a row would take
-  int tx = 32;
-  while (tx < cols && tx < 256) tx <<= 1;
-  const dim3 b(tx, 256 / tx);
-  const unsigned g = static_cast<unsigned>((a.rows + b.y - 1) / b.y);
-  if (vec) nebw::moe_combine_kernel<TY, TO, 8><<<g, b, 0, st>>>(a);
-  else nebw::moe_combine_kernel<TY, TO, 1><<<g, b, 0, st>>>(a);
+  const int segments = (a.H + 255) / 256;
+  const int64_t items = static_cast<int64_t>(a.rows) * segments;
+  if (vec && items < (1ll << 31)) {
+    const unsigned g = static_cast<unsigned>((items + 7) / 8);
+    if (a.k > 4) nebw::moe_combine_kernel<TY, TO, 8><<<g, 256, 0, st>>>(a, segments);
+    else if (a.k > 2) nebw::moe_combine_kernel<TY, TO, 4><<<g, 256, 0, st>>>(a, segments);
+    else nebw::moe_combine_kernel<TY, TO, 2><<<g, 256, 0, st>>>(a, segments);
+  } else {
+    nebw::moe_combine_any_kernel<TY, TO>
+        <<<static_cast<unsigned>((static_cast<int64_t>(a.rows) + 7) / 8), 256, 0, st>>>(a);
+  }
 }
 
 }  // namespace

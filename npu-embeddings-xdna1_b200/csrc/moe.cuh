@@ -22,7 +22,7 @@
 
 namespace nebw {
 
-constexpr int kRouteThreads = 512;
+constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteMaxExperts = 512;
 constexpr int kRouteMaxK = 16;
@@ -127,11 +127,52 @@ __device__ __forceinline__ void route_order(Key &a, Key &b) {
   b = lo;
 }
 
+// The D stages of a bitonic merge over N elements: descending order from a
+// bitonic sequence.
+template <int N, typename Key>
+__device__ __forceinline__ void route_merge(Key (&k)[N]) {
+#pragma unroll
+  for (int d = N / 2; d > 0; d >>= 1) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if ((i & d) == 0) route_order(k[i], k[i + d]);
+  }
+}
+
+// Eight keys in descending order (Batcher's odd-even merge sort, 19
+// exchanges).
+template <typename Key>
+__device__ __forceinline__ void route_sort8(Key (&k)[8]) {
+  constexpr int kNet[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6},
+                               {5, 7}, {1, 2}, {5, 6}, {0, 4}, {1, 5}, {2, 6}, {3, 7},
+                               {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+#pragma unroll
+  for (int i = 0; i < 19; ++i) route_order(k[kNet[i][0]], k[kNet[i][1]]);
+}
+
+// Eight more keys into the ordered list of the K largest.  Up to four places
+// an insertion is the shortest; longer lists sort the eight first: the K
+// largest of two ordered lists are max(a[i], b[K - 1 - i]), a bitonic
+// sequence that a merge orders again (35 exchanges for K = 8 against 64).
+template <int K, typename Key>
+__device__ __forceinline__ void route_add8(Key (&top)[K], Key (&k)[8]) {
+  if constexpr (K <= 4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int j = 0; j < K; ++j) route_order(top[j], k[i]);
+    }
+  } else {
+    route_sort8(k);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[K - 1 - i] = max(top[K - 1 - i], k[i]);
+    route_merge<K>(top);
+  }
+}
+
 // One row's choice by the 2^lg lanes that share it: each keeps the K largest
-// keys of its experts in order (insertion, unrolled and without a branch),
-// then lanes merge in pairs: the K largest of two ordered lists are max(a[i],
-// b[K - 1 - i]), which a bitonic pass orders again.  Every lane ends with the
-// row's list.
+// keys of its experts in order, then lanes merge in pairs.  Every lane ends
+// with the row's list.
 template <typename T, int K>
 __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int sub,
                                           typename RouteKey<T>::Key (&top)[K]) {
@@ -143,11 +184,7 @@ __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int su
   for (int e = sub * p.per; e < end; e += 8) {
     Key k[8];
     R::load8(l, e, p.experts, p.vec, k);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-#pragma unroll
-      for (int j = 0; j < K; ++j) route_order(top[j], k[i]);
-    }
+    route_add8<K>(top, k);
   }
   for (int o = 1; o < 1 << p.lg; o <<= 1) {
     Key other[K];
@@ -155,12 +192,7 @@ __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int su
     for (int i = 0; i < K; ++i) other[i] = __shfl_xor_sync(0xffffffffu, top[i], o);
 #pragma unroll
     for (int i = 0; i < K; ++i) top[i] = max(top[i], other[K - 1 - i]);
-#pragma unroll
-    for (int d = K / 2; d > 0; d >>= 1) {
-#pragma unroll
-      for (int i = 0; i < K; ++i)
-        if ((i & d) == 0) route_order(top[i], top[i + d]);
-    }
+    route_merge<K>(top);
   }
 }
 
@@ -236,11 +268,18 @@ __device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, 
   const int i0 = min(n, warp * run), i1 = min(n, i0 + run);
   const int *ids = p.ids + static_cast<int64_t>(r0) * p.k;
   int *mine = cnt + warp * E;
-  for (int i = i0; i < i1; i += 32) {
-    const int id = i + lane < i1 ? ids[i + lane] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
-    if (id >= 0 && (same & ((1u << lane) - 1)) == 0) mine[id] += __popc(same);
-    __syncwarp();
+  // (the ids of four groups are loaded together: the walk over a group
+  // waits for the counts of the one before, not for memory)
+  for (int ib = i0; ib < i1; ib += 128) {
+    int id[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) id[u] = ib + u * 32 + lane < i1 ? ids[ib + u * 32 + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const unsigned same = __match_any_sync(0xffffffffu, id[u]);
+      if (id[u] >= 0 && (same & ((1u << lane) - 1)) == 0) mine[id[u]] += __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < E; e += kRouteThreads) {
@@ -252,18 +291,24 @@ __device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, 
     }
   }
   __syncthreads();
-  for (int i = i0; i < i1; i += 32) {
-    const int id = i + lane < i1 ? ids[i + lane] : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
-    const unsigned below = same & ((1u << lane) - 1);
-    int place = -1;
-    if (id >= 0) place = mine[id] + __popc(below);
-    __syncwarp();
-    if (id >= 0 && below == 0) mine[id] += __popc(same);
-    __syncwarp();
-    if (i + lane < i1) {
-      p.row_dst[static_cast<int64_t>(r0) * p.k + i + lane] = place;
-      if (place >= 0) p.row_src[place] = r0 + (i + lane) / p.k;
+  for (int ib = i0; ib < i1; ib += 128) {
+    int id[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) id[u] = ib + u * 32 + lane < i1 ? ids[ib + u * 32 + lane] : -1;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = ib + u * 32 + lane;
+      const unsigned same = __match_any_sync(0xffffffffu, id[u]);
+      const unsigned below = same & ((1u << lane) - 1);
+      int place = -1;
+      if (id[u] >= 0) place = mine[id[u]] + __popc(below);
+      __syncwarp();
+      if (id[u] >= 0 && below == 0) mine[id[u]] += __popc(same);
+      __syncwarp();
+      if (i < i1) {
+        p.row_dst[static_cast<int64_t>(r0) * p.k + i] = place;
+        if (place >= 0) p.row_src[place] = r0 + i / p.k;
+      }
     }
   }
 }
@@ -360,9 +405,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_fused_kernel(const RouteA
 // out[t] = residual[t] + sum_j weights[t, j] * y[row_dst[t, j]], j ascending,
 // in fp32 with one rounding at the end; an entry without a place (row_dst
 // < 0) adds nothing and is not read.  HBM bounds it: k rows of y are read for
-// one written.  V = 8 columns a thread by 16-byte accesses (1 where the width
-// or an address does not allow them); the loads of four entries are issued
-// together.
+// one written.
 struct CombineArgs {
   const void *y;
   const int *row_dst;
@@ -376,94 +419,132 @@ struct CombineArgs {
   int *err;
 };
 
-template <int V>
-__device__ __forceinline__ void combine_load(const float *y, float (&f)[V]) {
-  if constexpr (V == 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4 *>(y));
-    const float4 b = __ldg(reinterpret_cast<const float4 *>(y) + 1);
-    f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
-    f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
-  } else {
-    f[0] = __ldg(y);
+// Eight columns of a row as they are stored, and their sum into acc.
+template <typename T>
+struct CombineVec;
+template <>
+struct CombineVec<__nv_bfloat16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const __nv_bfloat16 *y) {
+    u = __ldg(reinterpret_cast<const uint4 *>(y));
   }
-}
-template <int V>
-__device__ __forceinline__ void combine_load(const __nv_bfloat16 *y, float (&f)[V]) {
-  if constexpr (V == 8) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4 *>(y));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+  __device__ __forceinline__ void zero() { u = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void add(float w, float (&acc)[8]) const {
+    const uint32_t v[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      f[2 * i] = __uint_as_float(w[i] << 16);
-      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      acc[2 * i] = fmaf(w, __uint_as_float(v[i] << 16), acc[2 * i]);
+      acc[2 * i + 1] = fmaf(w, __uint_as_float(v[i] & 0xffff0000u), acc[2 * i + 1]);
     }
-  } else {
-    f[0] = __bfloat162float(*y);
+  }
+};
+template <>
+struct CombineVec<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float *y) {
+    a = __ldg(reinterpret_cast<const float4 *>(y));
+    b = __ldg(reinterpret_cast<const float4 *>(y) + 1);
+  }
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void add(float w, float (&acc)[8]) const {
+    const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+  }
+};
+
+// A row's places and weights, one entry a lane; entries without a place (or
+// with a bad one, which is reported) have place -1 and weight 0.
+__device__ __forceinline__ void combine_entries(const CombineArgs &p, int64_t row, int lane,
+                                                int &at, float &w) {
+  at = -1;
+  w = 0.f;
+  if (lane < p.k) {
+    at = __ldg(p.row_dst + row * p.k + lane);
+    w = __ldg(p.weights + row * p.k + lane);
+    if (at >= p.y_rows) {
+      record_err(p.err, kDevBadGroup);
+      at = -1;
+    }
+    if (at < 0) w = 0.f;
   }
 }
 
-template <typename TY, typename TO, int V>
-__global__ void __launch_bounds__(256) moe_combine_kernel(const CombineArgs p) {
-  const int row = blockIdx.x * blockDim.y + threadIdx.y;
+// A warp takes 256 columns of one row; the entries are read by as many lanes
+// at once, and the loads of up to BATCH rows of y are in flight together.
+template <typename TY, typename TO, int BATCH>
+__global__ void __launch_bounds__(256) moe_combine_kernel(const CombineArgs p, int segments) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int rows = p.rows_dev ? min(p.rows, max(0, __ldg(p.rows_dev))) : p.rows;
+  // items fit 32 bits where rows do not need more (checked by the caller)
+  const int row = static_cast<int>(static_cast<uint32_t>(item) / static_cast<uint32_t>(segments));
+  if (row >= rows) return;
+  const int c = (static_cast<int>(item) - row * segments) * 256 + lane * 8;
+  int at;
+  float w;
+  combine_entries(p, row, lane, at, w);
+  const bool live = c < p.H;
+  float acc[8];
+#pragma unroll
+  for (int v = 0; v < 8; ++v) acc[v] = 0.f;
+  for (int j0 = 0; j0 < p.k; j0 += BATCH) {
+    CombineVec<TY> f[BATCH];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int a = __shfl_sync(0xffffffffu, at, j0 + j);  // lanes from k on hold -1
+      f[j].zero();
+      if (live && a >= 0)
+        f[j].load(static_cast<const TY *>(p.y) + static_cast<int64_t>(a) * p.H + c);
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) f[j].add(__shfl_sync(0xffffffffu, w, j0 + j), acc);
+  }
+  if (!live) return;
+  const int64_t o = static_cast<int64_t>(row) * p.H + c;
+  if (p.residual) {  // not __ldg: residual may be out
+    const float4 *r4 = reinterpret_cast<const float4 *>(p.residual + o);
+    const float4 a = r4[0], b = r4[1];
+    acc[0] += a.x; acc[1] += a.y; acc[2] += a.z; acc[3] += a.w;
+    acc[4] += b.x; acc[5] += b.y; acc[6] += b.z; acc[7] += b.w;
+  }
+  if constexpr (sizeof(TO) == 4) {
+    float4 *out = reinterpret_cast<float4 *>(static_cast<float *>(p.out) + o);
+    out[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    out[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
+  } else {
+    *reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(p.out) + o) =
+        make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]),
+                   pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
+  }
+}
+
+// Any width and alignment, a column a lane.
+template <typename TY, typename TO>
+__global__ void __launch_bounds__(256) moe_combine_any_kernel(const CombineArgs p) {
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int rows = p.rows_dev ? min(p.rows, max(0, __ldg(p.rows_dev))) : p.rows;
   if (row >= rows) return;
-  const int *dst = p.row_dst + static_cast<int64_t>(row) * p.k;
-  const float *weights = p.weights + static_cast<int64_t>(row) * p.k;
-  for (int c = threadIdx.x * V; c < p.H; c += blockDim.x * V) {
-    const int64_t o = static_cast<int64_t>(row) * p.H + c;
-    float acc[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = 0.f;
-    for (int j0 = 0; j0 < p.k; j0 += 4) {
-      float f[4][V], w[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = j0 + j < p.k ? __ldg(dst + j0 + j) : -1;
-        w[j] = 0.f;
-#pragma unroll
-        for (int v = 0; v < V; ++v) f[j][v] = 0.f;
-        if (at >= p.y_rows) {
-          record_err(p.err, kDevBadGroup);
-        } else if (at >= 0) {
-          w[j] = __ldg(weights + j0 + j);
-          combine_load<V>(static_cast<const TY *>(p.y) + static_cast<int64_t>(at) * p.H + c, f[j]);
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = fmaf(w[j], f[j][v], acc[v]);
-      }
+  int at;
+  float w;
+  combine_entries(p, row, lane, at, w);
+  for (int c0 = 0; c0 < p.H; c0 += 32) {
+    const int c = c0 + lane;
+    float acc = 0.f;
+    for (int j = 0; j < p.k; ++j) {
+      const int a = __shfl_sync(0xffffffffu, at, j);
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      if (a < 0 || c >= p.H) continue;
+      const TY *y = static_cast<const TY *>(p.y) + static_cast<int64_t>(a) * p.H + c;
+      if constexpr (sizeof(TY) == 4) acc = fmaf(wj, *y, acc);
+      else acc = fmaf(wj, __bfloat162float(*y), acc);
     }
-    if (p.residual) {
-      float r[V];
-      if constexpr (V == 8) {  // not __ldg: residual may be out
-        const float4 *r4 = reinterpret_cast<const float4 *>(p.residual + o);
-        const float4 a = r4[0], b = r4[1];
-        r[0] = a.x; r[1] = a.y; r[2] = a.z; r[3] = a.w;
-        r[4] = b.x; r[5] = b.y; r[6] = b.z; r[7] = b.w;
-      } else {
-        r[0] = p.residual[o];
-      }
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] += r[v];
-    }
-    if constexpr (sizeof(TO) == 4) {
-      float *out = static_cast<float *>(p.out) + o;
-      if constexpr (V == 8) {
-        reinterpret_cast<float4 *>(out)[0] = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        reinterpret_cast<float4 *>(out)[1] = make_float4(acc[4], acc[5], acc[6], acc[7]);
-      } else {
-        *out = acc[0];
-      }
-    } else {
-      __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.out) + o;
-      if constexpr (V == 8)
-        *reinterpret_cast<uint4 *>(out) =
-            make_uint4(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]),
-                       pack_bf16x2(acc[4], acc[5]), pack_bf16x2(acc[6], acc[7]));
-      else
-        *out = __float2bfloat16_rn(acc[0]);
+    if (c < p.H) {
+      const int64_t o = static_cast<int64_t>(row) * p.H + c;
+      if (p.residual) acc += p.residual[o];
+      if constexpr (sizeof(TO) == 4) static_cast<float *>(p.out)[o] = acc;
+      else static_cast<__nv_bfloat16 *>(p.out)[o] = __float2bfloat16_rn(acc);
     }
   }
 }

@@ -231,7 +231,7 @@ struct Experts {
   int experts = 0;
   int64_t K = 0, N = 0;
   bool gated = false;
-  CUtensorMap map32, map128;  // [experts * N, K], box rows 32 / 128
+  CUtensorMap map32, map64, map128;  // [experts * N, K], box rows 32 / 64 / 128
 };
 
 // cos and sin of every position and frequency (nebw_stage_rope).
