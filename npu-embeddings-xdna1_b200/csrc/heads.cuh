@@ -64,8 +64,8 @@ __global__ void __launch_bounds__(256)
   table[i] = make_float2(static_cast<float>(c * scale), static_cast<float>(s * scale));
 }
 
-__device__ __forceinline__ int64_t head_position(const HeadArgs &p, int64_t row) {
-  int64_t at = p.pos[row];
+// The table row of position `at`.
+__device__ __forceinline__ int64_t head_position(const HeadArgs &p, int64_t at) {
   if (at < 0 || at >= p.max_pos) {  // reported; a valid entry is read instead
     record_err(p.err, kDevBadPosition);
     at = at < 0 ? 0 : p.max_pos - 1;
@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(256) heads_any_kernel(const HeadArgs p) {
   const int64_t hh = key ? h - p.q.heads : h;
   const T *x = static_cast<const T *>(side.x) + row * side.stride + hh * p.head_dim;
   T *out = static_cast<T *>(side.out) + row * side.out_stride + hh * p.head_dim;
-  const float2 *cs = p.n ? p.table + head_position(p, row) * p.n : nullptr;
+  const float2 *cs = p.n ? p.table + head_position(p, p.pos[row]) * p.n : nullptr;
   constexpr int kMax = kHeadMaxDim / 64;  // pairs a lane
   const int half = p.head_dim / 2;
   float a[kMax], b[kMax];
@@ -213,8 +213,14 @@ __device__ __forceinline__ void head_weights(const float *w, uint64_t (&f)[P]) {
   }
 }
 
+// Blocks an SM must hold, which bounds the registers.  Measured (us, at 4 / 3 /
+// 2 blocks; 49,999 rows of 16 + 16 heads of 128, bf16): no norm 132 / 131 /
+// 157 (and 83 / 92 / 92 for 65,539 rows of 32 heads of 64, pairs, a quarter
+// of the work), RMS 188 / 144 / 156, LayerNorm 270 / 224 / 178.
+constexpr int head_blocks(int norm) { return norm == kHeadNormNone ? 4 : norm == kHeadNormRms ? 3 : 2; }
+
 template <typename T, int NORM, bool PAIRS, int IT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, head_blocks(NORM))
     heads_vec_kernel(const HeadArgs p, int lg, int q_chunks, float inv_dim) {
   constexpr int V = HeadVec<T>::V, P = V / 2;
   const int lane = threadIdx.x & 31;
@@ -240,6 +246,7 @@ __global__ void __launch_bounds__(256)
   out += row * (key ? p.k.out_stride : p.q.out_stride) + head0 * p.head_dim;
   const int hop = per * p.head_dim;  // elements between a lane's heads
 
+  const int pos = turn ? __ldg(p.pos + row) : 0;  // looked at once the rows are on their way
   uint4 ua[IT], ub[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
@@ -254,7 +261,7 @@ __global__ void __launch_bounds__(256)
   uint64_t c2[P], s2[P];
   if (turn) {
     const float4 *t =
-        reinterpret_cast<const float4 *>(p.table + head_position(p, row) * p.n + slot * V);
+        reinterpret_cast<const float4 *>(p.table + head_position(p, pos) * p.n + slot * V);
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const float4 v = __ldg(t + i);

@@ -38,8 +38,17 @@ int set_grouped_attrs_ctas() {
   return set_grouped_attr<CTAS, nebw::kGrpBf16GeGLU>();
 }
 
-constexpr int kRouteSmem =
-    (nebw::kRouteWarps + 2) * nebw::kRouteMaxExperts * static_cast<int>(sizeof(int));
+// Shared memory of the placing kernels: starts and totals, and the row masks
+// and counts of as many tiles of 32 rows as fit beside them (one a warp at
+// most).
+constexpr int kRouteSmem = 100 * 1024;
+int route_tiles(int experts) {
+  const int fit = (kRouteSmem / (experts * static_cast<int>(sizeof(int))) - 2) / 2;
+  return std::min(fit, nebw::kRouteWarps);
+}
+size_t route_smem(int experts) {
+  return (2 + 2 * static_cast<size_t>(route_tiles(experts))) * experts * sizeof(int);
+}
 
 template <typename T>
 int set_route_attrs() {
@@ -231,8 +240,9 @@ int launch_heads(const nebw::HeadArgs &a, cudaStream_t st) {
     while ((2 * V << lg) < a.head_dim) ++lg;
     const int per = 32 >> lg;  // heads a warp takes at once
     const int most = std::max(a.q.heads, a.k.heads);
-    static const int kIt = std::getenv("HD_IT") ? std::atoi(std::getenv("HD_IT")) : 4;
-    const int it = std::min(kIt, most > 2 * per ? 4 : most > per ? 2 : 1);
+    // four turns a warp share its table entries and weights (144 us against
+    // 170 for two, on the RMS case at heads_vec_kernel)
+    const int it = most > 2 * per ? 4 : most > per ? 2 : 1;
     if (it == 4) launch_heads_vec<T, NORM, PAIRS, 4>(a, lg, per, st);
     else if (it == 2) launch_heads_vec<T, NORM, PAIRS, 2>(a, lg, per, st);
     else launch_heads_vec<T, NORM, PAIRS, 1>(a, lg, per, st);
@@ -350,10 +360,6 @@ int check_route(int64_t rows, int32_t experts, int32_t top_k) {
   return NEBW_OK;
 }
 
-size_t route_smem(int experts) {
-  return (nebw::kRouteWarps + 2) * static_cast<size_t>(experts) * sizeof(int);
-}
-
 template <typename T, int K>
 int launch_route(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
   const size_t smem = route_smem(a.experts);
@@ -434,8 +440,10 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
   while (a.lg < 4 && (1 << a.lg) < eights && (a.lg < 2 || (eights >> a.lg) > 4)) ++a.lg;
   a.per = (eights + (1 << a.lg) - 1) / (1 << a.lg) * 8;
   a.vec = experts % 8 == 0 && aligned(logits, 16) && stride * esz % 16 == 0;
-  const int blocks = static_cast<int>(route_blocks(rows, d->sm_count));
-  a.block_rows = static_cast<int>((rows + blocks - 1) / blocks);
+  a.tiles = route_tiles(experts);
+  int blocks = static_cast<int>(route_blocks(rows, d->sm_count));
+  a.block_rows = static_cast<int>(((rows + blocks - 1) / blocks + 31) / 32 * 32);
+  blocks = static_cast<int>((rows + a.block_rows - 1) / a.block_rows);
   return dtype == NEBW_F32 ? launch_route_k<float>(a, blocks, st)
                            : launch_route_k<__nv_bfloat16>(a, blocks, st);
 }

@@ -45,7 +45,8 @@ struct RouteArgs {
   int lg;           // 2^lg lanes share a row,
   int per;          // each with `per` consecutive experts (a multiple of 8)
   int vec;          // rows of whole, aligned 16-byte vectors
-  int block_rows;   // rows a block
+  int block_rows;   // rows a block, a multiple of 32
+  int tiles;        // tiles of 32 rows placed at once
 };
 
 __device__ __forceinline__ int route_rows(const RouteArgs &p) {
@@ -60,11 +61,12 @@ struct RouteKey;
 template <>
 struct RouteKey<__nv_bfloat16> {
   using Key = uint32_t;
-  static __device__ __forceinline__ Key make(uint32_t bits16, int e) {
-    const uint32_t u = bits16 == 0x8000u ? 0u : bits16;
-    const uint32_t o = u & 0x8000u ? u ^ 0xffffu : u | 0x8000u;  // ascending
-    // above -inf (0x007f) and up to +inf (0xff80); NaN of either sign is outside
-    return o > 0x007fu && o <= 0xff80u ? (o << 16) | (0xffffu - e) : 0u;
+  // v: a bf16 value's bits in the upper half
+  static __device__ __forceinline__ Key make(uint32_t v, int e) {
+    const float f = __uint_as_float(v) + 0.0f;  // -0 + 0 = +0
+    const int u = __float_as_int(f);
+    const uint32_t o = static_cast<uint32_t>(u ^ ((u >> 31) | static_cast<int>(0x80000000)));
+    return f > -INFINITY ? (o & 0xffff0000u) | (0xffffu - e) : 0u;
   }
   static __device__ __forceinline__ float value(Key k) {
     const uint32_t o = k >> 16;
@@ -78,11 +80,13 @@ struct RouteKey<__nv_bfloat16> {
       const uint4 u = __ldg(reinterpret_cast<const uint4 *>(l + e));
       const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = make(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu, e + i);
+      for (int i = 0; i < 8; ++i)
+        k[i] = make(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16, e + i);
     } else {
       const unsigned short *s = reinterpret_cast<const unsigned short *>(l);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) k[i] = e + i < n ? make(__ldg(s + e + i), e + i) : 0u;
+      for (int i = 0; i < 8; ++i)
+        k[i] = e + i < n ? make(static_cast<uint32_t>(__ldg(s + e + i)) << 16, e + i) : 0u;
     }
   }
 };
@@ -196,6 +200,26 @@ __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int su
   }
 }
 
+// Entry j of an ordered list (0 past its end).
+template <int K, typename Key>
+__device__ __forceinline__ Key route_pick(const Key (&top)[K], int j) {
+  Key k = 0;
+#pragma unroll
+  for (int i = 0; i < K; ++i)
+    if (i == j) k = top[i];
+  return k;
+}
+
+// The score of a chosen expert before it is normalised; `first` is the row's
+// largest logit.
+template <typename T>
+__device__ __forceinline__ float route_score(const RouteArgs &p, typename RouteKey<T>::Key key,
+                                             float first) {
+  const float v = RouteKey<T>::value(key);
+  if (p.sigmoid) return 1.0f / (1.0f + expf(-v));
+  return v == first ? 1.0f : expf(v - first);  // inf - inf is no number
+}
+
 // The choice of this block's rows, written out and counted per expert.
 template <typename T, int K>
 __device__ __forceinline__ void route_choose(const RouteArgs &p, int r0, int r1, int *count) {
@@ -226,90 +250,76 @@ __device__ __forceinline__ void route_choose(const RouteArgs &p, int r0, int r1,
       }
       for (int o = 1; o < 1 << p.lg; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    if (!live || sub != 0) continue;
-    float w[K];
+    // the row's lanes share its entries out: entry sub, sub + 2^lg, ...
+    const int lanes = 1 << p.lg;
     float chosen = 0.f;
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-      w[j] = 0.f;
-      if (j < p.k && top[j]) {
-        const float v = R::value(top[j]);
-        w[j] = p.sigmoid ? 1.0f / (1.0f + expf(-v)) : v == first ? 1.0f : expf(v - first);
-        chosen += w[j];
+    if (p.renorm) {
+      for (int j0 = 0; j0 < K; j0 += lanes) {
+        const typename R::Key mine = route_pick<K>(top, j0 + sub);
+        if (mine && j0 + sub < p.k) chosen += route_score<T>(p, mine, first);
+      }
+      for (int o = 1; o < lanes; o <<= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
+      sum = chosen;
+    }
+    float by = p.scale;
+    if (p.renorm || !p.sigmoid) by = sum > 0.f ? p.scale / sum : 0.f;
+    for (int j = sub; j < p.k; j += lanes) {
+      const typename R::Key mine = route_pick<K>(top, j);
+      const int id = mine ? R::expert(mine) : -1;
+      if (live) {
+        const int64_t at = static_cast<int64_t>(row) * p.k + j;
+        p.ids[at] = id;
+        p.weights[at] = mine ? route_score<T>(p, mine, first) * by : 0.f;
+        if (mine) atomicAdd(&count[id], 1);
       }
     }
-    if (p.renorm) sum = chosen;
-    const bool divide = p.renorm || !p.sigmoid;
-#pragma unroll
-    for (int j = 0; j < K; ++j) {
-      if (j < p.k) {
-        const int id = top[j] ? R::expert(top[j]) : -1;
-        if (divide) w[j] = sum > 0.f ? w[j] / sum : 0.f;
-        p.ids[static_cast<int64_t>(row) * p.k + j] = id;
-        p.weights[static_cast<int64_t>(row) * p.k + j] = w[j] * p.scale;
-        if (id >= 0) atomicAdd(&count[id], 1);
-      }
-    }
+    __syncwarp();
   }
 }
 
 // The grouped places of this block's rows.  start [experts]: the first place
-// of each expert for this block; cnt [warps, experts]: scratch.  The order
-// inside a block comes from a count per warp and a match within 32 entries.
-__device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, const int *start,
-                                            int *cnt) {
+// of each expert for this block; mask, pre [tiles, experts]: scratch.  A warp
+// takes a tile of 32 rows, a lane a row: bit r of mask[tile][e] says that row
+// r of the tile chose e, so an entry's place is its expert's count before the
+// tile and the bits below its own -- whatever order the bits were set in.
+__device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, int *start,
+                                            int *mask, int *pre) {
   const int E = p.experts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kRouteWarps * E; i += kRouteThreads) cnt[i] = 0;
-  __syncthreads();
-  // each warp a run of whole groups of 32 entries
-  const int n = (r1 - r0) * p.k;
-  const int run = (n + kRouteThreads - 1) / kRouteThreads * 32;
-  const int i0 = min(n, warp * run), i1 = min(n, i0 + run);
-  const int *ids = p.ids + static_cast<int64_t>(r0) * p.k;
-  int *mine = cnt + warp * E;
-  // (the ids of four groups are loaded together: the walk over a group
-  // waits for the counts of the one before, not for memory)
-  for (int ib = i0; ib < i1; ib += 128) {
-    int id[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) id[u] = ib + u * 32 + lane < i1 ? ids[ib + u * 32 + lane] : -1;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const unsigned same = __match_any_sync(0xffffffffu, id[u]);
-      if (id[u] >= 0 && (same & ((1u << lane) - 1)) == 0) mine[id[u]] += __popc(same);
-      __syncwarp();
-    }
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kRouteThreads) {
-    int at = start[e];
-    for (int w = 0; w < kRouteWarps; ++w) {
-      const int c = cnt[w * E + e];
-      cnt[w * E + e] = at;
-      at += c;
-    }
-  }
-  __syncthreads();
-  for (int ib = i0; ib < i1; ib += 128) {
-    int id[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) id[u] = ib + u * 32 + lane < i1 ? ids[ib + u * 32 + lane] : -1;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int i = ib + u * 32 + lane;
-      const unsigned same = __match_any_sync(0xffffffffu, id[u]);
-      const unsigned below = same & ((1u << lane) - 1);
-      int place = -1;
-      if (id[u] >= 0) place = mine[id[u]] + __popc(below);
-      __syncwarp();
-      if (id[u] >= 0 && below == 0) mine[id[u]] += __popc(same);
-      __syncwarp();
-      if (i < i1) {
-        p.row_dst[static_cast<int64_t>(r0) * p.k + i] = place;
-        if (place >= 0) p.row_src[place] = r0 + i / p.k;
+  for (int rb = r0; rb < r1; rb += p.tiles * 32) {
+    const int tiles = min(p.tiles, (r1 - rb + 31) / 32);
+    for (int i = threadIdx.x; i < tiles * E; i += kRouteThreads) mask[i] = 0;
+    __syncthreads();
+    const int row = rb + warp * 32 + lane;
+    const bool mine = warp < tiles && row < r1;
+    const int64_t at = static_cast<int64_t>(row) * p.k;
+    if (mine)
+      for (int j = 0; j < p.k; ++j) {
+        const int id = p.ids[at + j];
+        if (id >= 0) atomicOr(&mask[warp * E + id], 1 << lane);
       }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += kRouteThreads) {
+      int run = start[e];
+#pragma unroll 8
+      for (int t = 0; t < tiles; ++t) {
+        pre[t * E + e] = run;
+        run += __popc(mask[t * E + e]);
+      }
+      start[e] = run;
     }
+    __syncthreads();
+    if (mine)
+      for (int j = 0; j < p.k; ++j) {
+        const int id = p.ids[at + j];
+        int place = -1;
+        if (id >= 0) {
+          place = pre[warp * E + id] + __popc(mask[warp * E + id] & ((1 << lane) - 1));
+          p.row_src[place] = row;
+        }
+        p.row_dst[at + j] = place;
+      }
+    __syncthreads();
   }
 }
 
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
 __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs p) {
   extern __shared__ int sh[];
   const int E = p.experts;
-  int *start = sh, *total = sh + E, *cnt = sh + 2 * E;
+  int *start = sh, *total = sh + E, *mask = sh + 2 * E, *pre = mask + p.tiles * E;
   for (int e = threadIdx.x; e < 2 * E; e += kRouteThreads) sh[e] = 0;
   __syncthreads();
   // threads share the blocks' counts out among them, expert by expert
@@ -383,7 +393,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.block_rows;
   if (r0 < rows)
     route_place(p, static_cast<int>(r0),
-                static_cast<int>(min(static_cast<int64_t>(rows), r0 + p.block_rows)), start, cnt);
+                static_cast<int>(min(static_cast<int64_t>(rows), r0 + p.block_rows)), start, mask, pre);
 }
 
 // Few rows: one block chooses and places.
@@ -391,7 +401,7 @@ template <typename T, int K>
 __global__ void __launch_bounds__(kRouteThreads) route_fused_kernel(const RouteArgs p) {
   extern __shared__ int sh[];
   const int E = p.experts;
-  int *start = sh, *total = sh + E, *cnt = sh + 2 * E;
+  int *start = sh, *total = sh + E, *mask = sh + 2 * E, *pre = mask + p.tiles * E;
   for (int e = threadIdx.x; e < 2 * E; e += kRouteThreads) sh[e] = 0;
   __syncthreads();
   const int rows = route_rows(p);
@@ -399,7 +409,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_fused_kernel(const RouteA
   __syncthreads();
   route_scan(p, total, start, true);
   __syncthreads();
-  route_place(p, 0, rows, start, cnt);
+  route_place(p, 0, rows, start, mask, pre);
 }
 
 // out[t] = residual[t] + sum_j weights[t, j] * y[row_dst[t, j]], j ascending,
