@@ -50,22 +50,23 @@ size_t route_smem(int experts) {
   return (2 + 2 * static_cast<size_t>(route_tiles(experts))) * experts * sizeof(int);
 }
 
-template <typename T>
+template <int K>
 int set_route_attrs() {
   const auto a = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 1>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 2>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 4>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 8>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<T, 16>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<float, K, 0>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<float, K, 2>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<__nv_bfloat16, K, 0>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<__nv_bfloat16, K, 2>, a, kRouteSmem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_place_kernel<K>, a, kRouteSmem));
   return NEBW_OK;
 }
 
 int set_layer_op_attrs() {
-  if (int rc = set_route_attrs<float>()) return rc;
-  if (int rc = set_route_attrs<__nv_bfloat16>()) return rc;
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_place_kernel,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, kRouteSmem));
+  if (int rc = set_route_attrs<1>()) return rc;
+  if (int rc = set_route_attrs<2>()) return rc;
+  if (int rc = set_route_attrs<4>()) return rc;
+  if (int rc = set_route_attrs<8>()) return rc;
+  if (int rc = set_route_attrs<16>()) return rc;
   if (int rc = set_grouped_attrs_ctas<1>()) return rc;
   return set_grouped_attrs_ctas<2>();
 }
@@ -360,18 +361,30 @@ int check_route(int64_t rows, int32_t experts, int32_t top_k) {
   return NEBW_OK;
 }
 
-template <typename T, int K>
-int launch_route(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
+template <typename T, int K, int LG>
+int launch_route_lg(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
   const size_t smem = route_smem(a.experts);
   if (blocks == 1) {
-    nebw::route_fused_kernel<T, K><<<1, nebw::kRouteThreads, smem, st>>>(a);
+    nebw::route_fused_kernel<T, K, LG><<<1, nebw::kRouteThreads, smem, st>>>(a);
   } else {
-    nebw::route_choose_kernel<T, K><<<blocks, nebw::kRouteThreads, 0, st>>>(a);
+    nebw::route_choose_kernel<T, K, LG><<<blocks, nebw::kRouteThreads, 0, st>>>(a);
     NEBW_CUDA(cudaGetLastError());
-    nebw::route_place_kernel<<<blocks, nebw::kRouteThreads, smem, st>>>(a);
+    nebw::route_place_kernel<K><<<blocks, nebw::kRouteThreads, smem, st>>>(a);
   }
   NEBW_CUDA(cudaGetLastError());
   return NEBW_OK;
+}
+
+// Four lanes a row from three eights of experts on, else one.
+template <typename T, int K>
+int launch_route(nebw::RouteArgs a, int blocks, cudaStream_t st) {
+  const int eights = (a.experts + 7) / 8;
+  if (eights < 3) {
+    a.per = eights * 8;
+    return launch_route_lg<T, K, 0>(a, blocks, st);
+  }
+  a.per = (eights + 3) / 4 * 8;
+  return launch_route_lg<T, K, 2>(a, blocks, st);
 }
 
 // The list a lane keeps: the next power of two of top_k.
@@ -435,12 +448,9 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
   a.row_src = row_src;
   a.row_dst = row_dst;
   a.hist = static_cast<int *>(ws);
-  const int eights = (experts + 7) / 8;
-  // four lanes a row up to 128 experts, then as many as leave each 32
-  while (a.lg < 4 && (1 << a.lg) < eights && (a.lg < 2 || (eights >> a.lg) > 4)) ++a.lg;
-  a.per = (eights + (1 << a.lg) - 1) / (1 << a.lg) * 8;
   a.vec = experts % 8 == 0 && aligned(logits, 16) && stride * esz % 16 == 0;
   a.tiles = route_tiles(experts);
+  a.whole = (top_k == 4 || top_k == 8 || top_k == 16) && aligned(ids, 16) && aligned(row_dst, 16);
   int blocks = static_cast<int>(route_blocks(rows, d->sm_count));
   a.block_rows = static_cast<int>(((rows + blocks - 1) / blocks + 31) / 32 * 32);
   blocks = static_cast<int>((rows + a.block_rows - 1) / a.block_rows);

@@ -42,11 +42,11 @@ struct RouteArgs {
   int *row_src;     // [rows * k]: the row at each grouped place
   int *row_dst;     // [rows, k]: the place of each row's expert, -1 if none
   int *hist;        // [blocks, experts]; unused by one block
-  int lg;           // 2^lg lanes share a row,
-  int per;          // each with `per` consecutive experts (a multiple of 8)
+  int per;          // consecutive experts a lane looks at, a multiple of 8
   int vec;          // rows of whole, aligned 16-byte vectors
   int block_rows;   // rows a block, a multiple of 32
   int tiles;        // tiles of 32 rows placed at once
+  int whole;        // k is the list's length and rows of ids and row_dst are 16-byte vectors
 };
 
 __device__ __forceinline__ int route_rows(const RouteArgs &p) {
@@ -174,10 +174,10 @@ __device__ __forceinline__ void route_add8(Key (&top)[K], Key (&k)[8]) {
   }
 }
 
-// One row's choice by the 2^lg lanes that share it: each keeps the K largest
+// One row's choice by the 2^LG lanes that share it: each keeps the K largest
 // keys of its experts in order, then lanes merge in pairs.  Every lane ends
 // with the row's list.
-template <typename T, int K>
+template <typename T, int K, int LG>
 __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int sub,
                                           typename RouteKey<T>::Key (&top)[K]) {
   using R = RouteKey<T>;
@@ -190,7 +190,8 @@ __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int su
     R::load8(l, e, p.experts, p.vec, k);
     route_add8<K>(top, k);
   }
-  for (int o = 1; o < 1 << p.lg; o <<= 1) {
+#pragma unroll
+  for (int o = 1; o < 1 << LG; o <<= 1) {
     Key other[K];
 #pragma unroll
     for (int i = 0; i < K; ++i) other[i] = __shfl_xor_sync(0xffffffffu, top[i], o);
@@ -200,90 +201,127 @@ __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int su
   }
 }
 
-// Entry j of an ordered list (0 past its end).
-template <int K, typename Key>
-__device__ __forceinline__ Key route_pick(const Key (&top)[K], int j) {
-  Key k = 0;
-#pragma unroll
-  for (int i = 0; i < K; ++i)
-    if (i == j) k = top[i];
-  return k;
-}
-
 // The score of a chosen expert before it is normalised; `first` is the row's
 // largest logit.
-template <typename T>
-__device__ __forceinline__ float route_score(const RouteArgs &p, typename RouteKey<T>::Key key,
-                                             float first) {
-  const float v = RouteKey<T>::value(key);
+__device__ __forceinline__ float route_score(const RouteArgs &p, float v, float first) {
   if (p.sigmoid) return 1.0f / (1.0f + expf(-v));
   return v == first ? 1.0f : expf(v - first);  // inf - inf is no number
 }
 
 // The choice of this block's rows, written out and counted per expert.
-template <typename T, int K>
+template <typename T, int K, int LG>
 __device__ __forceinline__ void route_choose(const RouteArgs &p, int r0, int r1, int *count) {
   using R = RouteKey<T>;
+  using Key = typename R::Key;
+  constexpr int kLanes = 1 << LG, kRowsWarp = 32 >> LG;
+  constexpr int kMine = (K + kLanes - 1) / kLanes;  // entries a lane writes
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int sub = lane & ((1 << p.lg) - 1);
-  const int rows_warp = 32 >> p.lg;
-  for (int rb = r0 + warp * rows_warp; rb < r1; rb += kRouteWarps * rows_warp) {
-    const int row = rb + (lane >> p.lg);
+  const int sub = lane & (kLanes - 1);
+  for (int rb = r0 + warp * kRowsWarp; rb < r1; rb += kRouteWarps * kRowsWarp) {
+    const int row = rb + (lane >> LG);
     const bool live = row < r1;
     // lanes of a row that is not there walk the last one
     const T *l = static_cast<const T *>(p.logits) +
                  static_cast<int64_t>(live ? row : r1 - 1) * p.stride;
-    typename R::Key top[K];
-    route_row<T, K>(p, l, sub, top);
+    Key top[K];
+    route_row<T, K, LG>(p, l, sub, top);
     const float first = R::value(top[0]);
     float sum = 0.f;
     if (!p.sigmoid && !p.renorm) {
       const int end = min(p.experts, (sub + 1) * p.per);
       for (int e = sub * p.per; e < end; e += 8) {
-        typename R::Key k[8];
+        Key k[8];
         R::load8(l, e, p.experts, p.vec, k);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = R::value(k[i]);
-          if (k[i]) sum += v == first ? 1.0f : expf(v - first);  // inf - inf is no number
-        }
+        for (int i = 0; i < 8; ++i)
+          if (k[i]) sum += route_score(p, R::value(k[i]), first);
       }
-      for (int o = 1; o < 1 << p.lg; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
-    // the row's lanes share its entries out: entry sub, sub + 2^lg, ...
-    const int lanes = 1 << p.lg;
-    float chosen = 0.f;
-    if (p.renorm) {
-      for (int j0 = 0; j0 < K; j0 += lanes) {
-        const typename R::Key mine = route_pick<K>(top, j0 + sub);
-        if (mine && j0 + sub < p.k) chosen += route_score<T>(p, mine, first);
-      }
-      for (int o = 1; o < lanes; o <<= 1) chosen += __shfl_xor_sync(0xffffffffu, chosen, o);
-      sum = chosen;
+    // the row's lanes share its entries out: entry (i << LG) + sub, by halving
+    // the list once per bit of sub
+    Key mine[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) mine[i] = top[i];
+#pragma unroll
+    for (int b = 0; b < LG; ++b) {
+#pragma unroll
+      for (int i = 0; i < (K >> b) / 2; ++i) mine[i] = (sub >> b) & 1 ? mine[2 * i + 1] : mine[2 * i];
     }
+    float w[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int j = (i << LG) + sub;
+      // (a list shorter than the lanes: lanes from K on have no entry)
+      if (j >= p.k) mine[i] = 0;
+      w[i] = mine[i] ? route_score(p, R::value(mine[i]), first) : 0.f;
+      if (p.renorm) sum += w[i];
+    }
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     float by = p.scale;
     if (p.renorm || !p.sigmoid) by = sum > 0.f ? p.scale / sum : 0.f;
-    for (int j = sub; j < p.k; j += lanes) {
-      const typename R::Key mine = route_pick<K>(top, j);
-      const int id = mine ? R::expert(mine) : -1;
-      if (live) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int j = (i << LG) + sub;
+      if (live && j < p.k) {
+        const int id = mine[i] ? R::expert(mine[i]) : -1;
         const int64_t at = static_cast<int64_t>(row) * p.k + j;
         p.ids[at] = id;
-        p.weights[at] = mine ? route_score<T>(p, mine, first) * by : 0.f;
-        if (mine) atomicAdd(&count[id], 1);
+        p.weights[at] = w[i] * by;
+        if (mine[i]) atomicAdd(&count[id], 1);
       }
     }
     __syncwarp();
   }
 }
 
-// The grouped places of this block's rows.  start [experts]: the first place
+// A row's chosen experts, -1 past the last.
+template <int K>
+__device__ __forceinline__ void route_ids(const RouteArgs &p, int row, bool live, int (&id)[K]) {
+  const int *ids = p.ids + static_cast<int64_t>(row) * p.k;
+  if constexpr (K % 4 == 0) {
+    if (p.whole) {
+#pragma unroll
+      for (int j = 0; j < K; j += 4) {
+        const int4 v = live ? *reinterpret_cast<const int4 *>(ids + j) : make_int4(-1, -1, -1, -1);
+        id[j] = v.x;
+        id[j + 1] = v.y;
+        id[j + 2] = v.z;
+        id[j + 3] = v.w;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < K; ++j) id[j] = live && j < p.k ? ids[j] : -1;
+}
+
+// A row's places.
+template <int K>
+__device__ __forceinline__ void route_put(const RouteArgs &p, int row, const int (&place)[K]) {
+  int *dst = p.row_dst + static_cast<int64_t>(row) * p.k;
+  if constexpr (K % 4 == 0) {
+    if (p.whole) {
+#pragma unroll
+      for (int j = 0; j < K; j += 4)
+        *reinterpret_cast<int4 *>(dst + j) =
+            make_int4(place[j], place[j + 1], place[j + 2], place[j + 3]);
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < K; ++j)
+    if (j < p.k) dst[j] = place[j];
+}
+
+// The grouped places of this block's rows; id: those of the first tiles' rows.  start [experts]: the first place
 // of each expert for this block; mask, pre [tiles, experts]: scratch.  A warp
 // takes a tile of 32 rows, a lane a row: bit r of mask[tile][e] says that row
 // r of the tile chose e, so an entry's place is its expert's count before the
 // tile and the bits below its own -- whatever order the bits were set in.
+template <int K>
 __device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, int *start,
-                                            int *mask, int *pre) {
+                                            int *mask, int *pre, int (&id)[K]) {
   const int E = p.experts;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int rb = r0; rb < r1; rb += p.tiles * 32) {
@@ -292,12 +330,12 @@ __device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, 
     __syncthreads();
     const int row = rb + warp * 32 + lane;
     const bool mine = warp < tiles && row < r1;
-    const int64_t at = static_cast<int64_t>(row) * p.k;
-    if (mine)
-      for (int j = 0; j < p.k; ++j) {
-        const int id = p.ids[at + j];
-        if (id >= 0) atomicOr(&mask[warp * E + id], 1 << lane);
-      }
+    if (rb != r0) route_ids<K>(p, row, mine, id);
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < K; ++j)
+        if (id[j] >= 0) atomicOr(&mask[warp * E + id[j]], 1 << lane);
+    }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += kRouteThreads) {
       int run = start[e];
@@ -309,16 +347,18 @@ __device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, 
       start[e] = run;
     }
     __syncthreads();
-    if (mine)
-      for (int j = 0; j < p.k; ++j) {
-        const int id = p.ids[at + j];
-        int place = -1;
-        if (id >= 0) {
-          place = pre[warp * E + id] + __popc(mask[warp * E + id] & ((1 << lane) - 1));
-          p.row_src[place] = row;
+    if (mine) {
+      int place[K];
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        place[j] = -1;
+        if (id[j] >= 0) {
+          place[j] = pre[warp * E + id[j]] + __popc(mask[warp * E + id[j]] & ((1 << lane) - 1));
+          p.row_src[place[j]] = row;
         }
-        p.row_dst[at + j] = place;
       }
+      route_put<K>(p, row, place);
+    }
     __syncthreads();
   }
 }
@@ -350,7 +390,7 @@ __device__ __forceinline__ void route_scan(const RouteArgs &p, const int *total,
 }
 
 // The choice of every row, and each block's count of rows per expert.
-template <typename T, int K>
+template <typename T, int K, int LG>
 __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteArgs p) {
   __shared__ int count[kRouteMaxExperts];
   for (int e = threadIdx.x; e < p.experts; e += kRouteThreads) count[e] = 0;
@@ -358,8 +398,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
   const int rows = route_rows(p);
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.block_rows;
   if (r0 < rows)
-    route_choose<T, K>(p, static_cast<int>(r0),
-                       static_cast<int>(min(static_cast<int64_t>(rows), r0 + p.block_rows)), count);
+    route_choose<T, K, LG>(p, static_cast<int>(r0),
+                           static_cast<int>(min(static_cast<int64_t>(rows), r0 + p.block_rows)),
+                           count);
   __syncthreads();
   for (int e = threadIdx.x; e < p.experts; e += kRouteThreads)
     p.hist[static_cast<int64_t>(blockIdx.x) * p.experts + e] = count[e];
@@ -367,10 +408,18 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
 
 // The places: the counts of all blocks give each expert's start and this
 // block's start within it.
+template <int K>
 __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteArgs p) {
   extern __shared__ int sh[];
   const int E = p.experts;
   int *start = sh, *total = sh + E, *mask = sh + 2 * E, *pre = mask + p.tiles * E;
+  const int rows = route_rows(p);
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.block_rows;
+  const int64_t r1 = min(static_cast<int64_t>(rows), r0 + p.block_rows);
+  int id[K];  // on their way while the counts are summed
+  const int warp = threadIdx.x >> 5;
+  route_ids<K>(p, static_cast<int>(r0) + static_cast<int>(threadIdx.x),
+               warp < p.tiles && r0 + threadIdx.x < r1, id);
   for (int e = threadIdx.x; e < 2 * E; e += kRouteThreads) sh[e] = 0;
   __syncthreads();
   // threads share the blocks' counts out among them, expert by expert
@@ -378,6 +427,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
   while (lanes < E && lanes < kRouteThreads) lanes <<= 1;
   for (int e = threadIdx.x & (lanes - 1); e < E; e += lanes) {
     int before = 0, all = 0;
+#pragma unroll 8
     for (int b = threadIdx.x / lanes; b < gridDim.x; b += kRouteThreads / lanes) {
       const int c = p.hist[static_cast<int64_t>(b) * E + e];
       if (b < static_cast<int>(blockIdx.x)) before += c;
@@ -389,15 +439,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteA
   __syncthreads();
   route_scan(p, total, start, blockIdx.x == 0);
   __syncthreads();
-  const int rows = route_rows(p);
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.block_rows;
   if (r0 < rows)
-    route_place(p, static_cast<int>(r0),
-                static_cast<int>(min(static_cast<int64_t>(rows), r0 + p.block_rows)), start, mask, pre);
+    route_place<K>(p, static_cast<int>(r0), static_cast<int>(r1), start, mask, pre, id);
 }
 
 // Few rows: one block chooses and places.
-template <typename T, int K>
+template <typename T, int K, int LG>
 __global__ void __launch_bounds__(kRouteThreads) route_fused_kernel(const RouteArgs p) {
   extern __shared__ int sh[];
   const int E = p.experts;
@@ -405,11 +452,13 @@ __global__ void __launch_bounds__(kRouteThreads) route_fused_kernel(const RouteA
   for (int e = threadIdx.x; e < 2 * E; e += kRouteThreads) sh[e] = 0;
   __syncthreads();
   const int rows = route_rows(p);
-  if (rows > 0) route_choose<T, K>(p, 0, rows, total);
+  if (rows > 0) route_choose<T, K, LG>(p, 0, rows, total);
   __syncthreads();
   route_scan(p, total, start, true);
   __syncthreads();
-  route_place(p, 0, rows, start, mask, pre);
+  int id[K];
+  route_ids<K>(p, threadIdx.x, (threadIdx.x >> 5) < p.tiles && threadIdx.x < rows, id);
+  route_place<K>(p, 0, rows, start, mask, pre, id);
 }
 
 // out[t] = residual[t] + sum_j weights[t, j] * y[row_dst[t, j]], j ascending,
