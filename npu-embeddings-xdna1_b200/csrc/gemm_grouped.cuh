@@ -9,11 +9,18 @@
 // a gated weight's N columns are interleaved in groups of 64 = [32 up |
 // 32 gate] and the product is up * act(gate), N / 2 wide.
 //
-// A tile is 128 * CTAS rows of one expert by bn columns: a CTA pair on 256 x
-// 256 (tcgen05 cta_group::2, each CTA loading its 128 rows of A and of W) or
-// one CTA on 128 x bn, bn <= 128.  A list of tile counts per expert, built by
-// every block from off, gives a tile its expert, so the persistent blocks walk
-// one list whatever the groups are.  Roles of a block:
+// Two kernels with one list of tiles (counts per expert, built by every block
+// from off, so the persistent blocks walk one list whatever the groups are):
+//
+//   gemm_grouped_pair_kernel  a CTA pair (tcgen05 cta_group::2) takes 256
+//       columns of W and up to 256 rows of one group, with W as the product's
+//       M operand and the rows as its N operand: N is any multiple of 32, so a
+//       group of 40 rows costs 64 and not 256, and a group of 257 is cut into
+//       160 + 97.  The accumulator holds a column of C per TMEM lane.
+//   gemm_grouped_kernel  one CTA takes 128 rows by 128, 64 or 32 columns, rows
+//       as M: for so few rows that the columns have to spread over the SMs.
+//
+// Roles of a block:
 //   warp 0        W by TMA (and A, where its rows are grouped already), and
 //                 the stage's transaction bytes
 //   warp 1        tcgen05.mma (the pair's leader)
@@ -23,11 +30,11 @@
 //   warps 10-17   GATHER: A's rows, four at a time (tile::gather4), each warp
 //                 a share of the tile's rows with their indices in registers
 // A gather is issued by one lane for uniform operands; from 32 lanes of one
-// warp the same 32 gathers take turns on the issue path (80 clocks each,
-// measured: 2457 us for 65,542 rows, K 1024, N 8192).  Rows past the group
-// are not loaded: what lies in their place in shared memory reaches only
-// accumulator rows that are not stored.  All waits are bounded as in
-// gemm_tc_pair_kernel, whose barriers these are.
+// warp the same 32 gathers take turns on the issue path (80 clocks each).
+// Eight warps: 877 us on 65,542 rows, K 1024, N 8192, against 988 for four
+// and 1207 for two.  Rows past the group are not loaded: what lies in their
+// place in shared memory reaches only accumulators that are not stored.  All
+// waits are bounded as in gemm_tc_pair_kernel, whose barriers these are.
 #pragma once
 
 #include <cuda.h>
@@ -58,7 +65,7 @@ struct GroupedArgs {
   const int *row_src;  // [rows] or null
   int a_rows;          // A's rows
   int N, K;            // N as staged (2F for a gated weight)
-  int bn;              // tile columns: 256 (pairs); 128, 64 or 32
+  int bn;              // one CTA: tile columns, 128, 64 or 32
   const float *bias;   // [experts, N] in the container's column order, or null
   void *out;           // [rows, N or N / 2]
   int *err;
@@ -190,6 +197,20 @@ __device__ __forceinline__ GroupTile group_tile(const GroupTable &g, int t, int 
   return {e, g.off[e] + mb * bm, g.off[e + 1], i - mb * n_blocks};
 }
 
+// The same for the pair kernel: a group of m rows is cut into ceil(m / 256)
+// tiles of equal size, rounded up to 32 rows.
+__device__ __forceinline__ GroupTile group_tile_even(const GroupTable &g, int t, int n_blocks,
+                                                     int &e) {
+  while (t >= g.tile[e + 1]) ++e;
+  const int i = t - g.tile[e];
+  const int tb = i / n_blocks;
+  const int m = g.off[e + 1] - g.off[e];
+  const int tiles = (m + 255) / 256;
+  const int size = ((m + tiles - 1) / tiles + 31) / 32 * 32;
+  const int row = g.off[e] + tb * size;
+  return {e, row, min(row + size, g.off[e + 1]), i - tb * n_blocks};
+}
+
 // 32 accumulator columns of one row from GEMM column col0 on (a gated
 // epilogue: up columns, with their gates in rg), biased and activated: output
 // columns [c0, c0 + ncols).
@@ -284,17 +305,15 @@ __device__ __forceinline__ void grp_store(void *out, int64_t at, int ncols, cons
   }
 }
 
-template <int CTAS, int EPI, bool GATHER>
-__global__ void __cluster_dims__(CTAS, 1, 1)
-    __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
+template <int EPI, bool GATHER>
+__global__ void __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA,
                         const __grid_constant__ CUtensorMap tmA128,
                         const __grid_constant__ CUtensorMap tmW,
                         const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
   using S = GroupedShape;
   constexpr int kStages = S::kStages;
-  constexpr int kTileM = CTAS * kGemmBM;
-  constexpr int kAccCols = CTAS == 2 ? 256 : 128;  // TMEM columns of an accumulator
+  constexpr int kAccCols = 128;  // TMEM columns of an accumulator
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -312,12 +331,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int rank = CTAS == 2 ? static_cast<int>(cluster_ctarank()) : 0;
-  const bool leader = rank == 0;
-  const int bn = CTAS == 2 ? 256 : p.bn;
+  const int bn = p.bn;
   const int n_blocks = (p.N + bn - 1) / bn;
   const int num_kb = (p.K + kGemmBK - 1) / kGemmBK;
-  const int first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&tmA);
@@ -327,41 +343,28 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       // every gather warp arrives on every stage, also with no row to load:
       // one that did not could fall a phase behind the ring, whose parity
       // then reads the wrong way round
-      mbar_init(&full[s], 1 + (GATHER ? kGatherWarps * CTAS : 0));
+      mbar_init(&full[s], 1 + (GATHER ? kGatherWarps : 0));
       mbar_init(&empty[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 8 * CTAS);
+      mbar_init(&tempty[a], 8);
     }
     mbar_init(drain, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
-    if constexpr (CTAS == 2) {
-      tmem_alloc_pair(tmem_slot, 2 * kAccCols);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(tmem_slot, 2 * kAccCols);
-      tmem_relinquish();
-    }
+    tmem_alloc(tmem_slot, 2 * kAccCols);
+    tmem_relinquish();
   }
-  group_table_build(table, p, kTileM, n_blocks);
+  group_table_build(table, p, kGemmBM, n_blocks);
   tc_fence_before();
-  if constexpr (CTAS == 2) cluster_sync();
-  else __syncthreads();
+  __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int num_tiles = table.tile[p.experts];
   auto wait_all = [&](uint64_t *bar, uint32_t parity) -> bool {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
-  };
-  auto leader_bar = [&](uint64_t *bar) -> uint32_t {
-    return CTAS == 2 ? map_to_cta(smem_u32(bar), 0) : smem_u32(bar);
-  };
-  // of a tile's rows, how many lie in CTA c's 128
-  auto cta_rows = [&](const GroupTile &t, int c) -> int {
-    return min(max(t.end - t.row - c * kGemmBM, 0), kGemmBM);
   };
 
   if (warp == 0) {
@@ -370,31 +373,28 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       int stage = 0, e = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = first; tile < num_tiles && ok; tile += step) {
-        const GroupTile t = group_tile(table, tile, kTileM, n_blocks, e);
-        const int a_boxes = GATHER ? 0 : (cta_rows(t, rank) + kGroupedBox - 1) / kGroupedBox;
-        uint32_t bytes = static_cast<uint32_t>(bn) * kGemmBK * 2;
-        for (int c = 0; c < CTAS; ++c) {
-          const int m = cta_rows(t, c);
-          bytes += GATHER ? (m + 3) / 4 * 512
-                          : (m + kGroupedBox - 1) / kGroupedBox * (kGroupedBox * 128);
-        }
-        const int w_row = t.e * p.N + t.nb * bn + rank * (bn / CTAS);
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+        const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
+        const int m = min(t.end - t.row, kGemmBM);
+        const int a_boxes = GATHER ? 0 : (m + kGroupedBox - 1) / kGroupedBox;
+        const uint32_t bytes = static_cast<uint32_t>(bn) * kGemmBK * 2 +
+                               (GATHER ? (m + 3) / 4 * 512 : a_boxes * (kGroupedBox * 128));
+        const int w_row = t.e * p.N + t.nb * bn;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) {
             ok = false;
             break;
           }
-          if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
-          const uint32_t bar = leader_bar(&full[stage]);
-          grp_load<CTAS>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
+          mbar_arrive_expect_tx(&full[stage], bytes);
+          const uint32_t bar = smem_u32(&full[stage]);
+          grp_load<1>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
           if (a_boxes == kGemmBM / kGroupedBox) {
-            grp_load<CTAS>(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK,
-                           t.row + rank * kGemmBM);
+            grp_load<1>(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK,
+                        t.row);
           } else {
             for (int i = 0; i < a_boxes; ++i)
-              grp_load<CTAS>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
-                             kb * kGemmBK, t.row + rank * kGemmBM + i * kGroupedBox);
+              grp_load<1>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
+                             kb * kGemmBK, t.row + i * kGroupedBox);
           }
           if (++stage == kStages) {
             stage = 0;
@@ -414,15 +414,15 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       }
     }
   } else if (warp == 1) {
-    // ---------------- MMA issuer (the pair's leader) ----------------
-    if (leader) {
-      const uint32_t idesc = idesc_bf16_f32(kTileM, bn);
+    // ---------------- MMA issuer ----------------
+    {
+      const uint32_t idesc = idesc_bf16_f32(kGemmBM, bn);
       const bool elect = elect_one_sync();
       int stage = 0;
       uint32_t phase = 0;
       bool issued_any = false, ok = true;
       int local = 0;
-      for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
         const int acc = local & 1;
         if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
         tc_fence_after();
@@ -438,13 +438,9 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
           if (elect) {
 #pragma unroll
             for (int k = 0; k < kGemmBK / 16; ++k) {
-              if constexpr (CTAS == 2)
-                umma_bf16_pair(d_tmem, da + k * 2, dw + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
-              else
-                umma_bf16(d_tmem, da + k * 2, dw + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
+              umma_bf16(d_tmem, da + k * 2, dw + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
             }
-            if constexpr (CTAS == 2) umma_commit_pair(&empty[stage], 0x3);
-            else umma_commit(&empty[stage]);
+            umma_commit(&empty[stage]);
           }
           __syncwarp();
           issued_any = true;
@@ -454,15 +450,13 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
           }
         }
         if (ok && elect) {
-          if constexpr (CTAS == 2) umma_commit_pair(&tfull[acc], 0x3);
-          else umma_commit(&tfull[acc]);
+          umma_commit(&tfull[acc]);
         }
         __syncwarp();
       }
       if (issued_any) {
         if (elect) {
-          if constexpr (CTAS == 2) umma_commit_pair(drain, 0x1);
-          else umma_commit(drain);
+          umma_commit(drain);
         }
         __syncwarp();
         wait_all(drain, 0);
@@ -483,12 +477,12 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
     uint8_t *mine = staging + (warp - 2) * S::kWarpStaging;
     int slot = 0;
     int local = 0, e = 0;
-    for (int tile = first; tile < num_tiles; tile += step, ++local) {
+    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
       const int acc = local & 1;
       if (!wait_all(&tfull[acc], (local >> 1) & 1)) break;
       tc_fence_after();
-      const GroupTile t = group_tile(table, tile, kTileM, n_blocks, e);
-      const int row0 = t.row + rank * kGemmBM + quarter * 32;
+      const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
+      const int row0 = t.row + quarter * 32;
       const float *bias = p.bias ? p.bias + static_cast<int64_t>(t.e) * p.N : nullptr;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                              static_cast<uint32_t>(acc * kAccCols);
@@ -527,10 +521,7 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        // (the fence orders the TMEM reads; a releasing arrive would also wait
-        // for this thread's outstanding global accesses)
-        if constexpr (CTAS == 2) grp_arrive(map_to_cta(smem_u32(&tempty[acc]), 0));
-        else mbar_arrive(&tempty[acc]);
+        mbar_arrive(&tempty[acc]);
       }
     }
     if (lane == 0) bulk_wait_group_all();
@@ -541,13 +532,13 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
     int stage = 0, e = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = first; tile < num_tiles && ok; tile += step) {
-      const GroupTile t = group_tile(table, tile, kTileM, n_blocks, e);
-      const int count = min(max(cta_rows(t, rank) - kGatherRows * part, 0), kGatherRows);
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
+      const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
+      const int count = min(max(t.end - t.row - kGatherRows * part, 0), kGatherRows);
       int mine = 0;
       if (count > 0) {
         // past the group: its last row again, to fill a gather of four
-        const int at = t.row + rank * kGemmBM + kGatherRows * part + min(lane, count - 1);
+        const int at = t.row + kGatherRows * part + min(lane, count - 1);
         mine = __ldg(p.row_src + at);
         if (mine < 0 || mine >= p.a_rows) {
           record_err(p.err, kDevBadGroup);
@@ -564,11 +555,11 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
         }
         if (elect) {
           const uint32_t dst = smem_u32(sA + stage * S::kABytes) + part * (kGatherRows * 128);
-          const uint32_t bar = leader_bar(&full[stage]);
+          const uint32_t bar = smem_u32(&full[stage]);
 #pragma unroll
           for (int i = 0; i < kGatherRows / 4; ++i)
             if (4 * i < count)
-              grp_gather4<CTAS>(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
+              grp_gather4<1>(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
                                 src[4 * i + 2], src[4 * i + 3]);
           grp_arrive(bar);
         }
@@ -582,12 +573,378 @@ __global__ void __cluster_dims__(CTAS, 1, 1)
   }
 
   tc_fence_before();
-  if constexpr (CTAS == 2) cluster_sync();  // no CTA leaves while its pair may still signal it
-  else __syncthreads();
+  __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (CTAS == 2) tmem_dealloc_pair(tmem_base, 2 * kAccCols);
-    else tmem_dealloc(tmem_base, 2 * kAccCols);
+    tmem_dealloc(tmem_base, 2 * kAccCols);
+  }
+}
+
+// Both warps of an epilogue pair: wait, and whether `ok` held for both (each
+// arrives however its own wait ended, so neither is left behind).
+__device__ __forceinline__ bool grp_pair_and(int id, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.u32 p, %2, 0;\n\t"
+      "barrier.cta.red.and.pred q, %1, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(id), "r"(static_cast<uint32_t>(ok))
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void grp_pair_sync(int id) {
+  asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory");
+}
+
+// One value of C's column per lane, 32 rows: column `lane` of a 32 x 32 chunk
+// in the output map's swizzle (the transposed twin of grp_stage).  bf16 lanes
+// in pairs share a 32-bit word and rows differ in bank, so a store of one row
+// by the warp has no conflict.
+template <int EPI>
+__device__ __forceinline__ void grp_stage_t(const float (&v)[32], uint8_t *chunk, int lane) {
+  if constexpr (EPI == kGrpF32) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      *reinterpret_cast<float *>(chunk + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) +
+                                 (lane & 3) * 4) = v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+      *reinterpret_cast<__nv_bfloat16 *>(chunk + i * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) +
+                                         (lane & 7) * 2) = __float2bfloat16_rn(v[i]);
+  }
+}
+
+template <int EPI, bool GATHER>
+__global__ void __cluster_dims__(2, 1, 1)
+    __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
+    gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA,
+                             const __grid_constant__ CUtensorMap tmA128,
+                             const __grid_constant__ CUtensorMap tmW,
+                             const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
+  using S = GroupedShape;
+  constexpr int kStages = S::kStages;
+  constexpr int kAccCols = 256;  // TMEM columns of an accumulator: the tile's rows
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t *sA = smem;
+  uint8_t *sW = smem + kStages * S::kABytes;
+  uint8_t *staging = smem + kStages * S::kStageBytes;
+  uint64_t *full = reinterpret_cast<uint64_t *>(staging + S::kStagingBytes);
+  uint64_t *empty = full + kStages;
+  uint64_t *tfull = empty + kStages;
+  uint64_t *tempty = tfull + 2;
+  uint64_t *drain = tempty + 2;
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+  GroupTable &table =
+      *reinterpret_cast<GroupTable *>(staging + S::kStagingBytes + S::kBarBytes);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(cluster_ctarank());
+  const bool leader = rank == 0;
+  const int n_blocks = (p.N + 255) / 256;
+  const int num_kb = (p.K + kGemmBK - 1) / kGemmBK;
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmC);
+    for (int s = 0; s < kStages; ++s) {
+      // every gather warp arrives on every stage, also with no row to load:
+      // one that did not could fall a phase behind the ring, whose parity
+      // then reads the wrong way round
+      mbar_init(&full[s], 1 + (GATHER ? 2 * kGatherWarps : 0));
+      mbar_init(&empty[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull[a], 1);
+      mbar_init(&tempty[a], 16);
+    }
+    mbar_init(drain, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * kAccCols);
+    tmem_relinquish_pair();
+  }
+  group_table_build(table, p, 256, n_blocks);
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const int num_tiles = table.tile[p.experts];
+  auto wait_all = [&](uint64_t *bar, uint32_t parity) -> bool {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
+  };
+  // the product's N, a multiple of 32, and how many of the tile's rows lie in
+  // CTA c's half of it
+  auto tile_n = [](const GroupTile &t) -> int { return (t.end - t.row + 31) / 32 * 32; };
+  auto cta_rows = [&](const GroupTile &t, int c) -> int {
+    const int half = tile_n(t) / 2;
+    return min(max(t.end - t.row - c * half, 0), half);
+  };
+
+  if (warp == 0) {
+    // ---------------- W (and grouped A) producer, both CTAs ----------------
+    if (lane == 0) {
+      int stage = 0, e = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first; tile < num_tiles && ok; tile += step) {
+        const GroupTile t = group_tile_even(table, tile, n_blocks, e);
+        uint32_t bytes = 2 * S::kABytes;  // W
+        for (int c = 0; c < 2; ++c) {
+          const int m = cta_rows(t, c);
+          bytes += GATHER ? (m + 3) / 4 * 512
+                          : (m + kGroupedBox - 1) / kGroupedBox * (kGroupedBox * 128);
+        }
+        const int boxes = GATHER ? 0 : (cta_rows(t, rank) + kGroupedBox - 1) / kGroupedBox;
+        const int a_row = t.row + rank * (tile_n(t) / 2);
+        const int w_row = t.e * p.N + t.nb * 256 + rank * 128;
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
+          const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
+          grp_load<2>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
+          if (boxes == kGemmBM / kGroupedBox) {
+            grp_load<2>(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK, a_row);
+          } else {
+            for (int i = 0; i < boxes; ++i)
+              grp_load<2>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
+                          kb * kGemmBK, a_row + i * kGroupedBox);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+      }
+      // Tail: the MMAs have released every stage, so all loads of this CTA
+      // (the gathers too) have landed and all commits aimed at its barriers
+      // have arrived before it may exit.
+      for (int i = 0; i < kStages && ok; ++i) {
+        if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) break;
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------- MMA issuer (the leader) ----------------
+    if (leader) {
+      const bool elect = elect_one_sync();
+      int stage = 0, e = 0;
+      uint32_t phase = 0;
+      bool issued_any = false, ok = true;
+      int local = 0;
+      for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
+        const GroupTile t = group_tile_even(table, tile, n_blocks, e);
+        const uint32_t idesc = idesc_bf16_f32(256, tile_n(t));
+        const int acc = local & 1;
+        if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kAccCols);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!wait_all(&full[stage], phase)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t da = sdesc_kmajor_sw128(smem_u32(sA + stage * S::kABytes));
+          const uint64_t dw = sdesc_kmajor_sw128(smem_u32(sW + stage * S::kABytes));
+          if (elect) {
+#pragma unroll
+            for (int k = 0; k < kGemmBK / 16; ++k)
+              umma_bf16_pair(d_tmem, dw + k * 2, da + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
+            umma_commit_pair(&empty[stage], 0x3);
+          }
+          __syncwarp();
+          issued_any = true;
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (ok && elect) umma_commit_pair(&tfull[acc], 0x3);
+        __syncwarp();
+      }
+      if (issued_any) {
+        if (elect) umma_commit_pair(drain, 0x1);
+        __syncwarp();
+        wait_all(drain, 0);
+      }
+    }
+  } else if (warp < 10) {
+    // ---------------- epilogue ----------------
+    // TMEM lanes are W's columns: 32 of them a quarter, a warp for each half
+    // of the tile's rows.  A gated weight's quarters alternate between up and
+    // gate of the same 32 output columns, so the warps of quarters 2q and
+    // 2q + 1 work together: the gate's warp hands act(gate) over in shared
+    // memory, chunk by chunk in two buffers, and the up warp finishes.
+    constexpr bool kGated = grp_gated(EPI);
+    constexpr int kChunkBytes = EPI == kGrpF32 ? 4096 : 2048;
+    constexpr int kSlots = (kGated ? 4096 : S::kWarpStaging) / kChunkBytes;
+    const int quarter = warp & 3, half = (warp - 2) >> 2;
+    const bool gate = kGated && (quarter & 1);
+    const int pair = half * 2 + (quarter >> 1);  // gated: pair of warps
+    float *exchange = reinterpret_cast<float *>(staging + pair * 8192);
+    uint8_t *mine = kGated ? staging + 32768 + pair * 4096 : staging + (warp - 2) * S::kWarpStaging;
+    const int width = kGated ? p.N / 2 : p.N;
+    int slot = 0, buf = 0;
+    int local = 0, e = 0;
+    for (int tile = first; tile < num_tiles; tile += step, ++local) {
+      const int acc = local & 1;
+      bool ok = wait_all(&tfull[acc], (local >> 1) & 1);
+      if constexpr (kGated) ok = grp_pair_and(1 + pair, ok);
+      if (!ok) break;
+      tc_fence_after();
+      const GroupTile t = group_tile_even(table, tile, n_blocks, e);
+      // first W column of the quarter (of the pair of quarters), and of C
+      const int col = t.nb * 256 + rank * 128 + (kGated ? quarter & 2 : quarter) * 32;
+      const int c0 = kGated ? col / 2 : col;
+      const bool inside = c0 + lane < width;
+      float b = 0.f;
+      if (p.bias && inside)
+        b = __ldg(p.bias + static_cast<int64_t>(t.e) * p.N + c0 + lane + (gate ? width : 0));
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
+                             static_cast<uint32_t>(acc * kAccCols);
+      const int chunks = tile_n(t) / 32;
+      const int split = (chunks + 1) / 2;
+      if (c0 < width) {  // the same for both warps of a pair
+#pragma unroll 1
+        for (int c = half ? split : 0; c < (half ? chunks : split); ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(t_row + c * 32, r);
+          tmem_wait_ld_regs(r);
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2)
+            unpk2(add_x2(pk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), pk2(b, b)), v[i],
+                  v[i + 1]);
+          if constexpr (kGated) {
+            float *x = exchange + buf * 1024 + lane;
+            buf ^= 1;
+            if (gate) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                if constexpr (EPI == kGrpBf16SwiGLU) {
+                  v[i] = silu_fast(v[i]);
+                  v[i + 1] = silu_fast(v[i + 1]);
+                } else {
+                  gelu_erf_x2(v[i], v[i + 1]);
+                }
+                x[i * 32] = v[i];
+                x[i * 32 + 32] = v[i + 1];
+              }
+            }
+            // the buffer is written again two chunks on, past the next of
+            // these barriers, which the up warp reaches with this one read
+            grp_pair_sync(1 + pair);
+            if (gate) continue;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) v[i] *= x[i * 32];
+          } else if constexpr (EPI == kGrpBf16Gelu8) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) gelu8_x2(v[i], v[i + 1]);
+          } else if constexpr (EPI == kGrpBf16Erf) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) gelu_erf_x2(v[i], v[i + 1]);
+          }
+          const int row0 = t.row + c * 32;
+          if (row0 + 32 <= t.end) {
+            uint8_t *chunk = mine + slot * kChunkBytes;
+            if (++slot == kSlots) slot = 0;
+            if (lane == 0) bulk_wait_group_read<kSlots - 1>();
+            __syncwarp();
+            grp_stage_t<EPI>(v, chunk, lane);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_2d(&tmC, chunk, c0, row0);
+              bulk_commit_group();
+            }
+          } else if (inside) {
+            const int64_t at = static_cast<int64_t>(row0) * width + c0 + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              if (row0 + i < t.end) {
+                const int64_t o = at + static_cast<int64_t>(i) * width;
+                if constexpr (EPI == kGrpF32) static_cast<float *>(p.out)[o] = v[i];
+                else static_cast<__nv_bfloat16 *>(p.out)[o] = __float2bfloat16_rn(v[i]);
+              }
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      // (the fence orders the TMEM reads; a releasing arrive at cluster scope
+      // would also wait for this thread's outstanding accesses, a microsecond)
+      if (lane == 0) grp_arrive(map_to_cta(smem_u32(&tempty[acc]), 0));
+    }
+    if (lane == 0) bulk_wait_group_all();
+  } else if constexpr (GATHER) {
+    // ---------------- A by gathers (warps 10..17) ----------------
+    const int part = warp - 10;  // a share of this CTA's 128 rows
+    const bool elect = elect_one_sync();
+    int stage = 0, e = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int tile = first; tile < num_tiles && ok; tile += step) {
+      const GroupTile t = group_tile_even(table, tile, n_blocks, e);
+      const int count = min(max(cta_rows(t, rank) - kGatherRows * part, 0), kGatherRows);
+      int mine = 0;
+      if (count > 0) {
+        // past the group: its last row again, to fill a gather of four
+        const int at = t.row + rank * (tile_n(t) / 2) + kGatherRows * part + min(lane, count - 1);
+        mine = __ldg(p.row_src + at);
+        if (mine < 0 || mine >= p.a_rows) {
+          record_err(p.err, kDevBadGroup);
+          mine = 0;
+        }
+      }
+      int src[kGatherRows];
+#pragma unroll
+      for (int i = 0; i < kGatherRows; ++i) src[i] = __shfl_sync(0xffffffffu, mine, i);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!wait_all(&empty[stage], phase ^ 1u)) {
+          ok = false;
+          break;
+        }
+        if (elect) {
+          const uint32_t dst = smem_u32(sA + stage * S::kABytes) + part * (kGatherRows * 128);
+          const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
+#pragma unroll
+          for (int i = 0; i < kGatherRows / 4; ++i)
+            if (4 * i < count)
+              grp_gather4<2>(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
+                             src[4 * i + 2], src[4 * i + 3]);
+          grp_arrive(bar);
+        }
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync();  // no CTA leaves while its pair may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * kAccCols);
   }
 }
 

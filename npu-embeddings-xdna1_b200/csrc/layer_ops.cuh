@@ -18,24 +18,24 @@ int where_is(nebw_dev *d, const void *p, bool *on_device) {
   return NEBW_OK;
 }
 
-template <int CTAS, int EPI>
+template <int EPI>
 int set_grouped_attr() {
+  const auto a = cudaFuncAttributeMaxDynamicSharedMemorySize;
   const int smem = nebw::GroupedShape::kSmemBytes;
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<CTAS, EPI, false>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<CTAS, EPI, true>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<EPI, false>, a, smem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<EPI, true>, a, smem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_pair_kernel<EPI, false>, a, smem));
+  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_pair_kernel<EPI, true>, a, smem));
   return NEBW_OK;
 }
 
-template <int CTAS>
-int set_grouped_attrs_ctas() {
-  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16>()) return rc;
-  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16Gelu8>()) return rc;
-  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16Erf>()) return rc;
-  if (int rc = set_grouped_attr<CTAS, nebw::kGrpF32>()) return rc;
-  if (int rc = set_grouped_attr<CTAS, nebw::kGrpBf16SwiGLU>()) return rc;
-  return set_grouped_attr<CTAS, nebw::kGrpBf16GeGLU>();
+int set_grouped_attrs() {
+  if (int rc = set_grouped_attr<nebw::kGrpBf16>()) return rc;
+  if (int rc = set_grouped_attr<nebw::kGrpBf16Gelu8>()) return rc;
+  if (int rc = set_grouped_attr<nebw::kGrpBf16Erf>()) return rc;
+  if (int rc = set_grouped_attr<nebw::kGrpF32>()) return rc;
+  if (int rc = set_grouped_attr<nebw::kGrpBf16SwiGLU>()) return rc;
+  return set_grouped_attr<nebw::kGrpBf16GeGLU>();
 }
 
 // Shared memory of the placing kernels: starts and totals, and the row masks
@@ -67,8 +67,7 @@ int set_layer_op_attrs() {
   if (int rc = set_route_attrs<4>()) return rc;
   if (int rc = set_route_attrs<8>()) return rc;
   if (int rc = set_route_attrs<16>()) return rc;
-  if (int rc = set_grouped_attrs_ctas<1>()) return rc;
-  return set_grouped_attrs_ctas<2>();
+  return set_grouped_attrs();
 }
 
 }  // namespace
@@ -532,40 +531,41 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
 
 namespace {
 
-template <int CTAS, int EPI>
-void launch_grouped_epi(const CUtensorMap &mA, const CUtensorMap &mA128, const CUtensorMap &mW,
-                        const CUtensorMap &mC, const nebw::GroupedArgs &a, unsigned grid,
-                        cudaStream_t st) {
+struct GroupedMaps {
+  CUtensorMap a, a128, w, c;
+};
+
+template <int EPI>
+void launch_grouped_epi(const GroupedMaps &m, const nebw::GroupedArgs &a, bool pairs,
+                        unsigned grid, cudaStream_t st) {
   const size_t smem = nebw::GroupedShape::kSmemBytes;
-  if (a.row_src)
-    nebw::gemm_grouped_kernel<CTAS, EPI, true>
-        <<<grid, nebw::kGroupedGatherThreads, smem, st>>>(mA, mA128, mW, mC, a);
+  const int threads = a.row_src ? nebw::kGroupedGatherThreads : nebw::kGroupedThreads;
+  if (pairs && a.row_src)
+    nebw::gemm_grouped_pair_kernel<EPI, true><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
+  else if (pairs)
+    nebw::gemm_grouped_pair_kernel<EPI, false><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
+  else if (a.row_src)
+    nebw::gemm_grouped_kernel<EPI, true><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
   else
-    nebw::gemm_grouped_kernel<CTAS, EPI, false>
-        <<<grid, nebw::kGroupedThreads, smem, st>>>(mA, mA128, mW, mC, a);
+    nebw::gemm_grouped_kernel<EPI, false><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
 }
 
-// The most tiles that groups of `rows` rows in all can make: every group may
-// end in a part tile.
-int64_t grouped_tiles(int64_t rows, int64_t experts, int64_t tile_rows, int64_t n_blocks) {
-  return (rows / tile_rows + std::min(experts, rows)) * n_blocks;
-}
-
-template <int CTAS>
-int launch_grouped(nebw_dev *d, const CUtensorMap &mA, const CUtensorMap &mA128,
-                   const CUtensorMap &mW, const CUtensorMap &mC, int epi, const nebw::GroupedArgs &a, cudaStream_t st) {
-  const int64_t tiles = grouped_tiles(a.rows, a.experts, CTAS * nebw::kGemmBM,
-                                      (a.N + a.bn - 1) / a.bn);
+int launch_grouped(nebw_dev *d, const GroupedMaps &m, int epi, const nebw::GroupedArgs &a,
+                   bool pairs, cudaStream_t st) {
+  // the most tiles that the groups can make: every one may end in a part tile
+  const int64_t tile_rows = pairs ? 256 : nebw::kGemmBM, tile_cols = pairs ? 256 : a.bn;
+  const int64_t tiles = (a.rows / tile_rows + std::min(a.experts, a.rows)) *
+                        ((a.N + tile_cols - 1) / tile_cols);
   NEBW_REQUIRE(tiles < (1ll << 31), "grouped product too large");
   const unsigned g = static_cast<unsigned>(
-      CTAS * std::min<int64_t>(tiles, CTAS == 2 ? d->gemm_pairs : d->sm_count));
+      pairs ? 2 * std::min<int64_t>(tiles, d->gemm_pairs) : std::min<int64_t>(tiles, d->sm_count));
   switch (epi) {
-    case nebw::kGrpBf16: launch_grouped_epi<CTAS, nebw::kGrpBf16>(mA, mA128, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16Gelu8: launch_grouped_epi<CTAS, nebw::kGrpBf16Gelu8>(mA, mA128, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16Erf: launch_grouped_epi<CTAS, nebw::kGrpBf16Erf>(mA, mA128, mW, mC, a, g, st); break;
-    case nebw::kGrpF32: launch_grouped_epi<CTAS, nebw::kGrpF32>(mA, mA128, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16SwiGLU>(mA, mA128, mW, mC, a, g, st); break;
-    case nebw::kGrpBf16GeGLU: launch_grouped_epi<CTAS, nebw::kGrpBf16GeGLU>(mA, mA128, mW, mC, a, g, st); break;
+    case nebw::kGrpBf16: launch_grouped_epi<nebw::kGrpBf16>(m, a, pairs, g, st); break;
+    case nebw::kGrpBf16Gelu8: launch_grouped_epi<nebw::kGrpBf16Gelu8>(m, a, pairs, g, st); break;
+    case nebw::kGrpBf16Erf: launch_grouped_epi<nebw::kGrpBf16Erf>(m, a, pairs, g, st); break;
+    case nebw::kGrpF32: launch_grouped_epi<nebw::kGrpF32>(m, a, pairs, g, st); break;
+    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<nebw::kGrpBf16SwiGLU>(m, a, pairs, g, st); break;
+    case nebw::kGrpBf16GeGLU: launch_grouped_epi<nebw::kGrpBf16GeGLU>(m, a, pairs, g, st); break;
   }
   NEBW_CUDA(cudaGetLastError());
   return NEBW_OK;
@@ -624,24 +624,24 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   else if (c_dtype == NEBW_F32) epi = nebw::kGrpF32;
   else if (act == NEBW_ACT_GELU8) epi = nebw::kGrpBf16Gelu8;
   else if (act == NEBW_ACT_GELU_ERF) epi = nebw::kGrpBf16Erf;
-  CUtensorMap mA, mA128, mC;
-  if (int rc = make_tmap_kmajor(&mA, A, a_rows, K, row_src ? 1 : nebw::kGroupedBox)) return rc;
-  if (row_src) mA128 = mA;  // not used
-  else if (int rc = make_tmap_kmajor(&mA128, A, a_rows, K, nebw::kGemmBM)) return rc;
-  if (int rc = make_tmap_out(&mC, C, rows, w.gated ? N / 2 : N, c_dtype == NEBW_BF16)) return rc;
+  GroupedMaps m;
+  if (int rc = make_tmap_kmajor(&m.a, A, a_rows, K, row_src ? 1 : nebw::kGroupedBox)) return rc;
+  if (row_src) m.a128 = m.a;  // not used
+  else if (int rc = make_tmap_kmajor(&m.a128, A, a_rows, K, nebw::kGemmBM)) return rc;
+  if (int rc = make_tmap_out(&m.c, C, rows, w.gated ? N / 2 : N, c_dtype == NEBW_BF16)) return rc;
   const cudaStream_t st = pick_stream(d, stream);
   const int64_t groups = std::min<int64_t>(w.experts, rows);
-  static const int kThr = std::getenv("GRP_THR") ? std::atoi(std::getenv("GRP_THR")) : 384;
-  if (d->gemm_pairs > 0 && rows >= kThr * groups && N >= 256) {
-    a.bn = 256;
-    return launch_grouped<2>(d, mA, mA128, w.map128, mC, epi, a, st);
+  static const int kThr = std::getenv("GRP_THR") ? std::atoi(std::getenv("GRP_THR")) : 32;
+  if (d->gemm_pairs > 0 && rows >= kThr * groups && N >= 128) {
+    m.w = w.map128;
+    return launch_grouped(d, m, epi, a, true, st);
   }
   // one CTA a tile; narrower tiles while the groups' columns leave SMs idle
   a.bn = 128;
   const int least = w.gated ? 64 : 32;
   while (a.bn > least && groups * ((N + a.bn - 1) / a.bn) < d->sm_count) a.bn /= 2;
-  const CUtensorMap &mW = a.bn == 128 ? w.map128 : a.bn == 64 ? w.map64 : w.map32;
-  return launch_grouped<1>(d, mA, mA128, mW, mC, epi, a, st);
+  m.w = a.bn == 128 ? w.map128 : a.bn == 64 ? w.map64 : w.map32;
+  return launch_grouped(d, m, epi, a, false, st);
 }
 
 namespace {
