@@ -79,7 +79,8 @@ struct GroupedShape {
   static constexpr int kWarpStaging = 6 * 1024;  // one fp32 or three bf16 chunks
   static constexpr int kStagingBytes = 8 * kWarpStaging;
   static constexpr int kBarBytes = 256;
-  static constexpr int kTableBytes = 2 * (kGroupMaxExperts + 1) * 4;
+  static constexpr int kList = 128;  // tiles of a block looked up beforehand
+  static constexpr int kTableBytes = kList * 16 + 2 * (kGroupMaxExperts + 1) * 4 + 8;
   static constexpr int kSmemBytes =
       1024 + kStages * kStageBytes + kStagingBytes + kBarBytes + kTableBytes;
 };
@@ -133,16 +134,47 @@ __device__ __forceinline__ void grp_gather4(uint32_t dst, const void *tmap, uint
         : "memory");
 }
 
+// A tile of the list: expert, its rows [row, end) and the column block.
+struct alignas(16) GroupTile {
+  int e, row, end, nb;
+};
+
 // The groups in shared memory: off clamped to [0, rows] and ascending (a
-// fault is reported), and the first tile of every expert.
+// fault is reported), the first tile of every expert, and this block's first
+// tiles.
 struct GroupTable {
+  GroupTile list[GroupedShape::kList];
   int off[kGroupMaxExperts + 1];
   int tile[kGroupMaxExperts + 1];
 };
 static_assert(sizeof(GroupTable) == GroupedShape::kTableBytes, "table size");
 
+// Tile t.  EVEN: a group of m rows is cut into ceil(m / bm) tiles of equal
+// size, rounded up to 32 rows; otherwise into tiles of bm rows and a rest.
+template <bool EVEN>
+__device__ __forceinline__ GroupTile group_find(const GroupTable &g, const GroupedArgs &p, int t,
+                                                int bm, int n_blocks) {
+  int lo = 0, hi = p.experts;  // tile[lo] <= t < tile[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t >= g.tile[mid]) lo = mid;
+    else hi = mid;
+  }
+  const int i = t - g.tile[lo], b = i / n_blocks;
+  const int m = g.off[lo + 1] - g.off[lo];
+  int size = bm;
+  if constexpr (EVEN) {
+    const int tiles = (m + bm - 1) / bm;
+    size = ((m + tiles - 1) / tiles + 31) / 32 * 32;
+  }
+  const int row = g.off[lo] + b * size;
+  return {lo, row, min(row + size, g.off[lo + 1]), i - b * n_blocks};
+}
+
+// The table, for the tiles first, first + step, ... of this block.
+template <bool EVEN>
 __device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedArgs &p, int bm,
-                                                  int n_blocks) {
+                                                  int n_blocks, int first, int step) {
   for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) g.off[e] = __ldg(p.off + e);
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -181,34 +213,19 @@ __device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedAr
     if (bad && blockIdx.x == 0) record_err(p.err, kDevBadGroup);
   }
   __syncthreads();
+  const int last = g.tile[p.experts];
+  for (int i = threadIdx.x; i < GroupedShape::kList; i += blockDim.x) {
+    const int64_t t = first + static_cast<int64_t>(i) * step;
+    if (t < last) g.list[i] = group_find<EVEN>(g, p, static_cast<int>(t), bm, n_blocks);
+  }
+  __syncthreads();
 }
 
-// A tile of the list: expert, its rows [row, end) and the column block.
-struct GroupTile {
-  int e, row, end, nb;
-};
-
-// The tile `t`, walking on from expert `e` (t does not decrease from call to call).
-__device__ __forceinline__ GroupTile group_tile(const GroupTable &g, int t, int bm, int n_blocks,
-                                                int &e) {
-  while (t >= g.tile[e + 1]) ++e;
-  const int i = t - g.tile[e];
-  const int mb = i / n_blocks;
-  return {e, g.off[e] + mb * bm, g.off[e + 1], i - mb * n_blocks};
-}
-
-// The same for the pair kernel: a group of m rows is cut into ceil(m / 256)
-// tiles of equal size, rounded up to 32 rows.
-__device__ __forceinline__ GroupTile group_tile_even(const GroupTable &g, int t, int n_blocks,
-                                                     int &e) {
-  while (t >= g.tile[e + 1]) ++e;
-  const int i = t - g.tile[e];
-  const int tb = i / n_blocks;
-  const int m = g.off[e + 1] - g.off[e];
-  const int tiles = (m + 255) / 256;
-  const int size = ((m + tiles - 1) / tiles + 31) / 32 * 32;
-  const int row = g.off[e] + tb * size;
-  return {e, row, min(row + size, g.off[e + 1]), i - tb * n_blocks};
+// This block's tile number `local`, tile t.
+template <bool EVEN>
+__device__ __forceinline__ GroupTile group_tile(const GroupTable &g, const GroupedArgs &p,
+                                                int local, int t, int bm, int n_blocks) {
+  return local < GroupedShape::kList ? g.list[local] : group_find<EVEN>(g, p, t, bm, n_blocks);
 }
 
 // 32 accumulator columns of one row from GEMM column col0 on (a gated
@@ -357,7 +374,7 @@ __global__ void __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThrea
     tmem_alloc(tmem_slot, 2 * kAccCols);
     tmem_relinquish();
   }
-  group_table_build(table, p, kGemmBM, n_blocks);
+  group_table_build<false>(table, p, kGemmBM, n_blocks, blockIdx.x, gridDim.x);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -370,11 +387,11 @@ __global__ void __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThrea
   if (warp == 0) {
     // ---------------- W (and grouped A) producer ----------------
     if (lane == 0) {
-      int stage = 0, e = 0;
+      int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-        const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
+      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
+        const GroupTile t = group_tile<false>(table, p, local, tile, kGemmBM, n_blocks);
         const int m = min(t.end - t.row, kGemmBM);
         const int a_boxes = GATHER ? 0 : (m + kGroupedBox - 1) / kGroupedBox;
         const uint32_t bytes = static_cast<uint32_t>(bn) * kGemmBK * 2 +
@@ -476,12 +493,12 @@ __global__ void __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThrea
     const int width = kGated ? p.N / 2 : p.N;
     uint8_t *mine = staging + (warp - 2) * S::kWarpStaging;
     int slot = 0;
-    int local = 0, e = 0;
+    int local = 0;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
       const int acc = local & 1;
       if (!wait_all(&tfull[acc], (local >> 1) & 1)) break;
       tc_fence_after();
-      const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
+      const GroupTile t = group_tile<false>(table, p, local, tile, kGemmBM, n_blocks);
       const int row0 = t.row + quarter * 32;
       const float *bias = p.bias ? p.bias + static_cast<int64_t>(t.e) * p.N : nullptr;
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
@@ -529,11 +546,11 @@ __global__ void __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThrea
     // ---------------- A by gathers (warps 10..17) ----------------
     const int part = warp - 10;  // a share of this CTA's 128 rows
     const bool elect = elect_one_sync();
-    int stage = 0, e = 0;
+    int stage = 0, local = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x) {
-      const GroupTile t = group_tile(table, tile, kGemmBM, n_blocks, e);
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
+      const GroupTile t = group_tile<false>(table, p, local, tile, kGemmBM, n_blocks);
       const int count = min(max(t.end - t.row - kGatherRows * part, 0), kGatherRows);
       int mine = 0;
       if (count > 0) {
@@ -598,22 +615,76 @@ __device__ __forceinline__ void grp_pair_sync(int id) {
   asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory");
 }
 
-// One value of C's column per lane, 32 rows: column `lane` of a 32 x 32 chunk
-// in the output map's swizzle (the transposed twin of grp_stage).  bf16 lanes
-// in pairs share a 32-bit word and rows differ in bank, so a store of one row
-// by the warp has no conflict.
+// A 32 x 32 chunk of the accumulator, 32 lanes of the warp's quarter by 32
+// columns, as mma fragments (tcgen05.ld 16x256b): of lanes 8 q .. 8 q + 7 and
+// columns 8 c .. 8 c + 7, thread T holds lane T / 4, columns 2 (T % 4) and + 1,
+// in r[16 (q / 2) + 4 c + 2 (q % 2)] and the one after.
+__device__ __forceinline__ void grp_load_chunk(uint32_t taddr, uint32_t (&r)[32]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]),
+          "=r"(r[16 * h + 4]), "=r"(r[16 * h + 5]), "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]),
+          "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]), "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]),
+          "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]), "=r"(r[16 * h + 14]), "=r"(r[16 * h + 15])
+        : "r"(taddr + (static_cast<uint32_t>(16 * h) << 16))
+        : "memory");
+  tmem_wait_ld_regs(r);
+}
+
+// The biases of this thread's columns of a chunk (0 where there are none).
+__device__ __forceinline__ void grp_bias4(const float *bias, int c, int width, float (&b)[4]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) b[q] = bias && c + 8 * q < width ? __ldg(bias + c + 8 * q) : 0.f;
+}
+
+// The chunk as rows of C in shared memory, in the output map's swizzle
+// (make_tmap_out): bf16 by stmatrix.trans, four 8 x 8 blocks an instruction
+// (the four column blocks of eight rows: each lane names a 16-byte piece, and
+// the pieces of a block lie in different banks); fp32 value by value.
 template <int EPI>
 __device__ __forceinline__ void grp_stage_t(const float (&v)[32], uint8_t *chunk, int lane) {
   if constexpr (EPI == kGrpF32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      *reinterpret_cast<float *>(chunk + i * 128 + (((lane >> 2) ^ (i & 7)) << 4) +
-                                 (lane & 3) * 4) = v[i];
+    for (int i = 0; i < 32; ++i) {
+      const int c = (lane >> 2) + 8 * (2 * (i / 16) + (i % 4) / 2);
+      const int row = 8 * (i / 4 % 4) + 2 * (lane & 3) + i % 2;
+      *reinterpret_cast<float *>(chunk + row * 128 + (((c >> 2) ^ (row & 7)) << 4) + (c & 3) * 4) =
+          v[i];
+    }
   } else {
 #pragma unroll
-    for (int i = 0; i < 32; ++i)
-      *reinterpret_cast<__nv_bfloat16 *>(chunk + i * 64 + (((lane >> 3) ^ ((i >> 1) & 3)) << 4) +
-                                         (lane & 7) * 2) = __float2bfloat16_rn(v[i]);
+    for (int i = 0; i < 4; ++i) {  // rows 8 i .. 8 i + 7
+      const int row = 8 * i + (lane & 7), q = lane >> 3;
+      const uint32_t at = smem_u32(chunk + row * 64 + ((q ^ ((row >> 1) & 3)) << 4));
+      asm volatile(
+          "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at),
+          "r"(pack_bf16x2(v[4 * i], v[4 * i + 1])), "r"(pack_bf16x2(v[4 * i + 2], v[4 * i + 3])),
+          "r"(pack_bf16x2(v[16 + 4 * i], v[16 + 4 * i + 1])),
+          "r"(pack_bf16x2(v[16 + 4 * i + 2], v[16 + 4 * i + 3]))
+          : "memory");
+    }
+  }
+}
+
+// The staged rows [row0, end) of a chunk in which a group ends, by 16-byte
+// pieces (the width is a multiple of 8 elements).
+template <int EPI>
+__device__ __forceinline__ void grp_store_rows(void *out, const uint8_t *chunk, int row0, int end,
+                                               int c0, int width, int lane) {
+  constexpr int kPieces = EPI == kGrpF32 ? 8 : 4, kRows = 32 / kPieces;
+  constexpr int kSize = EPI == kGrpF32 ? 4 : 2, kPer = 16 / kSize;
+  const int piece = lane % kPieces;
+  if (c0 + piece * kPer >= width) return;
+  for (int i = lane / kPieces; i < 32 && row0 + i < end; i += kRows) {
+    const int sw = EPI == kGrpF32 ? i & 7 : (i >> 1) & 3;
+    const uint4 u = *reinterpret_cast<const uint4 *>(chunk + i * (kPieces * 16) +
+                                                     ((piece ^ sw) << 4));
+    *reinterpret_cast<uint4 *>(
+        static_cast<uint8_t *>(out) +
+        (static_cast<int64_t>(row0 + i) * width + c0 + piece * kPer) * kSize) = u;
   }
 }
 
@@ -672,7 +743,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     tmem_alloc_pair(tmem_slot, 2 * kAccCols);
     tmem_relinquish_pair();
   }
-  group_table_build(table, p, 256, n_blocks);
+  group_table_build<true>(table, p, 256, n_blocks, first, step);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
@@ -692,11 +763,11 @@ __global__ void __cluster_dims__(2, 1, 1)
   if (warp == 0) {
     // ---------------- W (and grouped A) producer, both CTAs ----------------
     if (lane == 0) {
-      int stage = 0, e = 0;
+      int stage = 0, local = 0;
       uint32_t phase = 0;
       bool ok = true;
-      for (int tile = first; tile < num_tiles && ok; tile += step) {
-        const GroupTile t = group_tile_even(table, tile, n_blocks, e);
+      for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
+        const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
         uint32_t bytes = 2 * S::kABytes;  // W
         for (int c = 0; c < 2; ++c) {
           const int m = cta_rows(t, c);
@@ -742,12 +813,12 @@ __global__ void __cluster_dims__(2, 1, 1)
     // ---------------- MMA issuer (the leader) ----------------
     if (leader) {
       const bool elect = elect_one_sync();
-      int stage = 0, e = 0;
+      int stage = 0;
       uint32_t phase = 0;
       bool issued_any = false, ok = true;
       int local = 0;
       for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-        const GroupTile t = group_tile_even(table, tile, n_blocks, e);
+        const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
         const uint32_t idesc = idesc_bf16_f32(256, tile_n(t));
         const int acc = local & 1;
         if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
@@ -786,102 +857,127 @@ __global__ void __cluster_dims__(2, 1, 1)
   } else if (warp < 10) {
     // ---------------- epilogue ----------------
     // TMEM lanes are W's columns: 32 of them a quarter, a warp for each half
-    // of the tile's rows.  A gated weight's quarters alternate between up and
-    // gate of the same 32 output columns, so the warps of quarters 2q and
-    // 2q + 1 work together: the gate's warp hands act(gate) over in shared
-    // memory, chunk by chunk in two buffers, and the up warp finishes.
+    // of the tile's rows, 32 x 32 chunks in the fragment layout that stmatrix
+    // turns over.  A gated weight's quarters alternate between up and gate of
+    // the same 32 output columns, so the warps of quarters 2q and 2q + 1 work
+    // on two chunks together: each hands the other its values of one chunk
+    // through shared memory and finishes the other.
     constexpr bool kGated = grp_gated(EPI);
     constexpr int kChunkBytes = EPI == kGrpF32 ? 4096 : 2048;
-    constexpr int kSlots = (kGated ? 4096 : S::kWarpStaging) / kChunkBytes;
+    constexpr int kSlots = kGated ? 1 : S::kWarpStaging / kChunkBytes;
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    const bool gate = kGated && (quarter & 1);
+    const int gate = kGated ? quarter & 1 : 0;
     const int pair = half * 2 + (quarter >> 1);  // gated: pair of warps
-    float *exchange = reinterpret_cast<float *>(staging + pair * 8192);
-    uint8_t *mine = kGated ? staging + 32768 + pair * 4096 : staging + (warp - 2) * S::kWarpStaging;
+    float4 *send = reinterpret_cast<float4 *>(staging + pair * 8192 + gate * 4096) + lane;
+    const float4 *receive =
+        reinterpret_cast<float4 *>(staging + pair * 8192 + (gate ^ 1) * 4096) + lane;
+    uint8_t *mine = kGated ? staging + 32768 + (warp - 2) * 2048
+                           : staging + (warp - 2) * S::kWarpStaging;
     const int width = kGated ? p.N / 2 : p.N;
-    int slot = 0, buf = 0;
-    int local = 0, e = 0;
+    int slot = 0;
+    int local = 0;
     for (int tile = first; tile < num_tiles; tile += step, ++local) {
       const int acc = local & 1;
+      const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
+      // first W column of the quarter (of the pair of quarters), and of C
+      const int col = t.nb * 256 + rank * 128 + (kGated ? quarter & 2 : quarter) * 32;
+      const int c0 = kGated ? col / 2 : col;
+      // this thread's columns of a chunk: c0 + lane / 4 + {0, 8, 16, 24}
+      float b[4], bg[4];
+      grp_bias4(p.bias ? p.bias + static_cast<int64_t>(t.e) * p.N : nullptr, c0 + (lane >> 2),
+                width, b);
+      if constexpr (kGated)
+        grp_bias4(p.bias ? p.bias + static_cast<int64_t>(t.e) * p.N + width : nullptr,
+                  c0 + (lane >> 2), width, bg);
       bool ok = wait_all(&tfull[acc], (local >> 1) & 1);
       if constexpr (kGated) ok = grp_pair_and(1 + pair, ok);
       if (!ok) break;
       tc_fence_after();
-      const GroupTile t = group_tile_even(table, tile, n_blocks, e);
-      // first W column of the quarter (of the pair of quarters), and of C
-      const int col = t.nb * 256 + rank * 128 + (kGated ? quarter & 2 : quarter) * 32;
-      const int c0 = kGated ? col / 2 : col;
-      const bool inside = c0 + lane < width;
-      float b = 0.f;
-      if (p.bias && inside)
-        b = __ldg(p.bias + static_cast<int64_t>(t.e) * p.N + c0 + lane + (gate ? width : 0));
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
                              static_cast<uint32_t>(acc * kAccCols);
       const int chunks = tile_n(t) / 32;
       const int split = (chunks + 1) / 2;
+      const int begin = half ? split : 0, end = half ? chunks : split;
       if (c0 < width) {  // the same for both warps of a pair
 #pragma unroll 1
-        for (int c = half ? split : 0; c < (half ? chunks : split); ++c) {
+        for (int c = begin; c < end; c += kGated ? 2 : 1) {
           uint32_t r[32];
-          tmem_ld_32x32b_x32(t_row + c * 32, r);
-          tmem_wait_ld_regs(r);
+          int at = c;  // the chunk this warp finishes
+          if constexpr (kGated) {
+            // up: keeps c, hands over c + 1; gate: hands over c, keeps c + 1
+            const bool two = c + 1 < end;
+            if (gate || two) {
+              grp_load_chunk(t_row + (gate ? c : c + 1) * 32, r);
+              // the other warp has read what this one handed over before
+              grp_pair_sync(1 + pair);
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                send[i * 32] = make_float4(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]),
+                                           __uint_as_float(r[4 * i + 2]),
+                                           __uint_as_float(r[4 * i + 3]));
+            } else {
+              grp_pair_sync(1 + pair);
+            }
+            at = gate ? c + 1 : c;
+            if (at < end) grp_load_chunk(t_row + at * 32, r);
+            grp_pair_sync(1 + pair);
+            if (at >= end) continue;
+          } else {
+            grp_load_chunk(t_row + c * 32, r);
+          }
+          // entry 4 i + j: column lane / 4 + 8 * (2 * (i / 4) + j / 2), row
+          // 8 * (i % 4) + 2 * (lane % 4) + j % 2
           float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2)
-            unpk2(add_x2(pk2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), pk2(b, b)), v[i],
-                  v[i + 1]);
-          if constexpr (kGated) {
-            float *x = exchange + buf * 1024 + lane;
-            buf ^= 1;
-            if (gate) {
+          for (int i = 0; i < 8; ++i) {
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                if constexpr (EPI == kGrpBf16SwiGLU) {
-                  v[i] = silu_fast(v[i]);
-                  v[i + 1] = silu_fast(v[i + 1]);
-                } else {
-                  gelu_erf_x2(v[i], v[i + 1]);
+            for (int j = 0; j < 4; j += 2) {
+              const float bj = b[2 * (i / 4) + j / 2];
+              float x0 = __uint_as_float(r[4 * i + j]), x1 = __uint_as_float(r[4 * i + j + 1]);
+              if constexpr (kGated) {
+                const float2 o = *(reinterpret_cast<const float2 *>(receive + i * 32) + j / 2);
+                const float gj = bg[2 * (i / 4) + j / 2];
+                float g0 = (gate ? x0 : o.x) + gj, g1 = (gate ? x1 : o.y) + gj;
+                if (gate) {
+                  x0 = o.x;
+                  x1 = o.y;
                 }
-                x[i * 32] = v[i];
-                x[i * 32 + 32] = v[i + 1];
+                x0 += bj;
+                x1 += bj;
+                if constexpr (EPI == kGrpBf16SwiGLU) {
+                  x0 *= silu_fast(g0);
+                  x1 *= silu_fast(g1);
+                } else {
+                  gelu_erf_x2(g0, g1);
+                  x0 *= g0;
+                  x1 *= g1;
+                }
+              } else {
+                x0 += bj;
+                x1 += bj;
+                if constexpr (EPI == kGrpBf16Gelu8) gelu8_x2(x0, x1);
+                if constexpr (EPI == kGrpBf16Erf) gelu_erf_x2(x0, x1);
               }
+              v[4 * i + j] = x0;
+              v[4 * i + j + 1] = x1;
             }
-            // the buffer is written again two chunks on, past the next of
-            // these barriers, which the up warp reaches with this one read
-            grp_pair_sync(1 + pair);
-            if (gate) continue;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= x[i * 32];
-          } else if constexpr (EPI == kGrpBf16Gelu8) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) gelu8_x2(v[i], v[i + 1]);
-          } else if constexpr (EPI == kGrpBf16Erf) {
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) gelu_erf_x2(v[i], v[i + 1]);
           }
-          const int row0 = t.row + c * 32;
+          uint8_t *chunk = mine + slot * kChunkBytes;
+          if (lane == 0) bulk_wait_group_read<kSlots - 1>();
+          __syncwarp();
+          grp_stage_t<EPI>(v, chunk, lane);
+          const int row0 = t.row + at * 32;
           if (row0 + 32 <= t.end) {
-            uint8_t *chunk = mine + slot * kChunkBytes;
-            if (++slot == kSlots) slot = 0;
-            if (lane == 0) bulk_wait_group_read<kSlots - 1>();
-            __syncwarp();
-            grp_stage_t<EPI>(v, chunk, lane);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
               tma_store_2d(&tmC, chunk, c0, row0);
               bulk_commit_group();
             }
-          } else if (inside) {
-            const int64_t at = static_cast<int64_t>(row0) * width + c0 + lane;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (row0 + i < t.end) {
-                const int64_t o = at + static_cast<int64_t>(i) * width;
-                if constexpr (EPI == kGrpF32) static_cast<float *>(p.out)[o] = v[i];
-                else static_cast<__nv_bfloat16 *>(p.out)[o] = __float2bfloat16_rn(v[i]);
-              }
-            }
+            if (++slot == kSlots) slot = 0;
+          } else {
+            __syncwarp();
+            grp_store_rows<EPI>(p.out, chunk, row0, t.end, c0, width, lane);
           }
           __syncwarp();
         }
@@ -897,11 +993,11 @@ __global__ void __cluster_dims__(2, 1, 1)
     // ---------------- A by gathers (warps 10..17) ----------------
     const int part = warp - 10;  // a share of this CTA's 128 rows
     const bool elect = elect_one_sync();
-    int stage = 0, e = 0;
+    int stage = 0, local = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = first; tile < num_tiles && ok; tile += step) {
-      const GroupTile t = group_tile_even(table, tile, n_blocks, e);
+    for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
+      const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
       const int count = min(max(cta_rows(t, rank) - kGatherRows * part, 0), kGatherRows);
       int mine = 0;
       if (count > 0) {
