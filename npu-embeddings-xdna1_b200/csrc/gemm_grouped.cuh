@@ -40,6 +40,7 @@
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "gemm_tc.cuh"
 #include "ptx.cuh"
@@ -544,23 +545,32 @@ __global__ void __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThrea
     if (lane == 0) bulk_wait_group_all();
   } else if constexpr (GATHER) {
     // ---------------- A by gathers (warps 10..17) ----------------
-    const int part = warp - 10;  // a share of this CTA's 128 rows
+    const int part = warp - 10;  // a share of the tile's 128 rows
     const bool elect = elect_one_sync();
     int stage = 0, local = 0;
     uint32_t phase = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
-      const GroupTile t = group_tile<false>(table, p, local, tile, kGemmBM, n_blocks);
-      const int count = min(max(t.end - t.row - kGatherRows * part, 0), kGatherRows);
-      int mine = 0;
-      if (count > 0) {
-        // past the group: its last row again, to fill a gather of four
-        const int at = t.row + kGatherRows * part + min(lane, count - 1);
-        mine = __ldg(p.row_src + at);
-        if (mine < 0 || mine >= p.a_rows) {
-          record_err(p.err, kDevBadGroup);
-          mine = 0;
-        }
+    // this warp's rows of a tile, and the lane's row of A for one of them;
+    // a tile's are read while the one before is loaded
+    auto count_of = [&](const GroupTile &t) -> int {
+      return min(max(t.end - t.row - kGatherRows * part, 0), kGatherRows);
+    };
+    auto index_of = [&](int l, int tile) -> int {
+      if (tile >= num_tiles) return 0;
+      const GroupTile t = group_tile<false>(table, p, l, tile, kGemmBM, n_blocks);
+      const int count = count_of(t);
+      // past the group: its last row again, to fill a gather of four
+      return count ? __ldg(p.row_src + t.row + kGatherRows * part + min(lane, count - 1)) : 0;
+    };
+    const int stride = gridDim.x;
+    int next = index_of(0, blockIdx.x);
+    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += stride, ++local) {
+      const int count = count_of(group_tile<false>(table, p, local, tile, kGemmBM, n_blocks));
+      int mine = next;
+      next = index_of(local + 1, tile + stride);
+      if (mine < 0 || mine >= p.a_rows) {
+        record_err(p.err, kDevBadGroup);
+        mine = 0;
       }
       int src[kGatherRows];
 #pragma unroll
@@ -644,28 +654,25 @@ __device__ __forceinline__ void grp_bias4(const float *bias, int c, int width, f
 // (make_tmap_out): bf16 by stmatrix.trans, four 8 x 8 blocks an instruction
 // (the four column blocks of eight rows: each lane names a 16-byte piece, and
 // the pieces of a block lie in different banks); fp32 value by value.
-template <int EPI>
 __device__ __forceinline__ void grp_stage_t(const float (&v)[32], uint8_t *chunk, int lane) {
-  if constexpr (EPI == kGrpF32) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      const int c = (lane >> 2) + 8 * (2 * (i / 16) + (i % 4) / 2);
-      const int row = 8 * (i / 4 % 4) + 2 * (lane & 3) + i % 2;
-      *reinterpret_cast<float *>(chunk + row * 128 + (((c >> 2) ^ (row & 7)) << 4) + (c & 3) * 4) =
-          v[i];
-    }
-  } else {
+  for (int i = 0; i < 32; ++i) {
+    const int c = (lane >> 2) + 8 * (2 * (i / 16) + (i % 4) / 2);
+    const int row = 8 * (i / 4 % 4) + 2 * (lane & 3) + i % 2;
+    *reinterpret_cast<float *>(chunk + row * 128 + (((c >> 2) ^ (row & 7)) << 4) + (c & 3) * 4) =
+        v[i];
+  }
+}
+// m[i]: entries 2 i and 2 i + 1 of the chunk as bf16.
+__device__ __forceinline__ void grp_stage_t(const uint32_t (&m)[16], uint8_t *chunk, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {  // rows 8 i .. 8 i + 7
-      const int row = 8 * i + (lane & 7), q = lane >> 3;
-      const uint32_t at = smem_u32(chunk + row * 64 + ((q ^ ((row >> 1) & 3)) << 4));
-      asm volatile(
-          "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at),
-          "r"(pack_bf16x2(v[4 * i], v[4 * i + 1])), "r"(pack_bf16x2(v[4 * i + 2], v[4 * i + 3])),
-          "r"(pack_bf16x2(v[16 + 4 * i], v[16 + 4 * i + 1])),
-          "r"(pack_bf16x2(v[16 + 4 * i + 2], v[16 + 4 * i + 3]))
-          : "memory");
-    }
+  for (int i = 0; i < 4; ++i) {  // rows 8 i .. 8 i + 7
+    const int row = 8 * i + (lane & 7), q = lane >> 3;
+    const uint32_t at = smem_u32(chunk + row * 64 + ((q ^ ((row >> 1) & 3)) << 4));
+    asm volatile(
+        "stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(at),
+        "r"(m[2 * i]), "r"(m[2 * i + 1]), "r"(m[8 + 2 * i]), "r"(m[8 + 2 * i + 1])
+        : "memory");
   }
 }
 
@@ -927,7 +934,8 @@ __global__ void __cluster_dims__(2, 1, 1)
           }
           // entry 4 i + j: column lane / 4 + 8 * (2 * (i / 4) + j / 2), row
           // 8 * (i % 4) + 2 * (lane % 4) + j % 2
-          float v[32];
+          // (narrowed as they are made: 16 registers a chunk instead of 32)
+          std::conditional_t<EPI == kGrpF32, float[32], uint32_t[16]> v;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
 #pragma unroll
@@ -958,14 +966,18 @@ __global__ void __cluster_dims__(2, 1, 1)
                 if constexpr (EPI == kGrpBf16Gelu8) gelu8_x2(x0, x1);
                 if constexpr (EPI == kGrpBf16Erf) gelu_erf_x2(x0, x1);
               }
-              v[4 * i + j] = x0;
-              v[4 * i + j + 1] = x1;
+              if constexpr (EPI == kGrpF32) {
+                v[4 * i + j] = x0;
+                v[4 * i + j + 1] = x1;
+              } else {
+                v[2 * i + j / 2] = pack_bf16x2(x0, x1);
+              }
             }
           }
           uint8_t *chunk = mine + slot * kChunkBytes;
           if (lane == 0) bulk_wait_group_read<kSlots - 1>();
           __syncwarp();
-          grp_stage_t<EPI>(v, chunk, lane);
+          grp_stage_t(v, chunk, lane);
           const int row0 = t.row + at * 32;
           if (row0 + 32 <= t.end) {
             fence_proxy_async_smem();
@@ -996,18 +1008,28 @@ __global__ void __cluster_dims__(2, 1, 1)
     int stage = 0, local = 0;
     uint32_t phase = 0;
     bool ok = true;
+    // this warp's rows of a tile, and the lane's row of A for one of them;
+    // a tile's are read while the one before is loaded
+    auto count_of = [&](const GroupTile &t) -> int {
+      return min(max(cta_rows(t, rank) - kGatherRows * part, 0), kGatherRows);
+    };
+    auto index_of = [&](int l, int tile) -> int {
+      if (tile >= num_tiles) return 0;
+      const GroupTile t = group_tile<true>(table, p, l, tile, 256, n_blocks);
+      const int count = count_of(t);
+      // past the group: its last row again, to fill a gather of four
+      return count ? __ldg(p.row_src + t.row + rank * (tile_n(t) / 2) + kGatherRows * part +
+                           min(lane, count - 1))
+                   : 0;
+    };
+    int next = index_of(0, first);
     for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-      const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
-      const int count = min(max(cta_rows(t, rank) - kGatherRows * part, 0), kGatherRows);
-      int mine = 0;
-      if (count > 0) {
-        // past the group: its last row again, to fill a gather of four
-        const int at = t.row + rank * (tile_n(t) / 2) + kGatherRows * part + min(lane, count - 1);
-        mine = __ldg(p.row_src + at);
-        if (mine < 0 || mine >= p.a_rows) {
-          record_err(p.err, kDevBadGroup);
-          mine = 0;
-        }
+      const int count = count_of(group_tile<true>(table, p, local, tile, 256, n_blocks));
+      int mine = next;
+      next = index_of(local + 1, tile + step);
+      if (mine < 0 || mine >= p.a_rows) {
+        record_err(p.err, kDevBadGroup);
+        mine = 0;
       }
       int src[kGatherRows];
 #pragma unroll
