@@ -9,21 +9,21 @@
 // a gated weight's N columns are interleaved in groups of 64 = [32 up |
 // 32 gate] and the product is up * act(gate), N / 2 wide.
 //
-// Two kernels with one list of tiles (counts per expert, built by every block
-// from off, so the persistent blocks walk one list whatever the groups are):
-//
-//   gemm_grouped_pair_kernel  a CTA pair (tcgen05 cta_group::2) takes 256
-//       columns of W and up to 256 rows of one group, with W as the product's
-//       M operand and the rows as its N operand: N is any multiple of 32, so a
-//       group of 40 rows costs 64 and not 256, and a group of 257 is cut into
-//       160 + 97.  The accumulator holds a column of C per TMEM lane.
-//   gemm_grouped_kernel  one CTA takes 128 rows by 128, 64 or 32 columns, rows
-//       as M: for so few rows that the columns have to spread over the SMs.
+// A CTA pair (tcgen05 cta_group::2) takes 256 columns of W and up to 256 rows
+// of one group, with W as the product's M operand and the rows as its N
+// operand: N is any multiple of 32, so a group of 40 rows costs 64 and not
+// 256, and a group of 257 is cut into 160 + 97.  The accumulator holds a
+// column of C per TMEM lane.  The persistent pairs walk one list of tiles,
+// whatever the groups are: every block builds it from off.  (One CTA on 128
+// rows by 128, 64 or 32 columns, rows as M, was no faster at any size tried:
+// 8.2 / 9.0 / 12.8 us for the pair against 8.2 / 8.9 / 14.1 us at best on 1,
+// 32 and 1024 rows of 2 of 8 experts, K and N 1024; 15.0 against 15.4 us on
+// 64 rows, K 768, N 3840.)
 //
 // Roles of a block:
 //   warp 0        W by TMA (and A, where its rows are grouped already), and
 //                 the stage's transaction bytes
-//   warp 1        tcgen05.mma (the pair's leader)
+//   warp 1        tcgen05.mma (the leader)
 //   warps 2-9     epilogue: TMEM -> bias, activation -> shared memory -> TMA
 //                 store of 32 x 32 chunks; the chunk in which a group ends is
 //                 stored row by row
@@ -66,7 +66,6 @@ struct GroupedArgs {
   const int *row_src;  // [rows] or null
   int a_rows;          // A's rows
   int N, K;            // N as staged (2F for a gated weight)
-  int bn;              // one CTA: tile columns, 128, 64 or 32
   const float *bias;   // [experts, N] in the container's column order, or null
   void *out;           // [rows, N or N / 2]
   int *err;
@@ -91,21 +90,6 @@ constexpr int kGatherWarps = 8;
 constexpr int kGatherRows = kGemmBM / kGatherWarps;
 constexpr int kGroupedGatherThreads = 320 + 32 * kGatherWarps;
 
-// A box of a K-major map into this CTA's shared memory, completing on the
-// barrier at `bar` (a shared::cluster address: the pair leader's).
-template <int CTAS>
-__device__ __forceinline__ void grp_load(void *smem_dst, const void *tmap, uint32_t bar, int32_t c0,
-                                         int32_t c1) {
-  if constexpr (CTAS == 2)
-    tma_load_2d_pair(smem_dst, tmap, bar, c0, c1);
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(smem_dst)),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(c1), "r"(bar)
-        : "memory");
-}
-
 // Arrive on a barrier of this cluster without ordering any memory access of
 // this thread before it.
 __device__ __forceinline__ void grp_arrive(uint32_t bar) {
@@ -114,25 +98,16 @@ __device__ __forceinline__ void grp_arrive(uint32_t bar) {
 }
 
 // Four rows of a K-major map (box 64 x 1) into 512 consecutive bytes of a
-// 128-byte-swizzled tile.
-template <int CTAS>
+// 128-byte-swizzled tile, completing on the barrier at `bar` (a
+// shared::cluster address: the leader's).
 __device__ __forceinline__ void grp_gather4(uint32_t dst, const void *tmap, uint32_t bar,
                                             int32_t c0, int32_t r0, int32_t r1, int32_t r2,
                                             int32_t r3) {
-  if constexpr (CTAS == 2)
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-        ".cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
-        "r"(bar)
-        : "memory");
-  else
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
-        "r"(bar)
-        : "memory");
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      ".cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(c0), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+      : "memory");
 }
 
 // A tile of the list: expert, its rows [row, end) and the column block.
@@ -150,12 +125,13 @@ struct GroupTable {
 };
 static_assert(sizeof(GroupTable) == GroupedShape::kTableBytes, "table size");
 
-// Tile t.  EVEN: a group of m rows is cut into ceil(m / bm) tiles of equal
-// size, rounded up to 32 rows; otherwise into tiles of bm rows and a rest.
-template <bool EVEN>
-__device__ __forceinline__ GroupTile group_find(const GroupTable &g, const GroupedArgs &p, int t,
-                                                int bm, int n_blocks) {
-  int lo = 0, hi = p.experts;  // tile[lo] <= t < tile[hi]
+constexpr int kGroupTileRows = 256, kGroupTileCols = 256;
+
+// Tile t: a group of m rows is cut into ceil(m / 256) tiles of equal size,
+// rounded up to 32 rows.
+__device__ __forceinline__ GroupTile group_find(const GroupTable &g, int experts, int t,
+                                                int n_blocks) {
+  int lo = 0, hi = experts;  // tile[lo] <= t < tile[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (t >= g.tile[mid]) lo = mid;
@@ -163,448 +139,60 @@ __device__ __forceinline__ GroupTile group_find(const GroupTable &g, const Group
   }
   const int i = t - g.tile[lo], b = i / n_blocks;
   const int m = g.off[lo + 1] - g.off[lo];
-  int size = bm;
-  if constexpr (EVEN) {
-    const int tiles = (m + bm - 1) / bm;
-    size = ((m + tiles - 1) / tiles + 31) / 32 * 32;
-  }
+  const int tiles = (m + kGroupTileRows - 1) / kGroupTileRows;
+  const int size = ((m + tiles - 1) / tiles + 31) / 32 * 32;
   const int row = g.off[lo] + b * size;
   return {lo, row, min(row + size, g.off[lo + 1]), i - b * n_blocks};
 }
 
-// The table, for the tiles first, first + step, ... of this block.
-template <bool EVEN>
-__device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedArgs &p, int bm,
-                                                  int n_blocks, int first, int step) {
-  for (int e = threadIdx.x; e <= p.experts; e += blockDim.x) g.off[e] = __ldg(p.off + e);
-  __syncthreads();
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    int hi = 0, tiles = 0;  // the running maximum of off, and the tiles so far
-    bool bad = false;
-    for (int e0 = 0; e0 <= p.experts; e0 += 32) {
-      const int e = e0 + lane;
-      const int raw = e <= p.experts ? g.off[e] : 0;
-      int v = min(max(raw, 0), p.rows);
-      bad |= e <= p.experts && raw != v;
+// off and tile, by one warp.
+__device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedArgs &p,
+                                                  int n_blocks, int lane) {
+  int hi = 0, tiles = 0;  // the running maximum of off, and the tiles so far
+  bool bad = false;
+  int raw[4];
+  for (int e0 = 0; e0 <= p.experts; e0 += 32) {
+    const int u = e0 / 32 % 4;
+    if (u == 0) {  // four loads together
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v = max(v, u);
-      }
-      v = max(v, hi);
-      bad |= e <= p.experts && v > raw;
-      // expert e - 1 is [off[e - 1], off[e]): its tiles end at tile[e]
-      int before = __shfl_up_sync(0xffffffffu, v, 1);
-      if (lane == 0) before = e0 ? hi : v;
-      int t = (v - before + bm - 1) / bm * n_blocks;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, t, o);
-        if (lane >= o) t += u;
-      }
-      t += tiles;
-      if (e <= p.experts) {
-        g.off[e] = v;
-        g.tile[e] = t;
-      }
-      hi = __shfl_sync(0xffffffffu, v, 31);
-      tiles = __shfl_sync(0xffffffffu, t, 31);
+      for (int i = 0; i < 4; ++i)
+        raw[i] = e0 + 32 * i + lane <= p.experts ? __ldg(p.off + e0 + 32 * i + lane) : 0;
     }
-    if (bad && blockIdx.x == 0) record_err(p.err, kDevBadGroup);
+    const int e = e0 + lane;
+    const int given = u == 0 ? raw[0] : u == 1 ? raw[1] : u == 2 ? raw[2] : raw[3];
+    int v = min(max(given, 0), p.rows);
+    bad |= e <= p.experts && given != v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int w = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v = max(v, w);
+    }
+    v = max(v, hi);
+    bad |= e <= p.experts && v > given;
+    // expert e - 1 is [off[e - 1], off[e]): its tiles end at tile[e]
+    int before = __shfl_up_sync(0xffffffffu, v, 1);
+    if (lane == 0) before = e0 ? hi : v;
+    int t = (v - before + kGroupTileRows - 1) / kGroupTileRows * n_blocks;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int w = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += w;
+    }
+    t += tiles;
+    if (e <= p.experts) {
+      g.off[e] = v;
+      g.tile[e] = t;
+    }
+    hi = __shfl_sync(0xffffffffu, v, 31);
+    tiles = __shfl_sync(0xffffffffu, t, 31);
   }
-  __syncthreads();
-  const int last = g.tile[p.experts];
-  for (int i = threadIdx.x; i < GroupedShape::kList; i += blockDim.x) {
-    const int64_t t = first + static_cast<int64_t>(i) * step;
-    if (t < last) g.list[i] = group_find<EVEN>(g, p, static_cast<int>(t), bm, n_blocks);
-  }
-  __syncthreads();
+  if (bad && blockIdx.x == 0) record_err(p.err, kDevBadGroup);
 }
 
 // This block's tile number `local`, tile t.
-template <bool EVEN>
-__device__ __forceinline__ GroupTile group_tile(const GroupTable &g, const GroupedArgs &p,
-                                                int local, int t, int bm, int n_blocks) {
-  return local < GroupedShape::kList ? g.list[local] : group_find<EVEN>(g, p, t, bm, n_blocks);
-}
-
-// 32 accumulator columns of one row from GEMM column col0 on (a gated
-// epilogue: up columns, with their gates in rg), biased and activated: output
-// columns [c0, c0 + ncols).
-template <int EPI>
-__device__ __forceinline__ void grp_finish(const float *bias, int width, int c0, int ncols,
-                                           const uint32_t (&r)[32], const uint32_t (&rg)[32],
-                                           float (&v)[32]) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-  if (bias) {
-    const float4 *b4 = reinterpret_cast<const float4 *>(bias + c0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (i * 4 < ncols) {
-        const float4 b = __ldg(b4 + i);
-        v[4 * i] += b.x;
-        v[4 * i + 1] += b.y;
-        v[4 * i + 2] += b.z;
-        v[4 * i + 3] += b.w;
-      }
-    }
-  }
-  if constexpr (grp_gated(EPI)) {
-    const float4 *b4 = bias ? reinterpret_cast<const float4 *>(bias + width + c0) : nullptr;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float g[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) g[j] = __uint_as_float(rg[4 * i + j]);
-      if (b4) {  // a gated width is a multiple of 32
-        const float4 b = __ldg(b4 + i);
-        g[0] += b.x;
-        g[1] += b.y;
-        g[2] += b.z;
-        g[3] += b.w;
-      }
-      if constexpr (EPI == kGrpBf16SwiGLU) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * i + j] *= silu_fast(g[j]);
-      } else {
-        gelu_erf_x2(g[0], g[1]);
-        gelu_erf_x2(g[2], g[3]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[4 * i + j] *= g[j];
-      }
-    }
-  } else if constexpr (EPI == kGrpBf16Gelu8) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) gelu8_x2(v[i], v[i + 1]);
-  } else if constexpr (EPI == kGrpBf16Erf) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) gelu_erf_x2(v[i], v[i + 1]);
-  }
-}
-
-// This lane's row of a 32 x 32 chunk in shared memory, in the output map's
-// swizzle (make_tmap_out): fp32 rows of 128 bytes, bf16 rows of 64.
-template <int EPI>
-__device__ __forceinline__ void grp_stage(const float (&v)[32], uint8_t *chunk, int lane) {
-  if constexpr (EPI == kGrpF32) {
-#pragma unroll
-    for (int q = 0; q < 8; ++q)
-      *reinterpret_cast<float4 *>(chunk + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-          make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<uint4 *>(chunk + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
-          make_uint4(pack_bf16x2(v[8 * q], v[8 * q + 1]), pack_bf16x2(v[8 * q + 2], v[8 * q + 3]),
-                     pack_bf16x2(v[8 * q + 4], v[8 * q + 5]),
-                     pack_bf16x2(v[8 * q + 6], v[8 * q + 7]));
-  }
-}
-
-// The same row straight to C.
-template <int EPI>
-__device__ __forceinline__ void grp_store(void *out, int64_t at, int ncols, const float (&v)[32]) {
-  if constexpr (EPI == kGrpF32) {
-    float4 *o = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i * 4 < ncols) o[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-  } else {
-    uint4 *o = reinterpret_cast<uint4 *>(static_cast<__nv_bfloat16 *>(out) + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (i * 8 < ncols)
-        o[i] = make_uint4(pack_bf16x2(v[8 * i], v[8 * i + 1]),
-                          pack_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                          pack_bf16x2(v[8 * i + 4], v[8 * i + 5]),
-                          pack_bf16x2(v[8 * i + 6], v[8 * i + 7]));
-  }
-}
-
-template <int EPI, bool GATHER>
-__global__ void __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
-    gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA,
-                        const __grid_constant__ CUtensorMap tmA128,
-                        const __grid_constant__ CUtensorMap tmW,
-                        const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
-  using S = GroupedShape;
-  constexpr int kStages = S::kStages;
-  constexpr int kAccCols = 128;  // TMEM columns of an accumulator
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>(
-      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t *sA = smem;
-  uint8_t *sW = smem + kStages * S::kABytes;
-  uint8_t *staging = smem + kStages * S::kStageBytes;
-  uint64_t *full = reinterpret_cast<uint64_t *>(staging + S::kStagingBytes);
-  uint64_t *empty = full + kStages;
-  uint64_t *tfull = empty + kStages;
-  uint64_t *tempty = tfull + 2;
-  uint64_t *drain = tempty + 2;
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
-  GroupTable &table =
-      *reinterpret_cast<GroupTable *>(staging + S::kStagingBytes + S::kBarBytes);
-
-  const int warp = threadIdx.x >> 5;
-  const int lane = threadIdx.x & 31;
-  const int bn = p.bn;
-  const int n_blocks = (p.N + bn - 1) / bn;
-  const int num_kb = (p.K + kGemmBK - 1) / kGemmBK;
-
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmC);
-    for (int s = 0; s < kStages; ++s) {
-      // every gather warp arrives on every stage, also with no row to load:
-      // one that did not could fall a phase behind the ring, whose parity
-      // then reads the wrong way round
-      mbar_init(&full[s], 1 + (GATHER ? kGatherWarps : 0));
-      mbar_init(&empty[s], 1);
-    }
-    for (int a = 0; a < 2; ++a) {
-      mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 8);
-    }
-    mbar_init(drain, 1);
-    fence_mbar_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, 2 * kAccCols);
-    tmem_relinquish();
-  }
-  group_table_build<false>(table, p, kGemmBM, n_blocks, blockIdx.x, gridDim.x);
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
-  const int num_tiles = table.tile[p.experts];
-  auto wait_all = [&](uint64_t *bar, uint32_t parity) -> bool {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err));
-  };
-
-  if (warp == 0) {
-    // ---------------- W (and grouped A) producer ----------------
-    if (lane == 0) {
-      int stage = 0, local = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
-        const GroupTile t = group_tile<false>(table, p, local, tile, kGemmBM, n_blocks);
-        const int m = min(t.end - t.row, kGemmBM);
-        const int a_boxes = GATHER ? 0 : (m + kGroupedBox - 1) / kGroupedBox;
-        const uint32_t bytes = static_cast<uint32_t>(bn) * kGemmBK * 2 +
-                               (GATHER ? (m + 3) / 4 * 512 : a_boxes * (kGroupedBox * 128));
-        const int w_row = t.e * p.N + t.nb * bn;
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) {
-            ok = false;
-            break;
-          }
-          mbar_arrive_expect_tx(&full[stage], bytes);
-          const uint32_t bar = smem_u32(&full[stage]);
-          grp_load<1>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
-          if (a_boxes == kGemmBM / kGroupedBox) {
-            grp_load<1>(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK,
-                        t.row);
-          } else {
-            for (int i = 0; i < a_boxes; ++i)
-              grp_load<1>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
-                             kb * kGemmBK, t.row + i * kGroupedBox);
-          }
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
-      // Tail: the MMAs have released every stage, so all loads of this CTA
-      // (the gathers too) have landed and all commits aimed at its barriers
-      // have arrived before it may exit.
-      for (int i = 0; i < kStages && ok; ++i) {
-        if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) break;
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // ---------------- MMA issuer ----------------
-    {
-      const uint32_t idesc = idesc_bf16_f32(kGemmBM, bn);
-      const bool elect = elect_one_sync();
-      int stage = 0;
-      uint32_t phase = 0;
-      bool issued_any = false, ok = true;
-      int local = 0;
-      for (int tile = blockIdx.x; tile < num_tiles && ok; tile += gridDim.x, ++local) {
-        const int acc = local & 1;
-        if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
-        tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kAccCols);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!wait_all(&full[stage], phase)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t da = sdesc_kmajor_sw128(smem_u32(sA + stage * S::kABytes));
-          const uint64_t dw = sdesc_kmajor_sw128(smem_u32(sW + stage * S::kABytes));
-          if (elect) {
-#pragma unroll
-            for (int k = 0; k < kGemmBK / 16; ++k) {
-              umma_bf16(d_tmem, da + k * 2, dw + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
-            }
-            umma_commit(&empty[stage]);
-          }
-          __syncwarp();
-          issued_any = true;
-          if (++stage == kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-        if (ok && elect) {
-          umma_commit(&tfull[acc]);
-        }
-        __syncwarp();
-      }
-      if (issued_any) {
-        if (elect) {
-          umma_commit(drain);
-        }
-        __syncwarp();
-        wait_all(drain, 0);
-      }
-    }
-  } else if (warp < 10) {
-    // ---------------- epilogue ----------------
-    // Two warps per TMEM lane quarter, half of the columns each.
-    constexpr bool kGated = grp_gated(EPI);
-    constexpr int kStep = kGated ? 64 : 32;  // accumulator columns a chunk takes
-    constexpr int kChunkBytes = EPI == kGrpF32 ? 4096 : 2048;
-    constexpr int kSlots = S::kWarpStaging / kChunkBytes;
-    const int quarter = warp & 3, half = (warp - 2) >> 2;
-    // whole chunks to each half, the first taking the larger share
-    const int split = (bn / kStep + 1) / 2 * kStep;
-    const int begin = half ? split : 0, end = half ? bn : split;
-    const int width = kGated ? p.N / 2 : p.N;
-    uint8_t *mine = staging + (warp - 2) * S::kWarpStaging;
-    int slot = 0;
-    int local = 0;
-    for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x, ++local) {
-      const int acc = local & 1;
-      if (!wait_all(&tfull[acc], (local >> 1) & 1)) break;
-      tc_fence_after();
-      const GroupTile t = group_tile<false>(table, p, local, tile, kGemmBM, n_blocks);
-      const int row0 = t.row + quarter * 32;
-      const float *bias = p.bias ? p.bias + static_cast<int64_t>(t.e) * p.N : nullptr;
-      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) +
-                             static_cast<uint32_t>(acc * kAccCols);
-      if (row0 < t.end) {  // warp-uniform
-#pragma unroll 1
-        for (int c = begin; c < end; c += kStep) {
-          const int col0 = t.nb * bn + c;
-          if (col0 >= p.N) break;
-          uint32_t r[32], rg[32];
-          tmem_ld_32x32b_x32(t_row + c, r);
-          if constexpr (kGated) tmem_ld_32x32b_x32(t_row + c + 32, rg);
-          tmem_wait_ld_regs(r);
-          if constexpr (kGated) tmem_wait_ld_regs(rg);
-          const int c0 = kGated ? col0 / 2 : col0;
-          const int ncols = min(32, width - c0);
-          float v[32];
-          grp_finish<EPI>(bias, width, c0, ncols, r, rg, v);
-          if (row0 + 32 <= t.end) {
-            uint8_t *chunk = mine + slot * kChunkBytes;
-            if (++slot == kSlots) slot = 0;
-            if (lane == 0) bulk_wait_group_read<kSlots - 1>();
-            __syncwarp();
-            grp_stage<EPI>(v, chunk, lane);
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&tmC, chunk, c0, row0);
-              bulk_commit_group();
-            }
-          } else if (row0 + lane < t.end) {
-            grp_store<EPI>(p.out, static_cast<int64_t>(row0 + lane) * width + c0, ncols, v);
-          }
-          __syncwarp();
-        }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&tempty[acc]);
-      }
-    }
-    if (lane == 0) bulk_wait_group_all();
-  } else if constexpr (GATHER) {
-    // ---------------- A by gathers (warps 10..17) ----------------
-    const int part = warp - 10;  // a share of the tile's 128 rows
-    const bool elect = elect_one_sync();
-    int stage = 0, local = 0;
-    uint32_t phase = 0;
-    bool ok = true;
-    // this warp's rows of a tile, and the lane's row of A for one of them;
-    // a tile's are read while the one before is loaded
-    auto count_of = [&](const GroupTile &t) -> int {
-      return min(max(t.end - t.row - kGatherRows * part, 0), kGatherRows);
-    };
-    auto index_of = [&](int l, int tile) -> int {
-      if (tile >= num_tiles) return 0;
-      const GroupTile t = group_tile<false>(table, p, l, tile, kGemmBM, n_blocks);
-      const int count = count_of(t);
-      // past the group: its last row again, to fill a gather of four
-      return count ? __ldg(p.row_src + t.row + kGatherRows * part + min(lane, count - 1)) : 0;
-    };
-    const int stride = gridDim.x;
-    int next = index_of(0, blockIdx.x);
-    for (int tile = blockIdx.x; tile < num_tiles && ok; tile += stride, ++local) {
-      const int count = count_of(group_tile<false>(table, p, local, tile, kGemmBM, n_blocks));
-      int mine = next;
-      next = index_of(local + 1, tile + stride);
-      if (mine < 0 || mine >= p.a_rows) {
-        record_err(p.err, kDevBadGroup);
-        mine = 0;
-      }
-      int src[kGatherRows];
-#pragma unroll
-      for (int i = 0; i < kGatherRows; ++i) src[i] = __shfl_sync(0xffffffffu, mine, i);
-      for (int kb = 0; kb < num_kb; ++kb) {
-        if (!wait_all(&empty[stage], phase ^ 1u)) {
-          ok = false;
-          break;
-        }
-        if (elect) {
-          const uint32_t dst = smem_u32(sA + stage * S::kABytes) + part * (kGatherRows * 128);
-          const uint32_t bar = smem_u32(&full[stage]);
-#pragma unroll
-          for (int i = 0; i < kGatherRows / 4; ++i)
-            if (4 * i < count)
-              grp_gather4<1>(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
-                                src[4 * i + 2], src[4 * i + 3]);
-          grp_arrive(bar);
-        }
-        __syncwarp();
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1u;
-        }
-      }
-    }
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    tc_fence_after();
-    tmem_dealloc(tmem_base, 2 * kAccCols);
-  }
+__device__ __forceinline__ GroupTile group_tile(const GroupTable &g, int experts, int local, int t,
+                                                int n_blocks) {
+  return local < GroupedShape::kList ? g.list[local] : group_find(g, experts, t, n_blocks);
 }
 
 // Both warps of an epilogue pair: wait, and whether `ok` held for both (each
@@ -642,6 +230,15 @@ __device__ __forceinline__ void grp_load_chunk(uint32_t taddr, uint32_t (&r)[32]
         : "r"(taddr + (static_cast<uint32_t>(16 * h) << 16))
         : "memory");
   tmem_wait_ld_regs(r);
+}
+
+// x / (1 + 2^(-x log2 e)) on two values: 2^x and 1 / x on the SFU (relative
+// errors of 2^-22 and 2^-23), far below the rounding of the product to bf16.
+__device__ __forceinline__ void grp_silu_x2(float &a, float &b) {
+  float t0, t1;
+  unpk2(mul_x2(pk2(a, b), pk2(-1.4426950408889634f, -1.4426950408889634f)), t0, t1);
+  unpk2(add_x2(pk2(ex2_approx(t0), ex2_approx(t1)), pk2(1.0f, 1.0f)), t0, t1);
+  unpk2(mul_x2(pk2(a, b), pk2(rcp_approx(t0), rcp_approx(t1))), a, b);
 }
 
 // The biases of this thread's columns of a chunk (0 where there are none).
@@ -698,7 +295,7 @@ __device__ __forceinline__ void grp_store_rows(void *out, const uint8_t *chunk, 
 template <int EPI, bool GATHER>
 __global__ void __cluster_dims__(2, 1, 1)
     __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
-    gemm_grouped_pair_kernel(const __grid_constant__ CUtensorMap tmA,
+    gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA,
                              const __grid_constant__ CUtensorMap tmA128,
                              const __grid_constant__ CUtensorMap tmW,
                              const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
@@ -728,10 +325,12 @@ __global__ void __cluster_dims__(2, 1, 1)
   const int num_kb = (p.K + kGemmBK - 1) / kGemmBK;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
-  if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmW);
-    tma_prefetch_desc(&tmC);
+  if (warp == 0) {
+    group_table_build(table, p, n_blocks, lane);
+  } else if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * kAccCols);
+    tmem_relinquish_pair();
+  } else if (warp == 2 && lane == 0) {
     for (int s = 0; s < kStages; ++s) {
       // every gather warp arrives on every stage, also with no row to load:
       // one that did not could fall a phase behind the ring, whose parity
@@ -745,14 +344,20 @@ __global__ void __cluster_dims__(2, 1, 1)
     }
     mbar_init(drain, 1);
     fence_mbar_init();
+  } else if (warp == 3 && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    if (!GATHER) tma_prefetch_desc(&tmA128);
+    tma_prefetch_desc(&tmW);
+    tma_prefetch_desc(&tmC);
   }
-  if (warp == 1) {
-    tmem_alloc_pair(tmem_slot, 2 * kAccCols);
-    tmem_relinquish_pair();
+  __syncthreads();
+  for (int i = threadIdx.x; i < S::kList; i += blockDim.x) {
+    const int64_t t = first + static_cast<int64_t>(i) * step;
+    if (t < table.tile[p.experts])
+      table.list[i] = group_find(table, p.experts, static_cast<int>(t), n_blocks);
   }
-  group_table_build<true>(table, p, 256, n_blocks, first, step);
   tc_fence_before();
-  cluster_sync();
+  cluster_sync();  // barriers and TMEM of both CTAs, this CTA's list
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   const int num_tiles = table.tile[p.experts];
@@ -774,7 +379,7 @@ __global__ void __cluster_dims__(2, 1, 1)
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-        const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
+        const GroupTile t = group_tile(table, p.experts, local, tile, n_blocks);
         uint32_t bytes = 2 * S::kABytes;  // W
         for (int c = 0; c < 2; ++c) {
           const int m = cta_rows(t, c);
@@ -791,12 +396,12 @@ __global__ void __cluster_dims__(2, 1, 1)
           }
           if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
           const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
-          grp_load<2>(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
+          tma_load_2d_pair(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
           if (boxes == kGemmBM / kGroupedBox) {
-            grp_load<2>(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK, a_row);
+            tma_load_2d_pair(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK, a_row);
           } else {
             for (int i = 0; i < boxes; ++i)
-              grp_load<2>(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
+              tma_load_2d_pair(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
                           kb * kGemmBK, a_row + i * kGroupedBox);
           }
           if (++stage == kStages) {
@@ -825,7 +430,7 @@ __global__ void __cluster_dims__(2, 1, 1)
       bool issued_any = false, ok = true;
       int local = 0;
       for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-        const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
+        const GroupTile t = group_tile(table, p.experts, local, tile, n_blocks);
         const uint32_t idesc = idesc_bf16_f32(256, tile_n(t));
         const int acc = local & 1;
         if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
@@ -885,7 +490,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     int local = 0;
     for (int tile = first; tile < num_tiles; tile += step, ++local) {
       const int acc = local & 1;
-      const GroupTile t = group_tile<true>(table, p, local, tile, 256, n_blocks);
+      const GroupTile t = group_tile(table, p.experts, local, tile, n_blocks);
       // first W column of the quarter (of the pair of quarters), and of C
       const int col = t.nb * 256 + rank * 128 + (kGated ? quarter & 2 : quarter) * 32;
       const int c0 = kGated ? col / 2 : col;
@@ -933,45 +538,40 @@ __global__ void __cluster_dims__(2, 1, 1)
             grp_load_chunk(t_row + c * 32, r);
           }
           // entry 4 i + j: column lane / 4 + 8 * (2 * (i / 4) + j / 2), row
-          // 8 * (i % 4) + 2 * (lane % 4) + j % 2
-          // (narrowed as they are made: 16 registers a chunk instead of 32)
+          // 8 * (i % 4) + 2 * (lane % 4) + j % 2, finished two at a time and
+          // narrowed as they are made (16 registers a chunk instead of 32)
           std::conditional_t<EPI == kGrpF32, float[32], uint32_t[16]> v;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-              const float bj = b[2 * (i / 4) + j / 2];
-              float x0 = __uint_as_float(r[4 * i + j]), x1 = __uint_as_float(r[4 * i + j + 1]);
-              if constexpr (kGated) {
-                const float2 o = *(reinterpret_cast<const float2 *>(receive + i * 32) + j / 2);
-                const float gj = bg[2 * (i / 4) + j / 2];
-                float g0 = (gate ? x0 : o.x) + gj, g1 = (gate ? x1 : o.y) + gj;
-                if (gate) {
-                  x0 = o.x;
-                  x1 = o.y;
-                }
-                x0 += bj;
-                x1 += bj;
-                if constexpr (EPI == kGrpBf16SwiGLU) {
-                  x0 *= silu_fast(g0);
-                  x1 *= silu_fast(g1);
-                } else {
-                  gelu_erf_x2(g0, g1);
-                  x0 *= g0;
-                  x1 *= g1;
-                }
-              } else {
-                x0 += bj;
-                x1 += bj;
-                if constexpr (EPI == kGrpBf16Gelu8) gelu8_x2(x0, x1);
-                if constexpr (EPI == kGrpBf16Erf) gelu_erf_x2(x0, x1);
+          for (int i = 0; i < 16; ++i) {
+            const float2 bias2 = make_float2(b[2 * (i / 8) + i % 2], b[2 * (i / 8) + i % 2]);
+            uint64_t x = pk2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
+            if constexpr (kGated) {
+              const float2 o = reinterpret_cast<const float2 *>(receive + i / 2 * 32)[i % 2];
+              uint64_t g = pk2(o.x, o.y);
+              if (gate) {  // the same for the whole warp
+                const uint64_t y = x;
+                x = g;
+                g = y;
               }
-              if constexpr (EPI == kGrpF32) {
-                v[4 * i + j] = x0;
-                v[4 * i + j + 1] = x1;
-              } else {
-                v[2 * i + j / 2] = pack_bf16x2(x0, x1);
-              }
+              const float bg1 = bg[2 * (i / 8) + i % 2];
+              g = add_x2(g, pk2(bg1, bg1));
+              float g0, g1;
+              unpk2(g, g0, g1);
+              if constexpr (EPI == kGrpBf16SwiGLU) grp_silu_x2(g0, g1);
+              else gelu_erf_x2(g0, g1);
+              x = mul_x2(add_x2(x, pk2(bias2.x, bias2.y)), pk2(g0, g1));
+            } else {
+              x = add_x2(x, pk2(bias2.x, bias2.y));
+            }
+            float x0, x1;
+            unpk2(x, x0, x1);
+            if constexpr (EPI == kGrpBf16Gelu8) gelu8_x2(x0, x1);
+            if constexpr (EPI == kGrpBf16Erf) gelu_erf_x2(x0, x1);
+            if constexpr (EPI == kGrpF32) {
+              v[2 * i] = x0;
+              v[2 * i + 1] = x1;
+            } else {
+              v[i] = pack_bf16x2(x0, x1);
             }
           }
           uint8_t *chunk = mine + slot * kChunkBytes;
@@ -1015,7 +615,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     };
     auto index_of = [&](int l, int tile) -> int {
       if (tile >= num_tiles) return 0;
-      const GroupTile t = group_tile<true>(table, p, l, tile, 256, n_blocks);
+      const GroupTile t = group_tile(table, p.experts, l, tile, n_blocks);
       const int count = count_of(t);
       // past the group: its last row again, to fill a gather of four
       return count ? __ldg(p.row_src + t.row + rank * (tile_n(t) / 2) + kGatherRows * part +
@@ -1024,7 +624,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     };
     int next = index_of(0, first);
     for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-      const int count = count_of(group_tile<true>(table, p, local, tile, 256, n_blocks));
+      const int count = count_of(group_tile(table, p.experts, local, tile, n_blocks));
       int mine = next;
       next = index_of(local + 1, tile + step);
       if (mine < 0 || mine >= p.a_rows) {
@@ -1045,7 +645,7 @@ __global__ void __cluster_dims__(2, 1, 1)
 #pragma unroll
           for (int i = 0; i < kGatherRows / 4; ++i)
             if (4 * i < count)
-              grp_gather4<2>(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
+              grp_gather4(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
                              src[4 * i + 2], src[4 * i + 3]);
           grp_arrive(bar);
         }

@@ -24,8 +24,6 @@ int set_grouped_attr() {
   const int smem = nebw::GroupedShape::kSmemBytes;
   NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<EPI, false>, a, smem));
   NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<EPI, true>, a, smem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_pair_kernel<EPI, false>, a, smem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_pair_kernel<EPI, true>, a, smem));
   return NEBW_OK;
 }
 
@@ -58,6 +56,25 @@ int set_route_attrs() {
   NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<__nv_bfloat16, K, 0>, a, kRouteSmem));
   NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<__nv_bfloat16, K, 2>, a, kRouteSmem));
   NEBW_CUDA(cudaFuncSetAttribute(nebw::route_place_kernel<K>, a, kRouteSmem));
+  return NEBW_OK;
+}
+
+// How many CTA pairs of the grouped product the GPU holds at once.
+int query_grouped_pairs(int *pairs) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * 74);
+  cfg.blockDim = dim3(nebw::kGroupedGatherThreads);
+  cfg.dynamicSmemBytes = nebw::GroupedShape::kSmemBytes;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  NEBW_CUDA(cudaOccupancyMaxActiveClusters(
+      pairs, nebw::gemm_grouped_kernel<nebw::kGrpBf16, true>, &cfg));
+  NEBW_REQUIRE(*pairs > 0, "this GPU holds no CTA pair of the grouped product");
   return NEBW_OK;
 }
 
@@ -511,9 +528,7 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   int rc = NEBW_OK;
   if (e != cudaSuccess)
     rc = set_error(NEBW_ECUDA, "expert weight staging failed: %s", cudaGetErrorString(e));
-  if (!rc) rc = make_tmap_kmajor(&w.map128, w.ptr, experts * N, K, 128);
-  if (!rc) rc = make_tmap_kmajor(&w.map64, w.ptr, experts * N, K, 64);
-  if (!rc) rc = make_tmap_kmajor(&w.map32, w.ptr, experts * N, K, 32);
+  if (!rc) rc = make_tmap_kmajor(&w.map, w.ptr, experts * N, K, 128);
   if (!rc) {
     try {
       d->experts[d->next_handle] = w;
@@ -536,36 +551,31 @@ struct GroupedMaps {
 };
 
 template <int EPI>
-void launch_grouped_epi(const GroupedMaps &m, const nebw::GroupedArgs &a, bool pairs,
-                        unsigned grid, cudaStream_t st) {
+void launch_grouped_epi(const GroupedMaps &m, const nebw::GroupedArgs &a, unsigned grid,
+                        cudaStream_t st) {
   const size_t smem = nebw::GroupedShape::kSmemBytes;
-  const int threads = a.row_src ? nebw::kGroupedGatherThreads : nebw::kGroupedThreads;
-  if (pairs && a.row_src)
-    nebw::gemm_grouped_pair_kernel<EPI, true><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
-  else if (pairs)
-    nebw::gemm_grouped_pair_kernel<EPI, false><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
-  else if (a.row_src)
-    nebw::gemm_grouped_kernel<EPI, true><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
+  if (a.row_src)
+    nebw::gemm_grouped_kernel<EPI, true>
+        <<<grid, nebw::kGroupedGatherThreads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
   else
-    nebw::gemm_grouped_kernel<EPI, false><<<grid, threads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
+    nebw::gemm_grouped_kernel<EPI, false>
+        <<<grid, nebw::kGroupedThreads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
 }
 
 int launch_grouped(nebw_dev *d, const GroupedMaps &m, int epi, const nebw::GroupedArgs &a,
-                   bool pairs, cudaStream_t st) {
+                   cudaStream_t st) {
   // the most tiles that the groups can make: every one may end in a part tile
-  const int64_t tile_rows = pairs ? 256 : nebw::kGemmBM, tile_cols = pairs ? 256 : a.bn;
-  const int64_t tiles = (a.rows / tile_rows + std::min(a.experts, a.rows)) *
-                        ((a.N + tile_cols - 1) / tile_cols);
-  NEBW_REQUIRE(tiles < (1ll << 31), "grouped product too large");
-  const unsigned g = static_cast<unsigned>(
-      pairs ? 2 * std::min<int64_t>(tiles, d->gemm_pairs) : std::min<int64_t>(tiles, d->sm_count));
+  const int64_t tiles = (a.rows / nebw::kGroupTileRows + std::min(a.experts, a.rows)) *
+                        int64_t{(a.N + nebw::kGroupTileCols - 1) / nebw::kGroupTileCols};
+  NEBW_REQUIRE(tiles < (1ll << 30), "grouped product too large");
+  const unsigned g = 2 * static_cast<unsigned>(std::min<int64_t>(tiles, d->grouped_pairs));
   switch (epi) {
-    case nebw::kGrpBf16: launch_grouped_epi<nebw::kGrpBf16>(m, a, pairs, g, st); break;
-    case nebw::kGrpBf16Gelu8: launch_grouped_epi<nebw::kGrpBf16Gelu8>(m, a, pairs, g, st); break;
-    case nebw::kGrpBf16Erf: launch_grouped_epi<nebw::kGrpBf16Erf>(m, a, pairs, g, st); break;
-    case nebw::kGrpF32: launch_grouped_epi<nebw::kGrpF32>(m, a, pairs, g, st); break;
-    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<nebw::kGrpBf16SwiGLU>(m, a, pairs, g, st); break;
-    case nebw::kGrpBf16GeGLU: launch_grouped_epi<nebw::kGrpBf16GeGLU>(m, a, pairs, g, st); break;
+    case nebw::kGrpBf16: launch_grouped_epi<nebw::kGrpBf16>(m, a, g, st); break;
+    case nebw::kGrpBf16Gelu8: launch_grouped_epi<nebw::kGrpBf16Gelu8>(m, a, g, st); break;
+    case nebw::kGrpBf16Erf: launch_grouped_epi<nebw::kGrpBf16Erf>(m, a, g, st); break;
+    case nebw::kGrpF32: launch_grouped_epi<nebw::kGrpF32>(m, a, g, st); break;
+    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<nebw::kGrpBf16SwiGLU>(m, a, g, st); break;
+    case nebw::kGrpBf16GeGLU: launch_grouped_epi<nebw::kGrpBf16GeGLU>(m, a, g, st); break;
   }
   NEBW_CUDA(cudaGetLastError());
   return NEBW_OK;
@@ -629,19 +639,8 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   if (row_src) m.a128 = m.a;  // not used
   else if (int rc = make_tmap_kmajor(&m.a128, A, a_rows, K, nebw::kGemmBM)) return rc;
   if (int rc = make_tmap_out(&m.c, C, rows, w.gated ? N / 2 : N, c_dtype == NEBW_BF16)) return rc;
-  const cudaStream_t st = pick_stream(d, stream);
-  const int64_t groups = std::min<int64_t>(w.experts, rows);
-  static const int kThr = std::getenv("GRP_THR") ? std::atoi(std::getenv("GRP_THR")) : 32;
-  if (d->gemm_pairs > 0 && rows >= kThr * groups && N >= 128) {
-    m.w = w.map128;
-    return launch_grouped(d, m, epi, a, true, st);
-  }
-  // one CTA a tile; narrower tiles while the groups' columns leave SMs idle
-  a.bn = 128;
-  const int least = w.gated ? 64 : 32;
-  while (a.bn > least && groups * ((N + a.bn - 1) / a.bn) < d->sm_count) a.bn /= 2;
-  m.w = a.bn == 128 ? w.map128 : a.bn == 64 ? w.map64 : w.map32;
-  return launch_grouped(d, m, epi, a, false, st);
+  m.w = w.map;
+  return launch_grouped(d, m, epi, a, pick_stream(d, stream));
 }
 
 namespace {

@@ -231,7 +231,7 @@ struct Experts {
   int experts = 0;
   int64_t K = 0, N = 0;
   bool gated = false;
-  CUtensorMap map32, map64, map128;  // [experts * N, K], box rows 32 / 64 / 128
+  CUtensorMap map;  // [experts * N, K], box rows 128
 };
 
 // cos and sin of every position and frequency (nebw_stage_rope).
@@ -259,6 +259,7 @@ struct nebw_dev {
   // CTA pairs the GPU can hold at once for the 2-CTA GEMM (0: use the
   // single-CTA kernel); NEBW_GEMM_CTAS=1 in the environment forces 0.
   int gemm_pairs = 0;
+  int grouped_pairs = 0;  // and for the grouped product
   // attention kernel: NEBW_ATTN_MMA (mma.sync flash) or NEBW_ATTN_TCGEN05
   // (UMMA/TMEM); see nebw_set_attention_kernel
   int attn_kind = NEBW_ATTN_TCGEN05;
@@ -729,6 +730,7 @@ int set_gemm_i8_attrs() {
 
 namespace {
 int set_layer_op_attrs();  // layer_ops.cuh
+int query_grouped_pairs(int *pairs);
 }
 
 extern "C" int nebw_open(int device, nebw_dev **out) {
@@ -766,6 +768,7 @@ extern "C" int nebw_open(int device, nebw_dev **out) {
                                  cudaSharedmemCarveoutMaxShared));
 
   if (int rc = query_gemm_pairs(&d->gemm_pairs)) return rc;
+  if (int rc = query_grouped_pairs(&d->grouped_pairs)) return rc;
   if (int rc = load_tensor_map_encoder()) return rc;
   *out = d.release();
   return NEBW_OK;
