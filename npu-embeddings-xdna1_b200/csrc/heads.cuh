@@ -157,60 +157,107 @@ __global__ void __launch_bounds__(256) heads_any_kernel(const HeadArgs p) {
   }
 }
 
-// The same with 16-byte accesses, where head_dim and rot_dim are multiples of
-// two vectors (V = 8 bf16 or 4 fp32 elements) and the rows and weights lie on
-// 16-byte boundaries.  A thread owns V pairs of a head: two vectors, at i and
-// n + i of the half layout, adjacent of the pairs layout (and of the part
-// that does not turn), so the rotation needs no exchange and a norm only the
-// shuffles of the 2^lg lanes that share a head.  A warp takes 32 / 2^lg heads
-// of one side of one row at a time, IT times: the table entries and the
-// norm's weights are read once for all of them, and all loads are issued
-// before the first is used.  The arithmetic is packed, two values an
-// instruction, which keeps the issue slots below half of what the bytes take.
-template <typename T>
-struct HeadVec;
+// The same in vectors of V elements, where head_dim is a multiple of two of
+// them, n of one, and the rows and weights lie on their boundaries: 16 bytes
+// (V = 8 bf16 or 4 fp32), or 8 or 4 for heads of odd widths.  A thread owns V
+// pairs of a head: two vectors, at i and n + i of the half layout, adjacent of
+// the pairs layout (and of the part that does not turn), so the rotation
+// needs no exchange and a norm only the shuffles of the 2^lg lanes that share
+// a head.  A warp takes 32 / 2^lg heads of one side of one row at a time, IT
+// times: the table entries and the norm's weights are read once for all of
+// them, and all loads are issued before the first is used.  The arithmetic is
+// packed, two values an instruction, which keeps the issue slots below half
+// of what the bytes take.
+template <int BYTES>
+struct HeadWord;
 template <>
-struct HeadVec<__nv_bfloat16> {
-  static constexpr int V = 8;
-  static __device__ __forceinline__ void unpack(const uint4 &u, uint64_t (&f)[4]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      f[i] = pk2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+struct HeadWord<16> {
+  using U = uint4;
+  static __device__ __forceinline__ void split(const uint4 &u, uint32_t (&w)[4]) {
+    w[0] = u.x;
+    w[1] = u.y;
+    w[2] = u.z;
+    w[3] = u.w;
   }
-  static __device__ __forceinline__ uint32_t pack1(uint64_t f) {
-    float a, b;
-    unpk2(f, a, b);
-    return pack_bf16x2(a, b);
-  }
-  static __device__ __forceinline__ uint4 pack(const uint64_t (&f)[4]) {
-    return make_uint4(pack1(f[0]), pack1(f[1]), pack1(f[2]), pack1(f[3]));
+  static __device__ __forceinline__ uint4 join(const uint32_t (&w)[4]) {
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <>
-struct HeadVec<float> {
-  static constexpr int V = 4;
-  static __device__ __forceinline__ void unpack(const uint4 &u, uint64_t (&f)[2]) {
-    f[0] = pk2(__uint_as_float(u.x), __uint_as_float(u.y));
-    f[1] = pk2(__uint_as_float(u.z), __uint_as_float(u.w));
+struct HeadWord<8> {
+  using U = uint2;
+  static __device__ __forceinline__ void split(const uint2 &u, uint32_t (&w)[2]) {
+    w[0] = u.x;
+    w[1] = u.y;
   }
-  static __device__ __forceinline__ uint4 pack(const uint64_t (&f)[2]) {
-    float a, b, c, d;
-    unpk2(f[0], a, b);
-    unpk2(f[1], c, d);
-    return make_uint4(__float_as_uint(a), __float_as_uint(b), __float_as_uint(c),
-                      __float_as_uint(d));
+  static __device__ __forceinline__ uint2 join(const uint32_t (&w)[2]) {
+    return make_uint2(w[0], w[1]);
+  }
+};
+template <>
+struct HeadWord<4> {
+  using U = uint32_t;
+  static __device__ __forceinline__ void split(const uint32_t &u, uint32_t (&w)[1]) { w[0] = u; }
+  static __device__ __forceinline__ uint32_t join(const uint32_t (&w)[1]) { return w[0]; }
+};
+
+template <typename T, int V>
+struct HeadVec {
+  static constexpr int P = V / 2, W = V * static_cast<int>(sizeof(T)) / 4;
+  using Word = HeadWord<4 * W>;
+  using U = typename Word::U;
+  static __device__ __forceinline__ void unpack(const U &u, uint64_t (&f)[P]) {
+    uint32_t w[W];
+    Word::split(u, w);
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      if constexpr (sizeof(T) == 2)
+        f[i] = pk2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      else
+        f[i] = pk2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    }
+  }
+  static __device__ __forceinline__ U pack(const uint64_t (&f)[P]) {
+    uint32_t w[W];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float a, b;
+      unpk2(f[i], a, b);
+      if constexpr (sizeof(T) == 2) {
+        w[i] = pack_bf16x2(a, b);
+      } else {
+        w[2 * i] = __float_as_uint(a);
+        w[2 * i + 1] = __float_as_uint(b);
+      }
+    }
+    return Word::join(w);
   }
 };
 
 template <int P>
 __device__ __forceinline__ void head_weights(const float *w, uint64_t (&f)[P]) {
+  if constexpr (P == 1) {
+    const float2 x = __ldg(reinterpret_cast<const float2 *>(w));
+    f[0] = pk2(x.x, x.y);
+  } else {
 #pragma unroll
-  for (int i = 0; i < P; i += 2) {
-    const float4 x = __ldg(reinterpret_cast<const float4 *>(w + 2 * i));
-    f[i] = pk2(x.x, x.y);
-    f[i + 1] = pk2(x.z, x.w);
+    for (int i = 0; i < P; i += 2) {
+      const float4 x = __ldg(reinterpret_cast<const float4 *>(w + 2 * i));
+      f[i] = pk2(x.x, x.y);
+      f[i + 1] = pk2(x.z, x.w);
+    }
   }
+}
+
+// cos and sin of the thread's pair number i from its packed entries.
+template <int P>
+__device__ __forceinline__ void head_entry(const uint64_t (&c2)[P], const uint64_t (&s2)[P], int i,
+                                           float &c, float &s) {
+  float lo, hi;
+  unpk2(c2[i / 2], lo, hi);
+  c = i & 1 ? hi : lo;
+  unpk2(s2[i / 2], lo, hi);
+  s = i & 1 ? hi : lo;
 }
 
 // Blocks an SM must hold, which bounds the registers.  Measured (us, at 4 / 3 /
@@ -219,10 +266,12 @@ __device__ __forceinline__ void head_weights(const float *w, uint64_t (&f)[P]) {
 // of the work), RMS 188 / 144 / 156, LayerNorm 270 / 224 / 178.
 constexpr int head_blocks(int norm) { return norm == kHeadNormNone ? 4 : norm == kHeadNormRms ? 3 : 2; }
 
-template <typename T, int NORM, bool PAIRS, int IT>
+template <typename T, int V, int NORM, bool PAIRS, int IT>
 __global__ void __launch_bounds__(256, head_blocks(NORM))
     heads_vec_kernel(const HeadArgs p, int lg, int q_chunks, float inv_dim) {
-  constexpr int V = HeadVec<T>::V, P = V / 2;
+  using Vec = HeadVec<T, V>;
+  using U = typename Vec::U;
+  constexpr int P = Vec::P;
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   int64_t rows = p.rows;
@@ -247,17 +296,16 @@ __global__ void __launch_bounds__(256, head_blocks(NORM))
   const int hop = per * p.head_dim;  // elements between a lane's heads
 
   const int pos = turn ? __ldg(p.pos + row) : 0;  // looked at once the rows are on their way
-  uint4 ua[IT], ub[IT];
+  U ua[IT], ub[IT];
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
-    ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
+    ua[i] = ub[i] = U{};
     if (live && head0 + i * per < heads) {
-      ua[i] = *reinterpret_cast<const uint4 *>(x + i * hop + e0);
-      ub[i] = *reinterpret_cast<const uint4 *>(x + i * hop + e1);
+      ua[i] = *reinterpret_cast<const U *>(x + i * hop + e0);
+      ub[i] = *reinterpret_cast<const U *>(x + i * hop + e1);
     }
   }
-  // cos and sin of the thread's pairs: two pairs a packed value (half), or
-  // one at a time (pairs)
+  // cos and sin of the thread's V pairs, two a packed value
   uint64_t c2[P], s2[P];
   if (turn) {
     const float4 *t =
@@ -285,8 +333,8 @@ __global__ void __launch_bounds__(256, head_blocks(NORM))
 #pragma unroll
   for (int i = 0; i < IT; ++i) {
     uint64_t a[P], b[P];
-    HeadVec<T>::unpack(ua[i], a);
-    HeadVec<T>::unpack(ub[i], b);
+    Vec::unpack(ua[i], a);
+    Vec::unpack(ub[i], b);
     if constexpr (NORM != kHeadNormNone) {
       if constexpr (NORM == kHeadNormLayer) {
         uint64_t m2 = 0;
@@ -331,23 +379,16 @@ __global__ void __launch_bounds__(256, head_blocks(NORM))
     }
     if (turn) {
       if constexpr (PAIRS) {
-        // a[v] and b[v] are a pair each; the table entries of pair v of a are
-        // half v % 2 of entry v / 2, those of b follow
+        // a[v] and b[v] are a pair each, number v and P + v of the thread's
 #pragma unroll
         for (int v = 0; v < P; ++v) {
-          float ca, cb, sa, sb, lo, hi, x0, x1;
-          unpk2(c2[v / 2], lo, hi);
-          ca = v & 1 ? hi : lo;
-          unpk2(s2[v / 2], lo, hi);
-          sa = v & 1 ? hi : lo;
-          unpk2(c2[(P + v) / 2], lo, hi);
-          cb = v & 1 ? hi : lo;
-          unpk2(s2[(P + v) / 2], lo, hi);
-          sb = v & 1 ? hi : lo;
+          float c, t, x0, x1;
+          head_entry<P>(c2, s2, v, c, t);
           unpk2(a[v], x0, x1);
-          a[v] = pk2(fmaf(-x1, sa, x0 * ca), fmaf(x0, sa, x1 * ca));
+          a[v] = pk2(fmaf(-x1, t, x0 * c), fmaf(x0, t, x1 * c));
+          head_entry<P>(c2, s2, P + v, c, t);
           unpk2(b[v], x0, x1);
-          b[v] = pk2(fmaf(-x1, sb, x0 * cb), fmaf(x0, sb, x1 * cb));
+          b[v] = pk2(fmaf(-x1, t, x0 * c), fmaf(x0, t, x1 * c));
         }
       } else {
 #pragma unroll
@@ -359,8 +400,8 @@ __global__ void __launch_bounds__(256, head_blocks(NORM))
       }
     }
     if (live && head0 + i * per < heads) {
-      *reinterpret_cast<uint4 *>(out + i * hop + e0) = HeadVec<T>::pack(a);
-      *reinterpret_cast<uint4 *>(out + i * hop + e1) = HeadVec<T>::pack(b);
+      *reinterpret_cast<U *>(out + i * hop + e0) = Vec::pack(a);
+      *reinterpret_cast<U *>(out + i * hop + e1) = Vec::pack(b);
     }
   }
 }

@@ -234,38 +234,52 @@ int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t
   return NEBW_OK;
 }
 
-template <typename T, int NORM, bool PAIRS, int IT>
-void launch_heads_vec(const nebw::HeadArgs &a, int lg, int per, cudaStream_t st) {
+template <typename T, int V, int NORM, bool PAIRS, int IT>
+int launch_heads_it(const nebw::HeadArgs &a, int lg, int per, cudaStream_t st) {
   const int q_chunks = (a.q.heads + per * IT - 1) / (per * IT);
   const int chunks = q_chunks + (a.k.heads + per * IT - 1) / (per * IT);
   const dim3 grid(static_cast<unsigned>((a.rows + 7) / 8), chunks);
-  nebw::heads_vec_kernel<T, NORM, PAIRS, IT>
+  nebw::heads_vec_kernel<T, V, NORM, PAIRS, IT>
       <<<grid, 256, 0, st>>>(a, lg, q_chunks, 1.0f / static_cast<float>(a.head_dim));
+  NEBW_CUDA(cudaGetLastError());
+  return NEBW_OK;
 }
 
-bool heads_vec_side(const nebw::HeadSide &s, size_t esz) {
-  return aligned(s.x, 16) && aligned(s.out, 16) && s.stride * esz % 16 == 0 &&
-         s.out_stride * esz % 16 == 0 && aligned(s.gamma, 16) && aligned(s.beta, 16);
+bool heads_vec_side(const nebw::HeadSide &s, size_t esz, int v) {
+  const size_t bytes = v * esz, weights = std::min<size_t>(16, v * sizeof(float));
+  return aligned(s.x, bytes) && aligned(s.out, bytes) && s.stride * esz % bytes == 0 &&
+         s.out_stride * esz % bytes == 0 && aligned(s.gamma, weights) && aligned(s.beta, weights);
+}
+
+// Whether vectors of v elements fit the heads (and a head a warp).
+bool heads_vec_fit(const nebw::HeadArgs &a, size_t esz, int v) {
+  return a.head_dim % (2 * v) == 0 && a.head_dim <= 64 * v && a.n % v == 0 &&
+         heads_vec_side(a.q, esz, v) && heads_vec_side(a.k, esz, v);
+}
+
+template <typename T, int V, int NORM, bool PAIRS>
+int launch_heads_vec(const nebw::HeadArgs &a, cudaStream_t st) {
+  int lg = 0;  // lanes a head
+  while ((2 * V << lg) < a.head_dim) ++lg;
+  const int per = 32 >> lg;  // heads a warp takes at once
+  if constexpr (V * sizeof(T) == 16) {
+    // four turns a warp share its table entries and weights (144 us against
+    // 170 for two, on the RMS case at heads_vec_kernel); one or two where the
+    // heads end there
+    const int most = std::max(a.q.heads, a.k.heads);
+    if (most <= per) return launch_heads_it<T, V, NORM, PAIRS, 1>(a, lg, per, st);
+    if (most <= 2 * per) return launch_heads_it<T, V, NORM, PAIRS, 2>(a, lg, per, st);
+  }
+  return launch_heads_it<T, V, NORM, PAIRS, 4>(a, lg, per, st);
 }
 
 template <typename T, int NORM, bool PAIRS>
 int launch_heads(const nebw::HeadArgs &a, cudaStream_t st) {
-  constexpr int V = nebw::HeadVec<T>::V;
-  if (a.head_dim % (2 * V) == 0 && a.n % V == 0 && heads_vec_side(a.q, sizeof(T)) &&
-      heads_vec_side(a.k, sizeof(T))) {
-    int lg = 0;  // lanes a head
-    while ((2 * V << lg) < a.head_dim) ++lg;
-    const int per = 32 >> lg;  // heads a warp takes at once
-    const int most = std::max(a.q.heads, a.k.heads);
-    // four turns a warp share its table entries and weights (144 us against
-    // 170 for two, on the RMS case at heads_vec_kernel)
-    const int it = most > 2 * per ? 4 : most > per ? 2 : 1;
-    if (it == 4) launch_heads_vec<T, NORM, PAIRS, 4>(a, lg, per, st);
-    else if (it == 2) launch_heads_vec<T, NORM, PAIRS, 2>(a, lg, per, st);
-    else launch_heads_vec<T, NORM, PAIRS, 1>(a, lg, per, st);
-    NEBW_CUDA(cudaGetLastError());
-    return NEBW_OK;
-  }
+  constexpr int V = 16 / sizeof(T);
+  if (heads_vec_fit(a, sizeof(T), V)) return launch_heads_vec<T, V, NORM, PAIRS>(a, st);
+  if constexpr (sizeof(T) == 2)
+    if (heads_vec_fit(a, sizeof(T), 4)) return launch_heads_vec<T, 4, NORM, PAIRS>(a, st);
+  if (heads_vec_fit(a, sizeof(T), 2)) return launch_heads_vec<T, 2, NORM, PAIRS>(a, st);
   const int heads = a.q.heads + a.k.heads;
   const int64_t blocks = (a.rows * heads + 7) / 8;
   NEBW_REQUIRE(blocks < (1ll << 31), "too many heads: %lld rows of %d",

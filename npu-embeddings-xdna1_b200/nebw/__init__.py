@@ -218,8 +218,10 @@ def _addr(x):
         return None
     if isinstance(x, int):
         return x
-    if hasattr(x, "data_ptr"):
+    try:
         return x.data_ptr()
+    except AttributeError:
+        pass
     if isinstance(x, np.ndarray):
         return x.ctypes.data
     raise TypeError(f"cannot take the address of {type(x)}")
