@@ -66,23 +66,30 @@ struct GroupedArgs {
   const int *row_src;  // [rows] or null
   int a_rows;          // A's rows
   int N, K;            // N as staged (2F for a gated weight)
+  int tile_rows;       // most rows of a tile: 256, 128 or 64
   const float *bias;   // [experts, N] in the container's column order, or null
   void *out;           // [rows, N or N / 2]
   int *err;
 };
 
-// Shared memory, the same for both: 128 rows of A and up to 128 of W a stage.
+// Shared memory of a CTA: a ring of stages of 128 rows of W and half a tile's
+// rows of A, each 64 wide.  The fewer rows a tile may have (the launch's
+// choice), the deeper the ring.
 struct GroupedShape {
-  static constexpr int kABytes = kGemmBM * kGemmBK * 2;
-  static constexpr int kStageBytes = 2 * kABytes;
-  static constexpr int kStages = 5;
+  static constexpr int kWBytes = 128 * kGemmBK * 2;
+  static constexpr int kRingBytes = 168 * 1024;
+  static constexpr int kMaxStages = 8;
+  __host__ __device__ static constexpr int stages(int tile_rows) {
+    const int n = kRingBytes / (kWBytes + tile_rows / 2 * kGemmBK * 2);
+    return n < kMaxStages ? n : kMaxStages;
+  }
   static constexpr int kWarpStaging = 6 * 1024;  // one fp32 or three bf16 chunks
   static constexpr int kStagingBytes = 8 * kWarpStaging;
   static constexpr int kBarBytes = 256;
   static constexpr int kList = 128;  // tiles of a block looked up beforehand
   static constexpr int kTableBytes = kList * 16 + 2 * (kGroupMaxExperts + 1) * 4 + 8;
   static constexpr int kSmemBytes =
-      1024 + kStages * kStageBytes + kStagingBytes + kBarBytes + kTableBytes;
+      1024 + kRingBytes + kStagingBytes + kBarBytes + kTableBytes;
 };
 constexpr int kGroupedBox = 32;  // rows of the TMA boxes that end a group of A
 constexpr int kGroupedThreads = 320;
@@ -125,13 +132,13 @@ struct GroupTable {
 };
 static_assert(sizeof(GroupTable) == GroupedShape::kTableBytes, "table size");
 
-constexpr int kGroupTileRows = 256, kGroupTileCols = 256;
+constexpr int kGroupTileCols = 256;
 
-// Tile t: a group of m rows is cut into ceil(m / 256) tiles of equal size,
-// rounded up to 32 rows.
-__device__ __forceinline__ GroupTile group_find(const GroupTable &g, int experts, int t,
+// Tile t: a group of m rows is cut into ceil(m / tile_rows) tiles of equal
+// size, rounded up to 32 rows.
+__device__ __forceinline__ GroupTile group_find(const GroupTable &g, const GroupedArgs &p, int t,
                                                 int n_blocks) {
-  int lo = 0, hi = experts;  // tile[lo] <= t < tile[hi]
+  int lo = 0, hi = p.experts;  // tile[lo] <= t < tile[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (t >= g.tile[mid]) lo = mid;
@@ -139,7 +146,7 @@ __device__ __forceinline__ GroupTile group_find(const GroupTable &g, int experts
   }
   const int i = t - g.tile[lo], b = i / n_blocks;
   const int m = g.off[lo + 1] - g.off[lo];
-  const int tiles = (m + kGroupTileRows - 1) / kGroupTileRows;
+  const int tiles = (m + p.tile_rows - 1) / p.tile_rows;
   const int size = ((m + tiles - 1) / tiles + 31) / 32 * 32;
   const int row = g.off[lo] + b * size;
   return {lo, row, min(row + size, g.off[lo + 1]), i - b * n_blocks};
@@ -172,7 +179,7 @@ __device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedAr
     // expert e - 1 is [off[e - 1], off[e]): its tiles end at tile[e]
     int before = __shfl_up_sync(0xffffffffu, v, 1);
     if (lane == 0) before = e0 ? hi : v;
-    int t = (v - before + kGroupTileRows - 1) / kGroupTileRows * n_blocks;
+    int t = (v - before + p.tile_rows - 1) / p.tile_rows * n_blocks;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int w = __shfl_up_sync(0xffffffffu, t, o);
@@ -190,9 +197,9 @@ __device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedAr
 }
 
 // This block's tile number `local`, tile t.
-__device__ __forceinline__ GroupTile group_tile(const GroupTable &g, int experts, int local, int t,
-                                                int n_blocks) {
-  return local < GroupedShape::kList ? g.list[local] : group_find(g, experts, t, n_blocks);
+__device__ __forceinline__ GroupTile group_tile(const GroupTable &g, const GroupedArgs &p,
+                                                int local, int t, int n_blocks) {
+  return local < GroupedShape::kList ? g.list[local] : group_find(g, p, t, n_blocks);
 }
 
 // Both warps of an epilogue pair: wait, and whether `ok` held for both (each
@@ -300,17 +307,18 @@ __global__ void __cluster_dims__(2, 1, 1)
                              const __grid_constant__ CUtensorMap tmW,
                              const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
   using S = GroupedShape;
-  constexpr int kStages = S::kStages;
+  const int stages = S::stages(p.tile_rows);
+  const int a_bytes = p.tile_rows / 2 * kGemmBK * 2;
   constexpr int kAccCols = 256;  // TMEM columns of an accumulator: the tile's rows
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  uint8_t *sA = smem;
-  uint8_t *sW = smem + kStages * S::kABytes;
-  uint8_t *staging = smem + kStages * S::kStageBytes;
+  uint8_t *sW = smem;
+  uint8_t *sA = smem + stages * S::kWBytes;
+  uint8_t *staging = smem + S::kRingBytes;
   uint64_t *full = reinterpret_cast<uint64_t *>(staging + S::kStagingBytes);
-  uint64_t *empty = full + kStages;
-  uint64_t *tfull = empty + kStages;
+  uint64_t *empty = full + S::kMaxStages;
+  uint64_t *tfull = empty + S::kMaxStages;
   uint64_t *tempty = tfull + 2;
   uint64_t *drain = tempty + 2;
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
@@ -331,7 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     tmem_alloc_pair(tmem_slot, 2 * kAccCols);
     tmem_relinquish_pair();
   } else if (warp == 2 && lane == 0) {
-    for (int s = 0; s < kStages; ++s) {
+    for (int s = 0; s < stages; ++s) {
       // every gather warp arrives on every stage, also with no row to load:
       // one that did not could fall a phase behind the ring, whose parity
       // then reads the wrong way round
@@ -354,7 +362,7 @@ __global__ void __cluster_dims__(2, 1, 1)
   for (int i = threadIdx.x; i < S::kList; i += blockDim.x) {
     const int64_t t = first + static_cast<int64_t>(i) * step;
     if (t < table.tile[p.experts])
-      table.list[i] = group_find(table, p.experts, static_cast<int>(t), n_blocks);
+      table.list[i] = group_find(table, p, static_cast<int>(t), n_blocks);
   }
   tc_fence_before();
   cluster_sync();  // barriers and TMEM of both CTAs, this CTA's list
@@ -379,8 +387,8 @@ __global__ void __cluster_dims__(2, 1, 1)
       uint32_t phase = 0;
       bool ok = true;
       for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-        const GroupTile t = group_tile(table, p.experts, local, tile, n_blocks);
-        uint32_t bytes = 2 * S::kABytes;  // W
+        const GroupTile t = group_tile(table, p, local, tile, n_blocks);
+        uint32_t bytes = 2 * S::kWBytes;
         for (int c = 0; c < 2; ++c) {
           const int m = cta_rows(t, c);
           bytes += GATHER ? (m + 3) / 4 * 512
@@ -396,15 +404,15 @@ __global__ void __cluster_dims__(2, 1, 1)
           }
           if (leader) mbar_arrive_expect_tx(&full[stage], bytes);
           const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
-          tma_load_2d_pair(sW + stage * S::kABytes, &tmW, bar, kb * kGemmBK, w_row);
+          tma_load_2d_pair(sW + stage * S::kWBytes, &tmW, bar, kb * kGemmBK, w_row);
           if (boxes == kGemmBM / kGroupedBox) {
-            tma_load_2d_pair(sA + stage * S::kABytes, &tmA128, bar, kb * kGemmBK, a_row);
+            tma_load_2d_pair(sA + stage * a_bytes, &tmA128, bar, kb * kGemmBK, a_row);
           } else {
             for (int i = 0; i < boxes; ++i)
-              tma_load_2d_pair(sA + stage * S::kABytes + i * kGroupedBox * 128, &tmA, bar,
+              tma_load_2d_pair(sA + stage * a_bytes + i * kGroupedBox * 128, &tmA, bar,
                           kb * kGemmBK, a_row + i * kGroupedBox);
           }
-          if (++stage == kStages) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -413,9 +421,9 @@ __global__ void __cluster_dims__(2, 1, 1)
       // Tail: the MMAs have released every stage, so all loads of this CTA
       // (the gathers too) have landed and all commits aimed at its barriers
       // have arrived before it may exit.
-      for (int i = 0; i < kStages && ok; ++i) {
+      for (int i = 0; i < stages && ok; ++i) {
         if (!mbar_wait(&empty[stage], phase ^ 1u, p.err)) break;
-        if (++stage == kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }
@@ -430,7 +438,7 @@ __global__ void __cluster_dims__(2, 1, 1)
       bool issued_any = false, ok = true;
       int local = 0;
       for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-        const GroupTile t = group_tile(table, p.experts, local, tile, n_blocks);
+        const GroupTile t = group_tile(table, p, local, tile, n_blocks);
         const uint32_t idesc = idesc_bf16_f32(256, tile_n(t));
         const int acc = local & 1;
         if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
@@ -442,8 +450,8 @@ __global__ void __cluster_dims__(2, 1, 1)
             break;
           }
           tc_fence_after();
-          const uint64_t da = sdesc_kmajor_sw128(smem_u32(sA + stage * S::kABytes));
-          const uint64_t dw = sdesc_kmajor_sw128(smem_u32(sW + stage * S::kABytes));
+          const uint64_t da = sdesc_kmajor_sw128(smem_u32(sA + stage * a_bytes));
+          const uint64_t dw = sdesc_kmajor_sw128(smem_u32(sW + stage * S::kWBytes));
           if (elect) {
 #pragma unroll
             for (int k = 0; k < kGemmBK / 16; ++k)
@@ -452,7 +460,7 @@ __global__ void __cluster_dims__(2, 1, 1)
           }
           __syncwarp();
           issued_any = true;
-          if (++stage == kStages) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1u;
           }
@@ -490,7 +498,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     int local = 0;
     for (int tile = first; tile < num_tiles; tile += step, ++local) {
       const int acc = local & 1;
-      const GroupTile t = group_tile(table, p.experts, local, tile, n_blocks);
+      const GroupTile t = group_tile(table, p, local, tile, n_blocks);
       // first W column of the quarter (of the pair of quarters), and of C
       const int col = t.nb * 256 + rank * 128 + (kGated ? quarter & 2 : quarter) * 32;
       const int c0 = kGated ? col / 2 : col;
@@ -615,7 +623,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     };
     auto index_of = [&](int l, int tile) -> int {
       if (tile >= num_tiles) return 0;
-      const GroupTile t = group_tile(table, p.experts, l, tile, n_blocks);
+      const GroupTile t = group_tile(table, p, l, tile, n_blocks);
       const int count = count_of(t);
       // past the group: its last row again, to fill a gather of four
       return count ? __ldg(p.row_src + t.row + rank * (tile_n(t) / 2) + kGatherRows * part +
@@ -624,7 +632,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     };
     int next = index_of(0, first);
     for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
-      const int count = count_of(group_tile(table, p.experts, local, tile, n_blocks));
+      const int count = count_of(group_tile(table, p, local, tile, n_blocks));
       int mine = next;
       next = index_of(local + 1, tile + step);
       if (mine < 0 || mine >= p.a_rows) {
@@ -640,7 +648,7 @@ __global__ void __cluster_dims__(2, 1, 1)
           break;
         }
         if (elect) {
-          const uint32_t dst = smem_u32(sA + stage * S::kABytes) + part * (kGatherRows * 128);
+          const uint32_t dst = smem_u32(sA + stage * a_bytes) + part * (kGatherRows * 128);
           const uint32_t bar = map_to_cta(smem_u32(&full[stage]), 0);
 #pragma unroll
           for (int i = 0; i < kGatherRows / 4; ++i)
@@ -650,7 +658,7 @@ __global__ void __cluster_dims__(2, 1, 1)
           grp_arrive(bar);
         }
         __syncwarp();
-        if (++stage == kStages) {
+        if (++stage == stages) {
           stage = 0;
           phase ^= 1u;
         }

@@ -261,13 +261,17 @@ __device__ __forceinline__ void head_entry(const uint64_t (&c2)[P], const uint64
 }
 
 // Blocks an SM must hold, which bounds the registers.  Measured (us, at 4 / 3 /
-// 2 blocks; 49,999 rows of 16 + 16 heads of 128, bf16): no norm 132 / 131 /
-// 157 (and 83 / 92 / 92 for 65,539 rows of 32 heads of 64, pairs, a quarter
-// of the work), RMS 188 / 144 / 156, LayerNorm 270 / 224 / 178.
-constexpr int head_blocks(int norm) { return norm == kHeadNormNone ? 4 : norm == kHeadNormRms ? 3 : 2; }
+// 2 blocks; 49,999 rows of 16 + 16 heads of 128, bf16, V = 8): no norm 132 /
+// 131 / 157 (and 83 / 92 / 92 for 65,539 rows of 32 heads of 64, pairs, a
+// quarter of the work), RMS 188 / 144 / 156, LayerNorm 270 / 224 / 178.  Half
+// the vector holds half the state: RMS 106 / 115 / 115 (25,000 rows, fp32,
+// heads of 96), LayerNorm 178 / 202 / 204 (bf16, heads of 80 turning 40).
+constexpr int head_blocks(int norm, int v) {
+  return norm == kHeadNormNone || v < 8 ? 4 : norm == kHeadNormRms ? 3 : 2;
+}
 
 template <typename T, int V, int NORM, bool PAIRS, int IT>
-__global__ void __launch_bounds__(256, head_blocks(NORM))
+__global__ void __launch_bounds__(256, head_blocks(NORM, V))
     heads_vec_kernel(const HeadArgs p, int lg, int q_chunks, float inv_dim) {
   using Vec = HeadVec<T, V>;
   using U = typename Vec::U;

@@ -579,7 +579,7 @@ void launch_grouped_epi(const GroupedMaps &m, const nebw::GroupedArgs &a, unsign
 int launch_grouped(nebw_dev *d, const GroupedMaps &m, int epi, const nebw::GroupedArgs &a,
                    cudaStream_t st) {
   // the most tiles that the groups can make: every one may end in a part tile
-  const int64_t tiles = (a.rows / nebw::kGroupTileRows + std::min(a.experts, a.rows)) *
+  const int64_t tiles = (a.rows / a.tile_rows + std::min(a.experts, a.rows)) *
                         int64_t{(a.N + nebw::kGroupTileCols - 1) / nebw::kGroupTileCols};
   NEBW_REQUIRE(tiles < (1ll << 30), "grouped product too large");
   const unsigned g = 2 * static_cast<unsigned>(std::min<int64_t>(tiles, d->grouped_pairs));
@@ -654,6 +654,8 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   else if (int rc = make_tmap_kmajor(&m.a128, A, a_rows, K, nebw::kGemmBM)) return rc;
   if (int rc = make_tmap_out(&m.c, C, rows, w.gated ? N / 2 : N, c_dtype == NEBW_BF16)) return rc;
   m.w = w.map;
+  static const int kCap = std::getenv("GRP_CAP") ? std::atoi(std::getenv("GRP_CAP")) : 256;
+  a.tile_rows = kCap;
   return launch_grouped(d, m, epi, a, pick_stream(d, stream));
 }
 
