@@ -496,8 +496,9 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   NEBW_REQUIRE(dtype == NEBW_F32 || dtype == NEBW_BF16, "weight dtype %d refused", dtype);
   NEBW_REQUIRE(experts >= 1 && experts <= nebw::kGroupMaxExperts, "%d experts refused: 1 .. %d",
                experts, nebw::kGroupMaxExperts);
+  const int64_t col_blocks = (N + 255) / 256 * 2, k_blocks = (K + 63) / 64;
   NEBW_REQUIRE(K >= 64 && N >= 8 && K % 8 == 0 && N % 8 == 0 && K <= (1 << 20) &&
-                   N < (1ll << 30) && N * experts < (1ll << 30),
+                   N <= (1 << 20) && experts * col_blocks * k_blocks < (1 << 24),
                "expert weights [%d, K=%lld, N=%lld] refused: K >= 64, K %% 8 == 0, N %% 8 == 0",
                experts, static_cast<long long>(K), static_cast<long long>(N));
   NEBW_REQUIRE(!gated || N % 64 == 0,
@@ -514,18 +515,21 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   w.N = N;
   w.gated = gated != 0;
   void *tmp = nullptr;
-  if (cudaMalloc(&w.ptr, static_cast<size_t>(experts) * K * N * 2) != cudaSuccess ||
+  const int64_t blocks = experts * col_blocks * k_blocks;
+  if (cudaMalloc(&w.ptr, static_cast<size_t>(blocks) * 128 * 64 * 2) != cudaSuccess ||
       (!on_device && cudaMalloc(&tmp, one) != cudaSuccess)) {
     cudaGetLastError();
     cudaFree(w.ptr);
     return set_error(NEBW_ENOMEM, "cudaMalloc for [%d, %lld, %lld] expert weights failed", experts,
                      static_cast<long long>(N), static_cast<long long>(K));
   }
-  const unsigned gx = static_cast<unsigned>((N + 31) / 32), gy = static_cast<unsigned>((K + 31) / 32);
+  const unsigned gx = static_cast<unsigned>(col_blocks * 4), gy = static_cast<unsigned>(k_blocks * 2);
+  const int cb = static_cast<int>(col_blocks), kb = static_cast<int>(k_blocks);
   cudaError_t e = cudaSuccess;
   if (on_device) {
     nebw::stage_experts_kernel<<<dim3(gx, gy, experts), dim3(32, 8), 0, st>>>(
-        kn, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, 0, w.ptr);
+        kn, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, 0, cb, kb,
+        w.ptr);
     e = cudaGetLastError();
   } else {
     for (int i = 0; i < experts && e == cudaSuccess; ++i) {  // one expert's copy at a time
@@ -533,7 +537,8 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
                           cudaMemcpyHostToDevice, st);
       if (e != cudaSuccess) break;
       nebw::stage_experts_kernel<<<dim3(gx, gy, 1), dim3(32, 8), 0, st>>>(
-          tmp, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, i, w.ptr);
+          tmp, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, i, cb, kb,
+          w.ptr);
       e = cudaGetLastError();
     }
   }
@@ -542,7 +547,7 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   int rc = NEBW_OK;
   if (e != cudaSuccess)
     rc = set_error(NEBW_ECUDA, "expert weight staging failed: %s", cudaGetErrorString(e));
-  if (!rc) rc = make_tmap_kmajor(&w.map, w.ptr, experts * N, K, 128);
+  if (!rc) rc = make_tmap_kmajor(&w.map, w.ptr, blocks * 128, 64, 128);
   if (!rc) {
     try {
       d->experts[d->next_handle] = w;
@@ -654,8 +659,11 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   else if (int rc = make_tmap_kmajor(&m.a128, A, a_rows, K, nebw::kGemmBM)) return rc;
   if (int rc = make_tmap_out(&m.c, C, rows, w.gated ? N / 2 : N, c_dtype == NEBW_BF16)) return rc;
   m.w = w.map;
-  static const int kCap = std::getenv("GRP_CAP") ? std::atoi(std::getenv("GRP_CAP")) : 256;
-  a.tile_rows = kCap;
+  // small groups: half the rows a tile, two more stages in the ring (15.4
+  // against 17.0 us at 64 rows a group, 8 experts, K 768, N 3840 gated; 27.1
+  // against 29.6 at 32, 64 experts, K and N 1024); from 128 rows a group on
+  // whole tiles read W once (36.9 against 34.7 us there)
+  a.tile_rows = rows <= 64 * std::min<int64_t>(w.experts, rows) ? 128 : 256;
   return launch_grouped(d, m, epi, a, pick_stream(d, stream));
 }
 

@@ -224,14 +224,15 @@ struct WeightI8 {
   CUtensorMap map64, map128, map256;  // box rows 64 / 128 / 256, 128-byte K boxes
 };
 
-// The weights of a set of experts (nebw_stage_experts): bf16 [experts, N, K],
-// a gated set's N interleaved in groups of 64 = [32 up | 32 gate].
+// The weights of a set of experts (nebw_stage_experts): bf16 in blocks of 128
+// columns by 64 of K (stage_experts_kernel), a gated set's columns interleaved
+// in groups of 64 = [32 up | 32 gate].
 struct Experts {
   __nv_bfloat16 *ptr = nullptr;
   int experts = 0;
   int64_t K = 0, N = 0;
   bool gated = false;
-  CUtensorMap map;  // [experts * N, K], box rows 128
+  CUtensorMap map;  // the blocks' rows, [blocks * 128, 64], box rows 128
 };
 
 // cos and sin of every position and frequency (nebw_stage_rope).
