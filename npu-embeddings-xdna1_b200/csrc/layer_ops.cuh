@@ -374,10 +374,17 @@ namespace {
 
 constexpr int kRouteMostBlocks = 256;  // no sm_100 GPU has more SMs
 
-// Blocks of the two-kernel form (1: the fused one): one an SM at most, which
-// keeps the counts that every block sums small, of 32 rows at least.
+// One block chooses and places up to about where the two-kernel form takes
+// over (measured equal at 190 rows of 64 experts by 8, 128 of 256 by 8, 1024
+// of 8 by 2: 6.7 / 9.5 / 6.3 us): that much work of its rows.
+bool route_fused(int64_t rows, int64_t experts, int64_t top_k) {
+  return rows * (experts + 16 * top_k) <= 40000;
+}
+
+// Blocks of the two-kernel form: one an SM at most, which keeps the counts
+// that every block sums small (two an SM: 28 us against 27 on 131,071 rows of
+// 64 experts by 8, 27 against 20 on 31,000 of 256), of 32 rows at least.
 int64_t route_blocks(int64_t rows, int sms) {
-  if (rows <= nebw::kRouteFusedRows) return 1;
   return std::min<int64_t>((rows + 31) / 32, std::min(sms, kRouteMostBlocks));
 }
 
@@ -394,7 +401,7 @@ int check_route(int64_t rows, int32_t experts, int32_t top_k) {
 template <typename T, int K, int LG>
 int launch_route_lg(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
   const size_t smem = route_smem(a.experts);
-  if (blocks == 1) {
+  if (blocks == 0) {
     nebw::route_fused_kernel<T, K, LG><<<1, nebw::kRouteThreads, smem, st>>>(a);
   } else {
     nebw::route_choose_kernel<T, K, LG><<<blocks, nebw::kRouteThreads, 0, st>>>(a);
@@ -431,7 +438,7 @@ int launch_route_k(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
 
 extern "C" int64_t nebw_moe_route_workspace(int64_t rows, int32_t experts, int32_t top_k) {
   if (check_route(rows, experts, top_k)) return -1;
-  if (rows <= nebw::kRouteFusedRows) return 0;
+  if (route_fused(rows, experts, top_k)) return 0;
   return int64_t{kRouteMostBlocks} * experts * static_cast<int64_t>(sizeof(int));
 }
 
@@ -481,9 +488,11 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
   a.vec = experts % 8 == 0 && aligned(logits, 16) && stride * esz % 16 == 0;
   a.tiles = route_tiles(experts);
   a.whole = (top_k == 4 || top_k == 8 || top_k == 16) && aligned(ids, 16) && aligned(row_dst, 16);
-  int blocks = static_cast<int>(route_blocks(rows, d->sm_count));
+  const bool fused = route_fused(rows, experts, top_k);
+  int blocks = fused ? 1 : static_cast<int>(route_blocks(rows, d->sm_count));
   a.block_rows = static_cast<int>(((rows + blocks - 1) / blocks + 31) / 32 * 32);
   blocks = static_cast<int>((rows + a.block_rows - 1) / a.block_rows);
+  if (fused) blocks = 0;  // no counts of blocks
   return dtype == NEBW_F32 ? launch_route_k<float>(a, blocks, st)
                            : launch_route_k<__nv_bfloat16>(a, blocks, st);
 }

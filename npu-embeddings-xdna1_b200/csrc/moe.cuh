@@ -26,7 +26,6 @@ constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteMaxExperts = 512;
 constexpr int kRouteMaxK = 16;
-constexpr int kRouteFusedRows = 256;  // up to here one block does it all
 
 struct RouteArgs {
   const void *logits;  // [rows, stride], fp32 or bf16

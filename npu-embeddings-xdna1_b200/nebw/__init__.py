@@ -227,6 +227,23 @@ def _addr(x):
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
+_INT32 = None  # torch.int32, once torch is in use
+
+
+def _i32(x):
+    """Device address of int32 values: a torch tensor of another dtype or with
+    gaps is refused (its bytes would be read as other numbers)."""
+    global _INT32
+    if x is None or isinstance(x, int):
+        return x
+    if _INT32 is None:
+        import torch
+        _INT32 = torch.int32
+    if x.dtype is not _INT32 or not x.is_contiguous():
+        raise TypeError("contiguous int32 values are required")
+    return x.data_ptr()
+
+
 def _dtype(t) -> int:
     """F32 or BF16 of a torch tensor."""
     name = str(t.dtype)
@@ -398,8 +415,8 @@ class Device:
         return hnd.value
 
     def row_positions(self, seq_off, seq_len, B, max_len, pos, stream=None):
-        _check(lib().nebw_row_positions(self.h, _addr(seq_off), _addr(seq_len), B, max_len,
-                                        _addr(pos), self._s(stream)))
+        _check(lib().nebw_row_positions(self.h, _i32(seq_off), _i32(seq_len), B, max_len,
+                                        _i32(pos), self._s(stream)))
 
     @staticmethod
     def _heads_dtype(q, k, dtype):
@@ -416,15 +433,15 @@ class Device:
              stream=None):
         """Rotary positions on the heads q and k (Heads, either may be None) (nebw_rope)."""
         _check(lib().nebw_rope(self.h, q, k, self._heads_dtype(q, k, dtype), rows,
-                               _addr(rows_dev), head_dim, rope, layout, _addr(pos),
+                               _i32(rows_dev), head_dim, rope, layout, _i32(pos),
                                self._s(stream)))
 
     def qk_norm_rope(self, q, k, rows, head_dim, norm=HEADNORM_RMS, eps=1e-6, rope=0, pos=None,
                      layout=ROPE_HALF, dtype=None, rows_dev=None, stream=None):
         """A norm of every head, then the rotation (rope 0: none) (nebw_qk_norm_rope)."""
         _check(lib().nebw_qk_norm_rope(self.h, q, k, self._heads_dtype(q, k, dtype), rows,
-                                       _addr(rows_dev), head_dim, norm, eps, rope, layout,
-                                       _addr(pos), self._s(stream)))
+                                       _i32(rows_dev), head_dim, norm, eps, rope, layout,
+                                       _i32(pos), self._s(stream)))
 
     # ---- experts -----------------------------------------------------------
     def stage_experts(self, w_ekn, gated: bool = False, stream=None) -> int:
@@ -451,27 +468,32 @@ class Device:
         (nebw_moe_route)."""
         if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < experts:
             raise ValueError("logits are rows of at least `experts` adjacent values")
-        _check(lib().nebw_moe_route(self.h, logits.data_ptr(), _dtype(logits),
-                                    max(logits.stride(0), experts), rows, _addr(rows_dev),
-                                    experts, top_k, score, int(renorm), scale, _addr(ids),
-                                    _addr(weights), _addr(group_off), _addr(row_src),
-                                    _addr(row_dst), _addr(workspace),
+        if logits.shape[0] < rows:
+            raise ValueError("fewer logit rows than rows")
+        stride = logits.stride(0) if rows > 1 else experts  # one row: torch may give any
+        _check(lib().nebw_moe_route(self.h, logits.data_ptr(), _dtype(logits), stride, rows,
+                                    _i32(rows_dev), experts, top_k, score, int(renorm), scale,
+                                    _i32(ids),
+                                    _addr(weights), _i32(group_off), _i32(row_src),
+                                    _i32(row_dst), _addr(workspace),
                                     workspace.numel() * workspace.element_size(),
                                     self._s(stream)))
 
     def gemm_grouped(self, weight, A, a_rows, group_off, rows, K, N, C_out, row_src=None,
                      bias=None, act=ACT_NONE, c_dtype=BF16, stream=None):
         """One product per expert over its group of rows (nebw_gemm_grouped)."""
-        _check(lib().nebw_gemm_grouped(self.h, weight, _addr(A), a_rows, _addr(row_src),
-                                       _addr(group_off), rows, K, N, _addr(bias), act,
+        _check(lib().nebw_gemm_grouped(self.h, weight, _addr(A), a_rows, _i32(row_src),
+                                       _i32(group_off), rows, K, N, _addr(bias), act,
                                        _addr(C_out), c_dtype, self._s(stream)))
 
     def moe_combine(self, y, row_dst, weights, rows, top_k, H, out, residual=None, rows_dev=None,
                     stream=None):
         """The experts' rows y (torch, [places, H]) weighted and summed per
         row (nebw_moe_combine)."""
-        _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y.shape[0], _addr(row_dst),
-                                      _addr(weights), rows, _addr(rows_dev), top_k, H,
+        if not (y.is_contiguous() and out.is_contiguous()):
+            raise ValueError("expert rows and output are contiguous")
+        _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y.shape[0], _i32(row_dst),
+                                      _addr(weights), rows, _i32(rows_dev), top_k, H,
                                       _addr(residual), out.data_ptr(), _dtype(out),
                                       self._s(stream)))
 

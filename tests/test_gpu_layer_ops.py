@@ -441,7 +441,29 @@ ROUTE_CASES = [
     (1, 1, 1), (1, 8, 2), (5, 4, 4), (31, 6, 2), (100, 8, 2), (300, 16, 16), (64, 64, 8),
     (33, 60, 6), (129, 128, 4), (200, 200, 8), (70, 256, 8), (40, 512, 16), (513, 8, 2),
     (1500, 64, 8), (2049, 33, 1),
+    # around where one block hands over to two kernels, and one block with
+    # more rows than it places at once
+    (190, 64, 8), (220, 64, 8), (1000, 8, 2), (1001, 8, 2), (1990, 4, 1),
 ]
+
+
+@pytest.mark.parametrize("rows,experts,k", [(170001, 4, 1), (131071, 64, 8), (400003, 8, 2)])
+def test_route_many_rows(device, rows, experts, k):
+    """Many rows (also more than a block places at once) against the stable sort."""
+    x = torch.randn(rows, experts, generator=gen(rows), device="cuda").bfloat16()
+    r = Routing(rows, experts, k).run(device, x, renorm=True)
+    device.sync()
+    ids = x.float().sort(dim=1, descending=True, stable=True).indices[:, :k]
+    assert torch.equal(r.ids.long(), ids)
+    order = ids.reshape(-1).sort(stable=True)
+    edges = torch.arange(experts + 1, device="cuda")
+    assert torch.equal(r.off.long(), torch.searchsorted(order.values, edges))
+    assert torch.equal(r.src.long(), order.indices // k)
+    place = torch.empty_like(order.indices)
+    place[order.indices] = torch.arange(rows * k, device="cuda")
+    assert torch.equal(r.dst.long().reshape(-1), place)
+    want = torch.softmax(x.double().gather(1, ids), 1)
+    assert ((r.weights.double() - want).abs() <= 100 * U * want).all()
 
 
 @pytest.mark.parametrize("score,renorm", [(0, False), (0, True), (1, False), (1, True)])
@@ -546,7 +568,9 @@ def test_route_empty_and_refusals(device):
     refused("score", score=2)
     refused("scale", scale=float("inf"))
     refused("null routing", ids=None)
-    refused("workspace", ws=r.ws[:1], rows=1 << 20)
+    refused("workspace", logits=torch.zeros(1 << 20, 8, device="cuda"), ws=x, rows=1 << 20)
+    with pytest.raises(ValueError):
+        device.moe_route(x, 5, 8, 2, r.ids, r.weights, r.off, r.src, r.dst, r.ws)
     wide = torch.zeros(1, 600, device="cuda")
     refused("experts", logits=wide, rows=1, experts=513)
     with pytest.raises(ValueError):
@@ -621,6 +645,8 @@ GROUP_CASES = [
     # several tiles a block, with part tiles among them: one CTA, and a pair
     ([130, 3, 257, 1, 90, 128, 0, 200] * 10, 192, 1024),
     ([2100, 1, 900, 513, 40, 2500] * 2, 192, 1536),
+    # small groups but for one, which the smaller tiles cut in three
+    ([300, 1, 2, 0, 5, 3, 1, 0, 2, 6], 128, 520),
 ]
 EPILOGUES = [  # gated, act, output
     (False, 0, "bf16"), (False, 0, "f32"), (False, 1, "bf16"), (False, 2, "bf16"),
@@ -662,6 +688,22 @@ def test_grouped_product_matches_64_bits(device, sizes, K, N, gather, bias, gate
         assert_close(c[:M], *grouped_reference(a, w, off, src, b, gated, act))
     finally:
         device.release_weight(h)
+
+
+def test_grouped_product_of_more_tiles_than_are_looked_up(device):
+    """512 experts of a row each, 19 column tiles: over 128 tiles a block."""
+    E, K, N = 512, 64, 4864
+    w = torch.randn(E, K, N, generator=gen(9), device="cuda").bfloat16()
+    a = torch.randn(E, K, generator=gen(10), device="cuda").bfloat16()
+    h = device.stage_experts(w)
+    c = torch.empty(E, N, dtype=torch.bfloat16, device="cuda")
+    off = torch.arange(E + 1, device="cuda").int()
+    device.gemm_grouped(h, a, E, off, E, K, N, c)
+    device.sync()
+    want = torch.einsum("ek,ekn->en", a.double(), w.double())
+    size = torch.einsum("ek,ekn->en", a.double().abs(), w.double().abs())
+    assert_close(c, want, (K + 2) * 2 * U * size)
+    device.release_weight(h)
 
 
 def test_grouped_product_does_not_mix_groups(device):
@@ -811,6 +853,24 @@ def test_grouped_refusals(device):
     device.release_weight(plain)
     device.release_weight(gated)
     refused("unknown expert", g, plain, a, 8, off, 8, 64, 64, c)
+
+
+def test_whole_numbers_of_another_dtype_are_refused(device):
+    """int64 indices (torch's default) would be read as other numbers."""
+    import nebw
+    x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
+    inv, _ = nebw.rope_freqs(10000.0, 64)
+    h = device.stage_rope(inv, 16)
+    w = device.stage_experts(np.zeros((1, 64, 64), np.float32))
+    with pytest.raises(TypeError):
+        device.rope(nebw.Heads.of(x, 1), None, 4, 64, h, torch.arange(4, device="cuda"))
+    with pytest.raises(TypeError):
+        device.gemm_grouped(w, x, 4, torch.tensor([0, 4], device="cuda"), 4, 64, 64, x.clone())
+    with pytest.raises(TypeError):  # every second value
+        device.moe_combine(x, torch.zeros(4, 2, dtype=torch.int32, device="cuda")[:, :1],
+                           torch.zeros(4, 1, device="cuda"), 4, 1, 64, x.clone())
+    device.release_weight(h)
+    device.release_weight(w)
 
 
 # ---------------------------------------------------------------------------
