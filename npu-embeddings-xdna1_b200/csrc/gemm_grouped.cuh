@@ -155,46 +155,56 @@ __device__ __forceinline__ GroupTile group_find(const GroupTable &g, const Group
   return {lo, row, min(row + size, g.off[lo + 1]), i - b * n_blocks};
 }
 
-// off and tile, by one warp.
+// off and tile, by one warp: four consecutive experts a lane, 128 a round.
 __device__ __forceinline__ void group_table_build(GroupTable &g, const GroupedArgs &p,
                                                   int n_blocks, int lane) {
-  int hi = 0, tiles = 0;  // the running maximum of off, and the tiles so far
+  int top = 0, tiles = 0;  // off's running maximum, and the tiles so far
   bool bad = false;
-  int raw[4];
-  for (int e0 = 0; e0 <= p.experts; e0 += 32) {
-    const int u = e0 / 32 % 4;
-    if (u == 0) {  // four loads together
+  for (int e0 = 0; e0 <= p.experts; e0 += 128) {
+    const int e = e0 + 4 * lane;
+    int v[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        raw[i] = e0 + 32 * i + lane <= p.experts ? __ldg(p.off + e0 + 32 * i + lane) : 0;
+    for (int i = 0; i < 4; ++i) v[i] = e + i <= p.experts ? __ldg(p.off + e + i) : 0;
+    // ascending and within [0, rows]: what is not is reported and clamped
+    int most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int c = max(min(max(v[i], 0), p.rows), most);
+      bad |= e + i <= p.experts && c != v[i];
+      most = v[i] = c;
     }
-    const int e = e0 + lane;
-    const int given = u == 0 ? raw[0] : u == 1 ? raw[1] : u == 2 ? raw[2] : raw[3];
-    int v = min(max(given, 0), p.rows);
-    bad |= e <= p.experts && given != v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int w = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v = max(v, w);
+      const int w = __shfl_up_sync(0xffffffffu, most, o);
+      if (lane >= o) most = max(most, w);
     }
-    v = max(v, hi);
-    bad |= e <= p.experts && v > given;
+    int before = __shfl_up_sync(0xffffffffu, most, 1);
+    before = lane ? max(before, top) : top;
     // expert e - 1 is [off[e - 1], off[e]): its tiles end at tile[e]
-    int before = __shfl_up_sync(0xffffffffu, v, 1);
-    if (lane == 0) before = e0 ? hi : v;
-    int t = (v - before + p.tile_rows - 1) / p.tile_rows * n_blocks;
+    int t[4], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bad |= e + i <= p.experts && v[i] < before;
+      v[i] = max(v[i], before);
+      if (e + i > 0) sum += (v[i] - before + p.tile_rows - 1) / p.tile_rows * n_blocks;
+      t[i] = sum;
+      before = v[i];
+    }
+    int all = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int w = __shfl_up_sync(0xffffffffu, t, o);
-      if (lane >= o) t += w;
+      const int w = __shfl_up_sync(0xffffffffu, all, o);
+      if (lane >= o) all += w;
     }
-    t += tiles;
-    if (e <= p.experts) {
-      g.off[e] = v;
-      g.tile[e] = t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (e + i <= p.experts) {
+        g.off[e + i] = v[i];
+        g.tile[e + i] = tiles + all - sum + t[i];
+      }
     }
-    hi = __shfl_sync(0xffffffffu, v, 31);
-    tiles = __shfl_sync(0xffffffffu, t, 31);
+    top = max(top, __shfl_sync(0xffffffffu, most, 31));
+    tiles += __shfl_sync(0xffffffffu, all, 31);
   }
   if (bad && blockIdx.x == 0) record_err(p.err, kDevBadGroup);
 }
@@ -553,36 +563,38 @@ __global__ void __cluster_dims__(2, 1, 1)
           // narrowed as they are made (16 registers a chunk instead of 32)
           std::conditional_t<EPI == kGrpF32, float[32], uint32_t[16]> v;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 bias2 = make_float2(b[2 * (i / 8) + i % 2], b[2 * (i / 8) + i % 2]);
-            uint64_t x = pk2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-            if constexpr (kGated) {
-              const float2 o = reinterpret_cast<const float2 *>(receive + i / 2 * 32)[i % 2];
-              uint64_t g = pk2(o.x, o.y);
-              if (gate) {  // the same for the whole warp
-                const uint64_t y = x;
-                x = g;
-                g = y;
+          for (int i = 0; i < 8; ++i) {
+            float4 o;
+            if constexpr (kGated) o = receive[i * 32];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int q = 2 * (i / 4) + j;
+              uint64_t x = pk2(__uint_as_float(r[4 * i + 2 * j]), __uint_as_float(r[4 * i + 2 * j + 1]));
+              if constexpr (kGated) {
+                uint64_t g = j ? pk2(o.z, o.w) : pk2(o.x, o.y);
+                if (gate) {  // the same for the whole warp
+                  const uint64_t y = x;
+                  x = g;
+                  g = y;
+                }
+                float g0, g1;
+                unpk2(add_x2(g, pk2(bg[q], bg[q])), g0, g1);
+                if constexpr (EPI == kGrpBf16SwiGLU) grp_silu_x2(g0, g1);
+                else gelu_erf_x2(g0, g1);
+                x = mul_x2(add_x2(x, pk2(b[q], b[q])), pk2(g0, g1));
+              } else {
+                x = add_x2(x, pk2(b[q], b[q]));
               }
-              const float bg1 = bg[2 * (i / 8) + i % 2];
-              g = add_x2(g, pk2(bg1, bg1));
-              float g0, g1;
-              unpk2(g, g0, g1);
-              if constexpr (EPI == kGrpBf16SwiGLU) grp_silu_x2(g0, g1);
-              else gelu_erf_x2(g0, g1);
-              x = mul_x2(add_x2(x, pk2(bias2.x, bias2.y)), pk2(g0, g1));
-            } else {
-              x = add_x2(x, pk2(bias2.x, bias2.y));
-            }
-            float x0, x1;
-            unpk2(x, x0, x1);
-            if constexpr (EPI == kGrpBf16Gelu8) gelu8_x2(x0, x1);
-            if constexpr (EPI == kGrpBf16Erf) gelu_erf_x2(x0, x1);
-            if constexpr (EPI == kGrpF32) {
-              v[2 * i] = x0;
-              v[2 * i + 1] = x1;
-            } else {
-              v[i] = pack_bf16x2(x0, x1);
+              float x0, x1;
+              unpk2(x, x0, x1);
+              if constexpr (EPI == kGrpBf16Gelu8) gelu8_x2(x0, x1);
+              if constexpr (EPI == kGrpBf16Erf) gelu_erf_x2(x0, x1);
+              if constexpr (EPI == kGrpF32) {
+                v[4 * i + 2 * j] = x0;
+                v[4 * i + 2 * j + 1] = x1;
+              } else {
+                v[2 * i + j] = pack_bf16x2(x0, x1);
+              }
             }
           }
           uint8_t *chunk = mine + slot * kChunkBytes;
