@@ -260,18 +260,39 @@ __device__ __forceinline__ void head_entry(const uint64_t (&c2)[P], const uint64
   s = i & 1 ? hi : lo;
 }
 
+// The weights (and biases) of pair number i, one packed value, folded into its
+// rotation: w the factors of the pair itself, x those of the pair with its
+// elements exchanged, c the constant part.
+template <int P, int NORM>
+__device__ __forceinline__ void head_fold_pair(const uint64_t (&c2)[P], const uint64_t (&s2)[P],
+                                               int i, uint64_t &w, uint64_t &x, uint64_t &c) {
+  float t, u, g0, g1;
+  head_entry<P>(c2, s2, i, t, u);
+  unpk2(w, g0, g1);
+  x = pk2(-g1 * u, g0 * u);
+  w = pk2(g0 * t, g1 * t);
+  if constexpr (NORM == kHeadNormLayer) {
+    float b0, b1;
+    unpk2(c, b0, b1);
+    c = pk2(fmaf(-b1, u, b0 * t), fmaf(b0, u, b1 * t));
+  }
+}
+
 // Blocks an SM must hold, which bounds the registers.  Measured (us, at 4 / 3 /
 // 2 blocks; 49,999 rows of 16 + 16 heads of 128, bf16, V = 8): no norm 132 /
 // 131 / 157 (and 83 / 92 / 92 for 65,539 rows of 32 heads of 64, pairs, a
-// quarter of the work), RMS 188 / 144 / 156, LayerNorm 270 / 224 / 178.  Half
+// quarter of the work), RMS 188 / 144 / 156, LayerNorm 270 / 234 / 173.  Half
 // the vector holds half the state: RMS 106 / 115 / 115 (25,000 rows, fp32,
-// heads of 96), LayerNorm 178 / 202 / 204 (bf16, heads of 80 turning 40).
-constexpr int head_blocks(int norm, int v) {
-  return norm == kHeadNormNone || v < 8 ? 4 : norm == kHeadNormRms ? 3 : 2;
+// heads of 96), LayerNorm 141 / 128 / 163 there and 174 / 194 / 198 for bf16
+// in 8-byte vectors (heads of 80, turning 40).
+constexpr int head_blocks(int norm, int v, int bytes) {
+  if (norm == kHeadNormNone) return 4;
+  if (norm == kHeadNormRms) return v < 8 ? 4 : 3;
+  return v >= 8 ? 2 : bytes == 16 ? 3 : 4;
 }
 
 template <typename T, int V, int NORM, bool PAIRS, int IT>
-__global__ void __launch_bounds__(256, head_blocks(NORM, V))
+__global__ void __launch_bounds__(256, head_blocks(NORM, V, V * static_cast<int>(sizeof(T))))
     heads_vec_kernel(const HeadArgs p, int lg, int q_chunks, float inv_dim) {
   using Vec = HeadVec<T, V>;
   using U = typename Vec::U;
@@ -321,16 +342,43 @@ __global__ void __launch_bounds__(256, head_blocks(NORM, V))
       s2[i] = pk2(v.y, v.w);
     }
   }
-  uint64_t ga[P], gb[P], ba[P], bb[P];
+  // A normed head's weights go into the rotation: with n = x / std (less its
+  // mean), a' = n_a (g_a c) - n_b (g_b s) + (b_a c - b_b s), and so for b'.
+  // That makes wa, wb the factors of a thread's own elements, xa, xb those of
+  // the ones they turn with, ca, cb the constant part.
+  uint64_t wa[P], wb[P], xa[P], xb[P], ca[P], cb[P];
   if constexpr (NORM != kHeadNormNone) {
     if (live) {
       const float *g = key ? p.k.gamma : p.q.gamma;
-      head_weights<P>(g + e0, ga);
-      head_weights<P>(g + e1, gb);
+      head_weights<P>(g + e0, wa);
+      head_weights<P>(g + e1, wb);
       if constexpr (NORM == kHeadNormLayer) {
-        const float *b = key ? p.k.beta : p.q.beta;
-        head_weights<P>(b + e0, ba);
-        head_weights<P>(b + e1, bb);
+        const float *w = key ? p.k.beta : p.q.beta;
+        head_weights<P>(w + e0, ca);
+        head_weights<P>(w + e1, cb);
+      }
+      if (turn) {
+        if constexpr (PAIRS) {
+#pragma unroll
+          for (int v = 0; v < P; ++v) {
+            head_fold_pair<P, NORM>(c2, s2, v, wa[v], xa[v], ca[v]);
+            head_fold_pair<P, NORM>(c2, s2, P + v, wb[v], xb[v], cb[v]);
+          }
+        } else {
+#pragma unroll
+          for (int v = 0; v < P; ++v) {
+            const uint64_t ns = s2[v] ^ 0x8000000080000000ull;
+            xa[v] = mul_x2(wb[v], ns);
+            xb[v] = mul_x2(wa[v], s2[v]);
+            wa[v] = mul_x2(wa[v], c2[v]);
+            wb[v] = mul_x2(wb[v], c2[v]);
+            if constexpr (NORM == kHeadNormLayer) {
+              const uint64_t a0 = ca[v];
+              ca[v] = fma_x2(cb[v], ns, mul_x2(a0, c2[v]));
+              cb[v] = fma_x2(a0, s2[v], mul_x2(cb[v], c2[v]));
+            }
+          }
+        }
       }
     }
   }
@@ -370,18 +418,28 @@ __global__ void __launch_bounds__(256, head_blocks(NORM, V))
       const uint64_t is2 = pk2(is, is);
 #pragma unroll
       for (int v = 0; v < P; ++v) {
-        a[v] = mul_x2(a[v], is2);
-        b[v] = mul_x2(b[v], is2);
+        uint64_t ya = mul_x2(a[v], wa[v]), yb = mul_x2(b[v], wb[v]);
+        if (turn) {
+          uint64_t pa = b[v], pb = a[v];  // what they turn with
+          if constexpr (PAIRS) {
+            float lo, hi;
+            unpk2(a[v], lo, hi);
+            pa = pk2(hi, lo);
+            unpk2(b[v], lo, hi);
+            pb = pk2(hi, lo);
+          }
+          ya = fma_x2(pa, xa[v], ya);
+          yb = fma_x2(pb, xb[v], yb);
+        }
         if constexpr (NORM == kHeadNormLayer) {
-          a[v] = fma_x2(a[v], ga[v], ba[v]);
-          b[v] = fma_x2(b[v], gb[v], bb[v]);
+          a[v] = fma_x2(ya, is2, ca[v]);
+          b[v] = fma_x2(yb, is2, cb[v]);
         } else {
-          a[v] = mul_x2(a[v], ga[v]);
-          b[v] = mul_x2(b[v], gb[v]);
+          a[v] = mul_x2(ya, is2);
+          b[v] = mul_x2(yb, is2);
         }
       }
-    }
-    if (turn) {
+    } else if (turn) {
       if constexpr (PAIRS) {
         // a[v] and b[v] are a pair each, number v and P + v of the thread's
 #pragma unroll
