@@ -5,23 +5,27 @@
 //
 // off comes from device memory, so a pass needs no host round trip.  src(p)
 // is row_src[p] (the routed row, gathered on the way into shared memory) or p.
-// W is [experts, N, K] bf16, one matrix over all experts to the tensor map;
-// a gated weight's N columns are interleaved in groups of 64 = [32 up |
-// 32 gate] and the product is up * act(gate), N / 2 wide.
+// W is staged in blocks of 128 columns by 64 of K (stage_experts_kernel); a
+// gated weight's N columns are interleaved in groups of 64 = [32 up | 32 gate]
+// and the product is up * act(gate), N / 2 wide.
 //
 // A CTA pair (tcgen05 cta_group::2) takes 256 columns of W and up to 256 rows
 // of one group, with W as the product's M operand and the rows as its N
-// operand: N is any multiple of 32, so a group of 40 rows costs 64 and not
-// 256, and a group of 257 is cut into 160 + 97.  (W streams through the M side
-// at 128 columns in 128 clocks a step of 16, however small N is: measured 0.26
-// us a K-block for one pair and 8 rows, 60 GB/s an SM.  From about 110 SMs on
-// that is more than HBM gives; a product with fewer column tiles than that is
-// bound by it.)  The accumulator holds a column of C per TMEM lane.  The persistent pairs walk one list of tiles,
-// whatever the groups are: every block builds it from off.  (One CTA on 128
+// operand, a multiple of 32, so that a part tile loads and finishes only the
+// rows it has; the accumulator holds a column of C per TMEM lane.  The
+// persistent pairs walk one list of tiles, whatever the groups are: every
+// block builds it from off.
+//
+// What bounds it: the tensor pipe for whole tiles, HBM for few rows a group,
+// and between them that W streams through the M side at 128 columns in 128
+// clocks a step of 16, however few the rows are (0.26 us a K-block for one
+// pair and 8 rows, 60 GB/s an SM: more than HBM gives from about 110 SMs on,
+// the bound of a product with fewer column tiles than that).  One CTA on 128
 // rows by 128, 64 or 32 columns, rows as M, was no faster at any size tried:
 // 8.2 / 9.0 / 12.8 us for the pair against 8.2 / 8.9 / 14.1 us at best on 1,
 // 32 and 1024 rows of 2 of 8 experts, K and N 1024; 15.0 against 15.4 us on
-// 64 rows, K 768, N 3840.)
+// 64 rows, K 768, N 3840.  Prefetching W into L2 8 to 32 K-blocks ahead was
+// slower throughout (53 against 51 us on 2011 rows of 64 experts, 16).
 //
 // Roles of a block:
 //   warp 0        W by TMA (and A, where its rows are grouped already), and
@@ -34,8 +38,9 @@
 //                 a share of the tile's rows with their indices in registers
 // A gather is issued by one lane for uniform operands; from 32 lanes of one
 // warp the same 32 gathers take turns on the issue path (80 clocks each).
-// Eight warps: 877 us on 65,542 rows, K 1024, N 8192, against 988 for four
-// and 1207 for two.  Rows past the group are not loaded: what lies in their
+// Eight warps: 850 us on 65,542 rows, K 1024, N 8192, against 893 for four and
+// 962 for sixteen, whose registers the epilogue then lacks (717 us for rows
+// that are grouped already).  Rows past the group are not loaded: what lies in their
 // place in shared memory reaches only accumulators that are not stored.  All
 // waits are bounded as in gemm_tc_pair_kernel, whose barriers these are.
 #pragma once
@@ -316,9 +321,9 @@ template <int EPI, bool GATHER>
 __global__ void __cluster_dims__(2, 1, 1)
     __launch_bounds__(GATHER ? kGroupedGatherThreads : kGroupedThreads, 1)
     gemm_grouped_kernel(const __grid_constant__ CUtensorMap tmA,
-                             const __grid_constant__ CUtensorMap tmA128,
-                             const __grid_constant__ CUtensorMap tmW,
-                             const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
+                        const __grid_constant__ CUtensorMap tmA128,
+                        const __grid_constant__ CUtensorMap tmW,
+                        const __grid_constant__ CUtensorMap tmC, const GroupedArgs p) {
   using S = GroupedShape;
   const int stages = S::stages(p.tile_rows);
   const int a_bytes = p.tile_rows / 2 * kGemmBK * 2;
@@ -423,7 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1)
           } else {
             for (int i = 0; i < boxes; ++i)
               tma_load_2d_pair(sA + stage * a_bytes + i * kGroupedBox * 128, &tmA, bar,
-                          kb * kGemmBK, a_row + i * kGroupedBox);
+                               kb * kGemmBK, a_row + i * kGroupedBox);
           }
           if (++stage == stages) {
             stage = 0;
@@ -569,7 +574,8 @@ __global__ void __cluster_dims__(2, 1, 1)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               const int q = 2 * (i / 4) + j;
-              uint64_t x = pk2(__uint_as_float(r[4 * i + 2 * j]), __uint_as_float(r[4 * i + 2 * j + 1]));
+              uint64_t x =
+                  pk2(__uint_as_float(r[4 * i + 2 * j]), __uint_as_float(r[4 * i + 2 * j + 1]));
               if constexpr (kGated) {
                 uint64_t g = j ? pk2(o.z, o.w) : pk2(o.x, o.y);
                 if (gate) {  // the same for the whole warp
@@ -669,7 +675,7 @@ __global__ void __cluster_dims__(2, 1, 1)
           for (int i = 0; i < kGatherRows / 4; ++i)
             if (4 * i < count)
               grp_gather4(dst + i * 512, &tmA, bar, kb * kGemmBK, src[4 * i], src[4 * i + 1],
-                             src[4 * i + 2], src[4 * i + 3]);
+                          src[4 * i + 2], src[4 * i + 3]);
           grp_arrive(bar);
         }
         __syncwarp();
@@ -694,7 +700,8 @@ __global__ void __cluster_dims__(2, 1, 1)
 // 16 KB in one piece, which a TMA box reads as 128 consecutive rows of 128
 // bytes (2 to 4% faster than the same boxes from [N, K] rows: 43.1 against
 // 44.0 us on 2011 rows of 64 experts, 15.2 against 16.0 on 128 rows of 8).
-// Column blocks come in twos; columns past N and K are zero.  For a gated weight column n takes column glu(n) of [up | gate].
+// Column blocks come in twos; columns past N and K are zero.  A gated weight's
+// column n takes column glu(n) of [up | gate].
 __global__ void stage_experts_kernel(const void *__restrict__ src, int src_bf16, int K, int N,
                                      int gated, int e0, int col_blocks, int k_blocks,
                                      __nv_bfloat16 *__restrict__ dst) {

@@ -76,7 +76,9 @@ __device__ __forceinline__ int64_t head_position(const HeadArgs &p, int64_t at) 
 __device__ __forceinline__ float head_load(const float *p) { return *p; }
 __device__ __forceinline__ float head_load(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void head_store(float *p, float v) { *p = v; }
-__device__ __forceinline__ void head_store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void head_store(__nv_bfloat16 *p, float v) {
+  *p = __float2bfloat16_rn(v);
+}
 
 // Any even head_dim up to 256 and any even rot_dim, elements one by one: a
 // warp per head, up to four pairs a lane.

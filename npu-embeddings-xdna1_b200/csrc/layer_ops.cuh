@@ -209,7 +209,8 @@ int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t
   NEBW_REQUIRE(h->heads > 0 && h->heads <= 4096, "%d %s heads refused", h->heads, what);
   const int64_t width = static_cast<int64_t>(h->heads) * head_dim;
   NEBW_REQUIRE(h->x && h->out, "null %s operand", what);
-  NEBW_REQUIRE(aligned(h->x, esz) && aligned(h->out, esz), "%s heads are not element-aligned", what);
+  NEBW_REQUIRE(aligned(h->x, esz) && aligned(h->out, esz), "%s heads are not element-aligned",
+               what);
   NEBW_REQUIRE(rows <= 1 || (h->stride >= width && h->out_stride >= width),
                "%s row stride refused: %lld and %lld for %lld elements a row", what,
                static_cast<long long>(h->stride), static_cast<long long>(h->out_stride),
@@ -532,7 +533,8 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
     return set_error(NEBW_ENOMEM, "cudaMalloc for [%d, %lld, %lld] expert weights failed", experts,
                      static_cast<long long>(N), static_cast<long long>(K));
   }
-  const unsigned gx = static_cast<unsigned>(col_blocks * 4), gy = static_cast<unsigned>(k_blocks * 2);
+  const unsigned gx = static_cast<unsigned>(col_blocks * 4);
+  const unsigned gy = static_cast<unsigned>(k_blocks * 2);
   const int cb = static_cast<int>(col_blocks), kb = static_cast<int>(k_blocks);
   cudaError_t e = cudaSuccess;
   if (on_device) {

@@ -244,7 +244,8 @@ __device__ __forceinline__ void route_choose(const RouteArgs &p, int r0, int r1,
 #pragma unroll
     for (int b = 0; b < LG; ++b) {
 #pragma unroll
-      for (int i = 0; i < (K >> b) / 2; ++i) mine[i] = (sub >> b) & 1 ? mine[2 * i + 1] : mine[2 * i];
+      for (int i = 0; i < (K >> b) / 2; ++i)
+        mine[i] = (sub >> b) & 1 ? mine[2 * i + 1] : mine[2 * i];
     }
     float w[kMine];
 #pragma unroll
@@ -313,9 +314,10 @@ __device__ __forceinline__ void route_put(const RouteArgs &p, int row, const int
     if (j < p.k) dst[j] = place[j];
 }
 
-// The grouped places of this block's rows; id: those of the first tiles' rows.  start [experts]: the first place
-// of each expert for this block; mask, pre [tiles, experts]: scratch.  A warp
-// takes a tile of 32 rows, a lane a row: bit r of mask[tile][e] says that row
+// The grouped places of this block's rows.  id: the experts of the first
+// tiles' rows; start [experts]: the first place of each expert for this
+// block; mask, pre [tiles, experts]: scratch.  A warp takes a tile of 32
+// rows, a lane a row: bit r of mask[tile][e] says that row
 // r of the tile chose e, so an entry's place is its expert's count before the
 // tile and the bits below its own -- whatever order the bits were set in.
 template <int K>

@@ -83,7 +83,8 @@ class Heads(C.Structure):
         h = cls(x.data_ptr(), out.data_ptr(), x.stride(0), out.stride(0), heads, 0, _addr(gamma),
                 _addr(beta))
         h.dtype = _dtype(x)
-        h.tensors = (x, out, gamma, beta)
+        h.tensors = tuple(t for t in (x, out, gamma, beta) if t is not None)
+        h.on_gpu = all(t.is_cuda for t in h.tensors)
         return h
 
 
@@ -227,21 +228,30 @@ def _addr(x):
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
-_INT32 = None  # torch.int32, once torch is in use
+_torch_types = {}  # dtype name -> torch dtype, once torch is in use
+
+
+def _typed(x, name: str):
+    """Device address of contiguous values of a dtype: a torch tensor of
+    another dtype, with gaps or in host memory is refused (its bytes would be
+    read as other numbers, or not at all)."""
+    if x is None or isinstance(x, int):
+        return x
+    want = _torch_types.get(name)
+    if want is None:
+        import torch
+        want = _torch_types[name] = getattr(torch, name)
+    if x.dtype is not want or not x.is_cuda or not x.is_contiguous():
+        raise TypeError(f"contiguous {name} values on the GPU are required")
+    return x.data_ptr()
 
 
 def _i32(x):
-    """Device address of int32 values: a torch tensor of another dtype or with
-    gaps is refused (its bytes would be read as other numbers)."""
-    global _INT32
-    if x is None or isinstance(x, int):
-        return x
-    if _INT32 is None:
-        import torch
-        _INT32 = torch.int32
-    if x.dtype is not _INT32 or not x.is_contiguous():
-        raise TypeError("contiguous int32 values are required")
-    return x.data_ptr()
+    return _typed(x, "int32")
+
+
+def _f32(x):
+    return _typed(x, "float32")
 
 
 def _dtype(t) -> int:
@@ -426,6 +436,8 @@ class Device:
             if d is not None:
                 if dtype is not None and dtype != d:
                     raise TypeError("query and key heads of different dtypes")
+                if not h.on_gpu:
+                    raise TypeError("heads on the GPU are required")
                 dtype = d
         return BF16 if dtype is None else dtype
 
@@ -470,31 +482,33 @@ class Device:
             raise ValueError("logits are rows of at least `experts` adjacent values")
         if logits.shape[0] < rows:
             raise ValueError("fewer logit rows than rows")
+        if not (logits.is_cuda and workspace.is_cuda and workspace.is_contiguous()):
+            raise TypeError("logits and a contiguous workspace on the GPU are required")
         stride = logits.stride(0) if rows > 1 else experts  # one row: torch may give any
         _check(lib().nebw_moe_route(self.h, logits.data_ptr(), _dtype(logits), stride, rows,
                                     _i32(rows_dev), experts, top_k, score, int(renorm), scale,
-                                    _i32(ids),
-                                    _addr(weights), _i32(group_off), _i32(row_src),
-                                    _i32(row_dst), _addr(workspace),
+                                    _i32(ids), _f32(weights), _i32(group_off), _i32(row_src),
+                                    _i32(row_dst), workspace.data_ptr(),
                                     workspace.numel() * workspace.element_size(),
                                     self._s(stream)))
 
     def gemm_grouped(self, weight, A, a_rows, group_off, rows, K, N, C_out, row_src=None,
                      bias=None, act=ACT_NONE, c_dtype=BF16, stream=None):
         """One product per expert over its group of rows (nebw_gemm_grouped)."""
-        _check(lib().nebw_gemm_grouped(self.h, weight, _addr(A), a_rows, _i32(row_src),
-                                       _i32(group_off), rows, K, N, _addr(bias), act,
-                                       _addr(C_out), c_dtype, self._s(stream)))
+        out = _typed(C_out, "bfloat16" if c_dtype == BF16 else "float32")
+        _check(lib().nebw_gemm_grouped(self.h, weight, _typed(A, "bfloat16"), a_rows,
+                                       _i32(row_src), _i32(group_off), rows, K, N, _f32(bias), act,
+                                       out, c_dtype, self._s(stream)))
 
     def moe_combine(self, y, row_dst, weights, rows, top_k, H, out, residual=None, rows_dev=None,
                     stream=None):
         """The experts' rows y (torch, [places, H]) weighted and summed per
         row (nebw_moe_combine)."""
-        if not (y.is_contiguous() and out.is_contiguous()):
-            raise ValueError("expert rows and output are contiguous")
+        if not (y.is_contiguous() and out.is_contiguous() and y.is_cuda and out.is_cuda):
+            raise TypeError("contiguous expert rows and output on the GPU are required")
         _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y.shape[0], _i32(row_dst),
-                                      _addr(weights), rows, _i32(rows_dev), top_k, H,
-                                      _addr(residual), out.data_ptr(), _dtype(out),
+                                      _f32(weights), rows, _i32(rows_dev), top_k, H,
+                                      _f32(residual), out.data_ptr(), _dtype(out),
                                       self._s(stream)))
 
 

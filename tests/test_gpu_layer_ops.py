@@ -203,7 +203,8 @@ def test_head_norm_without_rotation_and_one_side(device):
         side = nebw.Heads.of(x, heads, out=out, gamma=gamma)
         device.qk_norm_rope(side if q else None, side if k else None, rows, hd, eps=1e-6)
         device.sync()
-        assert_close(out, *heads_reference(x, heads, hd, [], 1.0, None, False, 1, gamma, None, 1e-6))
+        assert_close(out, *heads_reference(x, heads, hd, [], 1.0, None, False, 1, gamma, None,
+                                           1e-6))
 
 
 def test_head_rows_of_zeros_and_infinities(device):
@@ -265,6 +266,23 @@ def test_heads_live_rows_and_bad_positions(device):
             assert_close(out, *heads_reference(x, heads, hd, inv, scale, pos, False))
     finally:
         device.release_weight(h)
+
+
+def test_heads_past_32_bits(device):
+    """Rows whose element offsets need more than 32 bits."""
+    import nebw
+    rows, stride, hd = 36000, 1 << 17, 64
+    buf = torch.empty(rows, stride, dtype=torch.bfloat16, device="cuda")  # 9.4 GB
+    x = buf[:, 5 * hd:6 * hd]
+    x.copy_(torch.randn(rows, hd, generator=gen(14), device="cuda"))
+    before = x.clone()
+    inv, scale = nebw.rope_freqs(10000.0, hd)
+    h = device.stage_rope(inv, rows)
+    pos = torch.arange(rows, device="cuda").int()
+    device.rope(nebw.Heads.of(x, 1), None, rows, hd, h, pos)
+    device.sync()
+    assert_close(x, *heads_reference(before, 1, hd, inv, scale, pos, False))
+    device.release_weight(h)
 
 
 def test_rope_table_far_positions(device):
@@ -833,9 +851,15 @@ def test_grouped_refusals(device):
     refused("empty A", g, plain, a, 0, off, 8, 64, 64, c, row_src=off)
     refused("activation", g, plain, a, 8, off, 8, 64, 64, c, act=3)
     refused("activation", g, gated, a, 8, off, 8, 64, 64, c, act=2)
-    refused("bf16 output", g, plain, a, 8, off, 8, 64, 64, c, act=1, c_dtype=0)
-    refused("bf16 output", g, gated, a, 8, off, 8, 64, 64, c, c_dtype=0)
-    refused("output dtype", g, plain, a, 8, off, 8, 64, 64, c, c_dtype=7)
+    f = torch.zeros(8, 64, device="cuda")
+    refused("bf16 output", g, plain, a, 8, off, 8, 64, 64, f, act=1, c_dtype=0)
+    refused("bf16 output", g, gated, a, 8, off, 8, 64, 64, f, c_dtype=0)
+    refused("output dtype", g, plain, a, 8, off, 8, 64, 64, c.data_ptr(), c_dtype=7)
+    for bad in (a.float(), a.t(), a.cpu()):  # read as other numbers, or not at all
+        with pytest.raises(TypeError):
+            g(plain, bad, 8, off, 8, 64, 64, c)
+    with pytest.raises(TypeError):
+        g(plain, a, 8, off, 8, 64, 64, f)
     refused("null grouped", g, plain, None, 8, off, 8, 64, 64, c)
     refused("null grouped", g, plain, a, 8, None, 8, 64, 64, c)
     refused("aligned", g, plain, a.data_ptr() + 2, 7, off, 7, 64, 64, c)
@@ -855,8 +879,32 @@ def test_grouped_refusals(device):
     refused("unknown expert", g, plain, a, 8, off, 8, 64, 64, c)
 
 
+def test_grouped_product_and_combine_past_32_bits(device):
+    """An output of more than 2^31 elements, and the combine that reads it."""
+    M, K, N = 270000, 64, 8192
+    a = torch.randn(M, K, generator=gen(15), device="cuda").bfloat16()
+    w = torch.randn(2, K, N, generator=gen(16), device="cuda").bfloat16()
+    off = groups([M - 1000, 1000])
+    h = device.stage_experts(w)
+    c = torch.empty(M, N, dtype=torch.bfloat16, device="cuda")  # 4.4 GB
+    device.gemm_grouped(h, a, M, torch.from_numpy(off).cuda(), M, K, N, c)
+    rows = 50
+    dst = torch.stack([torch.arange(rows), M - 1 - torch.arange(rows)], 1).int().cuda()
+    weights = torch.rand(rows, 2, generator=gen(17), device="cuda")
+    out = torch.empty(rows, N, device="cuda")
+    device.moe_combine(c, dst, weights, rows, 2, N, out)
+    device.sync()
+    at = torch.cat([torch.arange(300), torch.arange(M - 1300, M)]).cuda()
+    want, err = grouped_reference(a[at], w, [0, 600, 1600], None, None, False, 0)
+    assert_close(c[at], want, err)
+    parts = c[dst.long()].double() * weights[:, :, None].double()
+    assert_close(out, parts.sum(1), 3 * U * parts.abs().sum(1))
+    device.release_weight(h)
+
+
 def test_whole_numbers_of_another_dtype_are_refused(device):
-    """int64 indices (torch's default) would be read as other numbers."""
+    """int64 indices (torch's default) would be read as other numbers, host
+    memory not at all."""
     import nebw
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device="cuda")
     inv, _ = nebw.rope_freqs(10000.0, 64)
@@ -864,6 +912,8 @@ def test_whole_numbers_of_another_dtype_are_refused(device):
     w = device.stage_experts(np.zeros((1, 64, 64), np.float32))
     with pytest.raises(TypeError):
         device.rope(nebw.Heads.of(x, 1), None, 4, 64, h, torch.arange(4, device="cuda"))
+    with pytest.raises(TypeError):
+        device.rope(nebw.Heads.of(x.cpu(), 1), None, 4, 64, h, torch.arange(4, device="cuda").int())
     with pytest.raises(TypeError):
         device.gemm_grouped(w, x, 4, torch.tensor([0, 4], device="cuda"), 4, 64, 64, x.clone())
     with pytest.raises(TypeError):  # every second value
@@ -924,7 +974,8 @@ def test_combine_in_place_residual_live_rows_and_bad_places(device):
         device.sync()
         live = max(0, min(live, rows))
         assert torch.equal(out[live:], x[live:])
-        assert_close(out[:live], want[:live], 3 * U * (parts.abs().sum(1) + x.double().abs())[:live])
+        size = parts.abs().sum(1) + x.double().abs()
+        assert_close(out[:live], want[:live], 3 * U * size[:live])
     bad = dst.clone()
     bad[5, 1] = rows * k
     out = torch.empty(rows, H, device="cuda")
