@@ -12,6 +12,13 @@
 // Everything whole is exact and has one order whatever the schedule: the
 // choice compares the logits themselves, and places come from counts, never
 // from the order in which blocks reach an atomic.
+//
+// Measured: 26.8 us for 131,071 rows of 64 bf16 logits by 8, whose bytes take
+// 5.2.  The choice is two thirds of it, bound by the min / max pipe (a row of
+// 64 takes 200 exchanges of keys); the places are the rest, a chain of short
+// steps behind one another.  (One warp a row, with a warp-wide maximum for
+// every chosen expert, and places by a match within 32 entries took 141 us.)
+// A few rows cost one launch: 3.1 us for 21 rows of 8 by 2.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -465,7 +472,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_fused_kernel(const RouteA
 // out[t] = residual[t] + sum_j weights[t, j] * y[row_dst[t, j]], j ascending,
 // in fp32 with one rounding at the end; an entry without a place (row_dst
 // < 0) adds nothing and is not read.  HBM bounds it: k rows of y are read for
-// one written.
+// one written, 120 us at 6.7 TB/s (1.03 of the copy rate) for 32,771 rows of
+// 8 x 1024 bf16 onto fp32 rows.
 struct CombineArgs {
   const void *y;
   const int *row_dst;
