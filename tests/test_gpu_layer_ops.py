@@ -538,10 +538,11 @@ def test_route_ties_masks_and_odd_values(device, dtype):
                      dst))
 
 
-def test_route_live_rows(device):
-    rows, experts, k = 1200, 16, 2
+@pytest.mark.parametrize("rows", [1200, 700])  # two kernels, and one block
+def test_route_live_rows(device, rows):
+    experts, k = 16, 2
     x = torch.randn(rows, experts, generator=gen(3), device="cuda")
-    for live in (0, 1, 511, 512, 513, 1199, 1200, 5000, -1):
+    for live in (0, 1, 31, 32, 511, 513, rows - 1, rows, 5000, -1):
         n = torch.tensor([live], dtype=torch.int32, device="cuda")
         r = Routing(rows, experts, k).run(device, x, rows_dev=n)
         device.sync()
@@ -769,6 +770,22 @@ def test_grouped_product_equals_one_product(device):
     assert ((c1 - c2).abs().double() <= 4 * (K + 2) * U * size).all()
     device.release_weight(one)
     device.release_weight(many)
+
+
+def test_grouped_product_without_the_pair_gemm(device, monkeypatch):
+    """NEBW_GEMM_CTAS=1 takes nebw_gemm off CTA pairs, not the grouped product."""
+    import nebw
+    monkeypatch.setenv("NEBW_GEMM_CTAS", "1")
+    other = nebw.Device(0, torch_stream=True)
+    K, N, off = 128, 64, groups([3, 0, 40])
+    w = torch.randn(3, K, N, generator=gen(18), device="cuda").bfloat16()
+    a = torch.randn(43, K, generator=gen(19), device="cuda").bfloat16()
+    c = torch.empty(43, N, dtype=torch.bfloat16, device="cuda")
+    h = other.stage_experts(w)
+    other.gemm_grouped(h, a, 43, torch.from_numpy(off).cuda(), 43, K, N, c)
+    other.sync()
+    assert_close(c, *grouped_reference(a, w, off, None, None, False, 0))
+    other.close()
 
 
 @pytest.mark.parametrize("source", ["numpy f32", "numpy bf16", "torch f32", "torch bf16", "cpu"])
