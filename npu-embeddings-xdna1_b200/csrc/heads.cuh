@@ -172,8 +172,9 @@ __global__ void __launch_bounds__(256) heads_any_kernel(const HeadArgs p) {
 // needs no exchange and a norm only the shuffles of the 2^lg lanes that share
 // a head.  A warp takes 32 / 2^lg heads of one side of one row at a time, IT
 // times: the table entries and the norm's weights are read once for all of
-// them, and all loads are issued before the first is used.  The arithmetic is
-// packed, two values an instruction, which keeps the issue slots below half
+// them, and all loads are issued before the first is used.  IT = 0 is for fewer
+// heads than a turn takes: a warp then goes over heads of several rows (18.7
+// us against 36.8 for 65,539 rows of 4 + 1 heads of 64).  The arithmetic is packed, two values an instruction, which keeps the issue slots below half
 // of what the bytes take.
 template <int BYTES>
 struct HeadWord;
@@ -304,11 +305,14 @@ __global__ void __launch_bounds__(256, head_blocks(NORM, V, V * static_cast<int>
   using Vec = HeadVec<T, V>;
   using U = typename Vec::U;
   constexpr int P = Vec::P;
+  constexpr bool FLAT = IT == 0;
+  constexpr int TURNS = FLAT ? 1 : IT;
   const int lane = threadIdx.x & 31;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  int64_t row = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
   int64_t rows = p.rows;
   if (p.rows_dev) rows = min(rows, static_cast<int64_t>(max(0, __ldg(p.rows_dev))));
-  if (row >= rows) return;
+  const uint32_t item = static_cast<uint32_t>(row) * (32 >> lg);  // FLAT: the warp's first head
+  if (!FLAT && row >= rows) return;
   const bool key = static_cast<int>(blockIdx.y) >= q_chunks;
   const int chunk = key ? blockIdx.y - q_chunks : blockIdx.y;
   const T *x = static_cast<const T *>(key ? p.k.x : p.q.x);
@@ -316,9 +320,18 @@ __global__ void __launch_bounds__(256, head_blocks(NORM, V, V * static_cast<int>
   const int heads = key ? p.k.heads : p.q.heads;
   const bool in_place = x == out;
   const int per = 32 >> lg, slot = lane & ((1 << lg) - 1);
-  const int head0 = chunk * IT * per + (lane >> lg);
+  int head0 = chunk * TURNS * per + (lane >> lg);
   const bool turn = slot * V < p.n;
   bool live = slot * 2 * V < p.head_dim;
+  if constexpr (FLAT) {
+    if (item >= static_cast<uint64_t>(rows) * heads) return;
+    row = (item + (lane >> lg)) / static_cast<uint32_t>(heads);
+    head0 = static_cast<int>(item + (lane >> lg) - static_cast<uint32_t>(row) * heads);
+    if (row >= rows) {  // (row 0 is read in its place)
+      live = false;
+      row = 0;
+    }
+  }
   // what does not turn and is not normed stays where it is
   if (NORM == kHeadNormNone && in_place) live = live && turn;
   const int e0 = turn && !PAIRS ? slot * V : slot * 2 * V;
@@ -328,9 +341,9 @@ __global__ void __launch_bounds__(256, head_blocks(NORM, V, V * static_cast<int>
   const int hop = per * p.head_dim;  // elements between a lane's heads
 
   const int pos = turn ? __ldg(p.pos + row) : 0;  // looked at once the rows are on their way
-  U ua[IT], ub[IT];
+  U ua[TURNS], ub[TURNS];
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
+  for (int i = 0; i < TURNS; ++i) {
     ua[i] = ub[i] = U{};
     if (live && head0 + i * per < heads) {
       ua[i] = *reinterpret_cast<const U *>(x + i * hop + e0);
@@ -390,7 +403,7 @@ __global__ void __launch_bounds__(256, head_blocks(NORM, V, V * static_cast<int>
     }
   }
 #pragma unroll
-  for (int i = 0; i < IT; ++i) {
+  for (int i = 0; i < TURNS; ++i) {
     uint64_t a[P], b[P];
     Vec::unpack(ua[i], a);
     Vec::unpack(ub[i], b);

@@ -237,9 +237,17 @@ int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t
 
 template <typename T, int V, int NORM, bool PAIRS, int IT>
 int launch_heads_it(const nebw::HeadArgs &a, int lg, int per, cudaStream_t st) {
-  const int q_chunks = (a.q.heads + per * IT - 1) / (per * IT);
-  const int chunks = q_chunks + (a.k.heads + per * IT - 1) / (per * IT);
-  const dim3 grid(static_cast<unsigned>((a.rows + 7) / 8), chunks);
+  int q_chunks, chunks;
+  int64_t warps = a.rows;
+  if constexpr (IT == 0) {  // heads of all rows in one list a side
+    q_chunks = a.q.heads > 0;
+    chunks = q_chunks + (a.k.heads > 0);
+    warps = (a.rows * std::max(a.q.heads, a.k.heads) + per - 1) / per;
+  } else {
+    q_chunks = (a.q.heads + per * IT - 1) / (per * IT);
+    chunks = q_chunks + (a.k.heads + per * IT - 1) / (per * IT);
+  }
+  const dim3 grid(static_cast<unsigned>((warps + 7) / 8), chunks);
   nebw::heads_vec_kernel<T, V, NORM, PAIRS, IT>
       <<<grid, 256, 0, st>>>(a, lg, q_chunks, 1.0f / static_cast<float>(a.head_dim));
   NEBW_CUDA(cudaGetLastError());
@@ -268,6 +276,8 @@ int launch_heads_vec(const nebw::HeadArgs &a, cudaStream_t st) {
     // 170 for two, on the RMS case at heads_vec_kernel); one or two where the
     // heads end there
     const int most = std::max(a.q.heads, a.k.heads);
+    if (most < per && a.rows * most < (1ll << 31))
+      return launch_heads_it<T, V, NORM, PAIRS, 0>(a, lg, per, st);
     if (most <= per) return launch_heads_it<T, V, NORM, PAIRS, 1>(a, lg, per, st);
     if (most <= 2 * per) return launch_heads_it<T, V, NORM, PAIRS, 2>(a, lg, per, st);
   }

@@ -234,11 +234,12 @@ def test_head_rows_of_zeros_and_infinities(device):
         device.release_weight(h)
 
 
-def test_heads_live_rows_and_bad_positions(device):
+@pytest.mark.parametrize("heads", [2, 16])  # several rows a warp, and one
+def test_heads_live_rows_and_bad_positions(device, heads):
     """Rows behind the live count stay; a position outside the table is
     reported and the nearest entry used."""
     import nebw
-    rows, heads, hd = 40, 2, 64
+    rows, hd = 40, 64
     g = gen(7)
     x = torch.randn(rows, heads * hd, generator=g, device="cuda").to(torch.bfloat16)
     inv, scale = nebw.rope_freqs(10000.0, hd)
