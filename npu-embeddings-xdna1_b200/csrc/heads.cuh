@@ -174,8 +174,9 @@ __global__ void __launch_bounds__(256) heads_any_kernel(const HeadArgs p) {
 // times: the table entries and the norm's weights are read once for all of
 // them, and all loads are issued before the first is used.  IT = 0 is for fewer
 // heads than a turn takes: a warp then goes over heads of several rows (18.7
-// us against 36.8 for 65,539 rows of 4 + 1 heads of 64).  The arithmetic is packed, two values an instruction, which keeps the issue slots below half
-// of what the bytes take.
+// us against 36.8 for 65,539 rows of 4 + 1 heads of 64).  The arithmetic is
+// packed, two values an instruction, which keeps the issue slots below half of
+// what the bytes take.
 template <int BYTES>
 struct HeadWord;
 template <>
