@@ -332,6 +332,13 @@ __global__ void __cluster_dims__(2, 1, 1)
   const int stages = S::stages(p.tile_rows);
   const int a_bytes = p.tile_rows / 2 * kGemmBK * 2;
   constexpr int kAccCols = 256;  // TMEM columns of an accumulator: the tile's rows
+  // bf16 output: two accumulators, the epilogue of one tile under the products
+  // of the next.  fp32 output shows what the tensor core cuts off as it adds up
+  // (towards zero, once a step of 16): all of TMEM goes to one tile, K in as
+  // many parts as fit (two of 256 rows, four of 128), which the epilogue adds.
+  // Error against 64 bits at K 1024 / 2048: one part 1.0e-6 / 2.1e-6, two
+  // 4.7e-7 / 1.0e-6, four - / 4.7e-7 (fp32 sums in torch: 2.5e-7 / 3.9e-7).
+  constexpr int kBuffers = EPI == kGrpF32 ? 1 : 2;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -353,6 +360,9 @@ __global__ void __cluster_dims__(2, 1, 1)
   const bool leader = rank == 0;
   const int n_blocks = (p.N + 255) / 256;
   const int num_kb = (p.K + kGemmBK - 1) / kGemmBK;
+  const int parts_fit = 512 / p.tile_rows;  // of K, fp32 output
+  const int part_kb = (num_kb + parts_fit - 1) / parts_fit;
+  const int parts = (num_kb + part_kb - 1) / part_kb;
   const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
 
   if (warp == 0) {
@@ -462,11 +472,17 @@ __global__ void __cluster_dims__(2, 1, 1)
       for (int tile = first; tile < num_tiles && ok; tile += step, ++local) {
         const GroupTile t = group_tile(table, p, local, tile, n_blocks);
         const uint32_t idesc = idesc_bf16_f32(256, tile_n(t));
-        const int acc = local & 1;
-        if (!wait_all(&tempty[acc], ((local >> 1) & 1) ^ 1u)) break;
+        const int acc = local % kBuffers;
+        if (!wait_all(&tempty[acc], ((local / kBuffers) & 1) ^ 1u)) break;
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kAccCols);
         for (int kb = 0; kb < num_kb; ++kb) {
+          int kb0 = 0;  // where the accumulator begins
+          uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * kAccCols);
+          if constexpr (EPI == kGrpF32) {
+            const int part = kb / part_kb;
+            kb0 = part * part_kb;
+            d_tmem += static_cast<uint32_t>(part * p.tile_rows);
+          }
           if (!wait_all(&full[stage], phase)) {
             ok = false;
             break;
@@ -477,7 +493,7 @@ __global__ void __cluster_dims__(2, 1, 1)
           if (elect) {
 #pragma unroll
             for (int k = 0; k < kGemmBK / 16; ++k)
-              umma_bf16_pair(d_tmem, dw + k * 2, da + k * 2, idesc, (kb | k) != 0 ? 1u : 0u);
+              umma_bf16_pair(d_tmem, dw + k * 2, da + k * 2, idesc, kb != kb0 || k != 0 ? 1u : 0u);
             umma_commit_pair(&empty[stage], 0x3);
           }
           __syncwarp();
@@ -519,7 +535,7 @@ __global__ void __cluster_dims__(2, 1, 1)
     int slot = 0;
     int local = 0;
     for (int tile = first; tile < num_tiles; tile += step, ++local) {
-      const int acc = local & 1;
+      const int acc = local % kBuffers;
       const GroupTile t = group_tile(table, p, local, tile, n_blocks);
       // first W column of the quarter (of the pair of quarters), and of C
       const int col = t.nb * 256 + rank * 128 + (kGated ? quarter & 2 : quarter) * 32;
@@ -531,7 +547,7 @@ __global__ void __cluster_dims__(2, 1, 1)
       if constexpr (kGated)
         grp_bias4(p.bias ? p.bias + static_cast<int64_t>(t.e) * p.N + width : nullptr,
                   c0 + (lane >> 2), width, bg);
-      bool ok = wait_all(&tfull[acc], (local >> 1) & 1);
+      bool ok = wait_all(&tfull[acc], (local / kBuffers) & 1);
       if constexpr (kGated) ok = grp_pair_and(1 + pair, ok);
       if (!ok) break;
       tc_fence_after();
@@ -566,6 +582,15 @@ __global__ void __cluster_dims__(2, 1, 1)
             if (at >= end) continue;
           } else {
             grp_load_chunk(t_row + c * 32, r);
+            if constexpr (EPI == kGrpF32) {
+              for (int part = 1; part < parts; ++part) {
+                uint32_t s[32];
+                grp_load_chunk(t_row + part * p.tile_rows + c * 32, s);
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                  r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(s[i]));
+              }
+            }
           }
           // entry 4 i + j: column lane / 4 + 8 * (2 * (i / 4) + j / 2), row
           // 8 * (i % 4) + 2 * (lane % 4) + j % 2, finished two at a time and

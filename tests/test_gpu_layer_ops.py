@@ -710,6 +710,36 @@ def test_grouped_product_matches_64_bits(device, sizes, K, N, gather, bias, gate
         device.release_weight(h)
 
 
+@pytest.mark.parametrize("K", [128, 136, 320, 1024, 1536, 1544, 2048, 4000])
+def test_grouped_fp32_output_over_long_products(device, K):
+    """fp32 output keeps K in parts: up to four of half tiles, two of whole ones.
+
+    The tensor core cuts its sum once a step of 16, by half a unit (2^-24 of
+    the running sum) on average.  The running sum of independent products grows
+    as the root of the steps, so S steps of a part lose S * 2^-24 * 2 / 3 of
+    the part, and parts of random sign lose the same of their sum.  At 2048
+    that is 1.3e-6; one part of K would lose four times as much."""
+    import nebw
+    sizes, N = [300, 0, 129, 1, 700, 128, 64], 520
+    off, E, M = groups(sizes), 7, sum(sizes)
+    g = gen(K)
+    w = (torch.randn(E, K, N, generator=g, device="cuda") / math.sqrt(K)).bfloat16()
+    a = torch.randn(M, K, generator=g, device="cuda").bfloat16()
+    c = torch.full((M, N), 7.0, device="cuda")
+    h = device.stage_experts(w)
+    try:
+        device.gemm_grouped(h, a, M, torch.from_numpy(off).cuda(), M, K, N, c, c_dtype=nebw.F32)
+        device.sync()
+        want, err = grouped_reference(a, w, off, None, None, False, 0)
+        assert_close(c, want, err)
+        parts = 4 if K > 1536 else 2
+        steps = -(-K // (64 * parts)) * 4
+        lost = ((c.double() - want).norm() / want.norm()).item()
+        assert lost < steps * 2.0 ** -24 * 2 / 3 + 4 * U
+    finally:
+        device.release_weight(h)
+
+
 def test_grouped_product_of_more_tiles_than_are_looked_up(device):
     """512 experts of a row each, 19 column tiles: over 128 tiles a block."""
     E, K, N = 512, 64, 4864
