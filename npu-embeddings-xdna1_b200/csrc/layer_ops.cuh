@@ -126,6 +126,7 @@ extern "C" int nebw_rope_freqs(double theta, int32_t rot_dim, const nebw_rope_sc
     const double len = static_cast<double>(s->orig_len);
     lo = std::max(0.0, std::floor(n * std::log(len / (fast * kTwoPi)) / std::log(theta)));
     hi = std::min(n - 1.0, std::ceil(n * std::log(len / (slow * kTwoPi)) / std::log(theta)));
+    if (hi < 0.0) lo = hi - 1.0;  // none turns `slow` times: all are scaled
     *scale = s->attn_scale > 0.0 ? s->attn_scale : 0.1 * std::log(s->factor) + 1.0;
   }
   for (int i = 0; i < n; ++i) {
@@ -190,12 +191,12 @@ extern "C" int nebw_stage_rope(nebw_dev *d, const double *inv_freq, int32_t n, i
 extern "C" int nebw_row_positions(nebw_dev *d, const int32_t *off, const int32_t *len, int32_t B,
                                   int32_t max_len, int32_t *pos, void *stream) {
   if (int rc = use_dev(d)) return rc;
-  NEBW_REQUIRE(off && len && pos, "null position operand");
   NEBW_REQUIRE(B >= 0 && B <= 65535 && max_len >= 0, "positions of %d sequences up to %d refused",
                B, max_len);
   if (B == 0 || max_len == 0) return NEBW_OK;
-  nebw::row_pos_kernel<<<dim3((max_len + 255) / 256, B), 256, 0, pick_stream(d, stream)>>>(off, len,
-                                                                                          pos);
+  NEBW_REQUIRE(off && len && pos, "null position operand");
+  const dim3 grid(static_cast<unsigned>((int64_t{max_len} + 255) / 256), B);
+  nebw::row_positions_kernel<<<grid, 256, 0, pick_stream(d, stream)>>>(off, len, max_len, pos);
   NEBW_CUDA(cudaGetLastError());
   return NEBW_OK;
 }
@@ -208,6 +209,10 @@ int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t
   if (!h || h->heads == 0) return NEBW_OK;
   NEBW_REQUIRE(h->heads > 0 && h->heads <= 4096, "%d %s heads refused", h->heads, what);
   const int64_t width = static_cast<int64_t>(h->heads) * head_dim;
+  if (rows == 0) {  // an empty tensor may have no address
+    side->heads = h->heads;
+    return NEBW_OK;
+  }
   NEBW_REQUIRE(h->x && h->out, "null %s operand", what);
   NEBW_REQUIRE(aligned(h->x, esz) && aligned(h->out, esz), "%s heads are not element-aligned",
                what);
@@ -727,7 +732,7 @@ extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t
                    y_rows < (1ll << 30),
                "%lld rows of %d experts refused", static_cast<long long>(rows), top_k);
   if (rows == 0) return NEBW_OK;
-  NEBW_REQUIRE(y && row_dst && weights && out, "null combine operand");
+  NEBW_REQUIRE((y || y_rows == 0) && row_dst && weights && out, "null combine operand");
   nebw::CombineArgs a{};
   a.y = y;
   a.row_dst = row_dst;

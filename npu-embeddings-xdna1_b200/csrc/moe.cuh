@@ -342,7 +342,7 @@ __device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, 
     if (mine) {
 #pragma unroll
       for (int j = 0; j < K; ++j)
-        if (id[j] >= 0) atomicOr(&mask[warp * E + id[j]], 1 << lane);
+        if (id[j] >= 0) atomicOr(&mask[warp * E + id[j]], static_cast<int>(1u << lane));
     }
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += kRouteThreads) {
@@ -361,7 +361,7 @@ __device__ __forceinline__ void route_place(const RouteArgs &p, int r0, int r1, 
       for (int j = 0; j < K; ++j) {
         place[j] = -1;
         if (id[j] >= 0) {
-          place[j] = pre[warp * E + id[j]] + __popc(mask[warp * E + id[j]] & ((1 << lane) - 1));
+          place[j] = pre[warp * E + id[j]] + __popc(mask[warp * E + id[j]] & ((1u << lane) - 1u));
           p.row_src[place[j]] = row;
         }
       }

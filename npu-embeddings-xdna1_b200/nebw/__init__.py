@@ -84,7 +84,9 @@ class Heads(C.Structure):
                 _addr(beta))
         h.dtype = _dtype(x)
         h.tensors = tuple(t for t in (x, out, gamma, beta) if t is not None)
-        h.on_gpu = all(t.is_cuda for t in h.tensors)
+        h.rows, h.width = x.shape
+        gpus = {t.get_device() for t in h.tensors}
+        h.gpu = gpus.pop() if len(gpus) == 1 else -1  # -1: not on one GPU
         return h
 
 
@@ -228,30 +230,13 @@ def _addr(x):
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
-_torch_types = {}  # dtype name -> torch dtype, once torch is in use
+_INT32 = _FLOAT32 = None  # torch's dtypes, once it is in use
 
 
-def _typed(x, name: str):
-    """Device address of contiguous values of a dtype: a torch tensor of
-    another dtype, with gaps or in host memory is refused (its bytes would be
-    read as other numbers, or not at all)."""
-    if x is None or isinstance(x, int):
-        return x
-    want = _torch_types.get(name)
-    if want is None:
-        import torch
-        want = _torch_types[name] = getattr(torch, name)
-    if x.dtype is not want or not x.is_cuda or not x.is_contiguous():
-        raise TypeError(f"contiguous {name} values on the GPU are required")
-    return x.data_ptr()
-
-
-def _i32(x):
-    return _typed(x, "int32")
-
-
-def _f32(x):
-    return _typed(x, "float32")
+def _torch_dtypes():
+    global _INT32, _FLOAT32
+    import torch
+    _INT32, _FLOAT32 = torch.int32, torch.float32
 
 
 def _dtype(t) -> int:
@@ -289,6 +274,7 @@ class Device:
         self.h = h
         self.index = index
         self.torch_stream = torch_stream
+        self._experts = {}  # handle -> (experts, K, N, columns of the output)
         self._raw_stream = None
         if torch_stream:
             # the current stream's handle without a Stream object around it
@@ -305,6 +291,41 @@ class Device:
             import torch
             return _stream(torch.cuda.current_stream(self.index))
         return None
+
+    def _typed(self, x, name: str, n: int = 0):
+        """Device address of n contiguous values of a dtype: a torch tensor of
+        another dtype, with gaps, in host memory, on another GPU or with fewer
+        values is refused (its bytes would be read as other numbers, or what
+        lies behind them)."""
+        if x is None or isinstance(x, int):
+            return x
+        import torch
+        if (x.dtype is not getattr(torch, name) or x.get_device() != self.index
+                or not x.is_contiguous()):
+            raise TypeError(f"contiguous {name} values on the handle's GPU are required")
+        if x.numel() < n:
+            raise ValueError(f"{x.numel()} {name} values where {n} are read or written")
+        return x.data_ptr()
+
+    # The two below are _typed without its lookups (a short call has half a
+    # dozen of them).
+    def _i32(self, x, n: int = 0):
+        if x is None or x.__class__ is int:
+            return x
+        if (x.dtype is _INT32 and x.get_device() == self.index and x.is_contiguous()
+                and x.numel() >= n):
+            return x.data_ptr()
+        _torch_dtypes()
+        return self._typed(x, "int32", n)
+
+    def _f32(self, x, n: int = 0):
+        if x is None or x.__class__ is int:
+            return x
+        if (x.dtype is _FLOAT32 and x.get_device() == self.index and x.is_contiguous()
+                and x.numel() >= n):
+            return x.data_ptr()
+        _torch_dtypes()
+        return self._typed(x, "float32", n)
 
     def close(self):
         if self.h:
@@ -425,35 +446,39 @@ class Device:
         return hnd.value
 
     def row_positions(self, seq_off, seq_len, B, max_len, pos, stream=None):
-        _check(lib().nebw_row_positions(self.h, _i32(seq_off), _i32(seq_len), B, max_len,
-                                        _i32(pos), self._s(stream)))
+        _check(lib().nebw_row_positions(self.h, self._i32(seq_off, B), self._i32(seq_len, B), B,
+                                        max_len, self._i32(pos), self._s(stream)))
 
-    @staticmethod
-    def _heads_dtype(q, k, dtype):
-        """The dtype of heads made by Heads.of, or the one given."""
+    def _heads_dtype(self, q, k, dtype, rows, head_dim):
+        """The dtype of heads made by Heads.of, which must hold the rows and
+        the elements a head, or the one given."""
         for h in (q, k):
             d = getattr(h, "dtype", None)
             if d is not None:
                 if dtype is not None and dtype != d:
                     raise TypeError("query and key heads of different dtypes")
-                if not h.on_gpu:
-                    raise TypeError("heads on the GPU are required")
+                if h.gpu != self.index:
+                    raise TypeError("heads on the handle's GPU are required")
+                if rows > h.rows or h.heads * head_dim > h.width:
+                    raise ValueError(f"{rows} rows of {h.heads} x {head_dim} in heads of "
+                                     f"[{h.rows}, {h.width}]")
                 dtype = d
         return BF16 if dtype is None else dtype
 
     def rope(self, q, k, rows, head_dim, rope, pos, layout=ROPE_HALF, dtype=None, rows_dev=None,
              stream=None):
         """Rotary positions on the heads q and k (Heads, either may be None) (nebw_rope)."""
-        _check(lib().nebw_rope(self.h, q, k, self._heads_dtype(q, k, dtype), rows,
-                               _i32(rows_dev), head_dim, rope, layout, _i32(pos),
-                               self._s(stream)))
+        dtype = self._heads_dtype(q, k, dtype, rows, head_dim)
+        _check(lib().nebw_rope(self.h, q, k, dtype, rows, self._i32(rows_dev, 1), head_dim, rope,
+                               layout, self._i32(pos, rows), self._s(stream)))
 
     def qk_norm_rope(self, q, k, rows, head_dim, norm=HEADNORM_RMS, eps=1e-6, rope=0, pos=None,
                      layout=ROPE_HALF, dtype=None, rows_dev=None, stream=None):
         """A norm of every head, then the rotation (rope 0: none) (nebw_qk_norm_rope)."""
-        _check(lib().nebw_qk_norm_rope(self.h, q, k, self._heads_dtype(q, k, dtype), rows,
-                                       _i32(rows_dev), head_dim, norm, eps, rope, layout,
-                                       _i32(pos), self._s(stream)))
+        dtype = self._heads_dtype(q, k, dtype, rows, head_dim)
+        _check(lib().nebw_qk_norm_rope(self.h, q, k, dtype, rows, self._i32(rows_dev, 1), head_dim,
+                                       norm, eps, rope, layout, self._i32(pos, rows),
+                                       self._s(stream)))
 
     # ---- experts -----------------------------------------------------------
     def stage_experts(self, w_ekn, gated: bool = False, stream=None) -> int:
@@ -465,11 +490,14 @@ class Device:
                 raise TypeError("weights are fp32, or bf16 bit patterns as uint16")
             dt = F32 if w.dtype == np.float32 else BF16
         else:
-            w, dt = w_ekn.contiguous(), _dtype(w_ekn)
+            w, dt = w_ekn, _dtype(w_ekn)
+            if not w.is_contiguous():  # a copy would be made on torch's stream, not on this one
+                raise ValueError("contiguous expert weights are required")
         E, K, N = w.shape
         hnd = C.c_uint64()
         _check(lib().nebw_stage_experts(self.h, _addr(w), dt, E, K, N, int(gated),
                                         self._s(stream), C.byref(hnd)))
+        self._experts[hnd.value] = (E, K, N, N // 2 if gated else N)
         return hnd.value
 
     def moe_route(self, logits, rows, experts, top_k, ids, weights, group_off, row_src, row_dst,
@@ -482,33 +510,46 @@ class Device:
             raise ValueError("logits are rows of at least `experts` adjacent values")
         if logits.shape[0] < rows:
             raise ValueError("fewer logit rows than rows")
-        if not (logits.is_cuda and workspace.is_cuda and workspace.is_contiguous()):
-            raise TypeError("logits and a contiguous workspace on the GPU are required")
+        if (logits.get_device() != self.index or workspace.get_device() != self.index
+                or not workspace.is_contiguous()):
+            raise TypeError("logits and a contiguous workspace on the handle's GPU are required")
         stride = logits.stride(0) if rows > 1 else experts  # one row: torch may give any
+        n = rows * top_k
         _check(lib().nebw_moe_route(self.h, logits.data_ptr(), _dtype(logits), stride, rows,
-                                    _i32(rows_dev), experts, top_k, score, int(renorm), scale,
-                                    _i32(ids), _f32(weights), _i32(group_off), _i32(row_src),
-                                    _i32(row_dst), workspace.data_ptr(),
+                                    self._i32(rows_dev, 1), experts, top_k, score, int(renorm),
+                                    scale, self._i32(ids, n), self._f32(weights, n),
+                                    self._i32(group_off, experts + 1), self._i32(row_src, n),
+                                    self._i32(row_dst, n), workspace.data_ptr(),
                                     workspace.numel() * workspace.element_size(),
                                     self._s(stream)))
 
     def gemm_grouped(self, weight, A, a_rows, group_off, rows, K, N, C_out, row_src=None,
                      bias=None, act=ACT_NONE, c_dtype=BF16, stream=None):
         """One product per expert over its group of rows (nebw_gemm_grouped)."""
-        out = _typed(C_out, "bfloat16" if c_dtype == BF16 else "float32")
-        _check(lib().nebw_gemm_grouped(self.h, weight, _typed(A, "bfloat16"), a_rows,
-                                       _i32(row_src), _i32(group_off), rows, K, N, _f32(bias), act,
-                                       out, c_dtype, self._s(stream)))
+        # (a handle that is not there is refused below)
+        e, k, n, width = self._experts.get(weight, (0, 0, 0, 0))
+        out = self._typed(C_out, "bfloat16" if c_dtype == BF16 else "float32", rows * width)
+        _check(lib().nebw_gemm_grouped(self.h, weight, self._typed(A, "bfloat16", a_rows * k),
+                                       a_rows, self._i32(row_src, rows),
+                                       self._i32(group_off, e + 1), rows, K, N,
+                                       self._f32(bias, e * n), act, out, c_dtype,
+                                       self._s(stream)))
 
     def moe_combine(self, y, row_dst, weights, rows, top_k, H, out, residual=None, rows_dev=None,
                     stream=None):
         """The experts' rows y (torch, [places, H]) weighted and summed per
         row (nebw_moe_combine)."""
-        if not (y.is_contiguous() and out.is_contiguous() and y.is_cuda and out.is_cuda):
-            raise TypeError("contiguous expert rows and output on the GPU are required")
-        _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y.shape[0], _i32(row_dst),
-                                      _f32(weights), rows, _i32(rows_dev), top_k, H,
-                                      _f32(residual), out.data_ptr(), _dtype(out),
+        if (y.get_device() != self.index or out.get_device() != self.index
+                or not (y.is_contiguous() and out.is_contiguous())):
+            raise TypeError("contiguous expert rows and output on the handle's GPU are required")
+        y_rows, n = y.shape[0], rows * top_k
+        if y.numel() < y_rows * H or out.numel() < rows * H:
+            raise ValueError(f"expert rows {tuple(y.shape)} and output {tuple(out.shape)} for "
+                             f"{rows} rows of {H}")
+        _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y_rows,
+                                      self._i32(row_dst, n), self._f32(weights, n), rows,
+                                      self._i32(rows_dev, 1), top_k, H,
+                                      self._f32(residual, rows * H), out.data_ptr(), _dtype(out),
                                       self._s(stream)))
 
 

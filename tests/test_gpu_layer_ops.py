@@ -338,6 +338,20 @@ def test_row_positions(device):
     assert torch.equal(pos.cpu(), want.int())
 
 
+def test_row_positions_stop_at_the_bound(device):
+    """Lengths past max_len are cut there, and an empty batch has no addresses."""
+    off = torch.tensor([0, 300], dtype=torch.int32, device="cuda")
+    n = torch.tensor([290, 7], dtype=torch.int32, device="cuda")
+    pos = torch.full((400,), -7, dtype=torch.int32, device="cuda")
+    device.row_positions(off, n, 2, 258, pos)
+    empty = off[:0].clone()
+    device.row_positions(empty, empty, 0, 258, empty)
+    device.sync()
+    want = torch.full((400,), -7)
+    want[:258], want[300:307] = torch.arange(258), torch.arange(7)
+    assert torch.equal(pos.cpu(), want.int())
+
+
 def test_heads_refusals(device):
     import nebw
     x = torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")
@@ -357,19 +371,20 @@ def test_heads_refusals(device):
         refused("without a rotary", device.rope, hd, None, 4, 64, 0, pos)
         refused("without positions", device.rope, hd, None, 4, 64, h, None)
         refused("more than head_dim", device.rope, hd, None, 4, 32, h, pos)
-        refused("head_dim 258", device.rope, hd, None, 4, 258, h, pos)
+        p = x.data_ptr()
+        raw = nebw.Heads(p, p, 128, 128, 2)
+        refused("head_dim 258", device.rope, raw, None, 4, 258, h, pos)
         refused("head_dim 63", device.rope, hd, None, 4, 63, h, pos)
         refused("layout", device.rope, hd, None, 4, 64, h, pos, layout=2)
         refused("no heads", device.rope, None, None, 4, 64, h, pos)
         refused("rows", device.rope, hd, None, -1, 64, h, pos)
-        refused("rows", device.rope, hd, None, 1 << 31, 64, h, pos)
+        refused("rows", device.rope, raw, None, 1 << 31, 64, h, pos.data_ptr())
         refused("head norm", device.qk_norm_rope, hd, None, 4, 64, norm=0)
         refused("head norm", device.qk_norm_rope, hd, None, 4, 64, norm=3)
         refused("eps", device.qk_norm_rope, hd, None, 4, 64, eps=float("nan"))
         refused("without its bias", device.qk_norm_rope, hd, None, 4, 64, norm=2)
         refused("without its weight", device.qk_norm_rope, nebw.Heads.of(x, 2), None, 4, 64)
-        refused("stride", device.rope, nebw.Heads.of(x, 2), None, 4, 128, h, pos)
-        p = x.data_ptr()
+        refused("stride", device.rope, raw, None, 4, 128, h, pos)
         refused("one row stride", device.rope, nebw.Heads(p, p, 128, 192, 2), None, 4, 64, h, pos)
         refused("aligned", device.rope, nebw.Heads(p + 1, p, 128, 128, 2), None, 4, 64, h, pos)
         refused("null query", device.rope, nebw.Heads(None, p, 128, 128, 2), None, 4, 64, h, pos)
@@ -381,7 +396,11 @@ def test_heads_refusals(device):
         refused("scale", device.stage_rope, inv, 16, float("nan"))
         refused("not finite", device.stage_rope, np.array([1.0, np.inf]), 16)
         assert torch.equal(x, torch.zeros_like(x))
+        for few in ((5, 64, h, pos), (4, 66, h, pos), (4, 64, h, pos[:3])):  # what is not there
+            with pytest.raises(ValueError):
+                device.rope(hd, None, *few)
         device.rope(hd, None, 0, 64, h, None)  # no rows: nothing to do
+        device.rope(nebw.Heads.of(x[:0].clone(), 2), None, 0, 64, h, pos[:0].clone())
         device.sync()
     finally:
         device.release_weight(h)
@@ -570,7 +589,7 @@ def test_route_strided_logits_and_repeat(device):
 
 def test_route_empty_and_refusals(device):
     import nebw
-    r = Routing(4, 8, 2)
+    r = Routing(40, 8, 2)  # room for what the calls below ask for
     x = torch.zeros(4, 8, device="cuda")
     device.moe_route(x[:0], 0, 8, 2, r.ids, r.weights, r.off, r.src, r.dst, r.ws)
     device.sync()
@@ -588,10 +607,17 @@ def test_route_empty_and_refusals(device):
     refused("score", score=2)
     refused("scale", scale=float("inf"))
     refused("null routing", ids=None)
-    refused("workspace", logits=torch.zeros(1 << 20, 8, device="cuda"), ws=x, rows=1 << 20)
+    few = r
+    r = Routing(1 << 20, 8, 2)
+    refused("workspace", logits=torch.zeros(1 << 20, 8, device="cuda"), ids=r.ids, ws=x,
+            rows=1 << 20)
+    with pytest.raises(ValueError):  # fewer values than the call writes
+        device.moe_route(torch.zeros(99, 8, device="cuda"), 99, 8, 2, few.ids, r.weights, r.off,
+                         r.src, r.dst, r.ws)
     with pytest.raises(ValueError):
         device.moe_route(x, 5, 8, 2, r.ids, r.weights, r.off, r.src, r.dst, r.ws)
     wide = torch.zeros(1, 600, device="cuda")
+    r.off = torch.zeros(514, dtype=torch.int32, device="cuda")
     refused("experts", logits=wide, rows=1, experts=513)
     with pytest.raises(ValueError):
         device.moe_route(x.t(), 8, 4, 2, r.ids, r.weights, r.off, r.src, r.dst, r.ws)
@@ -895,8 +921,15 @@ def test_grouped_refusals(device):
     refused("does not match", g, plain, a, 8, off, 8, 128, 64, c)
     refused("does not match", g, plain, a, 8, off, 8, 64, 128, c)
     refused("rows", g, plain, a, 8, off, -1, 64, 64, c)
-    refused("rows", g, plain, a, 8, off, 9, 64, 64, c)       # more groups than A has rows
-    refused("empty A", g, plain, a, 0, off, 8, 64, 64, c, row_src=off)
+    refused("rows", g, plain, a, 8, off, 9, 64, 64, c.data_ptr())  # more groups than A has rows
+    refused("empty A", g, plain, a, 0, off, 8, 64, 64, c, row_src=torch.zeros(8).int().cuda())
+    for few in ((a, 9, off, 8, 64, 64, c), (a, 8, off, 9, 64, 64, c), (a, 8, off[:2], 8, 64, 64, c)):
+        with pytest.raises(ValueError):  # fewer values than the call reads or writes
+            g(plain, *few)
+    with pytest.raises(ValueError):
+        g(plain, a, 8, off, 8, 64, 64, c, row_src=off)
+    with pytest.raises(ValueError):
+        g(plain, a, 8, off, 8, 64, 64, c, bias=torch.zeros(64, device="cuda"))
     refused("activation", g, plain, a, 8, off, 8, 64, 64, c, act=3)
     refused("activation", g, gated, a, 8, off, 8, 64, 64, c, act=2)
     f = torch.zeros(8, 64, device="cuda")
@@ -919,6 +952,8 @@ def test_grouped_refusals(device):
     refused("experts refused", device.stage_experts, np.zeros((513, 64, 8), np.float32))
     with pytest.raises(TypeError):
         device.stage_experts(np.zeros((2, 64, 64)))
+    with pytest.raises(ValueError):  # not as it lies in memory
+        device.stage_experts(torch.zeros(2, 64, 64, device="cuda").transpose(1, 2))
     g(plain, a, 8, off, 0, 64, 64, c)  # no rows: nothing to do
     device.sync()
     assert (c == 7.0).all()
@@ -1066,7 +1101,11 @@ def test_combine_refusals(device):
         assert e.value.code == 1
 
     refused("top_k", y, dst, w, 4, 0, 64, out)
-    refused("top_k", y, dst, w, 4, 17, 64, out)
+    many = torch.zeros(4, 17, device="cuda")
+    refused("top_k", y, many.int(), many, 4, 17, 64, out)
+    for few in ((y, dst, w, 5, 2, 64, out), (y, dst, w, 4, 2, 72, out), (y, dst, w[:3], 4, 2, 64, out)):
+        with pytest.raises(ValueError):  # fewer values than the call reads or writes
+            device.moe_combine(*few)
     refused("width", y, dst, w, 4, 2, 0, out)
     refused("rows", y, dst, w, -1, 2, 64, out)
     refused("null combine", y, None, w, 4, 2, 64, out)
@@ -1075,6 +1114,10 @@ def test_combine_refusals(device):
     device.moe_combine(y, dst, w, 0, 2, 64, out)
     device.sync()
     assert (out == 7.0).all()
+    # no expert's rows at all, and no place that would need one
+    device.moe_combine(y[:0].clone(), torch.full_like(dst, -1), w, 4, 2, 64, out)
+    device.sync()
+    assert (out == 0.0).all()
 
 
 # ---------------------------------------------------------------------------

@@ -53,6 +53,17 @@ def test_rope_freqs_yarn_and_bands():
     np.testing.assert_allclose((plain / inv)[turns >= 2.0], 1.0, rtol=1e-13)
 
 
+def test_rope_freqs_yarn_where_no_frequency_turns():
+    """A trained length in which not even the first frequency turns `slow`
+    times: all of them are divided."""
+    import nebw
+    n, theta, length, factor = 32, 10000.0, 4, 8.0
+    plain = theta ** (-np.arange(n) / n)
+    assert (length * plain / (2 * math.pi) < 1.0).all()
+    inv, _ = nebw.rope_freqs(theta, 2 * n, "yarn", factor, length, fast=32.0, slow=2.0)
+    np.testing.assert_allclose(plain / inv, factor, rtol=1e-12)
+
+
 @pytest.mark.parametrize("args,word", [
     ((10000.0, 7), "rotary width"),
     ((10000.0, 0), "rotary width"),
@@ -132,3 +143,47 @@ def test_heads_of_refuses_what_it_cannot_describe():
         nebw.Heads.of(x, 2, gamma=torch.zeros(96))
     with pytest.raises(TypeError):
         nebw.Heads.of(x.double(), 2)
+
+
+def test_operands_of_another_gpu_or_too_few_are_refused():
+    """The argument checks of the device calls, on a handle without a device
+    and tensors that only say where they are."""
+    torch = pytest.importorskip("torch")
+    import nebw
+
+    class On:
+        dtype = torch.int32
+
+        def __init__(self, gpu, n=4, whole=True):
+            self.gpu, self.n, self.whole = gpu, n, whole
+
+        def get_device(self):
+            return self.gpu
+
+        def is_contiguous(self):
+            return self.whole
+
+        def numel(self):
+            return self.n
+
+        def data_ptr(self):
+            return 64
+
+    d = nebw.Device.__new__(nebw.Device)
+    d.h, d.index = None, 1
+    assert d._i32(On(1), 4) == 64 and d._i32(None, 4) is None and d._i32(80, 4) == 80
+    for bad in (On(0), On(-1), On(1, whole=False)):
+        with pytest.raises(TypeError):
+            d._i32(bad)
+    with pytest.raises(TypeError):
+        d._f32(On(1))
+    with pytest.raises(ValueError):
+        d._i32(On(1), 5)
+    side = nebw.Heads.of(torch.zeros(4, 96), 2)
+    with pytest.raises(TypeError):  # host memory
+        d._heads_dtype(side, None, None, 4, 48)
+    side.gpu = 1
+    assert d._heads_dtype(side, None, None, 4, 48) == nebw.F32
+    for rows, dim in ((5, 48), (4, 50)):
+        with pytest.raises(ValueError):
+            d._heads_dtype(None, side, None, rows, dim)
