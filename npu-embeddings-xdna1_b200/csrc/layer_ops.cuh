@@ -59,7 +59,8 @@ int set_route_attrs() {
   return NEBW_OK;
 }
 
-// How many CTA pairs of the grouped product the GPU holds at once.
+// How many CTA pairs of the grouped product the GPU holds at once (none: the
+// product is refused, the rest of the library works).
 int query_grouped_pairs(int *pairs) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * 74);
@@ -74,7 +75,6 @@ int query_grouped_pairs(int *pairs) {
   cfg.numAttrs = 1;
   NEBW_CUDA(cudaOccupancyMaxActiveClusters(
       pairs, nebw::gemm_grouped_kernel<nebw::kGrpBf16, true>, &cfg));
-  NEBW_REQUIRE(*pairs > 0, "this GPU holds no CTA pair of the grouped product");
   return NEBW_OK;
 }
 
@@ -613,6 +613,7 @@ int launch_grouped(nebw_dev *d, const GroupedMaps &m, int epi, const nebw::Group
   const int64_t tiles = (a.rows / a.tile_rows + std::min(a.experts, a.rows)) *
                         int64_t{(a.N + nebw::kGroupTileCols - 1) / nebw::kGroupTileCols};
   NEBW_REQUIRE(tiles < (1ll << 30), "grouped product too large");
+  NEBW_REQUIRE(d->grouped_pairs > 0, "this GPU holds no CTA pair of the grouped product");
   const unsigned g = 2 * static_cast<unsigned>(std::min<int64_t>(tiles, d->grouped_pairs));
   switch (epi) {
     case nebw::kGrpBf16: launch_grouped_epi<nebw::kGrpBf16>(m, a, g, st); break;

@@ -1298,3 +1298,50 @@ def test_operators_on_another_stream(device):
         outs.append(out)
     assert torch.equal(*outs)
     device.release_weight(h)
+
+
+def test_two_threads_on_two_streams_at_once(device):
+    """Two threads with a stream and a workspace each share a handle and its
+    staged weights."""
+    import threading
+    rows, E, k, H, N = 700, 16, 2, 256, 512
+    w = torch.randn(E, H, N, generator=gen(41), device="cuda").bfloat16()
+    h = device.stage_experts(w)
+    xs = [torch.randn(rows, E, generator=gen(42 + i), device="cuda") for i in range(2)]
+    a = torch.randn(rows, H, generator=gen(44), device="cuda").bfloat16()
+    rs = [Routing(rows, E, k) for _ in range(4)]
+    ys = [torch.empty(rows * k, N, dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    outs = [torch.empty(rows, N, device="cuda") for _ in range(4)]
+
+    def run(i, slot, stream=None):
+        r = rs[slot]
+        device.moe_route(xs[i], rows, E, k, r.ids, r.weights, r.off, r.src, r.dst, r.ws,
+                         renorm=True, stream=stream)
+        device.gemm_grouped(h, a, rows, r.off, rows * k, H, N, ys[slot], row_src=r.src,
+                            stream=stream)
+        device.moe_combine(ys[slot], r.dst, r.weights, rows, k, N, outs[slot], stream=stream)
+
+    for i in range(2):
+        run(i, 2 + i)
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(i, stream):
+        try:
+            for _ in range(20):
+                run(i, i, stream)
+            stream.synchronize()
+        except Exception as e:  # pragma: no cover - the assertion below reports it
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i, torch.cuda.Stream())) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    device.sync()
+    assert not errors
+    for i in range(2):
+        assert torch.equal(outs[i], outs[2 + i]) and torch.equal(rs[i].off, rs[2 + i].off)
+    device.release_weight(h)
