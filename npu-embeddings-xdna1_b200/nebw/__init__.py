@@ -230,23 +230,24 @@ def _addr(x):
     raise TypeError(f"cannot take the address of {type(x)}")
 
 
-_INT32 = _FLOAT32 = None  # torch's dtypes, once it is in use
+_INT32 = _FLOAT32 = _BFLOAT16 = None  # torch's dtypes, once it is in use
 
 
 def _torch_dtypes():
-    global _INT32, _FLOAT32
+    global _INT32, _FLOAT32, _BFLOAT16
     import torch
-    _INT32, _FLOAT32 = torch.int32, torch.float32
+    _INT32, _FLOAT32, _BFLOAT16 = torch.int32, torch.float32, torch.bfloat16
 
 
 def _dtype(t) -> int:
     """F32 or BF16 of a torch tensor."""
-    name = str(t.dtype)
-    if name == "torch.bfloat16":
+    if _BFLOAT16 is None:
+        _torch_dtypes()
+    if t.dtype is _BFLOAT16:
         return BF16
-    if name == "torch.float32":
+    if t.dtype is _FLOAT32:
         return F32
-    raise TypeError(f"fp32 or bf16 is required, not {name}")
+    raise TypeError(f"fp32 or bf16 is required, not {t.dtype}")
 
 
 CUDA_STREAM_LEGACY = 1  # cudaStreamLegacy: the legacy default stream's handle
