@@ -337,7 +337,9 @@ int64_t nebw_moe_route_workspace(int64_t rows, int32_t experts, int32_t top_k);
  * >= experts in elements: a padded GEMM output's N).  The largest logits are
  * chosen, ties to the lower expert; -inf and NaN are never chosen.  Their
  * scores are the softmax over all experts or the sigmoid; renorm != 0 divides
- * by the sum of the chosen; then times scale.  Outputs, all device:
+ * by the sum of the chosen (0 for sigmoids of a row without a logit above
+ * -709.78, one masked by a lowest value); then times scale.  Outputs, all
+ * device:
  *   ids [rows, top_k], weights [rows, top_k] fp32, by falling logit
  *   group_off [experts + 1]: expert e has the places group_off[e] ..
  *     group_off[e + 1], its rows ascending

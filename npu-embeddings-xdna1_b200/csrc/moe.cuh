@@ -208,9 +208,19 @@ __device__ __forceinline__ void route_row(const RouteArgs &p, const T *l, int su
 }
 
 // The score of a chosen expert before it is normalised; `first` is the row's
-// largest logit.
+// largest logit.  Sigmoids that are divided by their sum are taken times
+// exp(-first) where first < 0: sigmoid(v) = exp(v) / (1 + exp(v)), so the first
+// one is 1 / (1 + exp(first)) > 1/2 and the sum neither vanishes (all logits
+// below -88.7) nor becomes so small that scale / sum overflows.  A row whose
+// first is below kRouteMasked, where exp(-first) leaves 64 bits too, is one
+// masked by some lowest value: its scores are 0.
+constexpr float kRouteMasked = -709.78f;  // -ln of the largest double
 __device__ __forceinline__ float route_score(const RouteArgs &p, float v, float first) {
-  if (p.sigmoid) return 1.0f / (1.0f + expf(-v));
+  if (p.sigmoid) {
+    if (p.renorm && first < 0.f)
+      return first < kRouteMasked ? 0.f : expf(v - first) / (1.0f + expf(v));
+    return 1.0f / (1.0f + expf(-v));
+  }
   return v == first ? 1.0f : expf(v - first);  // inf - inf is no number
 }
 

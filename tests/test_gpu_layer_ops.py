@@ -558,6 +558,35 @@ def test_route_ties_masks_and_odd_values(device, dtype):
                      dst))
 
 
+@pytest.mark.parametrize("scale", [1.0, 2.5])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_route_sigmoid_shares_of_very_low_logits(device, dtype, scale):
+    """Divided by the sum of the chosen, sigmoids that fp32 cannot hold are
+    still shares of one; a row of lowest values has no share to give."""
+    low = torch.finfo(TYPES[dtype]).min
+    x = torch.cat([
+        torch.tensor([[-200.0, -150.0, -300.0, -250.0, -400.0, -120.0],
+                      [-700.0, low, -708.0, low, -900.0, low], [low] * 6,
+                      [-712.0, -712.0, -3e4, low, low, low], [low, -1.0, low, low, low, 3.0], [-math.inf, -90.0, -math.inf, -91.0, -92.0, 0.0],
+                      [-math.inf, -90.0, -math.inf, -90.5, -92.0, -math.inf]], device="cuda"),
+        # around where exp(-x) leaves fp32, and its reciprocal the normal range
+        -torch.arange(80.0, 110.0, 0.125, device="cuda").reshape(-1, 6)]).to(TYPES[dtype])
+    for k in (1, 2, 3):
+        r = Routing(len(x), 6, k).run(device, x, score=1, renorm=True, scale=scale)
+        device.sync()
+        v = x.double()
+        best = v.sort(dim=1, descending=True, stable=True)
+        top, ids = best.values[:, :k], best.indices[:, :k]
+        there = top > -math.inf
+        # sigmoid(v) / sum = exp(v - log(1 + e^v)) / sum, from the logarithms
+        want = scale * torch.softmax(torch.nn.functional.logsigmoid(top), 1) * there
+        want = torch.where(top[:, :1] > -709.78, want, 0.0)
+        assert torch.equal(r.ids, torch.where(there, ids, -1).int())
+        # as Routing.check: two exp of arguments to ~100, sums, quotients, a product
+        got = r.weights.double()
+        assert ((got - want).abs() <= 700 * U * want + 1e-37).all(), (got, want)
+
+
 @pytest.mark.parametrize("rows", [1200, 700])  # two kernels, and one block
 def test_route_live_rows(device, rows):
     experts, k = 16, 2
