@@ -244,8 +244,10 @@ enum { NEBW_ROPE_HALF = 0, NEBW_ROPE_PAIRS = 1 };
  *   NTK     f_i of the base theta * factor^(n / (n - 1))
  *   YARN    f_i where it turns more than `fast` (0: 32) times within orig_len
  *           positions, f_i / factor where fewer than `slow` (0: 1) times,
- *           blended linearly over the index in between; the rotated values
- *           times attn_scale (0: 0.1 ln(factor) + 1)
+ *           blended linearly over the index in between (whole indices, from 0
+ *           to rot_dim - 1, of those two turns: the last may lie past the
+ *           last frequency); the rotated values times attn_scale (0:
+ *           0.1 ln(factor) + 1)
  *   BANDS   the same two ends (fast 0: 4, slow 0: 1), blended linearly over
  *           the number of turns, and no scale */
 enum {

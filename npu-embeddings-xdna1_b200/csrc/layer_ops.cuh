@@ -122,10 +122,12 @@ extern "C" int nebw_rope_freqs(double theta, int32_t rot_dim, const nebw_rope_sc
   if (kind == NEBW_ROPE_NTK) base = n > 1 ? theta * std::pow(s->factor, n / (n - 1.0)) : theta;
   double lo = 0.0, hi = 0.0;
   if (kind == NEBW_ROPE_YARN) {
-    // the index whose frequency turns beta times within the trained length
+    // the index whose frequency turns beta times within the trained length:
+    // past the last frequency where that still turns more often, bounded by
+    // rot_dim - 1 as the definition has it
     const double len = static_cast<double>(s->orig_len);
     lo = std::max(0.0, std::floor(n * std::log(len / (fast * kTwoPi)) / std::log(theta)));
-    hi = std::min(n - 1.0, std::ceil(n * std::log(len / (slow * kTwoPi)) / std::log(theta)));
+    hi = std::min(rot_dim - 1.0, std::ceil(n * std::log(len / (slow * kTwoPi)) / std::log(theta)));
     if (hi < 0.0) lo = hi - 1.0;  // none turns `slow` times: all are scaled
     *scale = s->attn_scale > 0.0 ? s->attn_scale : 0.1 * std::log(s->factor) + 1.0;
   }

@@ -53,6 +53,37 @@ def test_rope_freqs_yarn_and_bands():
     np.testing.assert_allclose((plain / inv)[turns >= 2.0], 1.0, rtol=1e-13)
 
 
+@pytest.mark.parametrize("theta,rot_dim,length,factor,fast,slow", [
+    (10000.0, 128, 4096, 16.0, 0, 0),
+    # the index that turns once lies past the last frequency
+    (1000.0, 32, 4096, 8.0, 0, 0), (1000.0, 64, 8192, 8.0, 0, 0), (10000.0, 64, 131072, 4.0, 0, 0),
+    (1000.0, 12, 4096, 2.0, 0, 0), (500000.0, 128, 8192, 8.0, 24.0, 0.25),
+    # past rot_dim - 1, where it is bounded; every frequency turns fast
+    (100.0, 16, 1 << 20, 8.0, 0, 0), (100.0, 16, 1 << 30, 8.0, 0, 0), (10000.0, 2, 4096, 4.0, 0, 0),
+])
+def test_rope_freqs_yarn_ramp(theta, rot_dim, length, factor, fast, slow):
+    """Every frequency against the definition: the indices of the two turn
+    counts, rounded outwards and held within [0, rot_dim - 1], a linear ramp
+    between them, and the frequencies blended by it."""
+    import nebw
+
+    def index(turns):
+        return rot_dim * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+    low = max(math.floor(index(fast or 32)), 0)
+    high = min(math.ceil(index(slow or 1)), rot_dim - 1)
+    inv, _ = nebw.rope_freqs(theta, rot_dim, "yarn", factor, length, fast, slow)
+    assert len(inv) == rot_dim // 2
+    for i, got in enumerate(inv):
+        plain = theta ** (-2.0 * i / rot_dim)
+        ramp = min(1.0, max(0.0, (i - low) / max(high - low, 1e-3)))
+        # a few roundings of pow and log in double
+        assert got == pytest.approx(plain / factor * ramp + plain * (1 - ramp), rel=1e-12), i
+        # and what the definition says of it in words
+        if length * plain / (2 * math.pi) > 2.0 * (fast or 32):
+            assert got == pytest.approx(plain, rel=1e-12)
+
+
 def test_rope_freqs_yarn_where_no_frequency_turns():
     """A trained length in which not even the first frequency turns `slow`
     times: all of them are divided."""
