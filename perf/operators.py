@@ -324,10 +324,8 @@ def _stage(s, c):
     descriptions of its heads, a workspace."""
     nebw, dev, op = _nebw(), _dev(), c["op"]
     if op in ("rope", "qk_norm_rope"):
-        inv, scale = nebw.rope_freqs(
-            c["theta"], c["rot_dim"], scaling=c["scaling"], factor=c["factor"],
-            orig_len=4096 if c["max_pos"] >= 4096 else 512)
-        s["rope"] = _Staged(dev.stage_rope(inv, c["max_pos"], scale))
+        inv, scale = _frequencies(c)  # the case's own set
+        s["rope"] = _Staged(dev.stage_rope(inv.numpy(), c["max_pos"], scale))
         for side in "qk":
             s[side + "_heads"] = nebw.Heads.of(
                 s[side], c[side + "_heads"], out=s[side + "_out"], gamma=s.get(side + "_gamma"),
