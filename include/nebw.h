@@ -274,7 +274,13 @@ int nebw_rope_freqs(double theta, int32_t rot_dim, const nebw_rope_scaling *scal
 int nebw_stage_rope(nebw_dev *dev, const double *inv_freq, int32_t n, int64_t max_pos,
                     double scale, uint64_t *handle);
 /* pos[seq_off[b] + s] = s for s < seq_len[b] (at most max_len): the packed
- * rows' positions in their sequences, from nebw_pack_offsets' outputs. */
+ * rows' positions in their sequences, from nebw_pack_offsets' outputs.  pos
+ * has `rows` entries; a row outside them is an NEBW_EDEVICE error at the next
+ * sync and is not written.  The other entries stay as they are. */
+int nebw_packed_positions(nebw_dev *dev, const int32_t *seq_off, const int32_t *seq_len, int32_t B,
+                          int32_t max_len, int64_t rows, int32_t *pos, void *stream);
+/* The same for a pos of B * max_len entries, the most that B sequences pack
+ * to. */
 int nebw_row_positions(nebw_dev *dev, const int32_t *seq_off, const int32_t *seq_len, int32_t B,
                        int32_t max_len, int32_t *pos, void *stream);
 

@@ -64,14 +64,19 @@ __global__ void __launch_bounds__(kRowWarps * 32)
   }
 }
 
-// Position of every packed row in its sequence (pos[seq_off[b] + s] = s),
-// grid (ceil(S / 256), B): the rotary QKV epilogue's per-row input.
+// Position of every packed row in its sequence (pos[seq_off[b] + s] = s for
+// s < min(seq_len[b], most)), grid (ceil(most / 256), B), a thread a position:
+// the rotary QKV epilogue's per-row input, and nebw_packed_positions.  pos has
+// `rows` entries; a row outside them is reported and not written.
 __global__ void __launch_bounds__(256)
-    row_pos_kernel(const int *__restrict__ seq_off, const int *__restrict__ seq_len,
-                   int *__restrict__ pos) {
+    row_pos_kernel(const int *__restrict__ seq_off, const int *__restrict__ seq_len, int most,
+                   int64_t rows, int *__restrict__ pos, int *err) {
   const int b = blockIdx.y;
-  const int s = blockIdx.x * blockDim.x + threadIdx.x;
-  if (s < __ldg(seq_len + b)) pos[__ldg(seq_off + b) + s] = s;
+  const int64_t s = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  if (s >= min(__ldg(seq_len + b), most)) return;
+  const int64_t at = __ldg(seq_off + b) + s;
+  if (at >= 0 && at < rows) pos[at] = static_cast<int>(s);
+  else record_err(err, kDevBadRow);
 }
 
 // SiLU as swiglu_cpu computes it: x / (1 + 2^max(-x log2 e, -120)).

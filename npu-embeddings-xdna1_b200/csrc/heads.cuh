@@ -56,16 +56,6 @@ struct HeadArgs {
   int *err;
 };
 
-// pos[off[b] + s] = s for s < min(len[b], most): a block row a sequence, a
-// thread a position.
-__global__ void __launch_bounds__(256)
-    row_positions_kernel(const int *__restrict__ off, const int *__restrict__ len, int most,
-                         int *__restrict__ pos) {
-  const int b = blockIdx.y;
-  const int64_t s = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-  if (s < min(__ldg(len + b), most)) pos[__ldg(off + b) + s] = static_cast<int>(s);
-}
-
 // cos and sin of every position and frequency, in double, scaled and rounded
 // once.
 __global__ void __launch_bounds__(256)

@@ -190,17 +190,26 @@ extern "C" int nebw_stage_rope(nebw_dev *d, const double *inv_freq, int32_t n, i
   return NEBW_OK;
 }
 
-extern "C" int nebw_row_positions(nebw_dev *d, const int32_t *off, const int32_t *len, int32_t B,
-                                  int32_t max_len, int32_t *pos, void *stream) {
+extern "C" int nebw_packed_positions(nebw_dev *d, const int32_t *off, const int32_t *len,
+                                     int32_t B, int32_t max_len, int64_t rows, int32_t *pos,
+                                     void *stream) {
   if (int rc = use_dev(d)) return rc;
   NEBW_REQUIRE(B >= 0 && B <= 65535 && max_len >= 0, "positions of %d sequences up to %d refused",
                B, max_len);
+  NEBW_REQUIRE(rows >= 0, "rows %lld refused", static_cast<long long>(rows));
   if (B == 0 || max_len == 0) return NEBW_OK;
-  NEBW_REQUIRE(off && len && pos, "null position operand");
+  NEBW_REQUIRE(off && len && (pos || rows == 0), "null position operand");
   const dim3 grid(static_cast<unsigned>((int64_t{max_len} + 255) / 256), B);
-  nebw::row_positions_kernel<<<grid, 256, 0, pick_stream(d, stream)>>>(off, len, max_len, pos);
+  nebw::row_pos_kernel<<<grid, 256, 0, pick_stream(d, stream)>>>(off, len, max_len, rows, pos,
+                                                                 d->d_err);
   NEBW_CUDA(cudaGetLastError());
   return NEBW_OK;
+}
+
+extern "C" int nebw_row_positions(nebw_dev *d, const int32_t *off, const int32_t *len, int32_t B,
+                                  int32_t max_len, int32_t *pos, void *stream) {
+  const int64_t rows = B > 0 && max_len > 0 ? int64_t{B} * max_len : 0;
+  return nebw_packed_positions(d, off, len, B, max_len, rows, pos, stream);
 }
 
 namespace {

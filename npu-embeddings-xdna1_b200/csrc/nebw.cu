@@ -95,6 +95,7 @@ const char *dev_err_name(int code) {
     case nebw::kDevBadLength: return "a sequence length is outside [1, seq]";
     case nebw::kDevBadShape: return "a kernel was handed a shape its launch cannot cover";
     case nebw::kDevBadPosition: return "a position is outside the staged rotary table";
+    case nebw::kDevBadRow: return "a packed row is outside its buffer";
     case nebw::kDevBadGroup: return "a group offset or grouped row index is out of range";
     default: return "unknown device error";
   }
@@ -1627,7 +1628,8 @@ int encode_device_bf16(nebw_model *m, Workspace &ws, bool prof, const int *ids, 
   const bool rope_fused = c.rope && ws.row_pos != nullptr;
   if (rope_fused) {
     const dim3 pg((S + 255) / 256, B);
-    nebw::row_pos_kernel<<<pg, 256, 0, st>>>(ws.off, ws.len, ws.row_pos);
+    nebw::row_pos_kernel<<<pg, 256, 0, st>>>(ws.off, ws.len, S, ws.rows_cap, ws.row_pos,
+                                             d->d_err);
     NEBW_CUDA(cudaGetLastError());
   }
   for (int L = 0; L < c.num_layers; ++L) {

@@ -23,6 +23,7 @@ enum DevErr : int {
   kDevBadShape = 4,      // a kernel was handed a shape its launch cannot cover
   kDevBadPosition = 5,   // a position outside the rotary table
   kDevBadGroup = 6,      // a group offset or a grouped row index out of range
+  kDevBadRow = 7,        // a packed row outside its buffer
 };
 
 constexpr uint64_t kWaitTimeoutNs = 2000ull * 1000ull * 1000ull;  // 2 s

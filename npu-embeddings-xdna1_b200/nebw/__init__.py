@@ -174,6 +174,7 @@ def lib() -> C.CDLL:
         "nebw_stage_rope": ([vp, C.POINTER(C.c_double), i32, i64, C.c_double,
                              C.POINTER(C.c_uint64)], C.c_int),
         "nebw_row_positions": ([vp, vp, vp, i32, i32, vp, vp], C.c_int),
+        "nebw_packed_positions": ([vp, vp, vp, i32, i32, i64, vp, vp], C.c_int),
         "nebw_rope": ([vp, C.POINTER(Heads), C.POINTER(Heads), C.c_int, i64, vp, i32, C.c_uint64,
                        C.c_int, vp, vp], C.c_int),
         "nebw_qk_norm_rope": ([vp, C.POINTER(Heads), C.POINTER(Heads), C.c_int, i64, vp, i32,
@@ -446,9 +447,16 @@ class Device:
                                      max_pos, scale, C.byref(hnd)))
         return hnd.value
 
-    def row_positions(self, seq_off, seq_len, B, max_len, pos, stream=None):
-        _check(lib().nebw_row_positions(self.h, self._i32(seq_off, B), self._i32(seq_len, B), B,
-                                        max_len, self._i32(pos), self._s(stream)))
+    def row_positions(self, seq_off, seq_len, B, max_len, pos, stream=None, rows=None):
+        """The packed rows' positions in their sequences (nebw_packed_positions):
+        pos has `rows` entries, all of a tensor's if not given (an address
+        needs them)."""
+        if rows is None:
+            if pos.__class__ is int:
+                raise ValueError("positions at an address need their number")
+            rows = pos.numel()
+        _check(lib().nebw_packed_positions(self.h, self._i32(seq_off, B), self._i32(seq_len, B), B,
+                                           max_len, rows, self._i32(pos, rows), self._s(stream)))
 
     def _heads_dtype(self, q, k, dtype, rows, head_dim):
         """The dtype of heads made by Heads.of, which must hold the rows and

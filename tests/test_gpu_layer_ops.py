@@ -352,6 +352,53 @@ def test_row_positions_stop_at_the_bound(device):
     assert torch.equal(pos.cpu(), want.int())
 
 
+@pytest.mark.parametrize("off,lens", [
+    ([0, 90], [5, 20]),          # past the end
+    ([-3, 40], [5, 20]),         # before the start
+    ([2 ** 31 - 1, 40], [5, 20]), ([-2 ** 31, 40], [5, 20]),
+    ([0, 100], [5, 1]),
+])
+def test_row_positions_outside_the_rows(device, off, lens):
+    """Offsets that leave pos are reported; what lies in it is written, what lies
+    around it (with room on both sides) stays."""
+    import nebw
+    buf = torch.full((300,), -7, dtype=torch.int32, device="cuda")
+    pos = buf[100:200]
+    o, n = (torch.tensor(v, device="cuda").int() for v in (off, lens))
+    device.row_positions(o, n, 2, 64, pos)
+    with pytest.raises(nebw.NebwError, match="packed row") as e:
+        device.sync()
+    assert e.value.code == 5
+    want = torch.full((300,), -7)
+    for a, m in zip(off, lens):
+        for s in range(m):
+            if 0 <= a + s < 100:
+                want[100 + a + s] = s
+    assert torch.equal(buf.cpu(), want.int())
+    device.sync()  # reported once
+    with pytest.raises(ValueError):  # fewer entries than said
+        device.row_positions(o, n, 2, 64, pos, rows=101)
+    with pytest.raises(nebw.NebwError, match="rows"):
+        device.row_positions(o, n, 2, 64, pos, rows=-1)
+
+
+def test_row_positions_by_address_and_of_whole_sequences(device):
+    """The entry point without a row count writes as many as the sequences can
+    have; an address comes with its number."""
+    import nebw
+    off, n = (torch.tensor(v, device="cuda").int() for v in ([0, 5], [5, 8]))
+    pos = torch.full((20,), -7, dtype=torch.int32, device="cuda")
+    want = torch.cat([torch.arange(5), torch.arange(8), torch.full((7,), -7)]).int()
+    rc = nebw.lib().nebw_row_positions(device.h, off.data_ptr(), n.data_ptr(), 2, 8,
+                                       pos.data_ptr(), nebw.CUDA_STREAM_LEGACY)
+    device.sync()
+    assert rc == 0 and torch.equal(pos.cpu(), want)
+    pos.fill_(-7)
+    device.row_positions(off, n, 2, 8, pos.data_ptr(), rows=13)
+    device.sync()
+    assert torch.equal(pos.cpu(), want)
+
+
 def test_heads_refusals(device):
     import nebw
     x = torch.zeros(4, 128, dtype=torch.bfloat16, device="cuda")

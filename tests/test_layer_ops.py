@@ -157,6 +157,18 @@ def test_null_device_is_refused_by_name():
         assert "null device handle" in L.nebw_last_error().decode(), name
 
 
+def test_positions_say_how_many_they_are():
+    """An address alone does not: nothing may be written without a bound."""
+    import nebw
+    L = nebw.lib()
+    assert L.nebw_packed_positions(None, None, None, 1, 1, 1, None, None) == 1
+    assert "null device handle" in L.nebw_last_error().decode()
+    d = nebw.Device.__new__(nebw.Device)
+    d.h, d.index = None, 0
+    with pytest.raises(ValueError):
+        d.row_positions(64, 64, 1, 8, 64)
+
+
 def test_heads_of_refuses_what_it_cannot_describe():
     torch = pytest.importorskip("torch")
     import nebw
