@@ -8,6 +8,12 @@ namespace {
 
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Arrays of 4-byte values (or null), which kernels read and write whole.
+template <typename... P>
+bool words(const P *...p) {
+  return (aligned(p, 4) && ...);
+}
+
 // Host or this device's memory; *on_device says which.
 int where_is(nebw_dev *d, const void *p, bool *on_device) {
   cudaPointerAttributes a;
@@ -199,6 +205,7 @@ extern "C" int nebw_packed_positions(nebw_dev *d, const int32_t *off, const int3
   NEBW_REQUIRE(rows >= 0, "rows %lld refused", static_cast<long long>(rows));
   if (B == 0 || max_len == 0) return NEBW_OK;
   NEBW_REQUIRE(off && len && (pos || rows == 0), "null position operand");
+  NEBW_REQUIRE(words(off, len, pos), "position operands are not aligned");
   const dim3 grid(static_cast<unsigned>((int64_t{max_len} + 255) / 256), B);
   nebw::row_pos_kernel<<<grid, 256, 0, pick_stream(d, stream)>>>(off, len, max_len, rows, pos,
                                                                  d->d_err);
@@ -354,6 +361,7 @@ int run_heads(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype, 
     NEBW_REQUIRE(2 * it->second.n <= head_dim, "a rotary width of %d is more than head_dim %d",
                  2 * it->second.n, head_dim);
     NEBW_REQUIRE(pos || rows == 0, "rotation without positions");
+    NEBW_REQUIRE(words(pos), "positions are not aligned");
     a.n = it->second.n;
     a.table = it->second.table;
     a.max_pos = it->second.max_pos;
@@ -363,6 +371,7 @@ int run_heads(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype, 
   if (int rc = check_heads(q, "query", head_dim, rows, esz, norm, &a.q)) return rc;
   if (int rc = check_heads(k, "key", head_dim, rows, esz, norm, &a.k)) return rc;
   NEBW_REQUIRE(a.q.heads + a.k.heads > 0, "no heads given");
+  NEBW_REQUIRE(words(rows_dev), "the live row count is not aligned");
   if (rows == 0) return NEBW_OK;
   a.rows = rows;
   a.rows_dev = rows_dev;
@@ -481,6 +490,8 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
                score);
   NEBW_REQUIRE(std::isfinite(scale), "routing scale %g refused", static_cast<double>(scale));
   NEBW_REQUIRE(group_off, "null routing output");
+  NEBW_REQUIRE(words(rows_dev, ids, weights, group_off, row_src, row_dst),
+               "routing operands are not aligned");
   const cudaStream_t st = pick_stream(d, stream);
   if (rows == 0) {
     NEBW_CUDA(cudaMemsetAsync(group_off, 0, (experts + 1) * sizeof(int), st));
@@ -544,6 +555,7 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   if (int rc = where_is(d, kn, &on_device)) return rc;
   const cudaStream_t st = pick_stream(d, stream);
   const size_t esz = dtype == NEBW_F32 ? 4 : 2;
+  NEBW_REQUIRE(!on_device || aligned(kn, esz), "expert weights are not aligned");
   const size_t one = static_cast<size_t>(K) * N * esz;
   Experts w;
   w.experts = experts;
@@ -675,6 +687,7 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
                static_cast<long long>(a_rows), static_cast<long long>(rows));
   NEBW_REQUIRE(aligned(A, 16) && aligned(C, 16) && aligned(bias, 16),
                "grouped operands must be 16-byte aligned");
+  NEBW_REQUIRE(words(group_off, row_src), "group offsets or row indices are not aligned");
   nebw::GroupedArgs a{};
   a.off = group_off;
   a.experts = w.experts;
@@ -745,6 +758,10 @@ extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t
                "%lld rows of %d experts refused", static_cast<long long>(rows), top_k);
   if (rows == 0) return NEBW_OK;
   NEBW_REQUIRE((y || y_rows == 0) && row_dst && weights && out, "null combine operand");
+  NEBW_REQUIRE(aligned(y, y_dtype == NEBW_F32 ? 4 : 2) &&
+                   aligned(out, out_dtype == NEBW_F32 ? 4 : 2) &&
+                   words(row_dst, weights, residual, rows_dev),
+               "combine operands are not aligned");
   nebw::CombineArgs a{};
   a.y = y;
   a.row_dst = row_dst;

@@ -1061,6 +1061,49 @@ def test_grouped_product_and_combine_past_32_bits(device):
     device.release_weight(h)
 
 
+def test_operands_off_their_values_boundaries_are_refused(device):
+    """Addresses between two values are refused before a kernel reads there."""
+    import nebw
+    rows, E, k, H = 4, 8, 2, 64
+    x = torch.zeros(rows, H, dtype=torch.bfloat16, device="cuda")
+    it = torch.zeros(64, dtype=torch.int32, device="cuda")
+    fl = torch.zeros(rows, H, device="cuda")
+    inv, _ = nebw.rope_freqs(10000.0, H)
+    rope = device.stage_rope(inv, 16)
+    w = device.stage_experts(np.zeros((1, H, H), np.float32))
+    a, p, f = x.data_ptr(), it.data_ptr(), fl.data_ptr()
+    L, st = nebw.lib(), nebw.CUDA_STREAM_LEGACY
+    side = nebw.Heads(a, a, H, H, 1)
+
+    def swap(args, i, by):
+        return [v + by if j == i else v for j, v in enumerate(args)]
+
+    calls = [  # the call, its arguments, where the addresses are, and by how much they are off
+        (L.nebw_packed_positions, [p, p, 1, 4, 4, p, st], (0, 1, 5), 2),
+        (L.nebw_row_positions, [p, p, 1, 4, p, st], (0, 1, 4), 1),
+        (L.nebw_rope, [side, None, nebw.BF16, rows, p, H, rope, 0, p, st], (4, 8), 2),
+        (L.nebw_qk_norm_rope, [nebw.Heads(a, a, H, H, 1, 0, f), None, nebw.BF16, rows, p, H, 1,
+                               1e-6, rope, 0, p, st], (4, 10), 2),
+        (L.nebw_moe_route, [f, nebw.F32, E, rows, p, E, k, 0, 0, 1.0, p, f, p, p, p, p, 64 * 4,
+                            st], (0, 4, 10, 11, 12, 13, 14, 15), 2),
+        (L.nebw_gemm_grouped, [w, a, rows, p, p, rows, H, H, None, 0, f, nebw.BF16, st], (3, 4), 2),
+        (L.nebw_moe_combine, [a, nebw.BF16, rows, p, f, rows, p, k, H, f, f, nebw.F32, st],
+         (3, 4, 6, 9, 10), 2),
+        (L.nebw_moe_combine, [a, nebw.BF16, rows, p, f, rows, p, k, H, None, a, nebw.BF16, st],
+         (0, 10), 1),
+    ]
+    for call, args, where, by in calls:
+        for i in where:
+            assert call(device.h, *swap(args, i, by)) == 1, (call.__name__, i)
+            assert "aligned" in L.nebw_last_error().decode(), (call.__name__, i)
+    hnd = (nebw.C.c_uint64 * 1)()
+    assert L.nebw_stage_experts(device.h, a + 1, nebw.BF16, 1, 64, 8, 0, st, hnd) == 1
+    assert "aligned" in L.nebw_last_error().decode()
+    device.sync()
+    device.release_weight(rope)
+    device.release_weight(w)
+
+
 def test_whole_numbers_of_another_dtype_are_refused(device):
     """int64 indices (torch's default) would be read as other numbers, host
     memory not at all."""
