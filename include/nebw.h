@@ -19,7 +19,12 @@
  *     wants the legacy default stream passes cudaStreamLegacy ((void*)0x1).
  *   - One nebw_dev per GPU.  Calls on different nebw_dev handles may run
  *     concurrently from different host threads; calls on one handle must not
- *     overlap.  Staged weights are immutable after staging.
+ *     overlap, but for these: staging and releasing operands, and the
+ *     operators of rotary and expert layers (nebw_packed_positions, nebw_rope,
+ *     nebw_qk_norm_rope, nebw_moe_route, nebw_gemm_grouped,
+ *     nebw_moe_combine), each call with outputs and a workspace of its own
+ *     and no handle that another thread is releasing.  Staged weights are
+ *     immutable after staging.
  */
 #ifndef NEBW_H
 #define NEBW_H

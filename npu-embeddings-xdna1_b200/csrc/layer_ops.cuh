@@ -186,14 +186,9 @@ extern "C" int nebw_stage_rope(nebw_dev *d, const double *inv_freq, int32_t n, i
     cudaFree(t.table);
     return set_error(NEBW_ECUDA, "rotary table staging failed: %s", cudaGetErrorString(e));
   }
-  try {
-    d->ropes[d->next_handle] = t;
-  } catch (const std::exception &) {
-    cudaFree(t.table);
-    return set_error(NEBW_ENOMEM, "no host memory for a rotary handle");
-  }
-  *handle = d->next_handle++;
-  return NEBW_OK;
+  const int rc = keep_staged(d, d->ropes, t, handle);
+  if (rc) cudaFree(t.table);
+  return rc;
 }
 
 extern "C" int nebw_packed_positions(nebw_dev *d, const int32_t *off, const int32_t *len,
@@ -355,16 +350,15 @@ int run_heads(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype, 
                layout);
   nebw::HeadArgs a{};
   if (rope) {
-    auto it = d->ropes.find(rope);
-    NEBW_REQUIRE(it != d->ropes.end(), "unknown rotary handle %llu",
-                 static_cast<unsigned long long>(rope));
-    NEBW_REQUIRE(2 * it->second.n <= head_dim, "a rotary width of %d is more than head_dim %d",
-                 2 * it->second.n, head_dim);
+    const RopeTable *t = find_staged(d, d->ropes, rope);
+    NEBW_REQUIRE(t, "unknown rotary handle %llu", static_cast<unsigned long long>(rope));
+    NEBW_REQUIRE(2 * t->n <= head_dim, "a rotary width of %d is more than head_dim %d", 2 * t->n,
+                 head_dim);
     NEBW_REQUIRE(pos || rows == 0, "rotation without positions");
     NEBW_REQUIRE(words(pos), "positions are not aligned");
-    a.n = it->second.n;
-    a.table = it->second.table;
-    a.max_pos = it->second.max_pos;
+    a.n = t->n;
+    a.table = t->table;
+    a.max_pos = t->max_pos;
     a.pos = pos;
   }
   const size_t esz = dtype == NEBW_F32 ? 4 : 2;
@@ -597,19 +591,9 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   if (e != cudaSuccess)
     rc = set_error(NEBW_ECUDA, "expert weight staging failed: %s", cudaGetErrorString(e));
   if (!rc) rc = make_tmap_kmajor(&w.map, w.ptr, blocks * 128, 64, 128);
-  if (!rc) {
-    try {
-      d->experts[d->next_handle] = w;
-    } catch (const std::exception &) {
-      rc = set_error(NEBW_ENOMEM, "no host memory for an expert weight handle");
-    }
-  }
-  if (rc) {
-    cudaFree(w.ptr);
-    return rc;
-  }
-  *handle = d->next_handle++;
-  return NEBW_OK;
+  if (!rc) rc = keep_staged(d, d->experts, w, handle);
+  if (rc) cudaFree(w.ptr);
+  return rc;
 }
 
 namespace {
@@ -657,10 +641,10 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
                                  int64_t K, int64_t N, const float *bias, int act, void *C,
                                  int c_dtype, void *stream) {
   if (int rc = use_dev(d)) return rc;
-  auto it = d->experts.find(weight);
-  NEBW_REQUIRE(it != d->experts.end(), "unknown expert weight handle %llu",
+  const Experts *staged = find_staged(d, d->experts, weight);
+  NEBW_REQUIRE(staged, "unknown expert weight handle %llu",
                static_cast<unsigned long long>(weight));
-  const Experts &w = it->second;
+  const Experts &w = *staged;
   NEBW_REQUIRE(K == w.K && N == w.N,
                "grouped product [rows, %lld] x [%lld, %lld] does not match the staged experts "
                "[%d, K=%lld, N=%lld]",

@@ -258,6 +258,7 @@ struct nebw_dev {
   std::map<uint64_t, Experts> experts;
   std::map<uint64_t, RopeTable> ropes;
   uint64_t next_handle = 1;
+  std::mutex staged;  // of the four maps and next_handle (find_staged, keep_staged)
   // CTA pairs the GPU can hold at once for the 2-CTA GEMM (0: use the
   // single-CTA kernel); NEBW_GEMM_CTAS=1 in the environment forces 0.
   int gemm_pairs = 0;
@@ -277,6 +278,29 @@ int use_dev(nebw_dev *d) {
 
 cudaStream_t pick_stream(nebw_dev *d, void *stream) {
   return stream ? static_cast<cudaStream_t>(stream) : d->stream;
+}
+
+// A staged operand by its handle (null: unknown).  The maps change while other
+// threads' calls look into them; what they hold stays where it is until it is
+// released.
+template <typename T>
+const T *find_staged(nebw_dev *d, const std::map<uint64_t, T> &map, uint64_t handle) {
+  std::lock_guard<std::mutex> lock(d->staged);
+  const auto it = map.find(handle);
+  return it == map.end() ? nullptr : &it->second;
+}
+
+// A new operand's handle.
+template <typename T>
+int keep_staged(nebw_dev *d, std::map<uint64_t, T> &map, const T &operand, uint64_t *handle) {
+  try {
+    std::lock_guard<std::mutex> lock(d->staged);
+    map.emplace(d->next_handle, operand);
+    *handle = d->next_handle++;
+  } catch (const std::exception &) {
+    return set_error(NEBW_ENOMEM, "no host memory for a staged operand's handle");
+  }
+  return NEBW_OK;
 }
 
 template <int BN, int EPI>
@@ -964,34 +988,31 @@ extern "C" int nebw_stage_weight(nebw_dev *d, const void *host_kn, int dtype, in
   NEBW_REQUIRE(handle != nullptr, "null handle output");
   Weight w;
   if (int rc = stage_weight(d, host_kn, dtype, K, N, &w)) return rc;
-  *handle = d->next_handle++;
-  d->weights[*handle] = w;
-  return NEBW_OK;
+  const int rc = keep_staged(d, d->weights, w, handle);
+  if (rc) cudaFree(w.ptr);
+  return rc;
 }
 
 extern "C" int nebw_release_weight(nebw_dev *d, uint64_t handle) {
   if (int rc = use_dev(d)) return rc;
-  auto it = d->weights.find(handle);
-  auto it8 = d->weights_i8.find(handle);
-  auto itx = d->experts.find(handle);
-  auto itr = d->ropes.find(handle);
-  NEBW_REQUIRE(it != d->weights.end() || it8 != d->weights_i8.end() || itx != d->experts.end() ||
-                   itr != d->ropes.end(),
-               "unknown weight handle %llu", static_cast<unsigned long long>(handle));
+  const Weight *w = find_staged(d, d->weights, handle);
+  const WeightI8 *w8 = find_staged(d, d->weights_i8, handle);
+  const Experts *x = find_staged(d, d->experts, handle);
+  const RopeTable *r = find_staged(d, d->ropes, handle);
+  NEBW_REQUIRE(w || w8 || x || r, "unknown weight handle %llu",
+               static_cast<unsigned long long>(handle));
   NEBW_CUDA(cudaStreamSynchronize(d->stream));
-  if (it != d->weights.end()) {
-    cudaFree(it->second.ptr);
-    d->weights.erase(it);
-  } else if (itx != d->experts.end()) {
-    cudaFree(itx->second.ptr);
-    d->experts.erase(itx);
-  } else if (itr != d->ropes.end()) {
-    cudaFree(itr->second.table);
-    d->ropes.erase(itr);
-  } else {
-    cudaFree(it8->second.ptr);
-    d->weights_i8.erase(it8);
+  void *memory = w ? static_cast<void *>(w->ptr)
+                 : x ? static_cast<void *>(x->ptr)
+                 : r ? static_cast<void *>(r->table) : static_cast<void *>(w8->ptr);
+  {
+    std::lock_guard<std::mutex> lock(d->staged);
+    d->weights.erase(handle);  // (in one of them)
+    d->weights_i8.erase(handle);
+    d->experts.erase(handle);
+    d->ropes.erase(handle);
   }
+  cudaFree(memory);
   return NEBW_OK;
 }
 
@@ -1003,10 +1024,9 @@ extern "C" int nebw_gemm(nebw_dev *d, uint64_t weight, const void *A, int64_t M,
                          int64_t N, const float *bias, const float *residual, int act, void *C,
                          int c_dtype, void *stream) {
   if (int rc = use_dev(d)) return rc;
-  auto it = d->weights.find(weight);
-  NEBW_REQUIRE(it != d->weights.end(), "unknown weight handle %llu",
-               static_cast<unsigned long long>(weight));
-  const Weight &w = it->second;
+  const Weight *staged = find_staged(d, d->weights, weight);
+  NEBW_REQUIRE(staged, "unknown weight handle %llu", static_cast<unsigned long long>(weight));
+  const Weight &w = *staged;
   NEBW_REQUIRE(K == w.K && N == w.N, "GEMM [M, %lld] x [%lld, %lld] does not match the staged "
                "weight [K=%lld, N=%lld]", static_cast<long long>(K), static_cast<long long>(K),
                static_cast<long long>(N), static_cast<long long>(w.K), static_cast<long long>(w.N));
@@ -1149,20 +1169,18 @@ extern "C" int nebw_stage_weight_i8(nebw_dev *d, const int8_t *host_kn, int64_t 
   NEBW_REQUIRE(host_kn && handle, "null argument");
   WeightI8 w;
   if (int rc = stage_i8(host_kn, K, N, w)) return rc;
-  const uint64_t h = d->next_handle++;
-  d->weights_i8[h] = w;
-  *handle = h;
-  return NEBW_OK;
+  const int rc = keep_staged(d, d->weights_i8, w, handle);
+  if (rc) cudaFree(w.ptr);
+  return rc;
 }
 
 extern "C" int nebw_gemm_i8_ex(nebw_dev *d, uint64_t weight, const int8_t *A, const float *sa,
                                int64_t M, int64_t K, int64_t N, const float *ws, const float *bias,
                                int act, void *C, int c_dtype, void *stream) {
   if (int rc = use_dev(d)) return rc;
-  auto it = d->weights_i8.find(weight);
-  NEBW_REQUIRE(it != d->weights_i8.end(), "unknown int8 weight handle %llu",
-               static_cast<unsigned long long>(weight));
-  const WeightI8 &w = it->second;
+  const WeightI8 *staged = find_staged(d, d->weights_i8, weight);
+  NEBW_REQUIRE(staged, "unknown int8 weight handle %llu", static_cast<unsigned long long>(weight));
+  const WeightI8 &w = *staged;
   NEBW_REQUIRE(K == w.K && N == w.N, "int8 GEMM [%lld x %lld] . [%lld x %lld] mismatch",
                static_cast<long long>(M), static_cast<long long>(K),
                static_cast<long long>(w.K), static_cast<long long>(w.N));

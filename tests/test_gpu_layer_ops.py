@@ -1464,3 +1464,65 @@ def test_two_threads_on_two_streams_at_once(device):
     for i in range(2):
         assert torch.equal(outs[i], outs[2 + i]) and torch.equal(rs[i].off, rs[2 + i].off)
     device.release_weight(h)
+
+
+def test_staging_beside_running_operators(device):
+    """One thread stages and releases tables and expert weights while two others
+    look their own up: each has what it staged."""
+    import threading
+
+    import nebw
+    rows, E, H, N, hd = 200, 4, 128, 128, 64
+    w = torch.randn(E, H, N, generator=gen(51), device="cuda").bfloat16()
+    a = torch.randn(rows, H, generator=gen(52), device="cuda").bfloat16()
+    off = torch.from_numpy(groups([50, 0, 100, 50])).cuda()
+    x = torch.randn(rows, 2 * hd, generator=gen(53), device="cuda").bfloat16()
+    pos = torch.arange(rows, device="cuda").int()
+    inv, _ = nebw.rope_freqs(10000.0, hd)
+    table, experts = device.stage_rope(inv, rows), device.stage_experts(w)
+    outs = [[torch.empty(rows, N, dtype=torch.bfloat16, device="cuda"), torch.empty_like(x)]
+            for _ in range(3)]
+    sides = [nebw.Heads.of(x, 2, out=o[1]) for o in outs]
+
+    def run(i, stream=None):
+        device.gemm_grouped(experts, a, rows, off, rows, H, N, outs[i][0], stream=stream)
+        device.rope(sides[i], None, rows, hd, table, pos, stream=stream)
+
+    run(2)
+    torch.cuda.synchronize()
+    stop, errors, seen = threading.Event(), [], set()
+
+    def work(i, stream):
+        try:
+            for _ in range(400):
+                run(i, stream)
+            stream.synchronize()
+        except Exception as e:  # pragma: no cover - the assertion below reports it
+            errors.append(e)
+
+    def stage():
+        try:
+            while not stop.is_set():
+                new = [device.stage_rope(inv, 64) for _ in range(3)]
+                new.append(device.stage_experts(np.zeros((1, 64, 64), np.float32)))
+                seen.update(new)
+                for h in new:
+                    device.release_weight(h)
+        except Exception as e:  # pragma: no cover
+            errors.append(e)
+
+    workers = [threading.Thread(target=work, args=(i, torch.cuda.Stream())) for i in range(2)]
+    stager = threading.Thread(target=stage)
+    for t in workers + [stager]:
+        t.start()
+    for t in workers:
+        t.join()
+    stop.set()
+    stager.join()
+    torch.cuda.synchronize()
+    device.sync()
+    assert not errors and seen and not seen & {table, experts}
+    for i in range(2):
+        assert torch.equal(outs[i][0], outs[2][0]) and torch.equal(outs[i][1], outs[2][1])
+    device.release_weight(table)
+    device.release_weight(experts)
