@@ -403,6 +403,7 @@ class Device:
 
     def release_weight(self, handle: int):
         _check(lib().nebw_release_weight(self.h, handle))
+        self._experts.pop(handle, None)
 
     def gemm(self, weight, A, M, K, N, C_out, bias=None, residual=None, act=ACT_NONE,
              c_dtype=BF16, stream=None):

@@ -157,6 +157,34 @@ def test_null_device_is_refused_by_name():
         assert "null device handle" in L.nebw_last_error().decode(), name
 
 
+def test_released_experts_are_forgotten(monkeypatch):
+    """What the handle's object knows of an expert weight goes with it."""
+    import nebw
+
+    class Lib:
+        rc = 0
+
+        def nebw_release_weight(self, h, handle):
+            return self.rc
+
+        def nebw_last_error(self):
+            return b"unknown weight handle"
+
+    stub = Lib()
+    monkeypatch.setattr(nebw, "lib", lambda: stub)
+    d = nebw.Device.__new__(nebw.Device)
+    d.h, d.index, d._experts = None, 0, {3: (2, 64, 64, 64), 4: (2, 64, 64, 64)}
+    d.release_weight(3)
+    assert list(d._experts) == [4]
+    d.release_weight(9)  # of another kind
+    stub.rc = 1
+    with pytest.raises(nebw.NebwError):
+        d.release_weight(4)
+    assert list(d._experts) == [4]
+    stub.rc = 0
+    d.release_weight(4)
+
+
 def test_positions_say_how_many_they_are():
     """An address alone does not: nothing may be written without a bound."""
     import nebw
