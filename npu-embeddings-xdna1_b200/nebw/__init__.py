@@ -461,7 +461,7 @@ class Device:
 
     def _heads_dtype(self, q, k, dtype, rows, head_dim):
         """The dtype of heads made by Heads.of, which must hold the rows and
-        the elements a head, or the one given."""
+        have head_dim elements each, or the one given."""
         for h in (q, k):
             d = getattr(h, "dtype", None)
             if d is not None:
@@ -472,6 +472,9 @@ class Device:
                 if rows > h.rows or h.heads * head_dim > h.width:
                     raise ValueError(f"{rows} rows of {h.heads} x {head_dim} in heads of "
                                      f"[{h.rows}, {h.width}]")
+                if h.heads * head_dim < h.width:  # (a norm's weights have their length too)
+                    raise NebwError(1, f"heads of {h.width // h.heads} elements are more than "
+                                       f"head_dim {head_dim}")
                 dtype = d
         return BF16 if dtype is None else dtype
 

@@ -216,6 +216,23 @@ def test_heads_of_refuses_what_it_cannot_describe():
         nebw.Heads.of(x.double(), 2)
 
 
+@pytest.mark.parametrize("heads,head_dim", [(2, 32), (2, 16), (1, 48), (4, 14)])
+def test_heads_of_another_width_are_refused(heads, head_dim):
+    """Heads made for one width are not read as so many narrower ones, with the
+    first part of a norm's weights."""
+    torch = pytest.importorskip("torch")
+    import nebw
+    side = nebw.Heads.of(torch.zeros(4, 96), heads, gamma=torch.ones(96 // heads))
+    side.gpu = 0
+    d = nebw.Device.__new__(nebw.Device)
+    d.h, d.index = None, 0
+    assert d._heads_dtype(side, None, None, 4, 96 // heads) == nebw.F32
+    for q, k in ((side, None), (None, side)):
+        with pytest.raises(nebw.NebwError, match=f"head_dim {head_dim}") as e:
+            d._heads_dtype(q, k, None, 4, head_dim)
+        assert e.value.code == 1
+
+
 def test_operands_of_another_gpu_or_too_few_are_refused():
     """The argument checks of the device calls, on a handle without a device
     and tensors that only say where they are."""
