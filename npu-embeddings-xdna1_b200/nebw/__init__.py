@@ -30,6 +30,7 @@ POOL_MEAN, POOL_CLS = 0, 1
 ROPE_HALF, ROPE_PAIRS = 0, 1
 HEADNORM_NONE, HEADNORM_RMS, HEADNORM_LAYER = 0, 1, 2
 ROUTE_SOFTMAX, ROUTE_SIGMOID = 0, 1
+MAX_TOP_K = 16  # experts of a row
 
 
 class NebwError(RuntimeError):
@@ -294,11 +295,12 @@ class Device:
             return _stream(torch.cuda.current_stream(self.index))
         return None
 
-    def _typed(self, x, name: str, n: int = 0):
+    def _typed(self, x, name: str, n: int = 0, width: int = 0):
         """Device address of n contiguous values of a dtype: a torch tensor of
         another dtype, with gaps, in host memory, on another GPU or with fewer
         values is refused (its bytes would be read as other numbers, or what
-        lies behind them)."""
+        lies behind them), and so are rows of another width, if one is given
+        (they would be read as rows of that width)."""
         if x is None or isinstance(x, int):
             return x
         import torch
@@ -307,27 +309,36 @@ class Device:
             raise TypeError(f"contiguous {name} values on the handle's GPU are required")
         if x.numel() < n:
             raise ValueError(f"{x.numel()} {name} values where {n} are read or written")
+        if width:
+            self._wide(x, width)
         return x.data_ptr()
 
-    # The two below are _typed without its lookups (a short call has half a
-    # dozen of them).
-    def _i32(self, x, n: int = 0):
-        if x is None or x.__class__ is int:
-            return x
-        if (x.dtype is _INT32 and x.get_device() == self.index and x.is_contiguous()
-                and x.numel() >= n):
-            return x.data_ptr()
-        _torch_dtypes()
-        return self._typed(x, "int32", n)
+    @staticmethod
+    def _wide(x, width: int):
+        if x.dim() > 1 and x.size(-1) != width:
+            raise ValueError(f"rows of {x.size(-1)} values where they are of {width}")
 
-    def _f32(self, x, n: int = 0):
+    # The two below are _typed without its lookups (a short call has half a
+    # dozen of them), and without a look at the width of exactly n values.
+    def _i32(self, x, n: int = 0, width: int = 0):
         if x is None or x.__class__ is int:
             return x
-        if (x.dtype is _FLOAT32 and x.get_device() == self.index and x.is_contiguous()
-                and x.numel() >= n):
-            return x.data_ptr()
+        if x.dtype is _INT32 and x.get_device() == self.index and x.is_contiguous():
+            have = x.numel()
+            if have == n or (have > n and not width):
+                return x.data_ptr()
         _torch_dtypes()
-        return self._typed(x, "float32", n)
+        return self._typed(x, "int32", n, width)
+
+    def _f32(self, x, n: int = 0, width: int = 0):
+        if x is None or x.__class__ is int:
+            return x
+        if x.dtype is _FLOAT32 and x.get_device() == self.index and x.is_contiguous():
+            have = x.numel()
+            if have == n or (have > n and not width):
+                return x.data_ptr()
+        _torch_dtypes()
+        return self._typed(x, "float32", n, width)
 
     def close(self):
         if self.h:
@@ -528,11 +539,12 @@ class Device:
             raise TypeError("logits and a contiguous workspace on the handle's GPU are required")
         stride = logits.stride(0) if rows > 1 else experts  # one row: torch may give any
         n = rows * top_k
+        wide = top_k if 0 < top_k <= min(MAX_TOP_K, experts) else 0  # others are refused below
         _check(lib().nebw_moe_route(self.h, logits.data_ptr(), _dtype(logits), stride, rows,
                                     self._i32(rows_dev, 1), experts, top_k, score, int(renorm),
-                                    scale, self._i32(ids, n), self._f32(weights, n),
+                                    scale, self._i32(ids, n, wide), self._f32(weights, n, wide),
                                     self._i32(group_off, experts + 1), self._i32(row_src, n),
-                                    self._i32(row_dst, n), workspace.data_ptr(),
+                                    self._i32(row_dst, n, wide), workspace.data_ptr(),
                                     workspace.numel() * workspace.element_size(),
                                     self._s(stream)))
 
@@ -541,29 +553,39 @@ class Device:
         """One product per expert over its group of rows (nebw_gemm_grouped)."""
         # (a handle that is not there is refused below)
         e, k, n, width = self._experts.get(weight, (0, 0, 0, 0))
-        out = self._typed(C_out, "bfloat16" if c_dtype == BF16 else "float32", rows * width)
-        _check(lib().nebw_gemm_grouped(self.h, weight, self._typed(A, "bfloat16", a_rows * k),
-                                       a_rows, self._i32(row_src, rows),
-                                       self._i32(group_off, e + 1), rows, K, N,
-                                       self._f32(bias, e * n), act, out, c_dtype,
-                                       self._s(stream)))
+        try:
+            out = self._typed(C_out, "bfloat16" if c_dtype == BF16 else "float32", rows * width,
+                              width)
+            A = self._typed(A, "bfloat16", a_rows * k, k)
+            bias = self._f32(bias, e * n, n)
+        except ValueError:
+            # what the library refuses without the operands is said first
+            _check(lib().nebw_gemm_grouped(self.h, weight, None, 0, None, None, 0, K, N, None, act,
+                                           None, c_dtype, None))
+            raise
+        _check(lib().nebw_gemm_grouped(self.h, weight, A, a_rows, self._i32(row_src, rows),
+                                       self._i32(group_off, e + 1), rows, K, N, bias, act, out,
+                                       c_dtype, self._s(stream)))
 
     def moe_combine(self, y, row_dst, weights, rows, top_k, H, out, residual=None, rows_dev=None,
                     stream=None):
-        """The experts' rows y (torch, [places, H]) weighted and summed per
-        row (nebw_moe_combine)."""
+        """The experts' rows y (torch, [.., H]) weighted and summed per row
+        (nebw_moe_combine)."""
         if (y.get_device() != self.index or out.get_device() != self.index
                 or not (y.is_contiguous() and out.is_contiguous())):
             raise TypeError("contiguous expert rows and output on the handle's GPU are required")
-        y_rows, n = y.shape[0], rows * top_k
-        if y.numel() < y_rows * H or out.numel() < rows * H:
-            raise ValueError(f"expert rows {tuple(y.shape)} and output {tuple(out.shape)} for "
-                             f"{rows} rows of {H}")
+        y_rows, n = y.numel() // H if H > 0 else 0, rows * top_k
+        if H > 0:  # (other widths are refused below)
+            self._wide(y, H)
+            self._wide(out, H)
+            if out.numel() < rows * H:
+                raise ValueError(f"output {tuple(out.shape)} for {rows} rows of {H}")
+        wide = top_k if 0 < top_k <= MAX_TOP_K else 0
         _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y_rows,
-                                      self._i32(row_dst, n), self._f32(weights, n), rows,
-                                      self._i32(rows_dev, 1), top_k, H,
-                                      self._f32(residual, rows * H), out.data_ptr(), _dtype(out),
-                                      self._s(stream)))
+                                      self._i32(row_dst, n, wide), self._f32(weights, n, wide),
+                                      rows, self._i32(rows_dev, 1), top_k, H,
+                                      self._f32(residual, rows * H, H), out.data_ptr(),
+                                      _dtype(out), self._s(stream)))
 
 
 ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3, "bands": 4}

@@ -216,6 +216,78 @@ def test_heads_of_refuses_what_it_cannot_describe():
         nebw.Heads.of(x.double(), 2)
 
 
+@pytest.fixture
+def host_calls(monkeypatch):
+    """A handle whose checks take host tensors, and the library calls that pass
+    them (each answered with success)."""
+    torch = pytest.importorskip("torch")
+    import nebw
+
+    class Lib:
+        calls = []
+
+        def __getattr__(self, name):
+            return lambda *args: self.calls.append((name, args)) or 0
+
+    stub = Lib()
+    stub.calls = []
+    monkeypatch.setattr(nebw, "lib", lambda: stub)
+    d = nebw.Device.__new__(nebw.Device)
+    # a host tensor's device number
+    d.h, d.index, d._raw_stream, d.torch_stream = None, torch.zeros(1).get_device(), None, False
+    d._experts = {}
+    return d, stub.calls
+
+
+def test_rows_of_another_width_are_refused(host_calls):
+    """Rows wider than the call says would be read, or written, at the wrong
+    places; other shapes with as many values a row are fine."""
+    torch = pytest.importorskip("torch")
+    import nebw
+    d, calls = host_calls
+    bf, i32 = torch.bfloat16, torch.int32
+    dst, w = torch.zeros(4, 2, dtype=i32), torch.zeros(4, 2)
+
+    def combine(y=torch.zeros(8, 64, dtype=bf), dst=dst, w=w, out=torch.zeros(4, 64), **kw):
+        d.moe_combine(y, dst, w, 4, 2, 64, out, **kw)
+
+    combine()
+    assert calls[-1][1][3] == 8
+    combine(y=torch.zeros(2, 8, 64, dtype=bf), dst=dst.flatten(), w=w.flatten(),
+            out=torch.zeros(5 * 64), residual=torch.zeros(1, 4, 64))
+    assert calls[-1][1][3] == 16  # all of its rows
+    for bad in (dict(y=torch.zeros(8, 96, dtype=bf)), dict(out=torch.zeros(4, 128)),
+                dict(residual=torch.zeros(4, 65)), dict(dst=torch.zeros(4, 3, dtype=i32)),
+                dict(w=torch.zeros(4, 4))):
+        with pytest.raises(ValueError):
+            combine(**bad)
+    d._experts[7] = (2, 64, 128, 64)  # gated
+
+    def grouped(a=torch.zeros(4, 64, dtype=bf), out=torch.zeros(4, 64, dtype=bf), bias=None):
+        d.gemm_grouped(7, a, 4, torch.zeros(3, dtype=i32), 4, 64, 128, out, bias=bias)
+
+    grouped()
+    grouped(torch.zeros(2, 3, 64, dtype=bf), torch.zeros(500, dtype=bf), torch.zeros(2, 128))
+    for bad in (dict(a=torch.zeros(4, 72, dtype=bf)), dict(out=torch.zeros(4, 128, dtype=bf)),
+                dict(bias=torch.zeros(2, 192))):
+        with pytest.raises(ValueError):
+            grouped(**bad)
+
+    def route(ids=dst, w=w, dst=dst):
+        d.moe_route(torch.zeros(4, 8), 4, 8, 2, ids, w, torch.zeros(9, dtype=i32),
+                    torch.zeros(8, dtype=i32), dst, torch.zeros(0))
+
+    route()
+    route(torch.zeros(9, 2, dtype=i32), torch.zeros(20), torch.zeros(4, 2, dtype=i32))
+    for bad in (dict(ids=torch.zeros(4, 4, dtype=i32)), dict(w=torch.zeros(4, 3)),
+                dict(dst=torch.zeros(4, 8, dtype=i32))):
+        with pytest.raises(ValueError):
+            route(**bad)
+    # (a refused product asked the library first, about no rows)
+    assert [a[6] for n, a in calls if n == "nebw_gemm_grouped"] == [4, 4, 0, 0, 0]
+    assert len(calls) == 9
+
+
 @pytest.mark.parametrize("heads,head_dim", [(2, 32), (2, 16), (1, 48), (4, 14)])
 def test_heads_of_another_width_are_refused(heads, head_dim):
     """Heads made for one width are not read as so many narrower ones, with the
