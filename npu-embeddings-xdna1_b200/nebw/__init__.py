@@ -529,13 +529,17 @@ class Device:
                   stream=None):
         """The top_k experts of each row of logits (a 2-D fp32 / bf16 torch
         tensor, its row stride kept) and the rows grouped by expert
-        (nebw_moe_route)."""
+        (nebw_moe_route).  workspace: a tensor of moe_route_workspace bytes,
+        or None where that is 0."""
         if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < experts:
             raise ValueError("logits are rows of at least `experts` adjacent values")
         if logits.shape[0] < rows:
             raise ValueError("fewer logit rows than rows")
-        if (logits.get_device() != self.index or workspace.get_device() != self.index
-                or not workspace.is_contiguous()):
+        ws, ws_bytes = None, 0
+        if workspace is not None:
+            ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        if (logits.get_device() != self.index or ws_bytes
+                and (workspace.get_device() != self.index or not workspace.is_contiguous())):
             raise TypeError("logits and a contiguous workspace on the handle's GPU are required")
         stride = logits.stride(0) if rows > 1 else experts  # one row: torch may give any
         n = rows * top_k
@@ -544,8 +548,7 @@ class Device:
                                     self._i32(rows_dev, 1), experts, top_k, score, int(renorm),
                                     scale, self._i32(ids, n, wide), self._f32(weights, n, wide),
                                     self._i32(group_off, experts + 1), self._i32(row_src, n),
-                                    self._i32(row_dst, n, wide), workspace.data_ptr(),
-                                    workspace.numel() * workspace.element_size(),
+                                    self._i32(row_dst, n, wide), ws, ws_bytes,
                                     self._s(stream)))
 
     def gemm_grouped(self, weight, A, a_rows, group_off, rows, K, N, C_out, row_src=None,

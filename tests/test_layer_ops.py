@@ -288,6 +288,24 @@ def test_rows_of_another_width_are_refused(host_calls):
     assert len(calls) == 9
 
 
+def test_route_without_a_workspace(host_calls):
+    """A call that needs no workspace takes none."""
+    torch = pytest.importorskip("torch")
+    import nebw
+    d, calls = host_calls
+    i32 = torch.int32
+    outs = (torch.zeros(4, 2, dtype=i32), torch.zeros(4, 2), torch.zeros(9, dtype=i32),
+            torch.zeros(8, dtype=i32), torch.zeros(4, 2, dtype=i32))
+    for ws, want in ((None, (None, 0)), (torch.zeros(0), (0, 0))):
+        d.moe_route(torch.zeros(4, 8), 4, 8, 2, *outs, ws)
+        assert calls[-1][1][-3:-1] == want
+    ws = torch.zeros(12, 2)
+    d.moe_route(torch.zeros(4, 8), 4, 8, 2, *outs, ws)
+    assert calls[-1][1][-3:-1] == (ws.data_ptr(), 96)
+    with pytest.raises(TypeError):
+        d.moe_route(torch.zeros(4, 8), 4, 8, 2, *outs, ws.t())
+
+
 @pytest.mark.parametrize("heads,head_dim", [(2, 32), (2, 16), (1, 48), (4, 14)])
 def test_heads_of_another_width_are_refused(heads, head_dim):
     """Heads made for one width are not read as so many narrower ones, with the
