@@ -293,7 +293,9 @@ int nebw_row_positions(nebw_dev *dev, const int32_t *seq_off, const int32_t *seq
  * elements at x + r * stride + h * head_dim (stride in elements: 3H for the Q
  * or K block of a Q|K|V row).  The results go to out in the same manner: out
  * == x with out_stride == stride works in place, otherwise the two must not
- * overlap.  Query and key head counts are independent. */
+ * overlap, nor may one side's results and the other's heads or results (where
+ * their strides are equal, as in Q|K|V rows, that is refused).  Query and key
+ * head counts are independent. */
 typedef struct nebw_heads {
   const void *x;
   void *out;
@@ -387,7 +389,8 @@ int nebw_gemm_grouped(nebw_dev *dev, uint64_t weight, const void *A, int64_t a_r
  * in row order, bf16 or fp32.  row_dst < 0 adds nothing and reads nothing;
  * row_dst >= y_rows is an NEBW_EDEVICE error at the next sync (and adds
  * nothing).  residual [rows, H] fp32 (NULL: none) may be out itself where out
- * is fp32.  rows_dev as in nebw_moe_route. */
+ * is fp32; otherwise out must not overlap it, nor y.  rows_dev as in
+ * nebw_moe_route. */
 int nebw_moe_combine(nebw_dev *dev, const void *y, int y_dtype, int64_t y_rows,
                      const int32_t *row_dst, const float *weights, int64_t rows,
                      const int32_t *rows_dev, int32_t top_k, int64_t H, const float *residual,

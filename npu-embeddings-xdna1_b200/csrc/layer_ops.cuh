@@ -14,6 +14,31 @@ bool words(const P *...p) {
   return (aligned(p, 4) && ...);
 }
 
+// Whether two pieces of memory (na, nb bytes) meet.
+bool meet(const void *a, int64_t na, const void *b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && x < y + nb && y < x + na;
+}
+
+// Whether any two rows of two blocks of `rows` rows meet: wa and wb bytes a
+// row, sa and sb from one to the next.  Blocks of one stride may interleave
+// (Q and K of Q|K|V rows); blocks of two strides that reach into one another
+// are taken to be apart.
+bool rows_meet(const void *a, int64_t sa, int64_t wa, const void *b, int64_t sb, int64_t wb,
+               int64_t rows) {
+  if (rows <= 1) return meet(a, wa, b, wb);
+  if (sa != sb) return false;
+  // row i of b lies d bytes behind row i + by of a, and before the next one
+  const int64_t off = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b) -
+                                           reinterpret_cast<uintptr_t>(a));
+  int64_t by = off / sa, d = off % sa;
+  if (d < 0) {
+    --by;
+    d += sa;
+  }
+  return (d < wa && std::abs(by) < rows) || (d + wb > sa && std::abs(by + 1) < rows);
+}
+
 // Host or this device's memory; *on_device says which.
 int where_is(nebw_dev *d, const void *p, bool *on_device) {
   cudaPointerAttributes a;
@@ -366,6 +391,19 @@ int run_heads(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype, 
   if (int rc = check_heads(k, "key", head_dim, rows, esz, norm, &a.k)) return rc;
   NEBW_REQUIRE(a.q.heads + a.k.heads > 0, "no heads given");
   NEBW_REQUIRE(words(rows_dev), "the live row count is not aligned");
+  const auto apart = [&](const nebw::HeadSide &s, bool out_s, const nebw::HeadSide &t) {
+    // s's rows (read or written) and t's written ones
+    const int64_t e = static_cast<int64_t>(esz), w = head_dim * e;
+    return s.heads == 0 || t.heads == 0 ||
+           !rows_meet(out_s ? s.out : s.x, (out_s ? s.out_stride : s.stride) * e, s.heads * w,
+                      t.out, t.out_stride * e, t.heads * w, rows);
+  };
+  if (rows > 0) {
+    NEBW_REQUIRE(a.q.x == a.q.out || apart(a.q, false, a.q), "query heads overlap their results");
+    NEBW_REQUIRE(a.k.x == a.k.out || apart(a.k, false, a.k), "key heads overlap their results");
+    NEBW_REQUIRE(apart(a.q, false, a.k) && apart(a.k, false, a.q) && apart(a.q, true, a.k),
+                 "query and key heads overlap");
+  }
   if (rows == 0) return NEBW_OK;
   a.rows = rows;
   a.rows_dev = rows_dev;
@@ -672,6 +710,9 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   NEBW_REQUIRE(aligned(A, 16) && aligned(C, 16) && aligned(bias, 16),
                "grouped operands must be 16-byte aligned");
   NEBW_REQUIRE(words(group_off, row_src), "group offsets or row indices are not aligned");
+  const int64_t c_bytes = rows * (w.gated ? N / 2 : N) * (c_dtype == NEBW_F32 ? 4 : 2);
+  NEBW_REQUIRE(!meet(A, a_rows * K * 2, C, c_bytes),
+               "a grouped product's output overlaps its rows");
   nebw::GroupedArgs a{};
   a.off = group_off;
   a.experts = w.experts;
@@ -746,6 +787,12 @@ extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t
                    aligned(out, out_dtype == NEBW_F32 ? 4 : 2) &&
                    words(row_dst, weights, residual, rows_dev),
                "combine operands are not aligned");
+  const int64_t out_bytes = rows * H * (out_dtype == NEBW_F32 ? 4 : 2);
+  NEBW_REQUIRE(!meet(y, y_rows * H * (y_dtype == NEBW_F32 ? 4 : 2), out, out_bytes),
+               "the combine's output overlaps the experts' rows");
+  NEBW_REQUIRE((residual == out && out_dtype == NEBW_F32) ||
+                   !meet(residual, residual ? rows * H * 4 : 0, out, out_bytes),
+               "the combine's output overlaps its residual");
   nebw::CombineArgs a{};
   a.y = y;
   a.row_dst = row_dst;

@@ -1104,6 +1104,76 @@ def test_operands_off_their_values_boundaries_are_refused(device):
     device.release_weight(w)
 
 
+def test_results_over_what_is_still_read_are_refused(device):
+    """Blocks run in no order: results may lie on their own operand, or beside
+    everything that another block reads or writes, and nowhere between."""
+    import nebw
+    rows, hd = 5, 64
+    buf = torch.zeros(40, 6 * hd, dtype=torch.bfloat16, device="cuda")
+    inv, _ = nebw.rope_freqs(10000.0, hd)
+    table = device.stage_rope(inv, 64)
+    pos = torch.arange(40, device="cuda").int()
+
+    def heads(at, n=1, out=None, rows=rows):
+        v = [buf.flatten()[i:i + rows * 6 * hd].view(rows, 6 * hd)[:, :n * hd]
+             for i in (at, at if out is None else out)]
+        return nebw.Heads.of(v[0], n, out=v[1])
+
+    wide = 6 * hd
+    fine = [  # query, key (offsets of their first elements, heads, offsets of the results)
+        (heads(0, 2), heads(2 * hd, 2)), (heads(0, 2, 4 * hd), heads(2 * hd, 2)),
+        (heads(0, 2, wide * rows), heads(2 * hd, 2, wide * rows + 2 * hd)),
+        (heads(wide, 3, 3 * hd), None), (heads(0, 3, wide * 2 + 3 * hd), None),
+        (heads(wide * rows, 1, 0), heads(hd, 1)),
+    ]
+    bad = [
+        (heads(0, 2, hd), None), (heads(hd, 2, 0), None), (heads(0, 2, wide), None),
+        (heads(wide * 2, 2, 0), None), (heads(0, 1, wide - hd + 8), heads(0, 2, wide * 20)),
+        (heads(0, 2), heads(0, 2)), (heads(0, 2), heads(hd, 2)),
+        (heads(0, 2, wide * 10), heads(4 * hd, 2, wide * 10)),
+        (heads(0, 2, 4 * hd), heads(4 * hd, 2, wide * 10)),
+        (heads(2 * hd, 4, wide * 10 + 2 * hd), heads(0, 2, wide * 11 - 2 * hd)),
+    ]
+    for q, k in fine:
+        device.rope(q, k, rows, hd, table, pos)
+    for q, k in bad:
+        for a, b in ((q, k), (k, q)):
+            with pytest.raises(nebw.NebwError, match="overlap") as e:
+                device.rope(a, b, rows, hd, table, pos)
+            assert e.value.code == 1
+    one = [nebw.Heads.of(buf[i:i + 1, :2 * hd], 2) for i in (0, 1)]
+    device.rope(*one, 1, hd, table, pos)  # a row each
+    with pytest.raises(nebw.NebwError, match="overlap"):
+        device.rope(one[0], nebw.Heads.of(buf[:1, hd:3 * hd], 2), 1, hd, table, pos)
+    device.release_weight(table)
+
+    E, K, N, M = 1, 64, 64, 16
+    w = device.stage_experts(np.zeros((E, K, N), np.float32))
+    flat = torch.zeros(4096, dtype=torch.bfloat16, device="cuda")
+    off = torch.tensor([0, M], device="cuda").int()
+    rows_of = lambda i, n: flat[i:i + n * K].view(n, K)  # noqa: E731
+    device.gemm_grouped(w, rows_of(0, M), M, off, M, K, N, rows_of(M * K, M))
+    for i in (0, 64, M * K - 64):
+        with pytest.raises(nebw.NebwError, match="overlap"):
+            device.gemm_grouped(w, rows_of(512, M), M, off, M, K, N, rows_of(512 + i, M))
+        with pytest.raises(nebw.NebwError, match="overlap"):
+            device.gemm_grouped(w, rows_of(512 + i, M), M, off, M, K, N, rows_of(512, M))
+    device.release_weight(w)
+
+    dst, wt = torch.zeros(4, 1, dtype=torch.int32, device="cuda"), torch.zeros(4, 1, device="cuda")
+    y, f = rows_of(0, 8), torch.zeros(1024, device="cuda")
+    device.moe_combine(y, dst, wt, 4, 1, K, rows_of(512, 4))
+    for i in (0, 448):
+        with pytest.raises(nebw.NebwError, match="overlap"):
+            device.moe_combine(y, dst, wt, 4, 1, K, rows_of(i, 4))
+    res = f[256:512].view(4, K)
+    device.moe_combine(y, dst, wt, 4, 1, K, res, residual=res)
+    for out in (f[192:448].view(4, K), f[260:516].view(4, K), res.view(torch.bfloat16).view(8, K)):
+        with pytest.raises(nebw.NebwError, match="overlap"):
+            device.moe_combine(y, dst, wt, 4, 1, K, out, residual=res)
+    device.sync()
+
+
 def test_whole_numbers_of_another_dtype_are_refused(device):
     """int64 indices (torch's default) would be read as other numbers, host
     memory not at all."""
