@@ -36,7 +36,11 @@
 extern "C" {
 #endif
 
+/* VERSION changes with what a function takes, REVISION with functions added
+ * within a version.  Revision 1: the operators of rotary and expert layers.
+ * (Version 5 of the library without nebw_abi_revision is revision 0.) */
 #define NEBW_ABI_VERSION 5
+#define NEBW_ABI_REVISION 1
 
 typedef enum nebw_status {
   NEBW_OK = 0,
@@ -67,6 +71,7 @@ typedef struct nebw_model nebw_model;
 /* Message of the calling thread's last failure ("" if none). */
 const char *nebw_last_error(void);
 int nebw_abi_version(void);
+int nebw_abi_revision(void);
 
 /* ---- device ------------------------------------------------------------
  * Replaces npu::Device (runtime/include/runtime/device.hpp:29-38) and the

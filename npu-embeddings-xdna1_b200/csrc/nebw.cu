@@ -739,6 +739,7 @@ int launch_pack(const int *len_in, int B, int S, int *len_out, int *off, int *er
 
 extern "C" const char *nebw_last_error(void) { return g_last_error.c_str(); }
 extern "C" int nebw_abi_version(void) { return NEBW_ABI_VERSION; }
+extern "C" int nebw_abi_revision(void) { return NEBW_ABI_REVISION; }
 
 template <int BN>
 int set_gemm_i8_attrs() {

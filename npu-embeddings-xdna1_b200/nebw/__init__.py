@@ -23,6 +23,7 @@ REPO_DIR = PKG_DIR.parent
 LIB_PATH = Path(os.environ["NEBW_LIB"]) if os.environ.get("NEBW_LIB") else PKG_DIR / "libnebw.so"
 HEADER_PATH = REPO_DIR / "include" / "nebw.h"
 
+ABI = (5, 1)  # NEBW_ABI_VERSION and _REVISION of include/nebw.h
 F32, BF16 = 0, 1
 ACT_NONE, ACT_GELU8, ACT_GELU_ERF = 0, 1, 2
 GATE_SILU, GATE_GELU_ERF = 0, 1
@@ -110,10 +111,16 @@ def lib() -> C.CDLL:
         raise FileNotFoundError(
             f"{LIB_PATH} is not built; run `python __graft_entry__.py build` (or build()) first")
     L = C.CDLL(str(LIB_PATH))
+    # a library of an earlier build is refused here, not at some later call
+    got = (L.nebw_abi_version(), L.nebw_abi_revision() if hasattr(L, "nebw_abi_revision") else 0)
+    if got[0] != ABI[0] or got[1] < ABI[1]:
+        raise NebwError(1, f"{LIB_PATH} is of another build: ABI {got[0]}.{got[1]}, and "
+                           f"{ABI[0]}.{ABI[1]} is required; run build() again")
     vp, i64, i32 = C.c_void_p, C.c_int64, C.c_int32
     sig = {
         "nebw_last_error": ([], C.c_char_p),
         "nebw_abi_version": ([], C.c_int),
+        "nebw_abi_revision": ([], C.c_int),
         "nebw_open": ([C.c_int, C.POINTER(vp)], C.c_int),
         "nebw_close": ([vp], C.c_int),
         "nebw_sync": ([vp], C.c_int),

@@ -139,6 +139,34 @@ def test_route_workspace():
             nebw.moe_route_workspace(rows, experts, k)
 
 
+def test_a_library_of_an_earlier_build_is_refused(tmp_path, monkeypatch):
+    """One that has the version but not what was added since is refused when it
+    is loaded."""
+    import re
+    import shutil
+    import subprocess
+
+    import nebw
+    text = nebw.HEADER_PATH.read_text()
+    here = tuple(int(re.search(rf"#define NEBW_ABI_{n} (\d+)", text)[1])
+                 for n in ("VERSION", "REVISION"))
+    assert here == nebw.ABI == (nebw.lib().nebw_abi_version(), nebw.lib().nebw_abi_revision())
+    cc = shutil.which("gcc")
+    if not cc:
+        pytest.skip("no C compiler")
+    src = "int nebw_abi_version(void) { return %d; }"
+    newer = src + " int nebw_abi_revision(void) { return %d; }"
+    for i, text in enumerate((src % here[0], newer % (here[0], here[1] - 1),
+                              newer % (here[0] + 1, here[1]))):
+        (tmp_path / f"{i}.c").write_text(text)
+        out = tmp_path / f"lib{i}.so"
+        subprocess.run([cc, "-shared", "-fPIC", "-o", out, tmp_path / f"{i}.c"], check=True)
+        monkeypatch.setattr(nebw, "_lib", None)
+        monkeypatch.setattr(nebw, "LIB_PATH", out)
+        with pytest.raises(nebw.NebwError, match="another build"):
+            nebw.lib()
+
+
 def test_null_device_is_refused_by_name():
     import nebw
     L = nebw.lib()
