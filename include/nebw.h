@@ -239,12 +239,18 @@ int nebw_layernorm_quant(nebw_dev *dev, float *x, const float *y, const float *g
 
 /* ---- rotary positions and norms of the query and key heads ----------------
  * For a maintainer whose encoder rotates other than the model passes do
- * (adjacent pairs, a part of each head, positions past the trained length,
- * few key heads), or norms each query and key head first.  They go between
- * nebw_gemm (Q|K|V) and nebw_attention.  Device buffers, asynchronous on
- * `stream`, no allocation, no workspace: they can be captured in a graph.  No
- * counterpart in the reference, whose one form (rotate-half over the whole
- * head) the QKV epilogue of a rotary model applies. */
+ * (adjacent pairs, a part of each head, positions past the trained length),
+ * or norms each query and key head first.  They go between nebw_gemm (Q|K|V)
+ * and nebw_attention, which takes bf16 rows of as many key as query heads, of
+ * 32 or 64; other heads (fewer key heads, other widths, fp32 rows) are for a
+ * caller's own attention: nothing else in this library reads them.
+ * nebw_attention wants Q times 1/sqrt(head_dim).  nebw_rope keeps what the QKV
+ * operand has folded in; a norm takes it out again, so that its query weights
+ * have to bring it: gamma / sqrt(head_dim), and beta / sqrt(head_dim) for
+ * NEBW_HEADNORM_LAYER.  Device buffers, asynchronous on `stream`, no
+ * allocation, no workspace: they can be captured in a graph.  No counterpart
+ * in the reference, whose one form (rotate-half over the whole head) the QKV
+ * epilogue of a rotary model applies. */
 
 /* Which elements of a head turn together, n = rot_dim / 2: HALF i and n + i,
  * PAIRS 2i and 2i + 1.  Elements from rot_dim on do not turn. */
@@ -326,7 +332,9 @@ int nebw_rope(nebw_dev *dev, const nebw_heads *q, const nebw_heads *k, int dtype
               const int32_t *rows_dev, int32_t head_dim, uint64_t rope, int layout,
               const int32_t *pos, void *stream);
 /* A norm of every query and key head over its head_dim, then the rotation of
- * nebw_rope (rope 0: none, pos may then be NULL), in one pass. */
+ * nebw_rope (rope 0: none, pos may then be NULL), in one pass.  For
+ * nebw_attention q->gamma (and q->beta) are the model's times
+ * 1/sqrt(head_dim). */
 int nebw_qk_norm_rope(nebw_dev *dev, const nebw_heads *q, const nebw_heads *k, int dtype,
                       int64_t rows, const int32_t *rows_dev, int32_t head_dim, int norm,
                       float eps, uint64_t rope, int layout, const int32_t *pos, void *stream);

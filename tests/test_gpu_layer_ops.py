@@ -352,6 +352,59 @@ def test_row_positions_stop_at_the_bound(device):
     assert torch.equal(pos.cpu(), want.int())
 
 
+@pytest.mark.parametrize("heads,hd", [(4, 64), (8, 32)])
+@pytest.mark.parametrize("norm", [1, 2])
+def test_normed_heads_ahead_of_attention(device, heads, hd, norm):
+    """The documented way: the softmax's 1/sqrt(head_dim) in the query norm's
+    weight and bias, the Q|K|V rows in place, then the framework's attention."""
+    import nebw
+    lens = [70, 1, 128, 33]
+    T, H, g = sum(lens), heads * hd, gen(60 + hd + norm)
+    qkv = torch.randn(T, 3 * H, generator=g, device="cuda").bfloat16()
+    gam = [1 + 0.2 * torch.randn(hd, generator=g, device="cuda") for _ in range(2)]
+    bet = [0.3 * torch.randn(hd, generator=g, device="cuda") for _ in range(2)]
+    by = 1.0 / math.sqrt(hd)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    off, pos = torch.empty(5, dtype=torch.int32, device="cuda"), torch.empty_like(qkv[:, 0]).int()
+    device.pack_offsets(n, 4, 128, n, off)
+    device.row_positions(off, n, 4, 128, pos)
+    inv, _ = nebw.rope_freqs(10000.0, hd)
+    table = device.stage_rope(inv, 128)
+    side = [heads_reference(qkv[:, i * H:(i + 1) * H], heads, hd, inv, 1.0, pos, False, norm,
+                            gam[i], bet[i], 1e-6)[0].view(T, heads, hd) for i in range(2)]
+    v = qkv[:, 2 * H:].double().view(T, heads, hd)
+
+    def attention(scale):
+        """ctx in 64 bits, the sum of p |v|, and the most a logit is off."""
+        out, size, most, at = [], [], [], 0
+        for m in lens:
+            s = slice(at, at + m)
+            p = torch.softmax(scale * torch.einsum("qhd,khd->hqk", side[0][s], side[1][s]), -1)
+            terms = scale * torch.einsum("qhd,khd->hqk", side[0][s].abs(), side[1][s].abs())
+            out.append(torch.einsum("hqk,khd->qhd", p, v[s]))
+            size.append(torch.einsum("hqk,khd->qhd", p, v[s].abs()))
+            most.append(terms.amax(-1).t()[:, :, None].expand(m, heads, hd))
+            at += m
+        return [torch.cat(t).reshape(T, H) for t in (out, size, most)]
+
+    q = nebw.Heads.of(qkv[:, :H], heads, gamma=gam[0] * by, beta=bet[0] * by)
+    k = nebw.Heads.of(qkv[:, H:2 * H], heads, gamma=gam[1], beta=bet[1])
+    device.qk_norm_rope(q, k, T, hd, norm=norm, eps=1e-6, rope=table, pos=pos)
+    ctx = torch.empty(T, H, dtype=torch.bfloat16, device="cuda")
+    device.attention(qkv, T, off, n, 4, 128, heads, hd, ctx)
+    device.sync()
+    want, size, most = attention(by)
+    # q and k are rounded to bf16 (2^-8 each of every term of a logit), which moves
+    # a probability and its sum by that exponent each; p is rounded to bf16
+    # (2^-8), the fp32 steps are below a tenth of it, and ctx is rounded
+    tol = (torch.expm1(2 * 2.0 ** -7 * most) + 1.2 * 2.0 ** -8) * size + 2.0 ** -8 * want.abs()
+    assert ((ctx.double() - want).abs() <= tol).all()
+    # without the scale the result would be another one
+    far = (attention(1.0)[0] - want).abs()
+    assert (far > 2 * tol).float().mean() > 0.2
+    device.release_weight(table)
+
+
 @pytest.mark.parametrize("off,lens", [
     ([0, 90], [5, 20]),          # past the end
     ([-3, 40], [5, 20]),         # before the start
