@@ -389,10 +389,18 @@ int nebw_moe_route(nebw_dev *dev, const void *logits, int dtype, int64_t stride,
  * = up * act(gate)), bf16, or fp32 with act NONE; bias [experts, N] fp32 in
  * the container's column order, or NULL; act NEBW_ACT_*, for gated weights
  * NEBW_GATE_*.  rows bounds group_off[experts]; rows of C in no group are
- * left as they are.  Products accumulate in fp32, one rounding.  group_off
- * that falls or leaves [0, rows], or a row_src outside A, is an NEBW_EDEVICE
- * error at the next sync (clamped, so nothing is read out of bounds).  A, C
- * and bias 16-byte aligned; C must not overlap A. */
+ * left as they are.  group_off that falls or leaves [0, rows], or a row_src
+ * outside A, is an NEBW_EDEVICE error at the next sync (clamped, so nothing is
+ * read out of bounds).  A, C and bias 16-byte aligned; C must not overlap A.
+ * Products accumulate in fp32 on the tensor cores, which cut the sum towards
+ * zero once every 16 of K.  bf16 output is rounded once after that.  fp32
+ * output sums K in two parts (four above K 1536, or where rows are 64 an
+ * expert or fewer) and adds them.  Its error against 64 bits, relative and by
+ * norm, as measured: at K 1024, 1536, 2048, 4096, 16384, 65536
+ *   random signs  4.7e-7  7.3e-7  4.7e-7  1.0e-6  4.4e-6  1.9e-5
+ *   one sign      9.0e-7  1.5e-6  8.0e-7  2.2e-6  1.4e-5  8.3e-5
+ * The four parts above K 1536 are of half as many rows a tile: 625 us where
+ * two parts take 413 (65,542 rows, K 4096, N 1024). */
 int nebw_gemm_grouped(nebw_dev *dev, uint64_t weight, const void *A, int64_t a_rows,
                       const int32_t *row_src, const int32_t *group_off, int64_t rows, int64_t K,
                       int64_t N, const float *bias, int act, void *C, int c_dtype, void *stream);

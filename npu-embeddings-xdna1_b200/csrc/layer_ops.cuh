@@ -741,9 +741,10 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   // whole tiles read W once (36.9 against 34.7 us there)
   a.tile_rows = rows <= 64 * std::min<int64_t>(w.experts, rows) ? 128 : 256;
   // fp32 output over a long K: half tiles leave room for four parts of K,
-  // which keeps the error under 1e-6 up to K 4096 (gemm_grouped_kernel).
-  // 65,542 rows, K 4096, N 1024: 625 us and 1.0e-6, whole tiles 413 us and
-  // 2.1e-6; at K 1536 whole tiles are at 7.3e-7.
+  // which halves what is cut off (gemm_grouped_kernel).  Errors of random
+  // signs at K 1536 / 2048 / 4096: two parts of whole tiles 7.3e-7 / 1.0e-6 /
+  // 2.1e-6, four of half ones 3.5e-7 / 4.7e-7 / 1.0e-6, which fp32 sums keep
+  // below 6.1e-7.  It costs 625 us against 413 (65,542 rows, K 4096, N 1024).
   if (c_dtype == NEBW_F32 && K > 1536) a.tile_rows = 128;
   return launch_grouped(d, m, epi, a, pick_stream(d, stream));
 }

@@ -895,6 +895,44 @@ def test_grouped_fp32_output_over_long_products(device, K):
         device.release_weight(h)
 
 
+@pytest.mark.parametrize("signed", [False, True])
+@pytest.mark.parametrize("K,rows,parts", [
+    (1024, 700, 2), (1536, 700, 2), (1544, 700, 4), (2048, 700, 4), (4000, 700, 4),
+    (1024, 60, 4), (2048, 60, 4), (16384, 300, 4)])
+def test_grouped_fp32_output_loses_its_part_of_one_sum(device, K, rows, parts, signed):
+    """P parts of K lose about 1/P of what one accumulator over all of K loses:
+    each step of 16 cuts by a share of the running sum, which in a part is as
+    long on average as its share of the steps, and the adding of P parts is exact
+    next to that.  nebw_gemm keeps one accumulator.  Half the parts would lose
+    twice as much: the bound lies between, at sqrt(2) / P.  Products of one sign,
+    whose cuts all go one way, show it as well."""
+    import nebw
+    N, g = 264, gen(K + rows)
+    a = torch.randn(rows, K, generator=g, device="cuda")
+    w = torch.randn(1, K, N, generator=g, device="cuda") / math.sqrt(K)
+    if signed:
+        a, w = a.abs(), w.abs()
+    a, w = a.bfloat16(), w.bfloat16()
+    want = a.double() @ w[0].double()
+    one = device.stage_weight(w[0].view(torch.int16).cpu().numpy().view(np.uint16))
+    many = device.stage_experts(w)
+    lost = []
+    for grouped in (False, True):
+        c = torch.empty(rows, N, device="cuda")
+        if grouped:
+            device.gemm_grouped(many, a, rows, torch.tensor([0, rows], device="cuda").int(), rows, K,
+                                N, c, c_dtype=nebw.F32)
+        else:
+            device.gemm(one, a, rows, K, N, c, c_dtype=nebw.F32)
+        device.sync()
+        lost.append(((c.double() - want).norm() / want.norm()).item())
+    assert lost[1] < math.sqrt(2) / parts * lost[0], lost
+    # and one unit of the running sum a step at most
+    assert lost[1] < K / (16 * parts) * 2.0 ** -23, lost
+    device.release_weight(one)
+    device.release_weight(many)
+
+
 def test_grouped_product_of_more_tiles_than_are_looked_up(device):
     """512 experts of a row each, 19 column tiles: over 128 tiles a block."""
     E, K, N = 512, 64, 4864
