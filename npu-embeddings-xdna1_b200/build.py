@@ -20,10 +20,10 @@ from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
-SOURCES = ["csrc/nebw.cu", "csrc/npue_file.cpp", "csrc/npue_pack.cpp"]
+SOURCES = ["csrc/nebw.cu", "csrc/layer_kernels.cu", "csrc/npue_file.cpp", "csrc/npue_pack.cpp"]
 # every header the library includes: a change to any of them rebuilds it
 DEPS = SOURCES + sorted(str(p.relative_to(PKG)) for p in (PKG / "csrc").glob("*.cuh")) + [
-    "csrc/npue_file.h", "csrc/npue_pack.h", "../include/nebw.h"]
+    "csrc/layer_kernels.h", "csrc/npue_file.h", "csrc/npue_pack.h", "../include/nebw.h"]
 NVCC_FLAGS = ["-std=c++17", "-O3", "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo",
               "-Xcompiler", "-fPIC", "-shared"]
 

@@ -724,6 +724,7 @@ __global__ void __cluster_dims__(2, 1, 1)
   }
 }
 
+#ifdef NEBW_LAYER_KERNELS
 // Expert weights [experts, K, N] (fp32 or bf16) to bf16 RNE blocks of 128
 // columns by 64 of K, [experts][column block][K block][128][64]: a block is
 // 16 KB in one piece, which a TMA box reads as 128 consecutive rows of 128
@@ -757,5 +758,6 @@ __global__ void stage_experts_kernel(const void *__restrict__ src, int src_bf16,
     dst[(block * 128 + n % 128) * 64 + k % 64] = __float2bfloat16_rn(tile[threadIdx.x][i]);
   }
 }
+#endif
 
 }  // namespace nebw

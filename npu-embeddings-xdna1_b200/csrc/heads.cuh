@@ -56,6 +56,7 @@ struct HeadArgs {
   int *err;
 };
 
+#ifdef NEBW_LAYER_KERNELS
 // cos and sin of every position and frequency, in double, scaled and rounded
 // once.
 __global__ void __launch_bounds__(256)
@@ -68,6 +69,7 @@ __global__ void __launch_bounds__(256)
   sincos(static_cast<double>(p) * inv_freq[i - p * n], &s, &c);
   table[i] = make_float2(static_cast<float>(c * scale), static_cast<float>(s * scale));
 }
+#endif
 
 // The table row of position `at`.
 __device__ __forceinline__ int64_t head_position(const HeadArgs &p, int64_t at) {

@@ -2,7 +2,8 @@
 // include/nebw.h: rotary positions, per-head norms, expert routing, grouped
 // products and the combine.  This file is part of the nebw.cu translation
 // unit (included at its end): it uses that file's device handle, tensor maps
-// and error reporting.  None of these has a counterpart in the reference.
+// and error reporting.  The kernels' launches are in layer_kernels.cu.  None of
+// these has a counterpart in the reference.
 
 namespace {
 
@@ -49,73 +50,13 @@ int where_is(nebw_dev *d, const void *p, bool *on_device) {
   return NEBW_OK;
 }
 
-template <int EPI>
-int set_grouped_attr() {
-  const auto a = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  const int smem = nebw::GroupedShape::kSmemBytes;
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<EPI, false>, a, smem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::gemm_grouped_kernel<EPI, true>, a, smem));
+// The grouped product's kernels, once a handle (when experts are staged).
+int ready_grouped(nebw_dev *d) {
+  std::lock_guard<std::mutex> lock(d->staged);
+  if (d->grouped_ready) return NEBW_OK;
+  NEBW_CUDA(nebw::ready_grouped(&d->grouped_pairs));
+  d->grouped_ready = true;
   return NEBW_OK;
-}
-
-int set_grouped_attrs() {
-  if (int rc = set_grouped_attr<nebw::kGrpBf16>()) return rc;
-  if (int rc = set_grouped_attr<nebw::kGrpBf16Gelu8>()) return rc;
-  if (int rc = set_grouped_attr<nebw::kGrpBf16Erf>()) return rc;
-  if (int rc = set_grouped_attr<nebw::kGrpF32>()) return rc;
-  if (int rc = set_grouped_attr<nebw::kGrpBf16SwiGLU>()) return rc;
-  return set_grouped_attr<nebw::kGrpBf16GeGLU>();
-}
-
-// Shared memory of the placing kernels: starts and totals, and the row masks
-// and counts of as many tiles of 32 rows as fit beside them (one a warp at
-// most).
-constexpr int kRouteSmem = 100 * 1024;
-int route_tiles(int experts) {
-  const int fit = (kRouteSmem / (experts * static_cast<int>(sizeof(int))) - 2) / 2;
-  return std::min(fit, nebw::kRouteWarps);
-}
-size_t route_smem(int experts) {
-  return (2 + 2 * static_cast<size_t>(route_tiles(experts))) * experts * sizeof(int);
-}
-
-template <int K>
-int set_route_attrs() {
-  const auto a = cudaFuncAttributeMaxDynamicSharedMemorySize;
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<float, K, 0>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<float, K, 2>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<__nv_bfloat16, K, 0>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_fused_kernel<__nv_bfloat16, K, 2>, a, kRouteSmem));
-  NEBW_CUDA(cudaFuncSetAttribute(nebw::route_place_kernel<K>, a, kRouteSmem));
-  return NEBW_OK;
-}
-
-// How many CTA pairs of the grouped product the GPU holds at once (none: the
-// product is refused, the rest of the library works).
-int query_grouped_pairs(int *pairs) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(2 * 74);
-  cfg.blockDim = dim3(nebw::kGroupedGatherThreads);
-  cfg.dynamicSmemBytes = nebw::GroupedShape::kSmemBytes;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = 2;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  NEBW_CUDA(cudaOccupancyMaxActiveClusters(
-      pairs, nebw::gemm_grouped_kernel<nebw::kGrpBf16, true>, &cfg));
-  return NEBW_OK;
-}
-
-int set_layer_op_attrs() {
-  if (int rc = set_route_attrs<1>()) return rc;
-  if (int rc = set_route_attrs<2>()) return rc;
-  if (int rc = set_route_attrs<4>()) return rc;
-  if (int rc = set_route_attrs<8>()) return rc;
-  if (int rc = set_route_attrs<16>()) return rc;
-  return set_grouped_attrs();
 }
 
 }  // namespace
@@ -201,9 +142,7 @@ extern "C" int nebw_stage_rope(nebw_dev *d, const double *inv_freq, int32_t n, i
   cudaError_t e =
       cudaMemcpyAsync(freq, inv_freq, n * sizeof(double), cudaMemcpyHostToDevice, d->stream);
   if (e == cudaSuccess) {
-    nebw::rope_table_kernel<<<static_cast<unsigned>((entries + 255) / 256), 256, 0, d->stream>>>(
-        freq, n, max_pos, scale, t.table);
-    e = cudaGetLastError();
+    e = nebw::launch_rope_table(freq, n, max_pos, scale, t.table, d->stream);
   }
   if (e == cudaSuccess) e = cudaStreamSynchronize(d->stream);
   cudaFree(freq);
@@ -278,86 +217,6 @@ int check_heads(const nebw_heads *h, const char *what, int32_t head_dim, int64_t
   return NEBW_OK;
 }
 
-template <typename T, int V, int NORM, bool PAIRS, int IT>
-int launch_heads_it(const nebw::HeadArgs &a, int lg, int per, cudaStream_t st) {
-  int q_chunks, chunks;
-  int64_t warps = a.rows;
-  if constexpr (IT == 0) {  // heads of all rows in one list a side
-    q_chunks = a.q.heads > 0;
-    chunks = q_chunks + (a.k.heads > 0);
-    warps = (a.rows * std::max(a.q.heads, a.k.heads) + per - 1) / per;
-  } else {
-    q_chunks = (a.q.heads + per * IT - 1) / (per * IT);
-    chunks = q_chunks + (a.k.heads + per * IT - 1) / (per * IT);
-  }
-  const dim3 grid(static_cast<unsigned>((warps + 7) / 8), chunks);
-  nebw::heads_vec_kernel<T, V, NORM, PAIRS, IT>
-      <<<grid, 256, 0, st>>>(a, lg, q_chunks, 1.0f / static_cast<float>(a.head_dim));
-  NEBW_CUDA(cudaGetLastError());
-  return NEBW_OK;
-}
-
-bool heads_vec_side(const nebw::HeadSide &s, size_t esz, int v) {
-  const size_t bytes = v * esz, weights = std::min<size_t>(16, v * sizeof(float));
-  return aligned(s.x, bytes) && aligned(s.out, bytes) && s.stride * esz % bytes == 0 &&
-         s.out_stride * esz % bytes == 0 && aligned(s.gamma, weights) && aligned(s.beta, weights);
-}
-
-// Whether vectors of v elements fit the heads (and a head a warp).
-bool heads_vec_fit(const nebw::HeadArgs &a, size_t esz, int v) {
-  return a.head_dim % (2 * v) == 0 && a.head_dim <= 64 * v && a.n % v == 0 &&
-         heads_vec_side(a.q, esz, v) && heads_vec_side(a.k, esz, v);
-}
-
-template <typename T, int V, int NORM, bool PAIRS>
-int launch_heads_vec(const nebw::HeadArgs &a, cudaStream_t st) {
-  int lg = 0;  // lanes a head
-  while ((2 * V << lg) < a.head_dim) ++lg;
-  const int per = 32 >> lg;  // heads a warp takes at once
-  if constexpr (V * sizeof(T) == 16) {
-    // four turns a warp share its table entries and weights (144 us against
-    // 170 for two, on the RMS case at heads_vec_kernel); one or two where the
-    // heads end there
-    const int most = std::max(a.q.heads, a.k.heads);
-    if (most < per && a.rows * most < (1ll << 31))
-      return launch_heads_it<T, V, NORM, PAIRS, 0>(a, lg, per, st);
-    if (most <= per) return launch_heads_it<T, V, NORM, PAIRS, 1>(a, lg, per, st);
-    if (most <= 2 * per) return launch_heads_it<T, V, NORM, PAIRS, 2>(a, lg, per, st);
-  }
-  return launch_heads_it<T, V, NORM, PAIRS, 4>(a, lg, per, st);
-}
-
-template <typename T, int NORM, bool PAIRS>
-int launch_heads(const nebw::HeadArgs &a, cudaStream_t st) {
-  constexpr int V = 16 / sizeof(T);
-  if (heads_vec_fit(a, sizeof(T), V)) return launch_heads_vec<T, V, NORM, PAIRS>(a, st);
-  if constexpr (sizeof(T) == 2)
-    if (heads_vec_fit(a, sizeof(T), 4)) return launch_heads_vec<T, 4, NORM, PAIRS>(a, st);
-  if (heads_vec_fit(a, sizeof(T), 2)) return launch_heads_vec<T, 2, NORM, PAIRS>(a, st);
-  const int heads = a.q.heads + a.k.heads;
-  const int64_t blocks = (a.rows * heads + 7) / 8;
-  NEBW_REQUIRE(blocks < (1ll << 31), "too many heads: %lld rows of %d",
-               static_cast<long long>(a.rows), heads);
-  nebw::heads_any_kernel<T, NORM, PAIRS><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-  NEBW_CUDA(cudaGetLastError());
-  return NEBW_OK;
-}
-
-template <typename T, int NORM>
-int launch_heads_layout(const nebw::HeadArgs &a, int layout, cudaStream_t st) {
-  return layout == NEBW_ROPE_PAIRS ? launch_heads<T, NORM, true>(a, st)
-                                   : launch_heads<T, NORM, false>(a, st);
-}
-
-template <typename T>
-int launch_heads_norm(const nebw::HeadArgs &a, int norm, int layout, cudaStream_t st) {
-  switch (norm) {
-    case NEBW_HEADNORM_RMS: return launch_heads_layout<T, nebw::kHeadNormRms>(a, layout, st);
-    case NEBW_HEADNORM_LAYER: return launch_heads_layout<T, nebw::kHeadNormLayer>(a, layout, st);
-    default: return launch_heads_layout<T, nebw::kHeadNormNone>(a, layout, st);
-  }
-}
-
 int run_heads(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype, int64_t rows,
               const int32_t *rows_dev, int32_t head_dim, int norm, float eps, uint64_t rope,
               int layout, const int32_t *pos, void *stream) {
@@ -410,9 +269,11 @@ int run_heads(nebw_dev *d, const nebw_heads *q, const nebw_heads *k, int dtype, 
   a.head_dim = head_dim;
   a.eps = eps;
   a.err = d->d_err;
-  const cudaStream_t st = pick_stream(d, stream);
-  return dtype == NEBW_F32 ? launch_heads_norm<float>(a, norm, layout, st)
-                           : launch_heads_norm<__nv_bfloat16>(a, norm, layout, st);
+  const bool f32 = dtype == NEBW_F32;
+  NEBW_REQUIRE(nebw::heads_fit(a, f32), "too many heads: %lld rows of %d",
+               static_cast<long long>(rows), a.q.heads + a.k.heads);
+  NEBW_CUDA(nebw::launch_heads(a, f32, norm, layout == NEBW_ROPE_PAIRS, pick_stream(d, stream)));
+  return NEBW_OK;
 }
 
 }  // namespace
@@ -464,42 +325,6 @@ int check_route(int64_t rows, int32_t experts, int32_t top_k) {
   NEBW_REQUIRE(rows >= 0 && rows < (1ll << 30) && rows * top_k < (1ll << 30),
                "%lld rows of %d experts refused", static_cast<long long>(rows), top_k);
   return NEBW_OK;
-}
-
-template <typename T, int K, int LG>
-int launch_route_lg(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
-  const size_t smem = route_smem(a.experts);
-  if (blocks == 0) {
-    nebw::route_fused_kernel<T, K, LG><<<1, nebw::kRouteThreads, smem, st>>>(a);
-  } else {
-    nebw::route_choose_kernel<T, K, LG><<<blocks, nebw::kRouteThreads, 0, st>>>(a);
-    NEBW_CUDA(cudaGetLastError());
-    nebw::route_place_kernel<K><<<blocks, nebw::kRouteThreads, smem, st>>>(a);
-  }
-  NEBW_CUDA(cudaGetLastError());
-  return NEBW_OK;
-}
-
-// Four lanes a row from three eights of experts on, else one.
-template <typename T, int K>
-int launch_route(nebw::RouteArgs a, int blocks, cudaStream_t st) {
-  const int eights = (a.experts + 7) / 8;
-  if (eights < 3) {
-    a.per = eights * 8;
-    return launch_route_lg<T, K, 0>(a, blocks, st);
-  }
-  a.per = (eights + 3) / 4 * 8;
-  return launch_route_lg<T, K, 2>(a, blocks, st);
-}
-
-// The list a lane keeps: the next power of two of top_k.
-template <typename T>
-int launch_route_k(const nebw::RouteArgs &a, int blocks, cudaStream_t st) {
-  if (a.k == 1) return launch_route<T, 1>(a, blocks, st);
-  if (a.k == 2) return launch_route<T, 2>(a, blocks, st);
-  if (a.k <= 4) return launch_route<T, 4>(a, blocks, st);
-  if (a.k <= 8) return launch_route<T, 8>(a, blocks, st);
-  return launch_route<T, 16>(a, blocks, st);
 }
 
 }  // namespace
@@ -556,15 +381,15 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
   a.row_dst = row_dst;
   a.hist = static_cast<int *>(ws);
   a.vec = experts % 8 == 0 && aligned(logits, 16) && stride * esz % 16 == 0;
-  a.tiles = route_tiles(experts);
+  a.tiles = nebw::route_tiles(experts);
   a.whole = (top_k == 4 || top_k == 8 || top_k == 16) && aligned(ids, 16) && aligned(row_dst, 16);
   const bool fused = route_fused(rows, experts, top_k);
   int blocks = fused ? 1 : static_cast<int>(route_blocks(rows, d->sm_count));
   a.block_rows = static_cast<int>(((rows + blocks - 1) / blocks + 31) / 32 * 32);
   blocks = static_cast<int>((rows + a.block_rows - 1) / a.block_rows);
   if (fused) blocks = 0;  // no counts of blocks
-  return dtype == NEBW_F32 ? launch_route_k<float>(a, blocks, st)
-                           : launch_route_k<__nv_bfloat16>(a, blocks, st);
+  NEBW_CUDA(nebw::launch_route(a, dtype == NEBW_F32, blocks, d->route_ready, st));
+  return NEBW_OK;
 }
 
 extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_t experts,
@@ -588,6 +413,7 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
   const cudaStream_t st = pick_stream(d, stream);
   const size_t esz = dtype == NEBW_F32 ? 4 : 2;
   NEBW_REQUIRE(!on_device || aligned(kn, esz), "expert weights are not aligned");
+  if (int rc = ready_grouped(d)) return rc;
   const size_t one = static_cast<size_t>(K) * N * esz;
   Experts w;
   w.experts = experts;
@@ -603,24 +429,15 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
     return set_error(NEBW_ENOMEM, "cudaMalloc for [%d, %lld, %lld] expert weights failed", experts,
                      static_cast<long long>(N), static_cast<long long>(K));
   }
-  const unsigned gx = static_cast<unsigned>(col_blocks * 4);
-  const unsigned gy = static_cast<unsigned>(k_blocks * 2);
-  const int cb = static_cast<int>(col_blocks), kb = static_cast<int>(k_blocks);
   cudaError_t e = cudaSuccess;
   if (on_device) {
-    nebw::stage_experts_kernel<<<dim3(gx, gy, experts), dim3(32, 8), 0, st>>>(
-        kn, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, 0, cb, kb,
-        w.ptr);
-    e = cudaGetLastError();
+    e = nebw::launch_stage_experts(kn, dtype == NEBW_BF16, K, N, w.gated, 0, experts, w.ptr, st);
   } else {
     for (int i = 0; i < experts && e == cudaSuccess; ++i) {  // one expert's copy at a time
       e = cudaMemcpyAsync(tmp, static_cast<const char *>(kn) + i * one, one,
                           cudaMemcpyHostToDevice, st);
       if (e != cudaSuccess) break;
-      nebw::stage_experts_kernel<<<dim3(gx, gy, 1), dim3(32, 8), 0, st>>>(
-          tmp, dtype == NEBW_BF16, static_cast<int>(K), static_cast<int>(N), w.gated, i, cb, kb,
-          w.ptr);
-      e = cudaGetLastError();
+      e = nebw::launch_stage_experts(tmp, dtype == NEBW_BF16, K, N, w.gated, i, 1, w.ptr, st);
     }
   }
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
@@ -636,23 +453,7 @@ extern "C" int nebw_stage_experts(nebw_dev *d, const void *kn, int dtype, int32_
 
 namespace {
 
-struct GroupedMaps {
-  CUtensorMap a, a128, w, c;
-};
-
-template <int EPI>
-void launch_grouped_epi(const GroupedMaps &m, const nebw::GroupedArgs &a, unsigned grid,
-                        cudaStream_t st) {
-  const size_t smem = nebw::GroupedShape::kSmemBytes;
-  if (a.row_src)
-    nebw::gemm_grouped_kernel<EPI, true>
-        <<<grid, nebw::kGroupedGatherThreads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
-  else
-    nebw::gemm_grouped_kernel<EPI, false>
-        <<<grid, nebw::kGroupedThreads, smem, st>>>(m.a, m.a128, m.w, m.c, a);
-}
-
-int launch_grouped(nebw_dev *d, const GroupedMaps &m, int epi, const nebw::GroupedArgs &a,
+int run_grouped(nebw_dev *d, const nebw::GroupedMaps &m, int epi, const nebw::GroupedArgs &a,
                    cudaStream_t st) {
   // the most tiles that the groups can make: every one may end in a part tile
   const int64_t tiles = (a.rows / a.tile_rows + std::min(a.experts, a.rows)) *
@@ -660,15 +461,7 @@ int launch_grouped(nebw_dev *d, const GroupedMaps &m, int epi, const nebw::Group
   NEBW_REQUIRE(tiles < (1ll << 30), "grouped product too large");
   NEBW_REQUIRE(d->grouped_pairs > 0, "this GPU holds no CTA pair of the grouped product");
   const unsigned g = 2 * static_cast<unsigned>(std::min<int64_t>(tiles, d->grouped_pairs));
-  switch (epi) {
-    case nebw::kGrpBf16: launch_grouped_epi<nebw::kGrpBf16>(m, a, g, st); break;
-    case nebw::kGrpBf16Gelu8: launch_grouped_epi<nebw::kGrpBf16Gelu8>(m, a, g, st); break;
-    case nebw::kGrpBf16Erf: launch_grouped_epi<nebw::kGrpBf16Erf>(m, a, g, st); break;
-    case nebw::kGrpF32: launch_grouped_epi<nebw::kGrpF32>(m, a, g, st); break;
-    case nebw::kGrpBf16SwiGLU: launch_grouped_epi<nebw::kGrpBf16SwiGLU>(m, a, g, st); break;
-    case nebw::kGrpBf16GeGLU: launch_grouped_epi<nebw::kGrpBf16GeGLU>(m, a, g, st); break;
-  }
-  NEBW_CUDA(cudaGetLastError());
+  NEBW_CUDA(nebw::launch_grouped(m, epi, a, g, st));
   return NEBW_OK;
 }
 
@@ -729,7 +522,7 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   else if (c_dtype == NEBW_F32) epi = nebw::kGrpF32;
   else if (act == NEBW_ACT_GELU8) epi = nebw::kGrpBf16Gelu8;
   else if (act == NEBW_ACT_GELU_ERF) epi = nebw::kGrpBf16Erf;
-  GroupedMaps m;
+  nebw::GroupedMaps m;
   if (int rc = make_tmap_kmajor(&m.a, A, a_rows, K, row_src ? 1 : nebw::kGroupedBox)) return rc;
   if (row_src) m.a128 = m.a;  // not used
   else if (int rc = make_tmap_kmajor(&m.a128, A, a_rows, K, nebw::kGemmBM)) return rc;
@@ -746,27 +539,8 @@ extern "C" int nebw_gemm_grouped(nebw_dev *d, uint64_t weight, const void *A, in
   // 2.1e-6, four of half ones 3.5e-7 / 4.7e-7 / 1.0e-6, which fp32 sums keep
   // below 6.1e-7.  It costs 625 us against 413 (65,542 rows, K 4096, N 1024).
   if (c_dtype == NEBW_F32 && K > 1536) a.tile_rows = 128;
-  return launch_grouped(d, m, epi, a, pick_stream(d, stream));
+  return run_grouped(d, m, epi, a, pick_stream(d, stream));
 }
-
-namespace {
-
-template <typename TY, typename TO>
-void launch_combine(const nebw::CombineArgs &a, bool vec, cudaStream_t st) {
-  const int segments = (a.H + 255) / 256;
-  const int64_t items = static_cast<int64_t>(a.rows) * segments;
-  if (vec && items < (1ll << 31)) {
-    const unsigned g = static_cast<unsigned>((items + 7) / 8);
-    if (a.k > 4) nebw::moe_combine_kernel<TY, TO, 8><<<g, 256, 0, st>>>(a, segments);
-    else if (a.k > 2) nebw::moe_combine_kernel<TY, TO, 4><<<g, 256, 0, st>>>(a, segments);
-    else nebw::moe_combine_kernel<TY, TO, 2><<<g, 256, 0, st>>>(a, segments);
-  } else {
-    nebw::moe_combine_any_kernel<TY, TO>
-        <<<static_cast<unsigned>((static_cast<int64_t>(a.rows) + 7) / 8), 256, 0, st>>>(a);
-  }
-}
-
-}  // namespace
 
 extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t y_rows,
                                 const int32_t *row_dst, const float *weights, int64_t rows,
@@ -807,14 +581,7 @@ extern "C" int nebw_moe_combine(nebw_dev *d, const void *y, int y_dtype, int64_t
   a.H = static_cast<int>(H);
   a.err = d->d_err;
   const bool vec = H % 8 == 0 && aligned(y, 16) && aligned(out, 16) && aligned(residual, 16);
-  const cudaStream_t st = pick_stream(d, stream);
-  if (y_dtype == NEBW_F32) {
-    if (out_dtype == NEBW_F32) launch_combine<float, float>(a, vec, st);
-    else launch_combine<float, __nv_bfloat16>(a, vec, st);
-  } else {
-    if (out_dtype == NEBW_F32) launch_combine<__nv_bfloat16, float>(a, vec, st);
-    else launch_combine<__nv_bfloat16, __nv_bfloat16>(a, vec, st);
-  }
-  NEBW_CUDA(cudaGetLastError());
+  NEBW_CUDA(nebw::launch_combine(a, y_dtype == NEBW_F32, out_dtype == NEBW_F32, vec,
+                                 pick_stream(d, stream)));
   return NEBW_OK;
 }

@@ -28,6 +28,7 @@
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
+#include <atomic>
 #include <cctype>
 #include <cmath>
 #include <cstdarg>
@@ -45,11 +46,9 @@
 #include "attention.cuh"
 #include "attention_tc.cuh"
 #include "gated.cuh"
-#include "gemm_grouped.cuh"
 #include "gemm_i8.cuh"
 #include "gemm_tc.cuh"
-#include "heads.cuh"
-#include "moe.cuh"
+#include "layer_kernels.h"
 #include "npue_file.h"
 #include "npue_pack.h"
 #include "ptx.cuh"
@@ -262,7 +261,12 @@ struct nebw_dev {
   // CTA pairs the GPU can hold at once for the 2-CTA GEMM (0: use the
   // single-CTA kernel); NEBW_GEMM_CTAS=1 in the environment forces 0.
   int gemm_pairs = 0;
-  int grouped_pairs = 0;  // and for the grouped product
+  // The kernels of rotary and expert layers are made ready by the first call
+  // that needs them (layer_ops.cuh), not by nebw_open, whose first call they
+  // would make 15 ms longer.
+  bool grouped_ready = false;  // under `staged`
+  int grouped_pairs = 0;       // CTA pairs for the grouped product
+  std::atomic<uint32_t> route_ready{0};  // a bit a kernel of the routing
   // attention kernel: NEBW_ATTN_MMA (mma.sync flash) or NEBW_ATTN_TCGEN05
   // (UMMA/TMEM); see nebw_set_attention_kernel
   int attn_kind = NEBW_ATTN_TCGEN05;
@@ -755,11 +759,6 @@ int set_gemm_i8_attrs() {
   return NEBW_OK;
 }
 
-namespace {
-int set_layer_op_attrs();  // layer_ops.cuh
-int query_grouped_pairs(int *pairs);
-}
-
 extern "C" int nebw_open(int device, nebw_dev **out) {
   NEBW_REQUIRE(out != nullptr, "null output handle");
   *out = nullptr;
@@ -784,7 +783,6 @@ extern "C" int nebw_open(int device, nebw_dev **out) {
   if (int rc = set_all_gemm_attrs()) return rc;
   if (int rc = set_gemm_i8_attrs<128>()) return rc;
   if (int rc = set_gemm_i8_attrs<256>()) return rc;
-  if (int rc = set_layer_op_attrs()) return rc;
   NEBW_CUDA(cudaFuncSetAttribute(nebw::attention_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  nebw::AttnTcShape<64>::kSmemBytes));
   NEBW_CUDA(cudaFuncSetAttribute(nebw::attention_tc_kernel<64>, cudaFuncAttributePreferredSharedMemoryCarveout,
@@ -795,7 +793,6 @@ extern "C" int nebw_open(int device, nebw_dev **out) {
                                  cudaSharedmemCarveoutMaxShared));
 
   if (int rc = query_gemm_pairs(&d->gemm_pairs)) return rc;
-  if (int rc = query_grouped_pairs(&d->grouped_pairs)) return rc;
   if (int rc = load_tensor_map_encoder()) return rc;
   *out = d.release();
   return NEBW_OK;

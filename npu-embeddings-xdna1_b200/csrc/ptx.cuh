@@ -115,6 +115,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, int *e
   return mbar_wait_for(bar, parity, err, kWaitTimeoutNs);
 }
 
+#ifndef NEBW_LAYER_KERNELS
 // Self-check of the bounded wait: one warp waits on an mbarrier that nothing
 // arrives on (its phase 0 never completes), for `limit_ns`.  No copy or
 // tensor-core product is in flight.  out[0] = 1 if the wait ran out (and
@@ -129,6 +130,7 @@ __global__ void wait_probe_kernel(uint64_t limit_ns, int *err, int *out) {
   const bool done = mbar_wait_for(&bar, 0, err, limit_ns);
   if (threadIdx.x == 0) out[0] = done ? 0 : 1;
 }
+#endif
 
 // ---- TMA ------------------------------------------------------------------
 

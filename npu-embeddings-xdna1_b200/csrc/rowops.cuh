@@ -24,6 +24,7 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
+#ifndef NEBW_LAYER_KERNELS
 // seq_off[0..B] = exclusive prefix sum of seq_len; seq_off[B] = T (the
 // packed token count).  Lengths outside [1, S] are reported (kDevBadLength)
 // and clamped so that nothing downstream indexes out of bounds.
@@ -59,6 +60,7 @@ __global__ void __launch_bounds__(1024)
   }
   if (tid == blockDim.x - 1) seq_off[B] = part[tid];
 }
+#endif
 
 // LayerNorm of one warp-owned row held as NV float4 per lane (H = 128*NV),
 // in place.
@@ -274,6 +276,7 @@ __global__ void __launch_bounds__(kRowWarps * 32)
 // before the square root; the result is rounded to fp32 once.
 constexpr int kPoolThreads = 256;
 
+#ifndef NEBW_LAYER_KERNELS
 __global__ void __launch_bounds__(kPoolThreads)
     pool_l2_kernel(const float *__restrict__ h, const int *__restrict__ seq_off,
                    const int *__restrict__ seq_len, int H, int cls, int l2,
@@ -322,7 +325,9 @@ __global__ void __launch_bounds__(kPoolThreads)
     if (c < H) out[static_cast<int64_t>(b) * H + c] = static_cast<float>(acc[k] / nrm);
   }
 }
+#endif
 
+#ifndef NEBW_LAYER_KERNELS
 // Weight staging: fp32 or bf16 [K, N] (the container's layout) to bf16
 // [N, K] (K-major, the UMMA B-operand layout the GEMM's tensor map tiles),
 // with round-to-nearest-even (to_bf16, host_kernels.hpp:157-161).
@@ -346,7 +351,9 @@ __global__ void stage_weight_kernel(const void *__restrict__ src, int src_bf16, 
     if (n < N && k < K) dst[static_cast<int64_t>(n) * K + k] = __float2bfloat16_rn(tile[threadIdx.x][i]);
   }
 }
+#endif
 
+#ifndef NEBW_LAYER_KERNELS
 // fp32 -> bf16 RNE, elementwise (the standalone narrow, for op-level use).
 __global__ void narrow_bf16_kernel(const float *__restrict__ x, int64_t n,
                                    __nv_bfloat16 *__restrict__ y) {
@@ -361,5 +368,6 @@ __global__ void narrow_bf16_kernel(const float *__restrict__ x, int64_t n,
     for (int64_t j = i; j < n; ++j) y[j] = __float2bfloat16_rn(x[j]);
   }
 }
+#endif
 
 }  // namespace nebw

@@ -1687,3 +1687,60 @@ def test_staging_beside_running_operators(device):
         assert torch.equal(outs[i][0], outs[2][0]) and torch.equal(outs[i][1], outs[2][1])
     device.release_weight(table)
     device.release_weight(experts)
+
+
+FIRST_CALLS = """
+import sys
+import numpy as np, torch
+sys.path[:0] = sys.argv[1:2]
+import nebw
+d = nebw.Device(0, torch_stream=True)
+rows, E, k, H = 300, 256, 8, 128
+g = torch.Generator(device="cuda").manual_seed(1)
+logits = torch.randn(rows, E, generator=g, device="cuda")
+a = torch.randn(rows, H, generator=g, device="cuda").bfloat16()
+x = torch.randn(rows, 2 * H, generator=g, device="cuda").bfloat16()
+gamma = torch.ones(64, device="cuda")
+pos = torch.arange(rows, device="cuda").int()
+w = d.stage_experts((torch.randn(E, H, H, generator=g, device="cuda") / 12).bfloat16())
+table = d.stage_rope(nebw.rope_freqs(10000.0, 64)[0], rows)
+it = dict(dtype=torch.int32, device="cuda")
+
+def buffers():
+    ws = torch.empty(nebw.moe_route_workspace(rows, E, k), dtype=torch.uint8, device="cuda")
+    return (torch.zeros(rows, k, **it), torch.zeros(rows, k, device="cuda"), torch.zeros(E + 1, **it),
+            torch.zeros(rows * k, **it), torch.zeros(rows, k, **it), ws,
+            torch.zeros(rows * k, H, dtype=torch.bfloat16, device="cuda"),
+            torch.zeros(rows, H, device="cuda"), torch.zeros_like(x))
+
+def run(ids, weights, off, src, dst, ws, y, out, turned, n):
+    d.moe_route(logits, n, E, k, ids, weights, off, src, dst, ws, renorm=True)
+    d.gemm_grouped(w, a, rows, off, rows * k, H, H, y, row_src=src)
+    d.moe_combine(y, dst, weights, n, k, H, out)
+    d.qk_norm_rope(nebw.Heads.of(x, 4, out=turned, gamma=gamma), None, rows, 64, rope=table, pos=pos)
+
+for n in (rows, 20):  # two routing kernels, and one
+    one, two = buffers(), buffers()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        run(*one, n)
+    graph.replay()
+    run(*two, n)
+    d.sync()
+    assert all(torch.equal(s, t) for s, t in zip(one[:5] + one[6:], two[:5] + two[6:]))
+    assert (one[7][:n] != 0).any()
+print("same")
+"""
+
+
+def test_first_calls_of_a_process_inside_a_capture(device):
+    """The operators' kernels are made ready by the first call that needs them:
+    that call may be one that a graph captures."""
+    import subprocess
+    import sys
+
+    from conftest import PKG
+    out = subprocess.run([sys.executable, "-c", FIRST_CALLS, str(PKG)], capture_output=True,
+                         text=True, timeout=300)
+    assert out.returncode == 0 and out.stdout.strip() == "same", out.stderr[-2000:]
