@@ -86,7 +86,7 @@ class Heads(C.Structure):
                 _addr(beta))
         h.dtype = _dtype(x)
         h.tensors = tuple(t for t in (x, out, gamma, beta) if t is not None)
-        h.rows, h.width = x.shape
+        h.rows, h.head_dim = x.shape[0], x.shape[1] // heads
         gpus = {t.get_device() for t in h.tensors}
         h.gpu = gpus.pop() if len(gpus) == 1 else -1  # -1: not on one GPU
         return h
@@ -306,18 +306,20 @@ class Device:
         """Device address of n contiguous values of a dtype: a torch tensor of
         another dtype, with gaps, in host memory, on another GPU or with fewer
         values is refused (its bytes would be read as other numbers, or what
-        lies behind them), and so are rows of another width, if one is given
-        (they would be read as rows of that width)."""
+        lies behind them), and so are more than n in rows of another width, if
+        one is given (they would be read as rows of that width)."""
         if x is None or isinstance(x, int):
             return x
         import torch
         if (x.dtype is not getattr(torch, name) or x.get_device() != self.index
                 or not x.is_contiguous()):
             raise TypeError(f"contiguous {name} values on the handle's GPU are required")
-        if x.numel() < n:
-            raise ValueError(f"{x.numel()} {name} values where {n} are read or written")
-        if width:
-            self._wide(x, width)
+        have = x.numel()
+        if have != n:
+            if have < n:
+                raise ValueError(f"{have} {name} values where {n} are read or written")
+            if width:
+                self._wide(x, width)
         return x.data_ptr()
 
     @staticmethod
@@ -326,7 +328,7 @@ class Device:
             raise ValueError(f"rows of {x.size(-1)} values where they are of {width}")
 
     # The two below are _typed without its lookups (a short call has half a
-    # dozen of them), and without a look at the width of exactly n values.
+    # dozen of them).
     def _i32(self, x, n: int = 0, width: int = 0):
         if x is None or x.__class__ is int:
             return x
@@ -487,12 +489,13 @@ class Device:
                     raise TypeError("query and key heads of different dtypes")
                 if h.gpu != self.index:
                     raise TypeError("heads on the handle's GPU are required")
-                if rows > h.rows or h.heads * head_dim > h.width:
-                    raise ValueError(f"{rows} rows of {h.heads} x {head_dim} in heads of "
-                                     f"[{h.rows}, {h.width}]")
-                if h.heads * head_dim < h.width:  # (a norm's weights have their length too)
-                    raise NebwError(1, f"heads of {h.width // h.heads} elements are more than "
-                                       f"head_dim {head_dim}")
+                if rows > h.rows or head_dim != h.head_dim:
+                    if rows > h.rows or head_dim > h.head_dim:
+                        raise ValueError(f"{rows} rows of {h.heads} x {head_dim} in heads of "
+                                         f"[{h.rows}, {h.heads} x {h.head_dim}]")
+                    # (a norm's weights have their length too)
+                    raise NebwError(1, f"heads of {h.head_dim} elements are more than head_dim "
+                                       f"{head_dim}")
                 dtype = d
         return BF16 if dtype is None else dtype
 
@@ -538,9 +541,10 @@ class Device:
         tensor, its row stride kept) and the rows grouped by expert
         (nebw_moe_route).  workspace: a tensor of moe_route_workspace bytes,
         or None where that is 0."""
-        if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < experts:
+        shape = logits.shape
+        if len(shape) != 2 or logits.stride(1) != 1 or shape[1] < experts:
             raise ValueError("logits are rows of at least `experts` adjacent values")
-        if logits.shape[0] < rows:
+        if shape[0] < rows:
             raise ValueError("fewer logit rows than rows")
         ws, ws_bytes = None, 0
         if workspace is not None:
@@ -550,7 +554,7 @@ class Device:
             raise TypeError("logits and a contiguous workspace on the handle's GPU are required")
         stride = logits.stride(0) if rows > 1 else experts  # one row: torch may give any
         n = rows * top_k
-        wide = top_k if 0 < top_k <= min(MAX_TOP_K, experts) else 0  # others are refused below
+        wide = top_k if 0 < top_k <= experts and top_k <= MAX_TOP_K else 0  # or refused below
         _check(lib().nebw_moe_route(self.h, logits.data_ptr(), _dtype(logits), stride, rows,
                                     self._i32(rows_dev, 1), experts, top_k, score, int(renorm),
                                     scale, self._i32(ids, n, wide), self._f32(weights, n, wide),
@@ -584,12 +588,16 @@ class Device:
         if (y.get_device() != self.index or out.get_device() != self.index
                 or not (y.is_contiguous() and out.is_contiguous())):
             raise TypeError("contiguous expert rows and output on the handle's GPU are required")
-        y_rows, n = y.numel() // H if H > 0 else 0, rows * top_k
+        y_rows, n = y.shape[0], rows * top_k
         if H > 0:  # (other widths are refused below)
-            self._wide(y, H)
-            self._wide(out, H)
-            if out.numel() < rows * H:
-                raise ValueError(f"output {tuple(out.shape)} for {rows} rows of {H}")
+            if y.numel() != y_rows * H:  # not rows of H: of another width, or in more dimensions
+                self._wide(y, H)
+                y_rows = y.numel() // H
+            have = out.numel()
+            if have != rows * H:
+                if have < rows * H:
+                    raise ValueError(f"output {tuple(out.shape)} for {rows} rows of {H}")
+                self._wide(out, H)
         wide = top_k if 0 < top_k <= MAX_TOP_K else 0
         _check(lib().nebw_moe_combine(self.h, y.data_ptr(), _dtype(y), y_rows,
                                       self._i32(row_dst, n, wide), self._f32(weights, n, wide),
