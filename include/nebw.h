@@ -349,9 +349,11 @@ int nebw_qk_norm_rope(nebw_dev *dev, const nebw_heads *q, const nebw_heads *k, i
 
 /* The weights of `experts` (up to 512) experts, [experts, K, N] row-major,
  * each the container's [K, N] operand, fp32 or bf16, in host memory or on
- * this device (then read on `stream`); staged once as bf16 RNE [experts, N,
- * K].  gated != 0: N = 2F = [up | gate] along N, F % 32 == 0, and the
- * grouped product forms up * act(gate).  K % 8 == 0, K >= 64, N % 8 == 0.
+ * this device (then read on `stream`); staged once as bf16 RNE in blocks of
+ * 128 columns by 64 of K: experts * ceil(N / 256) * ceil(K / 64) * 32 KB of
+ * device memory (N = 8 takes what 256 columns do).  gated != 0: N = 2F =
+ * [up | gate] along N, F % 32 == 0, and the grouped product forms up *
+ * act(gate).  K % 8 == 0, K >= 64, N % 8 == 0.
  * Released with nebw_release_weight.  Synchronous. */
 int nebw_stage_experts(nebw_dev *dev, const void *kn, int dtype, int32_t experts, int64_t K,
                        int64_t N, int gated, void *stream, uint64_t *handle);

@@ -16,10 +16,12 @@
 // persistent pairs walk one list of tiles, whatever the groups are: every
 // block builds it from off.
 //
-// Measured: 373 us for 65,542 grouped rows, K 4096, N 1024, 8 experts (1473
-// TFLOP/s, 0.89 of the measured cuBLAS burst); 830 us gathered, K 1024, gated
-// N 8192 (1326 TFLOP/s; 717 us without the gather); 42.5 us for 16,088 rows of
-// 64 experts, K 1024, gated N 1024; 14.0 us for 28 rows of 8, K 768, N 3840.
+// Measured, replayed from a graph: 373 us for 65,542 grouped rows, K 4096, N
+// 1024, 8 experts (1473 TFLOP/s, 0.89 of the measured cuBLAS burst); 830 us
+// gathered, K 1024, gated N 8192 (1326 TFLOP/s; 717 us without the gather);
+// 42.5 us for 16,088 rows of 64 experts, K 1024, gated N 1024; 14.0 us for 28
+// rows of 8, K 768, N 3840.  In a loop of calls, where the power cap lowers the
+// clock: 372 to 457 us (1200 TFLOP/s), 830 to 957 (1150), 45 to 53, 16.4.
 // What bounds it: the tensor pipe for whole tiles, HBM for few rows a group,
 // and between them that W streams through the M side at 128 columns in 128
 // clocks a step of 16, however few the rows are (0.26 us a K-block for one

@@ -18,9 +18,10 @@
 // rounding, of the rotated value, at the end.
 //
 // Each element is read once and written once and takes a handful of fp32
-// operations, so HBM bounds it: rotation alone 83 us at 6.5 TB/s (1.00 of the
-// copy rate) on 65,539 rows of 32 heads of 64, RMS norm and rotation 142 us at
-// 5.9 TB/s (0.91) on 49,999 rows of 32 heads of 128.  LayerNorm keeps half as
+// operations, so HBM bounds it.  Replayed from a graph: rotation alone 83 us at
+// 6.5 TB/s (1.00 of the copy rate) on 65,539 rows of 32 heads of 64, RMS norm
+// and rotation 142 us at 5.9 TB/s (0.91) on 49,999 rows of 32 heads of 128; as
+// calls among others 89 and 157.  LayerNorm keeps half as
 // many warps on an SM and reads at 0.75; heads whose lanes are no power of two
 // (80, 96) leave lanes idle, at 0.66 to 0.91.  Sharing a warp's lanes out over
 // such heads without a gap was slower (159 against 129 us, heads of 80).
@@ -295,7 +296,9 @@ __device__ __forceinline__ void head_fold_pair(const uint64_t (&c2)[P], const ui
 // quarter of the work), RMS 188 / 144 / 156, LayerNorm 270 / 234 / 173.  Half
 // the vector holds half the state: RMS 106 / 115 / 115 (25,000 rows, fp32,
 // heads of 96), LayerNorm 141 / 128 / 163 there and 174 / 194 / 198 for bf16
-// in 8-byte vectors (heads of 80, turning 40).
+// in 8-byte vectors (heads of 80, turning 40).  The bounds were chosen by time
+// and cost some spills with four turns a warp: 48 bytes (half layout) and 20
+// (pairs) for bf16 without a norm, 28 and 8 with RMS, 8 for fp32 RMS.
 constexpr int head_blocks(int norm, int v, int bytes) {
   if (norm == kHeadNormNone) return 4;
   if (norm == kHeadNormRms) return v < 8 ? 4 : 3;

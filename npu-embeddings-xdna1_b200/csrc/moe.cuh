@@ -13,12 +13,18 @@
 // choice compares the logits themselves, and places come from counts, never
 // from the order in which blocks reach an atomic.
 //
-// Measured: 26.8 us for 131,071 rows of 64 bf16 logits by 8, whose bytes take
-// 5.2.  The choice is two thirds of it, bound by the min / max pipe (a row of
-// 64 takes 200 exchanges of keys); the places are the rest, a chain of short
-// steps behind one another.  (One warp a row, with a warp-wide maximum for
-// every chosen expert, and places by a match within 32 entries took 141 us.)
-// A few rows cost one launch: 3.1 us for 21 rows of 8 by 2.
+// Measured: 26.8 us replayed from a graph (31 as a call among others) for
+// 131,071 rows of 64 bf16 logits by 8, whose bytes take 5.2.  The choice is
+// about 17 of it.  A lane orders 16 keys and merges twice with another (86
+// exchanges, 204 min and max instructions with what picks the larger): the ALU
+// pipe is 77% busy while an SM works, 59% over the whole launch, and the rest
+// is waiting, for logits that are read and used in one turn and for a fourth
+// turn that is half empty (896 rows a block, 256 a turn).  The places are the
+// other third, a chain of counts and barriers with the issue slots 23% busy.
+// (One warp a row, with a warp-wide maximum for every chosen expert, and places
+// by a match within 32 entries took 141 us.)  fp32 logits, whose keys take 64
+// bits, are 1.5 times as long; lists of 16 of them spill 96 bytes.  A few rows
+// cost one launch: 3.1 us for 21 rows of 8 by 2.
 #pragma once
 
 #include <cuda_bf16.h>
