@@ -473,7 +473,7 @@ class Device:
         pos has `rows` entries, all of a tensor's if not given (an address
         needs them)."""
         if rows is None:
-            if pos.__class__ is int:
+            if pos is None or pos.__class__ is int:
                 raise ValueError("positions at an address need their number")
             rows = pos.numel()
         _check(lib().nebw_packed_positions(self.h, self._i32(seq_off, B), self._i32(seq_len, B), B,

@@ -221,8 +221,9 @@ def test_positions_say_how_many_they_are():
     assert "null device handle" in L.nebw_last_error().decode()
     d = nebw.Device.__new__(nebw.Device)
     d.h, d.index = None, 0
-    with pytest.raises(ValueError):
-        d.row_positions(64, 64, 1, 8, 64)
+    for nowhere in (64, None):
+        with pytest.raises(ValueError):
+            d.row_positions(64, 64, 1, 8, nowhere)
 
 
 def test_heads_of_refuses_what_it_cannot_describe():
