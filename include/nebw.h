@@ -378,7 +378,8 @@ int64_t nebw_moe_route_workspace(int64_t rows, int32_t experts, int32_t top_k);
  * Where fewer than top_k can be chosen the rest have id -1, weight 0, row_dst
  * -1 and no place.  rows_dev (may be NULL): device count of live rows; the
  * outputs of rows behind it, and row_src from group_off[experts] on, are left
- * as they are.  The result does not depend on scheduling. */
+ * as they are.  Logits, outputs and workspace must not overlap.  The result
+ * does not depend on scheduling. */
 int nebw_moe_route(nebw_dev *dev, const void *logits, int dtype, int64_t stride, int64_t rows,
                    const int32_t *rows_dev, int32_t experts, int32_t top_k, int score, int renorm,
                    float scale, int32_t *ids, float *weights, int32_t *group_off,

@@ -364,6 +364,21 @@ extern "C" int nebw_moe_route(nebw_dev *d, const void *logits, int dtype, int64_
   NEBW_REQUIRE(ws_bytes >= need && (ws || need == 0),
                "routing workspace of %lld bytes refused: %lld are needed",
                static_cast<long long>(ws_bytes), static_cast<long long>(need));
+  // what one block reads or writes must not be what another writes
+  const int64_t each = rows * top_k * 4;
+  const struct {
+    const void *p;
+    int64_t bytes;
+  } parts[] = {{logits, ((rows - 1) * stride + experts) * static_cast<int64_t>(esz)},
+               {ids, each},
+               {weights, each},
+               {group_off, (experts + 1) * int64_t{4}},
+               {row_src, each},
+               {row_dst, each},
+               {ws, need}};
+  for (const auto &x : parts)
+    for (const auto *y = &x + 1; y != std::end(parts); ++y)
+      NEBW_REQUIRE(!meet(x.p, x.bytes, y->p, y->bytes), "routing operands overlap");
   nebw::RouteArgs a{};
   a.logits = logits;
   a.stride = stride;

@@ -1259,6 +1259,23 @@ def test_results_over_what_is_still_read_are_refused(device):
             device.moe_combine(y, dst, wt, 4, 1, K, rows_of(i, 4))
     res = f[256:512].view(4, K)
     device.moe_combine(y, dst, wt, 4, 1, K, res, residual=res)
+    r = Routing(1200, 8, 2)
+    x = torch.zeros(1200, 8, device="cuda")
+    given = [r.ids, r.weights, r.off, r.src, r.dst, r.ws]
+    device.moe_route(x, 1200, 8, 2, *given)
+    assert r.ws.numel()  # two kernels
+    for i, t in enumerate(given):
+        onto = x.flatten()[-t.numel():] if i == 1 else x.view(torch.int32).flatten()[-t.numel():]
+        for j, other in ((None, onto), *((j, u) for j, u in enumerate(given) if j != i)):
+            if j is not None:
+                at = other.view(torch.float32 if i == 1 else torch.int32).flatten()
+                if at.numel() < t.numel():
+                    continue
+                other = at[-t.numel():]
+            new = list(given)
+            new[i] = other.view(t.shape)
+            with pytest.raises(nebw.NebwError, match="overlap"):
+                device.moe_route(x, 1200, 8, 2, *new)
     for out in (f[192:448].view(4, K), f[260:516].view(4, K), res.view(torch.bfloat16).view(8, K)):
         with pytest.raises(nebw.NebwError, match="overlap"):
             device.moe_combine(y, dst, wt, 4, 1, K, out, residual=res)
